@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define INTENT_HIP_ABI_VERSION 20
+#define INTENT_HIP_ABI_VERSION 21
 
 enum IntentHipStatus {
   INTENT_HIP_OK = 0,
@@ -65,7 +65,9 @@ enum IntentHipOperator {
   INTENT_HIP_OP_CONTINUOUS_DECODE = 19,   /* rows = HEAD_GROUP, cols = head dimension */
   INTENT_HIP_OP_VARLEN_DECODE = 20,       /* rows = HEAD_GROUP, cols = head dimension */
   INTENT_HIP_OP_DECODE_MERGE = 21,        /* cols = head dimension */
-  INTENT_HIP_OP_MLA_PREFILL = 22          /* cols = D | P << 16 */
+  INTENT_HIP_OP_MLA_PREFILL = 22,         /* cols = D | P << 16 */
+  INTENT_HIP_OP_QK_NORM_ROPE = 23,        /* dtype F16 or BF16; rows = tokens, cols = head width */
+  INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD = 24
 };
 
 /* Epilogue activations of intent_hip_gemm (the Activation enum of contraction/gemm.py:10-12). */
@@ -469,6 +471,29 @@ int intent_hip_csr_spmm_f32(const int32_t *row_offsets, const int32_t *column_in
                             const float *values, const float *dense, float *out, int64_t rows,
                             int64_t cols, int64_t nnz, int64_t features, int64_t ldd, int64_t ldo,
                             void *stream);
+
+/* Root-mean-square norm of every query and key head and the rotation of its token's position, no reference counterpart.
+ * q [tokens, q_heads, d], k [tokens, kv_heads, d] and the outputs of the same shapes in f16 or bf16 (d at most 1024);
+ * weights f32 [d]; positions i32 [tokens] (clamped into the tables); cos, sin f32 [table, pairs], 2 * pairs <= d. A head's
+ * row x gives y = x * rsqrt(mean(x^2) + eps) * weight in f32, of which the pairs (i, i + pairs), or (2i, 2i + 1) when
+ * `interleaved`, are turned by the position's angles; one rounding at the end. Outputs may not overlap inputs.
+ * strides[16]: q[3], k[3], cos[2], sin[2], q_out[3], k_out[3]. */
+int intent_hip_qk_norm_rope(int dtype, const void *q, const void *k, const float *q_weight, const float *k_weight,
+                            const int32_t *positions, const float *cos, const float *sin, void *q_out, void *k_out,
+                            int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t table, int64_t pairs,
+                            const int64_t strides[16], float eps, int interleaved, void *stream);
+
+/* Its gradients: grad_q, grad_k in the storage type, and the weights' gradients (f32 [d]), sums over tokens and heads in a
+ * fixed order through the workspace (intent_hip_qk_norm_rope_backward_workspace_bytes bytes, 16-byte aligned).
+ * strides[22]: q[3], k[3], cos[2], sin[2], grad_q_out[3], grad_k_out[3], grad_q[3], grad_k[3]. */
+int intent_hip_qk_norm_rope_backward_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t d,
+                                                     size_t *bytes);
+int intent_hip_qk_norm_rope_backward(int dtype, const void *q, const void *k, const float *q_weight, const float *k_weight,
+                                     const int32_t *positions, const float *cos, const float *sin, const void *grad_q_out,
+                                     const void *grad_k_out, void *grad_q, void *grad_k, float *grad_q_weight,
+                                     float *grad_k_weight, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t d,
+                                     int64_t table, int64_t pairs, const int64_t strides[22], float eps, int interleaved,
+                                     void *workspace, size_t workspace_bytes, void *stream);
 
 /* Measurement probe (no counterpart in the reference): the box's own MFMA ceiling, reported by the
  * benchmark beside the published peak, as the measurement protocol asks for an MFMA

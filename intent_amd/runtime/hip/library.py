@@ -11,7 +11,7 @@ from pathlib import Path
 
 from ...diagnostics import CompilationStageError
 
-ABI_VERSION = 20
+ABI_VERSION = 21
 # INTENT_HIP_STATIC_SCRATCH_BYTES: the static scratch of intent_hip_csr_spmv_f32_static.
 STATIC_SCRATCH_BYTES = 32 << 20
 LIBRARY_NAME = "libintent_hip.so"
@@ -22,7 +22,7 @@ F32, F16, BF16 = 0, 1, 2
  OP_ATTENTION_FWD, OP_ATTENTION_BWD_DELTA, OP_ATTENTION_BWD_DQ, OP_ATTENTION_BWD_DKDV, OP_PAGED_DECODE_PARTIALS,
  OP_SPLITK_REDUCE, OP_CSR_SPMM_F32, OP_ATTENTION_VARLEN, OP_GEMM_I8, OP_QUANTIZED_GEMM,
  OP_ATTENTION_BIAS, OP_GROUPED_DECODE_PARTIALS, OP_CONTINUOUS_DECODE, OP_VARLEN_DECODE, OP_DECODE_MERGE,
- OP_MLA_PREFILL) = range(23)
+ OP_MLA_PREFILL, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD) = range(25)
 ACT_NONE, ACT_RELU = 0, 1
 
 _i64, _int, _p, _f32, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_size_t
@@ -108,6 +108,11 @@ SIGNATURES = {
     "intent_hip_csr_spmv_f32": (_int, (_p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _sz, _p)),
     "intent_hip_csr_spmv_f32_static": (_int, (_p, _p, _p, _p, _p, _i64, _i64, _i64, _p)),
     "intent_hip_csr_spmm_f32": (_int, (_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p)),
+    "intent_hip_qk_norm_rope": (_int, (_int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+                                       ctypes.POINTER(_i64), _f32, _int, _p)),
+    "intent_hip_qk_norm_rope_backward_workspace_bytes": (_int, (_i64, _i64, _i64, _i64, ctypes.POINTER(_sz))),
+    "intent_hip_qk_norm_rope_backward": (_int, (_int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,
+                                                _i64, _i64, _i64, ctypes.POINTER(_i64), _f32, _int, _p, _sz, _p)),
     "intent_hip_mfma_probe": (_int, (_int, _int, _i64, _i64, _p, _p)),
 }
 

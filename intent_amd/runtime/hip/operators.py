@@ -34,7 +34,10 @@ Recognised definitions (reference file:line of the semantics each kernel follows
   varlen_gqa_decode_with_sink_logits streaming/attention.py:672-754  intent_hip_varlen_decode_sink
   csr_spmm                sparse/csr_spmm.py:11-33         intent_hip_csr_spmm_f32
 
-(paths relative to python/intent/examples/kernels/ in the reference).
+(paths relative to python/intent/examples/kernels/ in the reference), and of this package alone:
+
+  qk_norm_rope_{f16,bf16}           normalization/qk_norm_rope.py  intent_hip_qk_norm_rope
+  qk_norm_rope_backward_{f16,bf16}  backward/qk_norm_rope.py       intent_hip_qk_norm_rope_backward
 
 Layout handling: kernels read rows with unit inner stride. An input whose inner
 stride is not 1 is copied into a contiguous device buffer at every launch (on
@@ -53,7 +56,7 @@ from ...diagnostics import CompilationStageError
 from ..torch_views import raw_stream_getter
 from .library import (BF16, F16, F32, STATIC_SCRATCH_BYTES, OP_ATTENTION_BWD_DELTA, OP_ATTENTION_BWD_DKDV, OP_ATTENTION_BWD_DQ,
                       OP_ATTENTION_FWD, OP_ATTENTION_FWD_F16, OP_ATTENTION_BIAS, OP_ATTENTION_VARLEN, OP_MLA_PREFILL, OP_CSR_SPMV_F32, OP_GEMM, OP_GEMM_F32, OP_GEMM_I8, OP_QUANTIZED_GEMM,
-                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
+                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
 
 
 @dataclass
@@ -940,6 +943,83 @@ def _csr_spmm(lib, bound, constexprs, device):
                   lambda: lib.kernel_resources(OP_CSR_SPMM_F32, F32, rows, features))
 
 
+# ------------------------------------------------------------------------------ norm and rotation of heads
+def _interleaved(constexprs) -> int:
+    value = constexprs["INTERLEAVED"]
+    if not isinstance(value, bool):
+        raise CompilationStageError("provider_configuration", f"INTERLEAVED must be a bool, got {value!r}")
+    return int(value)
+
+
+def _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, before):
+    """The views as the kernels read them, and the extents (tokens, q_heads, kv_heads, d, table, pairs)."""
+    tokens, q_heads, d = q.shape
+    table, pairs = cos.shape
+    if 2 * pairs > d:
+        raise ValueError(f"{pairs} rotated pairs do not fit heads of width {d}")
+    if pairs and not table and tokens:
+        raise ValueError("the rotation tables hold no position")
+    views = [_readable(t, keep, before) for t in (q, k, q_weight, k_weight, positions, cos, sin)]
+    return views, (tokens, q_heads, k.shape[1], d, table, pairs)
+
+
+def _norm_rope(dtype_code):
+    """qk_norm_rope: q and k rows are read through their own strides (a projection's slices), staged only where their
+    inner stride is not 1."""
+    def plan(lib, bound, constexprs, device):
+        q, k, q_weight, k_weight, positions, cos, sin, q_out, k_out, eps = bound.arguments
+        interleaved = _interleaved(constexprs)
+        keep, before, after = list(bound.arguments[:9]), [], []
+        views, extents = _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, before)
+        outs = [_writable(t, keep, after) for t in (q_out, k_out)]
+        strides = _strides(views[0], views[1], views[5], views[6], *outs)
+        keep.append(strides)
+        fn = lib.fn["qk_norm_rope"]
+        args = (dtype_code, *(t.data_ptr() for t in (*views, *outs)), *extents, strides, float(eps), interleaved)
+        return Launch("intent_hip_qk_norm_rope", lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
+                      tuple(zip(("tokens", "q_heads", "kv_heads", "d", "table", "pairs"), extents)),
+                      lambda: lib.kernel_resources(OP_QK_NORM_ROPE, dtype_code, extents[0], extents[3]))
+    return plan
+
+
+def _norm_rope_backward(dtype_code):
+    """qk_norm_rope_backward: workgroups keep their share of the weights' gradients, summed in order through a workspace."""
+    def plan(lib, bound, constexprs, device):
+        import ctypes
+
+        (q, k, q_weight, k_weight, positions, cos, sin, grad_q_out, grad_k_out, grad_q, grad_k, grad_q_weight, grad_k_weight,
+         eps) = bound.arguments
+        interleaved = _interleaved(constexprs)
+        if _static_workspace():
+            raise CompilationStageError(
+                "provider_preparation", "qk_norm_rope_backward sums the weights' gradients through a workspace; "
+                "backend_options workspace='static' has none for it, use workspace='prepare'")
+        keep, before, after = list(bound.arguments[:13]), [], []
+        views, extents = _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, before)
+        grads = [_readable(t, keep, before) for t in (grad_q_out, grad_k_out)]
+        outs = [_writable(t, keep, after) for t in (grad_q, grad_k, grad_q_weight, grad_k_weight)]
+        strides = _strides(views[0], views[1], views[5], views[6], *grads, *outs[:2])
+        keep.append(strides)
+        size = ctypes.c_size_t(0)
+        lib.check(lib.fn["qk_norm_rope_backward_workspace_bytes"](*extents[:4], ctypes.byref(size)), "provider_preparation")
+        args = (dtype_code, *(t.data_ptr() for t in (*views, *grads, *outs)), *extents, strides, float(eps), interleaved)
+        run = _workspace_run(lib.fn["qk_norm_rope_backward"], args, size.value, device, keep)
+        return Launch("intent_hip_qk_norm_rope_backward", run, tuple(keep), tuple(before), tuple(after),
+                      tuple(zip(("tokens", "q_heads", "kv_heads", "d", "table", "pairs"), extents))
+                      + (("workspace_bytes", size.value),),
+                      lambda: lib.kernel_resources(OP_QK_NORM_ROPE_BACKWARD, dtype_code, extents[0], extents[3]))
+    return plan
+
+
+def _norm_rope_signature(element, backward):
+    rows, table, weight = _view(IN, element, 3), _view(IN, "f32", 2), _view(IN, "f32", 1)
+    inputs = (rows, rows, weight, weight, _view(IN, "i32", 1), table, table)
+    out, out_weight = _view(OUT, element, 3), _view(OUT, "f32", 1)
+    if backward:
+        return (*inputs, rows, rows, out, out, out_weight, out_weight, ("scalar", "f32"))
+    return (*inputs, out, out, ("scalar", "f32"))
+
+
 _SPECS = (
     OperatorSpec("stable_softmax", (_view(IN, "f32", 2), _view(OUT, "f32", 2)), (), _softmax_fwd(F32), True),
     OperatorSpec("stable_softmax_f16", (_view(IN, "f16", 2), _view(OUT, "f16", 2)), (), _softmax_fwd(F16), True),
@@ -1015,6 +1095,11 @@ _SPECS = (
                               _view(OUT, "f32", 2)), (), _csr_spmm, derived=(("R", "R1", -1),)),
     OperatorSpec("csr_spmv", (_view(IN, "i32", 1), _view(IN, "i32", 1), _view(IN, "f32", 1), _view(IN, "f32", 1),
                               _view(OUT, "f32", 1)), (), _csr_spmv, derived=(("R", "R1", -1),)),
+    OperatorSpec("qk_norm_rope_f16", _norm_rope_signature("f16", False), ("INTERLEAVED",), _norm_rope(F16)),
+    OperatorSpec("qk_norm_rope_bf16", _norm_rope_signature("bf16", False), ("INTERLEAVED",), _norm_rope(BF16)),
+    OperatorSpec("qk_norm_rope_backward_f16", _norm_rope_signature("f16", True), ("INTERLEAVED",), _norm_rope_backward(F16)),
+    OperatorSpec("qk_norm_rope_backward_bf16", _norm_rope_signature("bf16", True), ("INTERLEAVED",),
+                 _norm_rope_backward(BF16)),
 )
 
 SPECS = {spec.name: spec for spec in _SPECS}
@@ -1038,6 +1123,9 @@ ENTRY_POINTS = {
     "varlen_gqa_decode_with_sink_logits": "intent_hip_varlen_decode_sink",
     "splitk_attention_f32_to_f16_reduce": "intent_hip_splitk_reduce_f32_to_f16",
     "csr_spmm": "intent_hip_csr_spmm_f32", "csr_spmv": "intent_hip_csr_spmv_f32",
+    "qk_norm_rope_f16": "intent_hip_qk_norm_rope", "qk_norm_rope_bf16": "intent_hip_qk_norm_rope",
+    "qk_norm_rope_backward_f16": "intent_hip_qk_norm_rope_backward",
+    "qk_norm_rope_backward_bf16": "intent_hip_qk_norm_rope_backward",
 }
 assert set(ENTRY_POINTS) == set(SPECS)
 

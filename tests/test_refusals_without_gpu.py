@@ -1,0 +1,51 @@
+"""The entry points without a reference counterpart refuse bad requests on the host, before any HIP call; empty work is a
+successful no-op."""
+import ctypes
+
+from intent_amd.runtime.hip import library as hiplib
+
+F16, BF16 = hiplib.F16, hiplib.BF16
+
+
+def strides(*groups):
+    values = [s for group in groups for s in group]
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def test_norm_rope():
+    lib = hiplib.library()
+    err = lambda: lib.fn["last_error"]()  # noqa: E731
+    good = [(1024, 128, 1), (1024, 128, 1), (64, 1), (64, 1), (1024, 128, 1), (1024, 128, 1)]
+
+    def call(dtype=F16, q=16, positions=16, tokens=4, heads=8, kv=2, d=128, table=100, pairs=64, groups=good):
+        return lib.fn["qk_norm_rope"](dtype, q, 16, 16, 16, positions, 16, 16, 16, 16, tokens, heads, kv, d, table, pairs,
+                                      strides(*groups), 1e-6, 0, None)
+
+    assert call(dtype=hiplib.F32) == 1 and b"dtype" in err()
+    assert call(tokens=-1) == 1 and b"negative" in err()
+    assert call(pairs=65) == 1 and b"do not fit" in err()
+    assert call(d=1025) == 2 and b"1024" in err()
+    assert call(q=None) == 1 and b"null" in err()
+    assert call(positions=None) == 1 and b"null" in err()
+    assert call(table=0) == 1 and b"hold no position" in err()
+    assert call(groups=[(1024, 128, 2)] + good[1:]) == 1 and b"unit inner stride" in err()
+    assert call(groups=[(-1024, 128, 1)] + good[1:]) == 1 and b"negative stride" in err()
+    assert call(groups=good[:2] + [(64, 2)] + good[3:]) == 1 and b"tables" in err()
+    assert call(tokens=2 ** 40) == 2
+    assert call(tokens=0, q=None) == 0 and call(d=0, pairs=0) == 0 and call(heads=0, kv=0) == 0
+
+    size = ctypes.c_size_t(0)
+    query = lib.fn["qk_norm_rope_backward_workspace_bytes"]
+    assert query(16384, 32, 8, 128, ctypes.byref(size)) == 0 and 0 < size.value <= 1026 * 128 * 4
+    assert query(0, 32, 8, 128, ctypes.byref(size)) == 0 and size.value == 0
+    assert query(16384, 32, 8, 128, None) == 1 and query(-1, 32, 8, 128, ctypes.byref(size)) == 1
+    assert query(4, 32, 8, 128, ctypes.byref(size)) == 0
+    rows = [(1024, 128, 1)] * 4
+
+    def back(workspace=256, bytes_=size.value, grad=16, weight=16, tokens=4, d=128):
+        return lib.fn["qk_norm_rope_backward"](BF16, 16, 16, 16, 16, 16, 16, 16, grad, 16, 16, 16, weight, 16, tokens, 8, 2, d,
+                                               100, 32, strides(*good[:4], *rows), 1e-6, 1, workspace, bytes_, None)
+
+    assert back(workspace=None) == 5 and b"workspace" in err()
+    assert back(bytes_=16) == 5 and back(workspace=264) == 5
+    assert back(grad=None) == 1 and back(weight=None) == 1 and back(d=2000) == 2
