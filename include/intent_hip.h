@@ -67,7 +67,9 @@ enum IntentHipOperator {
   INTENT_HIP_OP_DECODE_MERGE = 21,        /* cols = head dimension */
   INTENT_HIP_OP_MLA_PREFILL = 22,         /* cols = D | P << 16 */
   INTENT_HIP_OP_QK_NORM_ROPE = 23,        /* dtype F16 or BF16; rows = tokens, cols = head width */
-  INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD = 24
+  INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD = 24,
+  INTENT_HIP_OP_PAGED_CACHE_APPEND = 25,  /* dtype F16 or BF16, for both */
+  INTENT_HIP_OP_PAGED_CACHE_READ = 26
 };
 
 /* Epilogue activations of intent_hip_gemm (the Activation enum of contraction/gemm.py:10-12). */
@@ -494,6 +496,28 @@ int intent_hip_qk_norm_rope_backward(int dtype, const void *q, const void *k, co
                                      float *grad_k_weight, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t d,
                                      int64_t table, int64_t pairs, const int64_t strides[22], float eps, int interleaved,
                                      void *workspace, size_t workspace_bytes, void *stream);
+
+/* Rows written into, and read back from, a paged cache of e4m3 elements with a shared power of two per 32; no reference
+ * counterpart. Elements [pages, ps, kv_heads, d] (keys) and [.., dv] (values), one byte each; exponents u8 [pages, ps,
+ * kv_heads, d / 32]: value = element * 2^(exponent - 127), 255 = NaN. Sequence s holds the logical pages page_offsets[s] ..
+ * page_offsets[s + 1] of page_indices [positions]; tables i32. k [rows, kv_heads, d], v [rows, kv_heads, dv] in f16 or bf16.
+ *   append: rows cu_seqlens[s] .. cu_seqlens[s + 1] become the last positions of sequence s, lengths[s] tokens long with them.
+ *           A block's exponent is the smallest e >= -127 with max |x| <= 448 * 2^e over its finite values; elements are
+ *           rounded to nearest even, NaN and infinities held as NaN. A page that is appended to belongs to one sequence.
+ *   read:   row cu_seqlens[s] + i is position i of sequence s in the rows' type, 0 where the tables have no page.
+ * Rows outside every sequence, positions outside the tables and pages outside the cache are left alone. d and dv are
+ * multiples of 32; rows 16-byte aligned with strides in multiples of 8, elements with strides in multiples of 16.
+ * strides[22]: k[3], v[3], key elements[4], key exponents[4], value elements[4], value exponents[4]. */
+int intent_hip_paged_cache_append(int dtype, const void *k, const void *v, void *key_cache, uint8_t *key_exponents,
+                                  void *value_cache, uint8_t *value_exponents, const int32_t *cu_seqlens,
+                                  const int32_t *page_offsets, const int32_t *page_indices, const int32_t *lengths,
+                                  int64_t rows, int64_t sequences, int64_t kv_heads, int64_t d, int64_t dv, int64_t pages,
+                                  int64_t ps, int64_t positions, const int64_t strides[22], void *stream);
+int intent_hip_paged_cache_read(int dtype, const void *key_cache, const uint8_t *key_exponents, const void *value_cache,
+                                const uint8_t *value_exponents, const int32_t *cu_seqlens, const int32_t *page_offsets,
+                                const int32_t *page_indices, void *k, void *v, int64_t rows, int64_t sequences,
+                                int64_t kv_heads, int64_t d, int64_t dv, int64_t pages, int64_t ps, int64_t positions,
+                                const int64_t strides[22], void *stream);
 
 /* Measurement probe (no counterpart in the reference): the box's own MFMA ceiling, reported by the
  * benchmark beside the published peak, as the measurement protocol asks for an MFMA

@@ -38,6 +38,8 @@ Recognised definitions (reference file:line of the semantics each kernel follows
 
   qk_norm_rope_{f16,bf16}           normalization/qk_norm_rope.py  intent_hip_qk_norm_rope
   qk_norm_rope_backward_{f16,bf16}  backward/qk_norm_rope.py       intent_hip_qk_norm_rope_backward
+  paged_cache_append_{f16,bf16}     streaming/mx_cache.py          intent_hip_paged_cache_append
+  paged_cache_read_{f16,bf16}       streaming/mx_cache.py          intent_hip_paged_cache_read
 
 Layout handling: kernels read rows with unit inner stride. An input whose inner
 stride is not 1 is copied into a contiguous device buffer at every launch (on
@@ -49,6 +51,7 @@ from __future__ import annotations
 
 import contextlib
 import contextvars
+import functools
 from dataclasses import dataclass, field
 from typing import Callable
 
@@ -56,7 +59,7 @@ from ...diagnostics import CompilationStageError
 from ..torch_views import raw_stream_getter
 from .library import (BF16, F16, F32, STATIC_SCRATCH_BYTES, OP_ATTENTION_BWD_DELTA, OP_ATTENTION_BWD_DKDV, OP_ATTENTION_BWD_DQ,
                       OP_ATTENTION_FWD, OP_ATTENTION_FWD_F16, OP_ATTENTION_BIAS, OP_ATTENTION_VARLEN, OP_MLA_PREFILL, OP_CSR_SPMV_F32, OP_GEMM, OP_GEMM_F32, OP_GEMM_I8, OP_QUANTIZED_GEMM,
-                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
+                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
 
 
 @dataclass
@@ -88,7 +91,7 @@ class OperatorSpec:
         return ENTRY_POINTS[self.name]
 
 
-IN, OUT = 0, 1
+IN, OUT, INOUT = 0, 1, 2
 
 
 def _view(access, dtype, rank):
@@ -1020,6 +1023,83 @@ def _norm_rope_signature(element, backward):
     return (*inputs, out, out, ("scalar", "f32"))
 
 
+# ------------------------------------------------------------------------------ paged cache of 8 bits
+_MX_BLOCK = 32
+
+
+def _cache_strides(name, elements, exponents) -> tuple:
+    """The strides of a cache's elements and exponents as the kernels take them (0 along an axis of one). A cache is never
+    staged: its pages are read, and written, in place."""
+    width = elements.shape[3]
+    if width % _MX_BLOCK or exponents.shape[3] * _MX_BLOCK != width:
+        raise ValueError(f"{name} rows are blocks of {_MX_BLOCK} elements with one exponent each; got widths {width} and "
+                         f"{exponents.shape[3]}")
+    if elements.numel() and not _aligned(elements, 16):
+        raise ValueError(f"{name} elements need unit inner stride, other strides in multiples of 16 and a 16-byte aligned "
+                         f"start, got strides {tuple(elements.stride())}")
+    if not _aligned(exponents, 1):
+        raise ValueError(f"{name} exponents need unit inner stride, got strides {tuple(exponents.stride())}")
+    return (*_outer_strides(elements), 1, *_outer_strides(exponents), 1)
+
+
+def _outer_strides(tensor) -> tuple:
+    return tuple(st if n > 1 else 0 for st, n in zip(tensor.stride()[:-1], tensor.shape[:-1]))
+
+
+def _paged_cache(dtype_code, reading: bool):
+    """paged_cache_append / paged_cache_read: the same tables and strides, the rows read or written."""
+    def plan(lib, bound, constexprs, device):
+        import ctypes
+
+        if reading:
+            *cache, cu, page_offsets, page_indices, k, v = bound.arguments
+            lengths = None
+        else:
+            k, v, *cache, cu, page_offsets, page_indices, lengths = bound.arguments
+            if lengths.shape[0] + 1 != cu.shape[0]:
+                raise ValueError(f"cu_seqlens and page_offsets need sequence_lengths.shape[0] + 1 = {lengths.shape[0] + 1} "
+                                 f"entries, got {cu.shape[0]}")
+        if cu.shape[0] < 1:
+            raise ValueError("cu_seqlens needs an entry per sequence and one more")
+        keep, before, after = list(bound.arguments), [], []
+        held = (*_cache_strides("key", *cache[:2]), *_cache_strides("value", *cache[2:]))
+        rows = [_writable(t, keep, after, 8) if reading else _readable(t, keep, before, 8) for t in (k, v)]
+        if reading and after:      # a staged output starts as the caller's, whose rows behind the last sequence stay
+            before += [functools.partial(staged.copy_, out) for staged, out in zip(rows, (k, v)) if staged is not out]
+        strides = (ctypes.c_int64 * 22)(*(x for t in rows for x in (*_outer_strides(t), 1)), *held)
+        tables = [_readable(t, keep, before) for t in (cu, page_offsets, page_indices)]
+        keep += rows + [strides]
+        pages, ps, kv_heads, d = cache[0].shape
+        extents = (k.shape[0], cu.shape[0] - 1, kv_heads, d, cache[2].shape[3], pages, ps, page_indices.shape[0])
+        pointers = tuple(t.data_ptr() for t in cache)
+        if reading:
+            fn, entry, op = lib.fn["paged_cache_read"], "intent_hip_paged_cache_read", OP_PAGED_CACHE_READ
+            args = (dtype_code, *pointers, *(t.data_ptr() for t in (*tables, *rows)), *extents, strides)
+        else:
+            fn, entry, op = lib.fn["paged_cache_append"], "intent_hip_paged_cache_append", OP_PAGED_CACHE_APPEND
+            tables.append(_readable(lengths, keep, before))
+            args = (dtype_code, *(t.data_ptr() for t in rows), *pointers, *(t.data_ptr() for t in tables), *extents, strides)
+        return Launch(entry, lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
+                      tuple(zip(("rows", "sequences", "kv_heads", "d", "dv", "pages", "ps", "positions"), extents)),
+                      lambda: lib.kernel_resources(op, dtype_code, extents[0], d))
+    return plan
+
+
+def _cache_signature(access):
+    elements, exponents = _view(access, "f8e4m3fn", 4), _view(access, "u8", 4)
+    return (elements, exponents, elements, exponents)
+
+
+def _append_signature(element):
+    rows, table = _view(IN, element, 3), _view(IN, "i32", 1)
+    return (rows, rows, *_cache_signature(INOUT), table, table, table, table)
+
+
+def _read_signature(element):
+    rows, table = _view(OUT, element, 3), _view(IN, "i32", 1)
+    return (*_cache_signature(IN), table, table, table, rows, rows)
+
+
 _SPECS = (
     OperatorSpec("stable_softmax", (_view(IN, "f32", 2), _view(OUT, "f32", 2)), (), _softmax_fwd(F32), True),
     OperatorSpec("stable_softmax_f16", (_view(IN, "f16", 2), _view(OUT, "f16", 2)), (), _softmax_fwd(F16), True),
@@ -1100,6 +1180,10 @@ _SPECS = (
     OperatorSpec("qk_norm_rope_backward_f16", _norm_rope_signature("f16", True), ("INTERLEAVED",), _norm_rope_backward(F16)),
     OperatorSpec("qk_norm_rope_backward_bf16", _norm_rope_signature("bf16", True), ("INTERLEAVED",),
                  _norm_rope_backward(BF16)),
+    OperatorSpec("paged_cache_append_f16", _append_signature("f16"), (), _paged_cache(F16, False)),
+    OperatorSpec("paged_cache_append_bf16", _append_signature("bf16"), (), _paged_cache(BF16, False)),
+    OperatorSpec("paged_cache_read_f16", _read_signature("f16"), (), _paged_cache(F16, True)),
+    OperatorSpec("paged_cache_read_bf16", _read_signature("bf16"), (), _paged_cache(BF16, True)),
 )
 
 SPECS = {spec.name: spec for spec in _SPECS}
@@ -1126,6 +1210,8 @@ ENTRY_POINTS = {
     "qk_norm_rope_f16": "intent_hip_qk_norm_rope", "qk_norm_rope_bf16": "intent_hip_qk_norm_rope",
     "qk_norm_rope_backward_f16": "intent_hip_qk_norm_rope_backward",
     "qk_norm_rope_backward_bf16": "intent_hip_qk_norm_rope_backward",
+    "paged_cache_append_f16": "intent_hip_paged_cache_append", "paged_cache_append_bf16": "intent_hip_paged_cache_append",
+    "paged_cache_read_f16": "intent_hip_paged_cache_read", "paged_cache_read_bf16": "intent_hip_paged_cache_read",
 }
 assert set(ENTRY_POINTS) == set(SPECS)
 

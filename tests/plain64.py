@@ -37,3 +37,24 @@ def norm_rope_backward(x, weight, grad, positions, cos, sin, eps, interleaved):
     grad_x = r * (inner - u * (inner * u).mean(-1, keepdim=True))
     grad_size = r * (inner_size + u.abs() * (inner_size * u.abs()).mean(-1, keepdim=True))
     return grad_x, grad_size, (g * u).sum((0, 1)), (size * u.abs()).sum((0, 1))
+
+
+def quantise(x):
+    """Elements and exponent bytes of rows [..., D] in blocks of 32: the smallest e >= -127 with max |x| <= 448 * 2^e over
+    the finite values, x * 2^-e rounded to e4m3 (four significant bits, multiples of 2^-9 below 2^-6, halves to even)."""
+    blocks = x.double().unflatten(-1, (-1, 32))
+    size = torch.where(blocks.isfinite(), blocks.abs(), 0.0).amax(-1)
+    mantissa, exponent = torch.frexp(size)                       # size = mantissa * 2^exponent, mantissa in [0.5, 1)
+    power = torch.where(size > 0, exponent - 9 + (mantissa > 0.875).int(), -127).clamp_min(-127)
+    scaled = torch.ldexp(blocks, -power[..., None])
+    _, at = torch.frexp(scaled)
+    step = torch.ldexp(torch.ones_like(scaled), (at - 1).clamp_min(-6) - 3)
+    elements = torch.where(blocks.isfinite(), torch.round(scaled / step) * step, float("nan"))
+    return elements.flatten(-2), power + 127
+
+
+def dequantise(elements, exponents):
+    """What e4m3 elements (any float type) and exponent bytes stand for."""
+    power = exponents.int() - 127
+    scale = torch.where(exponents == 255, float("nan"), torch.ldexp(torch.ones(power.shape, dtype=torch.float64), power))
+    return elements.double() * scale.repeat_interleave(32, -1)

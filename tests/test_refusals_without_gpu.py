@@ -49,3 +49,33 @@ def test_norm_rope():
     assert back(workspace=None) == 5 and b"workspace" in err()
     assert back(bytes_=16) == 5 and back(workspace=264) == 5
     assert back(grad=None) == 1 and back(weight=None) == 1 and back(d=2000) == 2
+
+
+def test_paged_cache():
+    lib = hiplib.library()
+    err = lambda: lib.fn["last_error"]()  # noqa: E731
+    rows, held, powers = (1024, 128, 1), (65536, 1024, 128, 1), (2048, 32, 4, 1)
+
+    def call(reading=False, dtype=F16, k=16, keys=16, cu=16, n=4, b=2, heads=8, d=128, dv=128, pages=9, ps=64, positions=4,
+             groups=(rows, rows, held, powers, held, powers), lengths=16):
+        tail = (n, b, heads, d, dv, pages, ps, positions, strides(*groups), None)
+        if reading:
+            return lib.fn["paged_cache_read"](dtype, keys, 16, 16, 16, cu, 16, 16, k, 16, *tail)
+        return lib.fn["paged_cache_append"](dtype, k, 16, keys, 16, 16, 16, cu, 16, 16, lengths, *tail)
+
+    for reading in (False, True):
+        assert call(reading, dtype=hiplib.F32) == 1 and b"F16 or BF16" in err()
+        assert call(reading, n=-1) == 1 and b"negative" in err()
+        assert call(reading, d=48) == 2 and b"blocks of 32" in err()
+        assert call(reading, k=None) == 1 and call(reading, keys=None) == 1 and call(reading, cu=None) == 1
+        assert call(reading, k=18) == 2 and b"aligned" in err()
+        assert call(reading, keys=24) == 2 and b"aligned" in err()
+        assert call(reading, ps=0) == 1 and b"no token" in err()
+        assert call(reading, groups=((1028, 128, 1), rows, held, powers, held, powers)) == 2
+        assert call(reading, groups=(rows, rows, (65536, 1024, 136, 1), powers, held, powers)) == 2
+        assert call(reading, groups=(rows, rows, held, (2048, 32, 4, 2), held, powers)) == 1 and b"unit inner" in err()
+        assert call(reading, groups=(rows, (-1024, 128, 1), held, powers, held, powers)) == 1
+        assert call(reading, heads=2 ** 28) == 2 and call(reading, n=2 ** 40) == 2
+        assert call(reading, n=0) == 0 and call(reading, b=0) == 0 and call(reading, heads=0) == 0
+    assert call(lengths=None) == 1
+    assert call(pages=0) == 0 and call(positions=0) == 0            # nowhere to write
