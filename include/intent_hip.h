@@ -69,7 +69,8 @@ enum IntentHipOperator {
   INTENT_HIP_OP_QK_NORM_ROPE = 23,        /* dtype F16 or BF16; rows = tokens, cols = head width */
   INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD = 24,
   INTENT_HIP_OP_PAGED_CACHE_APPEND = 25,  /* dtype F16 or BF16, for both */
-  INTENT_HIP_OP_PAGED_CACHE_READ = 26
+  INTENT_HIP_OP_PAGED_CACHE_READ = 26,
+  INTENT_HIP_OP_PAGED_GQA_DECODE_MX = 27  /* dtype F16 or BF16; rows = HEAD_GROUP, cols = head width */
 };
 
 /* Epilogue activations of intent_hip_gemm (the Activation enum of contraction/gemm.py:10-12). */
@@ -518,6 +519,23 @@ int intent_hip_paged_cache_read(int dtype, const void *key_cache, const uint8_t 
                                 const int32_t *page_indices, void *k, void *v, int64_t rows, int64_t sequences,
                                 int64_t kv_heads, int64_t d, int64_t dv, int64_t pages, int64_t ps, int64_t positions,
                                 const int64_t strides[22], void *stream);
+
+/* Attention of one new token per sequence over that cache (keys and values of one width d: 64, 96, 128, 192 or 256), no
+ * reference counterpart. q and output [batch, q_heads, d] in f16 or bf16, q_heads = kv_heads * head_group; query head h uses
+ * key head h / head_group over the positions below lengths[s] that the tables have a page for; 0 where there is none. Keys
+ * and values are taken in the query's type, sums are f32, one rounding at the end. page_offsets [batch + 1] do not decrease;
+ * pages outside the cache have no token. The pages of a sequence are cut into jobs whose states a second kernel joins through
+ * the workspace (intent_hip_paged_gqa_decode_mx_workspace_bytes bytes, 16-byte aligned; 0 where one job holds every page).
+ * Nothing depends on the host's knowledge of offsets and lengths, so they may change under a captured graph.
+ * strides[22]: q[3], key elements[4], key exponents[4], value elements[4], value exponents[4], output[3]. */
+int intent_hip_paged_gqa_decode_mx_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_group,
+                                                   int64_t d, int64_t ps, int64_t positions, size_t *bytes);
+int intent_hip_paged_gqa_decode_mx(int dtype, const void *q, const void *key_cache, const uint8_t *key_exponents,
+                                   const void *value_cache, const uint8_t *value_exponents, const int32_t *page_offsets,
+                                   const int32_t *page_indices, const int32_t *lengths, void *output, int64_t batch,
+                                   int64_t q_heads, int64_t kv_heads, int64_t head_group, int64_t d, int64_t pages, int64_t ps,
+                                   int64_t positions, const int64_t strides[22], float scale, void *workspace,
+                                   size_t workspace_bytes, void *stream);
 
 /* Measurement probe (no counterpart in the reference): the box's own MFMA ceiling, reported by the
  * benchmark beside the published peak, as the measurement protocol asks for an MFMA

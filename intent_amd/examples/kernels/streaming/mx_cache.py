@@ -19,6 +19,8 @@ signature.
 import intent_amd as intent
 import intent_amd.language as I
 
+from intent_amd.examples.kernels.streaming.attention import causal_pairs
+
 BLOCK = 32
 LARGEST = 448.0
 
@@ -149,3 +151,71 @@ def paged_cache_read_bf16(
 ):
     read_rows(key_cache, key_exponents, cu_seqlens, page_offsets, page_indices, k, I.bf16)
     read_rows(value_cache, value_exponents, cu_seqlens, page_offsets, page_indices, v, I.bf16)
+
+
+@intent.fn
+def decode_head(query, k_rows, v_rows, scale, element):
+    """One query head over its sequence's rows: f32 throughout, rounded at the end; 0 where there is no row."""
+    logits = I.matmul(query, k_rows, transpose_rhs=True, acc_dtype=I.f32) * (scale * I.LOG2E)
+    live = I.reduce.any(causal_pairs(I.indices(I.domain(0, 1)), I.indices(I.domain(0, k_rows.shape[0])), False), axis=1)
+    peak = I.reduce(logits, axis=1, identity=-I.inf, combine=I.maximum_num)
+    weights = I.exp2(logits - peak[:, None], approximate=True, flush_to_zero=True)
+    mixed = I.matmul(weights, I.cast(v_rows, I.f32), acc_dtype=I.f32)
+    return I.cast(I.select(live[:, None], mixed / I.reduce.sum(weights, axis=1)[:, None], 0.0), element)
+
+
+@intent.fn
+def decode_rows(q, key_cache, key_exponents, value_cache, value_exponents, page_offsets, page_indices, sequence_lengths, output,
+                scale, group, element):
+    P, PS = key_cache.shape[0], key_cache.shape[1]
+    for s in I.parallel(I.domain(0, q.shape[0])):
+        held = (I.cast(page_offsets[s + 1], I.index) - I.cast(page_offsets[s], I.index)) * PS
+        position = I.indices(I.domain(0, I.minimum(I.cast(sequence_lengths[s], I.index), held)))
+        slot = slot_of(page_offsets, page_indices, s, position, PS)
+        place = I.members(slot, (slot.page >= 0) & (slot.page < P))
+        for h in I.parallel(I.domain(0, q.shape[1])):
+            shared = h // group
+            keys = dequantise(key_cache[place.page, place.place, shared, :], key_exponents[place.page, place.place, shared, :], element)
+            values = dequantise(value_cache[place.page, place.place, shared, :], value_exponents[place.page, place.place, shared, :],
+                                element)
+            output[s, h, :] = decode_head(I.reshape(q[s, h, :], (1, q.shape[2])), keys, values, scale, element)[0]
+
+
+@intent.kernel
+def paged_gqa_decode_mx_f16(
+    q: I.In[I.f16, ("B", "HQ", "D")],
+    key_cache: I.In[I.f8e4m3fn, ("P", "PS", "HK", "D")],
+    key_exponents: I.In[I.u8, ("P", "PS", "HK", "DB")],
+    value_cache: I.In[I.f8e4m3fn, ("P", "PS", "HK", "D")],
+    value_exponents: I.In[I.u8, ("P", "PS", "HK", "DB")],
+    page_offsets: I.In[I.i32, ("B_PLUS_1",)],
+    page_indices: I.In[I.i32, ("S",)],
+    sequence_lengths: I.In[I.i32, ("B",)],
+    output: I.Out[I.f16, ("B", "HQ", "D")],
+    scale: I.f32,
+    HEAD_GROUP: I.Constexpr[int],
+):
+    """Query head h of sequence s over the positions below sequence_lengths[s] that the tables have a page for, with the keys
+    and values of head h // HEAD_GROUP; 0 where there is none. page_offsets do not decrease; pages reserved beyond a
+    sequence's length are not read. D is 64, 96, 128, 192 or 256. Any head group; the work is cut over each sequence's
+    pages and joined within the call."""
+    decode_rows(q, key_cache, key_exponents, value_cache, value_exponents, page_offsets, page_indices, sequence_lengths, output,
+                scale, HEAD_GROUP, I.f16)
+
+
+@intent.kernel
+def paged_gqa_decode_mx_bf16(
+    q: I.In[I.bf16, ("B", "HQ", "D")],
+    key_cache: I.In[I.f8e4m3fn, ("P", "PS", "HK", "D")],
+    key_exponents: I.In[I.u8, ("P", "PS", "HK", "DB")],
+    value_cache: I.In[I.f8e4m3fn, ("P", "PS", "HK", "D")],
+    value_exponents: I.In[I.u8, ("P", "PS", "HK", "DB")],
+    page_offsets: I.In[I.i32, ("B_PLUS_1",)],
+    page_indices: I.In[I.i32, ("S",)],
+    sequence_lengths: I.In[I.i32, ("B",)],
+    output: I.Out[I.bf16, ("B", "HQ", "D")],
+    scale: I.f32,
+    HEAD_GROUP: I.Constexpr[int],
+):
+    decode_rows(q, key_cache, key_exponents, value_cache, value_exponents, page_offsets, page_indices, sequence_lengths, output,
+                scale, HEAD_GROUP, I.bf16)

@@ -40,6 +40,7 @@ Recognised definitions (reference file:line of the semantics each kernel follows
   qk_norm_rope_backward_{f16,bf16}  backward/qk_norm_rope.py       intent_hip_qk_norm_rope_backward
   paged_cache_append_{f16,bf16}     streaming/mx_cache.py          intent_hip_paged_cache_append
   paged_cache_read_{f16,bf16}       streaming/mx_cache.py          intent_hip_paged_cache_read
+  paged_gqa_decode_mx_{f16,bf16}    streaming/mx_cache.py          intent_hip_paged_gqa_decode_mx
 
 Layout handling: kernels read rows with unit inner stride. An input whose inner
 stride is not 1 is copied into a contiguous device buffer at every launch (on
@@ -59,7 +60,7 @@ from ...diagnostics import CompilationStageError
 from ..torch_views import raw_stream_getter
 from .library import (BF16, F16, F32, STATIC_SCRATCH_BYTES, OP_ATTENTION_BWD_DELTA, OP_ATTENTION_BWD_DKDV, OP_ATTENTION_BWD_DQ,
                       OP_ATTENTION_FWD, OP_ATTENTION_FWD_F16, OP_ATTENTION_BIAS, OP_ATTENTION_VARLEN, OP_MLA_PREFILL, OP_CSR_SPMV_F32, OP_GEMM, OP_GEMM_F32, OP_GEMM_I8, OP_QUANTIZED_GEMM,
-                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
+                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ, OP_PAGED_GQA_DECODE_MX, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
 
 
 @dataclass
@@ -1085,6 +1086,44 @@ def _paged_cache(dtype_code, reading: bool):
     return plan
 
 
+def _paged_decode_mx(dtype_code):
+    """paged_gqa_decode_mx: jobs of a sequence's pages, whose states a second kernel joins through a workspace; none where
+    one job holds every page."""
+    def plan(lib, bound, constexprs, device):
+        import ctypes
+
+        q, *cache, page_offsets, page_indices, lengths, output, scale = bound.arguments
+        group = _positive_constexpr(constexprs, "HEAD_GROUP")
+        batch, q_heads, d = q.shape
+        pages, ps, kv_heads, _ = cache[0].shape
+        if kv_heads * group != q_heads:
+            raise ValueError(f"query heads ({q_heads}) must equal key/value heads ({kv_heads}) * HEAD_GROUP ({group})")
+        if page_offsets.shape[0] != batch + 1:
+            raise ValueError(f"page_offsets must hold batch + 1 = {batch + 1} entries, got {page_offsets.shape[0]}")
+        keep, before, after = list(bound.arguments[:9]), [], []
+        held = (*_cache_strides("key", *cache[:2]), *_cache_strides("value", *cache[2:]))
+        qk, outk = _readable(q, keep, before, 8), _writable(output, keep, after)
+        tables = [_readable(t, keep, before) for t in (page_offsets, page_indices, lengths)]
+        strides = (ctypes.c_int64 * 22)(*_outer_strides(qk), 1, *held, *_outer_strides(outk), 1)
+        keep += [qk, outk, strides]
+        size = ctypes.c_size_t(0)
+        lib.check(lib.fn["paged_gqa_decode_mx_workspace_bytes"](batch, q_heads, kv_heads, group, d, ps, page_indices.shape[0],
+                                                                ctypes.byref(size)), "provider_preparation")
+        fn = lib.fn["paged_gqa_decode_mx"]
+        args = (dtype_code, *(t.data_ptr() for t in (qk, *cache, *tables, outk)), batch, q_heads, kv_heads, group, d, pages, ps,
+                page_indices.shape[0], strides, float(scale))
+        if size.value:
+            _decode_workspace("paged_gqa_decode_mx")
+            run = _workspace_run(fn, args, size.value, device, keep)
+        else:
+            run = lambda stream: fn(*args, None, 0, stream)  # noqa: E731
+        return Launch("intent_hip_paged_gqa_decode_mx", run, tuple(keep), tuple(before), tuple(after),
+                      (("batch", batch), ("q_heads", q_heads), ("kv_heads", kv_heads), ("d", d), ("pages", pages), ("ps", ps),
+                       ("positions", page_indices.shape[0]), ("workspace_bytes", size.value)),
+                      lambda: lib.kernel_resources(OP_PAGED_GQA_DECODE_MX, dtype_code, group, d))
+    return plan
+
+
 def _cache_signature(access):
     elements, exponents = _view(access, "f8e4m3fn", 4), _view(access, "u8", 4)
     return (elements, exponents, elements, exponents)
@@ -1098,6 +1137,11 @@ def _append_signature(element):
 def _read_signature(element):
     rows, table = _view(OUT, element, 3), _view(IN, "i32", 1)
     return (*_cache_signature(IN), table, table, table, rows, rows)
+
+
+def _decode_mx_signature(element):
+    rows, table = _view(IN, element, 3), _view(IN, "i32", 1)
+    return (rows, *_cache_signature(IN), table, table, table, _view(OUT, element, 3), ("scalar", "f32"))
 
 
 _SPECS = (
@@ -1184,6 +1228,8 @@ _SPECS = (
     OperatorSpec("paged_cache_append_bf16", _append_signature("bf16"), (), _paged_cache(BF16, False)),
     OperatorSpec("paged_cache_read_f16", _read_signature("f16"), (), _paged_cache(F16, True)),
     OperatorSpec("paged_cache_read_bf16", _read_signature("bf16"), (), _paged_cache(BF16, True)),
+    OperatorSpec("paged_gqa_decode_mx_f16", _decode_mx_signature("f16"), ("HEAD_GROUP",), _paged_decode_mx(F16)),
+    OperatorSpec("paged_gqa_decode_mx_bf16", _decode_mx_signature("bf16"), ("HEAD_GROUP",), _paged_decode_mx(BF16)),
 )
 
 SPECS = {spec.name: spec for spec in _SPECS}
@@ -1212,6 +1258,7 @@ ENTRY_POINTS = {
     "qk_norm_rope_backward_bf16": "intent_hip_qk_norm_rope_backward",
     "paged_cache_append_f16": "intent_hip_paged_cache_append", "paged_cache_append_bf16": "intent_hip_paged_cache_append",
     "paged_cache_read_f16": "intent_hip_paged_cache_read", "paged_cache_read_bf16": "intent_hip_paged_cache_read",
+    "paged_gqa_decode_mx_f16": "intent_hip_paged_gqa_decode_mx", "paged_gqa_decode_mx_bf16": "intent_hip_paged_gqa_decode_mx",
 }
 assert set(ENTRY_POINTS) == set(SPECS)
 

@@ -58,3 +58,22 @@ def dequantise(elements, exponents):
     power = exponents.int() - 127
     scale = torch.where(exponents == 255, float("nan"), torch.ldexp(torch.ones(power.shape, dtype=torch.float64), power))
     return elements.double() * scale.repeat_interleave(32, -1)
+
+
+def decode(q, keys, values, page_offsets, page_indices, lengths, scale):
+    """q [B, HQ, D] over caches [P, PS, HK, D] of values (float64): (output, sum of weight * |value| over weights)."""
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    size = torch.zeros(q.shape, dtype=torch.float64)
+    pages, ps, heads = keys.shape[:3]
+    group = q.shape[1] // heads
+    for b in range(q.shape[0]):
+        slots = [(int(page_indices[i]), p) for i in range(int(page_offsets[b]), int(page_offsets[b + 1])) for p in range(ps)]
+        slots = [(page, p) for page, p in slots[:max(0, int(lengths[b]))] if 0 <= page < pages]
+        if not slots:
+            continue
+        at = torch.tensor(slots).unbind(1)
+        for h in range(q.shape[1]):
+            k, v = keys[at][:, h // group], values[at][:, h // group]
+            weights = torch.softmax(k @ q[b, h].double() * scale, 0)
+            out[b, h], size[b, h] = weights @ v, weights @ v.abs()
+    return out, size

@@ -79,3 +79,32 @@ def test_paged_cache():
         assert call(reading, n=0) == 0 and call(reading, b=0) == 0 and call(reading, heads=0) == 0
     assert call(lengths=None) == 1
     assert call(pages=0) == 0 and call(positions=0) == 0            # nowhere to write
+
+
+def test_decode_mx():
+    lib = hiplib.library()
+    err = lambda: lib.fn["last_error"]()  # noqa: E731
+    rows, held, powers = (4096, 128, 1), (65536, 1024, 128, 1), (2048, 32, 4, 1)
+
+    def call(dtype=F16, q=16, keys=16, out=16, b=2, heads=32, kv=8, group=4, d=128, pages=9, ps=64, positions=4,
+             groups=(rows, held, powers, held, powers, rows), workspace=None, size=0):
+        return lib.fn["paged_gqa_decode_mx"](dtype, q, keys, 16, 16, 16, 16, 16, 16, out, b, heads, kv, group, d, pages, ps,
+                                             positions, strides(*groups), 0.1, workspace, size, None)
+
+    assert call(dtype=hiplib.F32) == 1 and b"F16 or BF16" in err()
+    assert call(b=-1) == 1 and call(group=3) == 1 and b"HEAD_GROUP" in err()
+    assert call(d=80) == 2 and b"head widths" in err()
+    assert call(q=None) == 1 and call(keys=None) == 1 and call(out=None) == 1
+    assert call(q=18) == 2 and call(keys=24) == 2
+    assert call(groups=(rows, (65536, 1024, 136, 1), powers, held, powers, rows)) == 2
+    assert call(groups=(rows, held, powers, held, powers, (4096, 128, 2))) == 1
+    assert call(groups=((-4096, 128, 1), held, powers, held, powers, rows)) == 1
+    assert call(b=2 ** 30) == 2 and call(positions=2 ** 30) == 2
+    assert call(b=0) == 0 and call(heads=0, kv=0) == 0
+    size = ctypes.c_size_t(0)
+    query = lib.fn["paged_gqa_decode_mx_workspace_bytes"]
+    assert query(2, 32, 8, 4, 128, 64, 4, ctypes.byref(size)) == 0 and size.value == 0       # one job of 256 tokens
+    assert query(8, 32, 8, 4, 128, 64, 1000, ctypes.byref(size)) == 0 and size.value > 0
+    assert call(b=8, positions=1000, size=size.value) == 5 and b"workspace" in err()
+    assert call(b=8, positions=1000, workspace=256, size=size.value - 1) == 5
+    assert query(8, 32, 8, 4, 128, 64, 1000, None) == 1 and query(8, 32, 8, 3, 128, 64, 1000, ctypes.byref(size)) == 1
