@@ -70,7 +70,8 @@ enum IntentHipOperator {
   INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD = 24,
   INTENT_HIP_OP_PAGED_CACHE_APPEND = 25,  /* dtype F16 or BF16, for both */
   INTENT_HIP_OP_PAGED_CACHE_READ = 26,
-  INTENT_HIP_OP_PAGED_GQA_DECODE_MX = 27  /* dtype F16 or BF16; rows = HEAD_GROUP, cols = head width */
+  INTENT_HIP_OP_PAGED_GQA_DECODE_MX = 27, /* dtype F16 or BF16; rows = HEAD_GROUP, cols = head width */
+  INTENT_HIP_OP_LINEAR_MXFP4 = 28         /* dtype F16 or BF16; rows = m, cols = n */
 };
 
 /* Epilogue activations of intent_hip_gemm (the Activation enum of contraction/gemm.py:10-12). */
@@ -536,6 +537,13 @@ int intent_hip_paged_gqa_decode_mx(int dtype, const void *q, const void *key_cac
                                    int64_t q_heads, int64_t kv_heads, int64_t head_group, int64_t d, int64_t pages, int64_t ps,
                                    int64_t positions, const int64_t strides[22], float scale, void *workspace,
                                    size_t workspace_bytes, void *stream);
+
+/* y = x W^T with 4-bit weights, no reference counterpart. x [m, k] and y [m, n] in f16 or bf16; weight [n, k / 2] bytes of
+ * two e2m1 elements, the even column in the low four bits; exponents u8 [n, k / 32]: W[n, k] = element * 2^(exponent - 127) in
+ * the type of x, 255 = NaN. f32 sums, one rounding at the end. k a multiple of 32; rows of x and of the weight 16-byte
+ * aligned. ldw and lde are in bytes. */
+int intent_hip_linear_mxfp4(int dtype, const void *x, const uint8_t *weight, const uint8_t *exponents, void *y, int64_t m,
+                            int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t lde, int64_t ldy, void *stream);
 
 /* Measurement probe (no counterpart in the reference): the box's own MFMA ceiling, reported by the
  * benchmark beside the published peak, as the measurement protocol asks for an MFMA

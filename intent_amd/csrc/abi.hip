@@ -160,6 +160,7 @@ extern "C" int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int6
     case INTENT_HIP_OP_PAGED_CACHE_APPEND: return paged_cache_resources(dtype, 0, out);
     case INTENT_HIP_OP_PAGED_CACHE_READ: return paged_cache_resources(dtype, 1, out);
     case INTENT_HIP_OP_PAGED_GQA_DECODE_MX: return mx_decode_resources(dtype, rows, cols, out);
+    case INTENT_HIP_OP_LINEAR_MXFP4: return linear_mxfp4_resources(dtype, rows, out);
     case INTENT_HIP_OP_GEMM_I8: return gemm_i8_resources(rows, cols, out);
     case INTENT_HIP_OP_QUANTIZED_GEMM:
       return quantized_gemm_resources(nullptr, nullptr, nullptr, nullptr, rows, (cols + 7) / 8 * 8, 64, 64, 64, 64, 64, out);

@@ -55,6 +55,7 @@ int paged_decode_resources(int64_t batch, int64_t kv_heads, int64_t group, int64
 int spmm_resources(int64_t features, IntentHipKernelResources *out);
 int norm_rope_resources(int dtype, int backward, IntentHipKernelResources *out);
 int paged_cache_resources(int dtype, int reading, IntentHipKernelResources *out);
+int linear_mxfp4_resources(int dtype, int64_t m, IntentHipKernelResources *out);
 int mx_decode_resources(int dtype, int64_t group, int64_t d, IntentHipKernelResources *out);
 
 // f32 products of few output tiles (gemm_f32_few.hip); `workspace` may be null (one workgroup per tile).

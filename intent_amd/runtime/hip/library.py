@@ -23,7 +23,7 @@ F32, F16, BF16 = 0, 1, 2
  OP_SPLITK_REDUCE, OP_CSR_SPMM_F32, OP_ATTENTION_VARLEN, OP_GEMM_I8, OP_QUANTIZED_GEMM,
  OP_ATTENTION_BIAS, OP_GROUPED_DECODE_PARTIALS, OP_CONTINUOUS_DECODE, OP_VARLEN_DECODE, OP_DECODE_MERGE,
  OP_MLA_PREFILL, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ,
- OP_PAGED_GQA_DECODE_MX) = range(28)
+ OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4) = range(29)
 ACT_NONE, ACT_RELU = 0, 1
 
 _i64, _int, _p, _f32, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_size_t
@@ -118,6 +118,7 @@ SIGNATURES = {
     "intent_hip_paged_cache_read": (_int, (_int, *[_p] * 9, *[_i64] * 8, ctypes.POINTER(_i64), _p)),
     "intent_hip_paged_gqa_decode_mx_workspace_bytes": (_int, (*[_i64] * 7, ctypes.POINTER(_sz))),
     "intent_hip_paged_gqa_decode_mx": (_int, (_int, *[_p] * 9, *[_i64] * 8, ctypes.POINTER(_i64), _f32, _p, _sz, _p)),
+    "intent_hip_linear_mxfp4": (_int, (_int, *[_p] * 4, *[_i64] * 7, _p)),
     "intent_hip_mfma_probe": (_int, (_int, _int, _i64, _i64, _p, _p)),
 }
 

@@ -41,6 +41,7 @@ Recognised definitions (reference file:line of the semantics each kernel follows
   paged_cache_append_{f16,bf16}     streaming/mx_cache.py          intent_hip_paged_cache_append
   paged_cache_read_{f16,bf16}       streaming/mx_cache.py          intent_hip_paged_cache_read
   paged_gqa_decode_mx_{f16,bf16}    streaming/mx_cache.py          intent_hip_paged_gqa_decode_mx
+  linear_mxfp4_{f16,bf16}           contraction/linear_mxfp4.py    intent_hip_linear_mxfp4
 
 Layout handling: kernels read rows with unit inner stride. An input whose inner
 stride is not 1 is copied into a contiguous device buffer at every launch (on
@@ -60,7 +61,7 @@ from ...diagnostics import CompilationStageError
 from ..torch_views import raw_stream_getter
 from .library import (BF16, F16, F32, STATIC_SCRATCH_BYTES, OP_ATTENTION_BWD_DELTA, OP_ATTENTION_BWD_DKDV, OP_ATTENTION_BWD_DQ,
                       OP_ATTENTION_FWD, OP_ATTENTION_FWD_F16, OP_ATTENTION_BIAS, OP_ATTENTION_VARLEN, OP_MLA_PREFILL, OP_CSR_SPMV_F32, OP_GEMM, OP_GEMM_F32, OP_GEMM_I8, OP_QUANTIZED_GEMM,
-                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ, OP_PAGED_GQA_DECODE_MX, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
+                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ, OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
 
 
 @dataclass
@@ -1120,7 +1121,7 @@ def _paged_decode_mx(dtype_code):
         return Launch("intent_hip_paged_gqa_decode_mx", run, tuple(keep), tuple(before), tuple(after),
                       (("batch", batch), ("q_heads", q_heads), ("kv_heads", kv_heads), ("d", d), ("pages", pages), ("ps", ps),
                        ("positions", page_indices.shape[0]), ("workspace_bytes", size.value)),
-                      lambda: lib.kernel_resources(OP_PAGED_GQA_DECODE_MX, dtype_code, group, d))
+                      lambda: lib.kernel_resources(OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4, dtype_code, group, d))
     return plan
 
 
@@ -1142,6 +1143,29 @@ def _read_signature(element):
 def _decode_mx_signature(element):
     rows, table = _view(IN, element, 3), _view(IN, "i32", 1)
     return (rows, *_cache_signature(IN), table, table, table, _view(OUT, element, 3), ("scalar", "f32"))
+
+
+# ------------------------------------------------------------------------------ 4-bit weights
+def _linear_mxfp4(dtype_code):
+    """linear_mxfp4: x is staged where its layout is not the kernel's; a weight never is."""
+    def plan(lib, bound, constexprs, device):
+        x, weight, exponents, out = bound.arguments
+        (m, k), n = x.shape, weight.shape[0]
+        if k % _MX_BLOCK or weight.shape[1] * 2 != k or exponents.shape[1] * _MX_BLOCK != k:
+            raise ValueError(f"weights of K = {k} are blocks of {_MX_BLOCK} elements: [N, K / 2] bytes and [N, K / {_MX_BLOCK}] "
+                             f"exponents, got {tuple(weight.shape)} and {tuple(exponents.shape)}")
+        if not _aligned(weight, 16) or not _aligned(exponents, 1):
+            raise ValueError(f"weights need unit inner stride, rows in multiples of 16 bytes and a 16-byte aligned start, and "
+                             f"their exponents unit inner stride; got strides {tuple(weight.stride())} and "
+                             f"{tuple(exponents.stride())}")
+        keep, before, after = [x, weight, exponents, out], [], []
+        xk, outk = _readable(x, keep, before, 8), _writable(out, keep, after)
+        fn = lib.fn["linear_mxfp4"]
+        args = (dtype_code, xk.data_ptr(), weight.data_ptr(), exponents.data_ptr(), outk.data_ptr(), m, n, k,
+                *(_outer_strides(t)[0] for t in (xk, weight, exponents, outk)))
+        return Launch("intent_hip_linear_mxfp4", lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
+                      (("m", m), ("n", n), ("k", k)), lambda: lib.kernel_resources(OP_LINEAR_MXFP4, dtype_code, m, n))
+    return plan
 
 
 _SPECS = (
@@ -1230,6 +1254,10 @@ _SPECS = (
     OperatorSpec("paged_cache_read_bf16", _read_signature("bf16"), (), _paged_cache(BF16, True)),
     OperatorSpec("paged_gqa_decode_mx_f16", _decode_mx_signature("f16"), ("HEAD_GROUP",), _paged_decode_mx(F16)),
     OperatorSpec("paged_gqa_decode_mx_bf16", _decode_mx_signature("bf16"), ("HEAD_GROUP",), _paged_decode_mx(BF16)),
+    OperatorSpec("linear_mxfp4_f16", (_view(IN, "f16", 2), _view(IN, "u8", 2), _view(IN, "u8", 2), _view(OUT, "f16", 2)), (),
+                 _linear_mxfp4(F16)),
+    OperatorSpec("linear_mxfp4_bf16", (_view(IN, "bf16", 2), _view(IN, "u8", 2), _view(IN, "u8", 2), _view(OUT, "bf16", 2)), (),
+                 _linear_mxfp4(BF16)),
 )
 
 SPECS = {spec.name: spec for spec in _SPECS}
@@ -1259,6 +1287,7 @@ ENTRY_POINTS = {
     "paged_cache_append_f16": "intent_hip_paged_cache_append", "paged_cache_append_bf16": "intent_hip_paged_cache_append",
     "paged_cache_read_f16": "intent_hip_paged_cache_read", "paged_cache_read_bf16": "intent_hip_paged_cache_read",
     "paged_gqa_decode_mx_f16": "intent_hip_paged_gqa_decode_mx", "paged_gqa_decode_mx_bf16": "intent_hip_paged_gqa_decode_mx",
+    "linear_mxfp4_f16": "intent_hip_linear_mxfp4", "linear_mxfp4_bf16": "intent_hip_linear_mxfp4",
 }
 assert set(ENTRY_POINTS) == set(SPECS)
 

@@ -77,3 +77,10 @@ def decode(q, keys, values, page_offsets, page_indices, lengths, scale):
             weights = torch.softmax(k @ q[b, h].double() * scale, 0)
             out[b, h], size[b, h] = weights @ v, weights @ v.abs()
     return out, size
+
+
+def unpack_e2m1(weight, exponents):
+    """[N, K / 2] bytes and [N, K / 32] exponent bytes as float64 [N, K]."""
+    table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+    code = torch.stack((weight & 15, weight >> 4), -1).flatten(-2).long()
+    return dequantise(torch.where(code >= 8, -table[code % 8], table[code % 8]), exponents)

@@ -108,3 +108,20 @@ def test_decode_mx():
     assert call(b=8, positions=1000, size=size.value) == 5 and b"workspace" in err()
     assert call(b=8, positions=1000, workspace=256, size=size.value - 1) == 5
     assert query(8, 32, 8, 4, 128, 64, 1000, None) == 1 and query(8, 32, 8, 3, 128, 64, 1000, ctypes.byref(size)) == 1
+
+
+def test_linear_mxfp4():
+    lib = hiplib.library()
+    err = lambda: lib.fn["last_error"]()  # noqa: E731
+
+    def call(dtype=F16, x=16, w=16, y=16, m=4, n=8, k=64, ldx=64, ldw=32, lde=2, ldy=8):
+        return lib.fn["linear_mxfp4"](dtype, x, w, 16, y, m, n, k, ldx, ldw, lde, ldy, None)
+
+    assert call(dtype=hiplib.F32) == 1 and b"F16 or BF16" in err()
+    assert call(m=-1) == 1 and call(ldw=-32) == 1 and b"negative" in err()
+    assert call(k=48) == 2 and b"blocks of 32" in err()
+    assert call(x=None) == 1 and call(w=None) == 1 and call(y=None) == 1 and b"null" in err()
+    assert call(x=24) == 2 and call(ldx=65) == 2 and b"aligned" in err()
+    assert call(w=24) == 2 and call(ldw=40) == 2 and b"weight rows" in err()
+    assert call(m=2 ** 21) == 2 and call(n=2 ** 30) == 2
+    assert call(m=0, x=None) == 0 and call(n=0) == 0
