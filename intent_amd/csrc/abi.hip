@@ -155,8 +155,8 @@ extern "C" int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int6
     case INTENT_HIP_OP_MLA_PREFILL:
       return attention_resources(INTENT_HIP_F16, rows, cols & 0xFFFF, cols >> 16, 3, out);
     case INTENT_HIP_OP_CSR_SPMM_F32: return spmm_resources(cols, out);
-    case INTENT_HIP_OP_QK_NORM_ROPE: return norm_rope_resources(dtype, 0, out);
-    case INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD: return norm_rope_resources(dtype, 1, out);
+    case INTENT_HIP_OP_QK_NORM_ROPE: return norm_rope_resources(dtype, 0, cols, 0, 0, 0, out);   // aligned rows
+    case INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD: return norm_rope_resources(dtype, 1, cols, 0, 0, 0, out);
     case INTENT_HIP_OP_PAGED_CACHE_APPEND: return paged_cache_resources(dtype, 0, out);
     case INTENT_HIP_OP_PAGED_CACHE_READ: return paged_cache_resources(dtype, 1, out);
     case INTENT_HIP_OP_PAGED_GQA_DECODE_MX: return mx_decode_resources(dtype, rows, cols, out);
@@ -205,6 +205,10 @@ extern "C" int intent_hip_call_resources(int op, int dtype, const int64_t *facts
     case INTENT_HIP_OP_PAGED_DECODE_PARTIALS:
       if (const int rc = takes(7)) return rc;
       return paged_decode_resources(f[0], f[1], f[2], f[3], f[4], f[5], f[6], out);
+    case INTENT_HIP_OP_QK_NORM_ROPE: case INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD:
+      if (const int rc = takes(4)) return rc;
+      return norm_rope_resources(dtype, op == INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD, f[0], f[1], f[2] != 0,
+                                 static_cast<uint64_t>(f[3]), out);
   }
   return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "operator code %d has no facts of a call", op);
 }

@@ -968,6 +968,17 @@ def _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, befor
     return views, (tokens, q_heads, k.shape[1], d, table, pairs)
 
 
+def _mixed(*views) -> int:
+    """Every address, and every outer stride in bytes, or-ed: what the views' common alignment can be read from."""
+    mixed = 0
+    for t in views:
+        if t.numel():
+            mixed |= t.data_ptr()
+            for st in t.stride()[:-1]:
+                mixed |= st * t.element_size()
+    return mixed
+
+
 def _norm_rope(dtype_code):
     """qk_norm_rope: q and k rows are read through their own strides (a projection's slices), staged only where their
     inner stride is not 1."""
@@ -983,7 +994,8 @@ def _norm_rope(dtype_code):
         args = (dtype_code, *(t.data_ptr() for t in (*views, *outs)), *extents, strides, float(eps), interleaved)
         return Launch("intent_hip_qk_norm_rope", lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
                       tuple(zip(("tokens", "q_heads", "kv_heads", "d", "table", "pairs"), extents)),
-                      lambda: lib.kernel_resources(OP_QK_NORM_ROPE, dtype_code, extents[0], extents[3]))
+                      lambda: lib.call_resources(OP_QK_NORM_ROPE, dtype_code, extents[3], extents[5], interleaved,
+                                                 _mixed(*views[:4], *views[5:], *outs)))
     return plan
 
 
@@ -1012,7 +1024,8 @@ def _norm_rope_backward(dtype_code):
         return Launch("intent_hip_qk_norm_rope_backward", run, tuple(keep), tuple(before), tuple(after),
                       tuple(zip(("tokens", "q_heads", "kv_heads", "d", "table", "pairs"), extents))
                       + (("workspace_bytes", size.value),),
-                      lambda: lib.kernel_resources(OP_QK_NORM_ROPE_BACKWARD, dtype_code, extents[0], extents[3]))
+                      lambda: lib.call_resources(OP_QK_NORM_ROPE_BACKWARD, dtype_code, extents[3], extents[5], interleaved,
+                                                 _mixed(*views[:4], *views[5:], *grads, *outs[:2])))
     return plan
 
 
