@@ -68,7 +68,7 @@ enum IntentHipOperator {
   INTENT_HIP_OP_MLA_PREFILL = 22,         /* cols = D | P << 16 */
   INTENT_HIP_OP_QK_NORM_ROPE = 23,        /* dtype F16 or BF16; rows = tokens, cols = head width */
   INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD = 24,
-  INTENT_HIP_OP_PAGED_CACHE_APPEND = 25,  /* dtype F16 or BF16, for both */
+  INTENT_HIP_OP_PAGED_CACHE_APPEND = 25,  /* dtype F16 or BF16; rows, cols = kv_heads * (d + dv), for both */
   INTENT_HIP_OP_PAGED_CACHE_READ = 26,
   INTENT_HIP_OP_PAGED_GQA_DECODE_MX = 27, /* dtype F16 or BF16; rows = HEAD_GROUP, cols = head width */
   INTENT_HIP_OP_LINEAR_MXFP4 = 28         /* dtype F16 or BF16; rows = m, cols = n */

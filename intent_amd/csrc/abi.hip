@@ -157,8 +157,8 @@ extern "C" int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int6
     case INTENT_HIP_OP_CSR_SPMM_F32: return spmm_resources(cols, out);
     case INTENT_HIP_OP_QK_NORM_ROPE: return norm_rope_resources(dtype, 0, cols, 0, 0, 0, out);   // aligned rows
     case INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD: return norm_rope_resources(dtype, 1, cols, 0, 0, 0, out);
-    case INTENT_HIP_OP_PAGED_CACHE_APPEND: return paged_cache_resources(dtype, 0, out);
-    case INTENT_HIP_OP_PAGED_CACHE_READ: return paged_cache_resources(dtype, 1, out);
+    case INTENT_HIP_OP_PAGED_CACHE_APPEND: return paged_cache_resources(dtype, 0, rows, cols, out);
+    case INTENT_HIP_OP_PAGED_CACHE_READ: return paged_cache_resources(dtype, 1, rows, cols, out);
     case INTENT_HIP_OP_PAGED_GQA_DECODE_MX: return mx_decode_resources(dtype, rows, cols, out);
     case INTENT_HIP_OP_LINEAR_MXFP4: return linear_mxfp4_resources(dtype, rows, out);
     case INTENT_HIP_OP_GEMM_I8: return gemm_i8_resources(rows, cols, out);

@@ -12,6 +12,7 @@ constexpr int kMxBlock = 32;
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bfloat2_t __attribute__((ext_vector_type(2)));
 typedef short short2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 
 // The scale operand of the conversions, whose exponent field alone counts (2^-127 has a field of zero).
 __device__ __forceinline__ float mx_scale(int exponent) {
@@ -35,16 +36,32 @@ __device__ __forceinline__ int mx_exponent_e4m3(float size) {
   return e < 0 ? 0 : e;
 }
 
-// Four values as e4m3 elements at a block's scale. |value| <= 448 * scale or not finite; what is not finite is held as NaN
-// (the conversion itself would take an infinity to 448).
-__device__ __forceinline__ uint32_t mx_quad_e4m3(float a, float b, float c, float d, float scale) {
-  const auto settled = [](float v) {
-    return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u ? __uint_as_float(__float_as_uint(v) | 0x7FC00000u) : v;
-  };
+// Four e4m3 elements of two pairs of 16-bit values of type E, at a block's scale: finite magnitudes of at most 448 * scale
+// (the conversion itself would take an infinity to 448), or NaN.
+template <typename E>
+__device__ __forceinline__ uint32_t mx_quad_e4m3(uint32_t low, uint32_t high, float scale) {
   short2_t word = {0, 0};
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, settled(a), settled(b), scale, false);
-  word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, settled(c), settled(d), scale, true);
+  if constexpr (__is_same(E, f16_t)) {
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(word, __builtin_bit_cast(half2_t, low), scale, false);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(word, __builtin_bit_cast(half2_t, high), scale, true);
+  } else {
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(word, __builtin_bit_cast(bfloat2_t, low), scale, false);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(word, __builtin_bit_cast(bfloat2_t, high), scale, true);
+  }
   return __builtin_bit_cast(uint32_t, word);
+}
+
+// Two 16-bit values with what is not finite taken out (to 0), or turned into NaN.
+template <typename E, bool kNaN>
+__device__ __forceinline__ uint32_t mx_settled(uint32_t pair) {
+  constexpr uint32_t inf = __is_same(E, f16_t) ? 0x7C00u : 0x7F80u;
+  const auto one = [](uint32_t v) { return (v & inf) != inf ? v : kNaN ? v | 0x7FFFu : 0u; };
+  return one(pair & 0xFFFFu) | one(pair >> 16) << 16;
+}
+
+// The larger of each half of two pairs of 16-bit magnitudes (sign bits clear: they order as whole numbers).
+__device__ __forceinline__ uint32_t mx_larger(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
 }
 
 // The sequence of packed row `row`: the number of sequences among the first `sequences` that end at or before it, found 64
@@ -68,10 +85,9 @@ struct PageTable {
   const int32_t *offsets, *indices;
   int64_t positions, pages;
   int ps;
-  // The page of logical page `at` of sequence s, or -1.
-  __device__ __forceinline__ int64_t page(int s, int64_t at) const {
-    const int64_t first = offsets[s], last = offsets[s + 1];
-    if (at < 0 || at >= last - first || first < 0 || first + at >= positions) return -1;
+  // The page of logical page `at` of a sequence that holds `held` of them from offsets entry `first` on, or -1.
+  __device__ __forceinline__ int64_t page(int64_t first, int64_t held, int64_t at) const {
+    if (at < 0 || at >= held || first < 0 || first + at >= positions) return -1;
     const int64_t page = indices[first + at];
     return page < 0 || page >= pages ? -1 : page;
   }

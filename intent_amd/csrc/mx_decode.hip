@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
     for (int u = 0; u < 2; ++u) {
       if constexpr (kUniform) {
         const int64_t at = p0 + u * 16;
-        int64_t page = at < end ? p.table.page(s, at / p.table.ps) : -1;
+        int64_t page = at < end ? p.table.page(p.table.offsets[s], p.table.offsets[s + 1] - static_cast<int64_t>(p.table.offsets[s]), at / p.table.ps) : -1;
         int64_t slot = at % p.table.ps;
         valid[u] = page < 0 ? 0 : static_cast<int>(end - at < 16 ? end - at : 16);
         if (page < 0) page = slot = 0;             // any 16 rows of the cache: their weights are 0
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
         }
       } else {
         const auto find = [&](int64_t at, int64_t &page, int64_t &slot) {
-          page = at < end ? p.table.page(s, at / p.table.ps) : -1;
+          page = at < end ? p.table.page(p.table.offsets[s], p.table.offsets[s + 1] - static_cast<int64_t>(p.table.offsets[s]), at / p.table.ps) : -1;
           slot = at % p.table.ps;
           const bool live = page >= 0;
           if (!live) page = slot = 0;

@@ -149,20 +149,25 @@ __global__ __launch_bounds__(kWaves * kWave) void norm_rope_backward_any(NormRop
 }
 
 // grad_w[which][d]: the workgroups' partial sums, in a fixed order. One workgroup per 16 dimensions of the queries' or the
-// keys' weight; 16 threads share a dimension.
-__global__ __launch_bounds__(256) void norm_rope_fold(const float *partial, int blocks, int d, float *dq, float *dk) {
-  __shared__ float sums[16][17];
+// keys' weight; 64 threads share a dimension (a row's 16 values are half a line), so few loads wait for each other.
+constexpr int kFoldParts = 64;
+__global__ __launch_bounds__(16 * kFoldParts) void norm_rope_fold(const float *partial, int blocks, int d, float *dq, float *dk) {
+  __shared__ float sums[kFoldParts][17];
   const int column = threadIdx.x & 15, part = threadIdx.x >> 4, at = blockIdx.x * 16 + column;
   const int which = blockIdx.y;
   float total = 0.0f;
-  if (at < d)
-    for (int i = part; i < blocks; i += 16) total += partial[(static_cast<int64_t>(i) * 2 + which) * d + at];
+  if (at < d) {
+#pragma unroll 8
+    for (int i = part; i < blocks; i += kFoldParts) total += partial[(static_cast<int64_t>(i) * 2 + which) * d + at];
+  }
   sums[part][column] = total;
   __syncthreads();
-  if (part == 0 && at < d) {
-    for (int i = 1; i < 16; ++i) total += sums[i][column];
-    (which ? dk : dq)[at] = total;
+#pragma unroll
+  for (int half = kFoldParts / 2; half >= 1; half /= 2) {
+    if (part < half) sums[part][column] += sums[part + half][column];
+    __syncthreads();
   }
+  if (part == 0 && at < d) (which ? dk : dq)[at] = sums[0][column];
 }
 
 // ---------------------------------------------------------------- rows of 16-byte pieces
@@ -407,7 +412,7 @@ __global__ __launch_bounds__(kWaves * kWave) void norm_rope_backward_rows(NormRo
 
 // Workgroups of the backward pass: as many as the chip holds at once, fewer where a wave would have no token (or no row).
 int backward_blocks(int64_t tokens, int64_t q_heads, int64_t kv_heads) {
-  const int64_t rows = tokens * (q_heads + kv_heads), wanted = (rows + kWaves - 1) / kWaves, most = 4 * device_cus();
+  const int64_t rows = tokens * (q_heads + kv_heads), wanted = (rows + kWaves - 1) / kWaves, most = 2 * device_cus();
   return static_cast<int>(wanted < most ? wanted : most);
 }
 
@@ -639,7 +644,7 @@ extern "C" int intent_hip_qk_norm_rope_backward(int dtype, const void *q, const 
       launch_backward<bf16_t>(p, blocks, partial, as_stream(stream));
     if (hipPeekAtLastError() != hipSuccess) return launch_status("norm_rope_backward");
   }
-  norm_rope_fold<<<dim3(static_cast<unsigned>((d + 15) / 16), 2), 256, 0, as_stream(stream)>>>(
+  norm_rope_fold<<<dim3(static_cast<unsigned>((d + 15) / 16), 2), 16 * kFoldParts, 0, as_stream(stream)>>>(
       partial, blocks, static_cast<int>(d), grad_q_weight, grad_k_weight);
   return hipPeekAtLastError() != hipSuccess ? launch_status("norm_rope_fold") : INTENT_HIP_OK;
 }

@@ -1096,7 +1096,7 @@ def _paged_cache(dtype_code, reading: bool):
             args = (dtype_code, *(t.data_ptr() for t in rows), *pointers, *(t.data_ptr() for t in tables), *extents, strides)
         return Launch(entry, lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
                       tuple(zip(("rows", "sequences", "kv_heads", "d", "dv", "pages", "ps", "positions"), extents)),
-                      lambda: lib.kernel_resources(op, dtype_code, extents[0], d))
+                      lambda: lib.kernel_resources(op, dtype_code, extents[0], kv_heads * (d + extents[4])))
     return plan
 
 
