@@ -124,6 +124,7 @@ int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int64_t cols,
  *   ATTENTION_BWD_DKDV     batch, q_heads, head_group, sq, sk, d, causal, whether it has a workspace of the size it names
  *                          (of the kernels of one call the first, not the fold)
  *   PAGED_DECODE_PARTIALS  batch, kv_heads, head_group, d, positions, ps, splits
+ *   PAGED_GQA_DECODE_MX    batch, kv_heads, head_group, d, ps, positions (of the two kernels of a joined call the first)
  *   QK_NORM_ROPE, QK_NORM_ROPE_BACKWARD  d, pairs, interleaved, every address and stride in bytes of the rows, weights and
  *                          tables, or-ed */
 int intent_hip_call_resources(int op, int dtype, const int64_t *facts, int count, struct IntentHipKernelResources *out);

@@ -14,10 +14,8 @@ typedef __bf16 bfloat2_t __attribute__((ext_vector_type(2)));
 typedef short short2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 
-// The scale operand of the conversions, whose exponent field alone counts (2^-127 has a field of zero).
-__device__ __forceinline__ float mx_scale(int exponent) {
-  return __uint_as_float(exponent == 0 ? 0x00400000u : static_cast<uint32_t>(exponent) << 23);
-}
+// The scale operand of the conversions: its exponent field alone counts, and a field of 0 is 2^-127 there.
+__device__ __forceinline__ float mx_scale(int exponent) { return __uint_as_float(static_cast<uint32_t>(exponent) << 23); }
 
 // The elements 2 * kHalf and 2 * kHalf + 1 of four e4m3 elements, as two 16-bit values of type E.
 template <typename E, bool kHalf>

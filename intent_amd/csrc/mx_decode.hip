@@ -8,8 +8,8 @@
 //
 // Design. The page range of a sequence is cut into jobs of `job_pages` pages; job j of the flat list belongs to the last
 // sequence s with page_offsets[s] / job_pages + s <= j, which every wave finds by itself, so no table of work is made and
-// lengths may change under a captured graph. A workgroup takes a job of one key head, its waves 32 keys in turn; nothing
-// but the waves' final states goes through the LDS:
+// lengths may change under a captured graph. A workgroup takes a job of one key head, its waves 32 keys in turn; only their
+// final states go through the LDS, and the states of a sequence's jobs through the workspace to mx_decode_merge:
 //   * scores: v_mfma_f32_16x16x32 with 16 keys as rows and 16 query heads as columns. The sum over a head's dimensions may
 //     run in any order, so lane (r, g) takes dimensions g D / 4 .. of key r as they lie in memory, converts them with its
 //     blocks' scales, and the query is laid out to match.
@@ -18,7 +18,11 @@
 //   * values: lane (c, g) loads its columns of its own 8 keys and pairs them with v_perm, for 16 columns a product.
 //   * the running maximum is raised (and the sums scaled down) only when a score passes it by 2^8, so most steps have no
 //     cross-lane move at all; weights up to 2^8 are far inside either type.
-// Bound by the cache's bytes.
+// Bound by the cache's bytes once there are many jobs (64 sequences of 8191, 8 key heads of 128: 191 us, 5.1 TB/s; the loads
+// alone take as long); with few jobs by a step's chain of instructions, about 430 of a wave (1.2 us where it runs alone).
+#include <stdio.h>
+
+#include <algorithm>
 #include <type_traits>
 
 #include "mx.hpp"
@@ -27,9 +31,13 @@ namespace intent_hip {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWaves = 4;
 constexpr int kStep = 32;              // keys of a wave's step: two tiles of 16
 constexpr float kSlack = 8.0f;
+constexpr uint32_t kSigns = 0x80008000u;
+constexpr int kMany = 6, kFew = 2;     // workgroups a CU is given
+constexpr int kLong = 256;            // tokens of a job: from here on it is one of many
+constexpr int kLeast = 128;
+constexpr int kWhole = 2048, kWholeOne = 768;   // tokens of all sequences and of one, up to here each is one job
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -55,37 +63,52 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// Two values rounded to E, the first in the low half.
+// Two non-negative weights in two parts of type E each: `high` cut off to its bits, `low` what that left, cut off too; 2^-20
+// (f16) and 2^-14 (bf16) of a weight are left out.
 template <typename E>
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-  return static_cast<uint32_t>(from_f32<E>(a).bits) | static_cast<uint32_t>(from_f32<E>(b).bits) << 16;
-}
-template <typename E>
-__device__ __forceinline__ float unpack(uint32_t word, int half) {
-  return to_f32(E{static_cast<uint16_t>(half ? word >> 16 : word)});
+__device__ __forceinline__ void parts(float a, float b, uint32_t &high, uint32_t &low) {
+  if constexpr (std::is_same_v<E, f16_t>) {
+    const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    high = __builtin_bit_cast(uint32_t, h);
+    low = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(h[0]), b - static_cast<float>(h[1])));
+  } else {
+    const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
+    high = __builtin_amdgcn_perm(v, u, 0x07060302);
+    low = __builtin_amdgcn_perm(__float_as_uint(b - __uint_as_float(v & 0xFFFF0000u)), __float_as_uint(a - __uint_as_float(u & 0xFFFF0000u)),
+                                0x07060302);
+  }
 }
 
-// The sequence of job `job`: sequence s's jobs begin at offsets[s] / job_pages + s.
-__device__ __forceinline__ int job_sequence(const Decode &p, int job) {
+// A sequence: its first entry of the page indices, and its tokens: what its length and its pages both have; none in a cache
+// without a page.
+struct Sequence {
+  int s, first, tokens;
+  __device__ __forceinline__ void settle(const Decode &p, int next, int length) {
+    const int64_t held = static_cast<int64_t>(max(0, next - first)) * p.table.ps;
+    tokens = p.table.pages == 0 || length < 0 ? 0 : length < held ? length : static_cast<int>(held);
+  }
+};
+
+// The sequence of job `job` (the wave's): the last whose jobs, from offsets[s] / job_pages + s on, begin at or before it.
+// Found by all lanes of the wave, who then hold what is known of 64 candidates.
+__device__ __forceinline__ Sequence job_sequence(const Decode &p, int job) {
   const int lane = threadIdx.x & 63;
-  int first = 0, count = p.batch;
-  while (count > 0) {
+  int first = 0, count = p.batch - 1;          // it is one of first .. first + count
+  while (count >= kWave) {
     const int step = (count + 63) / 64;
     const int at = (lane + 1) * step;
     const bool past = at <= count && static_cast<int64_t>(p.table.offsets[first + at] / p.job_pages) + first + at <= job;
     const int steps = __popcll(__ballot(past));
     first += steps * step;
-    count = step == 1 ? 0 : min(step - 1, count - steps * step);
+    count = min(step - 1, count - steps * step);
   }
-  return first;
-}
-
-// Tokens of sequence s: what its length and its pages both have; none in a cache without a page.
-__device__ __forceinline__ int64_t sequence_tokens(const Decode &p, int s) {
-  if (p.table.pages == 0) return 0;
-  const int64_t pages = static_cast<int64_t>(p.table.offsets[s + 1]) - p.table.offsets[s];
-  const int64_t held = (pages < 0 ? 0 : pages) * p.table.ps, length = p.lengths[s];
-  return length < held ? (length < 0 ? 0 : length) : held;
+  const bool in = lane <= count;
+  const int s = first + (in ? lane : 0), begin = p.table.offsets[s], next = p.table.offsets[s + 1], length = p.lengths[s];
+  const bool past = lane > 0 && in && static_cast<int64_t>(begin / p.job_pages) + s <= job;
+  const int at = __popcll(__ballot(past));
+  Sequence found{first + at, __builtin_amdgcn_readlane(begin, at), 0};
+  found.settle(p, __builtin_amdgcn_readlane(next, at), __builtin_amdgcn_readlane(length, at));
+  return found;
 }
 
 // How a lane's columns of the values lie: `kWide` runs of 128 columns (8 bytes a lane), then one of 64 (4) and one of 32 (2).
@@ -95,7 +118,16 @@ struct Columns {
   static constexpr bool kHalf = kRest >= 64, kQuarter = kRest % 64 != 0;
   static constexpr int kRuns = kWide + kHalf + kQuarter;
   static constexpr int kTiles = D / 16;          // products of 16 columns
+  // Column of lane r in product j.
+  static __device__ __forceinline__ int column(int j, int r) {
+    if (j < kWide * 8) return j / 8 * 128 + r * 8 + j % 8;
+    if (kHalf && j < kWide * 8 + 4) return kWide * 128 + r * 4 + (j - kWide * 8);
+    return D - 32 + r * 2 + (j - (kTiles - 2));
+  }
 };
+
+// Waves of a SIMD: what the accumulators, the query and a step's loads leave room for.
+constexpr int waves_per_simd(int width) { return width <= 64 ? 4 : width <= 128 ? 3 : width <= 256 ? 2 : 1; }
 
 template <int D>
 struct Step {                                     // what a lane loads for 32 keys
@@ -103,31 +135,30 @@ struct Step {                                     // what a lane loads for 32 ke
   uint8_t ke[2][D / 32];
   uint2 v[8][Columns<D>::kRuns];                  // [key][run]
   uint8_t ve[8][Columns<D>::kRuns];
+  int valid[2];                                   // kUniform: how many keys of a tile have a token
+  unsigned live;                                  // else: a bit for each of the lane's keys of the values
 };
 
-// kUniform: a tile of 16 keys lies in one page (PS is a multiple of 16), so its address is the wave's.
-template <typename E, int D, int QT, bool kUniform>
-__global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
+// kUniform: a tile of 16 keys lies in one page (PS is a multiple of 16), so its address is the wave's, and a lane's place in
+// it stays the same.
+template <typename E, int D, int QT, bool kUniform, int W>
+__global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_per_simd(D * QT)))) void mx_decode(Decode p) {
   using C = Columns<D>;
   constexpr int kChunks = D / 32;
-  constexpr int kState = QT * C::kTiles * 4;      // accumulators of a lane
-  __shared__ float sums_s[kWaves / 2][kState][kWave];
-  __shared__ float peak_s[kWaves][QT * 16], total_s[kWaves][QT * 16];
-
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Key heads of a job run on one XCD, close in time: pages with their heads side by side share lines.
+  __shared__ float sums_s[W][C::kTiles * 4][kWave], peak_s[W][16], total_s[W][16];
+  // Key heads of a job run on one XCD at about the same time: pages with their heads side by side share lines.
   const int n = static_cast<int>(gridDim.x), xcd = static_cast<int>(blockIdx.x) % 8;
   const int item = xcd * (n / 8) + (xcd < n % 8 ? xcd : n % 8) + static_cast<int>(blockIdx.x) / 8;
   const int ht = item % p.head_tiles, kh = item / p.head_tiles % p.kv_heads, job = item / p.head_tiles / p.kv_heads;
-  const int s = job_sequence(p, job);
-  if (s >= p.batch) return;
-  const int64_t tokens = sequence_tokens(p, s);
-  const int64_t begin = static_cast<int64_t>(job - (p.table.offsets[s] / p.job_pages + s)) * p.job_pages * p.table.ps;
-  int64_t end = begin + static_cast<int64_t>(p.job_pages) * p.table.ps;
-  end = end < tokens ? end : tokens;
-  // A sequence without a token is its first job's, which writes the 0 itself where no states are merged.
-  if (begin < 0 || (begin >= end && (begin > 0 || p.peak != nullptr))) return;
+  const Sequence sequence = job_sequence(p, job);
+  const int s = sequence.s, place = job - (sequence.first / p.job_pages + s);        // of the job among the sequence's
+  const int64_t begin = static_cast<int64_t>(place) * p.job_pages * p.table.ps, size = static_cast<int64_t>(p.job_pages) * p.table.ps;
+  // A sequence without a token is its first job's, which writes the 0 itself where no states are joined.
+  if (place < 0 || (begin >= sequence.tokens && (place > 0 || p.peak != nullptr))) return;
+  const int tokens = static_cast<int>(sequence.tokens - begin < size ? sequence.tokens - begin : size);      // of the job
+  const int index0 = sequence.first + place * p.job_pages;           // its first entry of the page indices
   const int head0 = kh * p.group + ht * QT * 16, heads = min(QT * 16, p.group - ht * QT * 16);
 
   uint4 q[QT][kChunks];
@@ -139,7 +170,14 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
       if (t * 16 + r < heads)
         q[t][c] = *reinterpret_cast<const uint4 *>(p.q + s * p.qs[0] + (head0 + t * 16 + r) * p.qs[1] + g * (D / 4) + c * 8);
     }
-  const float c1 = p.scale * kLog2e;
+  // The sign of the scale goes to the query, so that scores order as their products do.
+  const float c1 = fabsf(p.scale) * kLog2e;
+  if (p.scale < 0.0f)
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        q[t][c] = make_uint4(q[t][c].x ^ kSigns, q[t][c].y ^ kSigns, q[t][c].z ^ kSigns, q[t][c].w ^ kSigns);
   f32x4_t acc[QT][C::kTiles];
   float peak[QT], total[QT];
 #pragma unroll
@@ -150,67 +188,31 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
     for (int j = 0; j < C::kTiles; ++j) acc[t][j] = f32x4_t{0, 0, 0, 0};
   }
 
-  // Row addresses of a key: page * stride + place * stride. `valid`: how many of a tile's keys count (kUniform), or a bit
-  // per key of the lane (bits 0, 1: its keys of the scores; 8 + i: its keys of the values).
-  const auto load = [&](Step<D> &x, int64_t p0, int(&valid)[2], unsigned &bits) {
-    const auto keys = [&](int u, const uint8_t *k, const uint8_t *ke) {
+  // A key's elements and exponents, and a value's, from a row's start and this lane's offset in it.
+  const auto key = [&](Step<D> &x, int u, const uint8_t *k, const uint8_t *ke, unsigned ko, unsigned keo) {
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        x.k[u][c] = *reinterpret_cast<const uint2 *>(k + g * (D / 4) + c * 8);
-        x.ke[u][c] = ke[(g * (D / 4) + c * 8) / 32];
-      }
-    };
-    const auto values = [&](int i, const uint8_t *v, const uint8_t *ve) {
+    for (int c = 0; c < kChunks; ++c) {
+      x.k[u][c] = *reinterpret_cast<const uint2 *>(k + ko + g * (D / 4) + c * 8);
+      x.ke[u][c] = ke[keo + (g * (D / 4) + c * 8) / 32];
+    }
+  };
+  const auto value = [&](Step<D> &x, int i, const uint8_t *v, const uint8_t *ve, unsigned vo, unsigned veo) {
 #pragma unroll
-      for (int w = 0; w < C::kWide; ++w) {
-        x.v[i][w] = *reinterpret_cast<const uint2 *>(v + w * 128 + r * 8);
-        x.ve[i][w] = ve[w * 4 + r / 4];
-      }
-      if constexpr (C::kHalf) {
-        x.v[i][C::kWide].x = *reinterpret_cast<const uint32_t *>(v + C::kWide * 128 + r * 4);
-        x.ve[i][C::kWide] = ve[C::kWide * 4 + r / 8];
-      }
-      if constexpr (C::kQuarter) {
-        x.v[i][C::kRuns - 1].x = *reinterpret_cast<const uint16_t *>(v + D - 32 + r * 2);
-        x.ve[i][C::kRuns - 1] = ve[D / 32 - 1];
-      }
-    };
-    bits = 0;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if constexpr (kUniform) {
-        const int64_t at = p0 + u * 16;
-        int64_t page = at < end ? p.table.page(p.table.offsets[s], p.table.offsets[s + 1] - static_cast<int64_t>(p.table.offsets[s]), at / p.table.ps) : -1;
-        int64_t slot = at % p.table.ps;
-        valid[u] = page < 0 ? 0 : static_cast<int>(end - at < 16 ? end - at : 16);
-        if (page < 0) page = slot = 0;             // any 16 rows of the cache: their weights are 0
-        keys(u, p.k + page * p.ks[0] + (slot + r) * p.ks[1] + kh * p.ks[2], p.ke + page * p.kes[0] + (slot + r) * p.kes[1] + kh * p.kes[2]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t at_slot = slot + g * 4 + i;
-          values(u * 4 + i, p.v + page * p.vs[0] + at_slot * p.vs[1] + kh * p.vs[2], p.ve + page * p.ves[0] + at_slot * p.ves[1] + kh * p.ves[2]);
-        }
-      } else {
-        const auto find = [&](int64_t at, int64_t &page, int64_t &slot) {
-          page = at < end ? p.table.page(p.table.offsets[s], p.table.offsets[s + 1] - static_cast<int64_t>(p.table.offsets[s]), at / p.table.ps) : -1;
-          slot = at % p.table.ps;
-          const bool live = page >= 0;
-          if (!live) page = slot = 0;
-          return live;
-        };
-        int64_t page, slot;
-        bits |= static_cast<unsigned>(find(p0 + u * 16 + r, page, slot)) << u;
-        keys(u, p.k + page * p.ks[0] + slot * p.ks[1] + kh * p.ks[2], p.ke + page * p.kes[0] + slot * p.kes[1] + kh * p.kes[2]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bits |= static_cast<unsigned>(find(p0 + u * 16 + g * 4 + i, page, slot)) << (8 + u * 4 + i);
-          values(u * 4 + i, p.v + page * p.vs[0] + slot * p.vs[1] + kh * p.vs[2], p.ve + page * p.ves[0] + slot * p.ves[1] + kh * p.ves[2]);
-        }
-      }
+    for (int w = 0; w < C::kWide; ++w) {
+      x.v[i][w] = *reinterpret_cast<const uint2 *>(v + vo + w * 128 + r * 8);
+      x.ve[i][w] = ve[veo + w * 4 + r / 4];
+    }
+    if constexpr (C::kHalf) {
+      x.v[i][C::kWide].x = *reinterpret_cast<const uint32_t *>(v + vo + C::kWide * 128 + r * 4);
+      x.ve[i][C::kWide] = ve[veo + C::kWide * 4 + r / 8];
+    }
+    if constexpr (C::kQuarter) {
+      x.v[i][C::kRuns - 1].x = *reinterpret_cast<const uint16_t *>(v + vo + D - 32 + r * 2);
+      x.ve[i][C::kRuns - 1] = ve[veo + D / 32 - 1];
     }
   };
 
-  const auto fold = [&](Step<D> &x, const int(&valid)[2], unsigned bits) {
+  const auto fold = [&](Step<D> &x) {
     // Scores of keys 16 u + 4 g + i against head 16 t + r.
     f32x4_t sc[QT][2];
 #pragma unroll
@@ -230,10 +232,10 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
     bool whole = true;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      live[i] = kUniform ? g * 4 + (i & 3) < valid[i >> 2] : (bits >> (8 + i) & 1) != 0;
+      live[i] = kUniform ? g * 4 + (i & 3) < x.valid[i >> 2] : (x.live >> i & 1) != 0;
       whole = whole && live[i];
     }
-    const bool all = kUniform ? valid[0] == 16 && valid[1] == 16 : __all(whole);
+    const bool all = kUniform ? x.valid[0] == 16 && x.valid[1] == 16 : __all(whole);
     if (!all) {
       // What lies in places without a token has no weight, and must not turn a zero weight into NaN.
 #pragma unroll
@@ -245,13 +247,10 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
     uint4 hi[QT], lo[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      float z[8], most = -INFINITY;
+      float z[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        z[i] = sc[t][i >> 2][i & 3] * c1;
-        if (!all && !live[i]) z[i] = -INFINITY;
-        most = fmaxf(most, z[i]);
-      }
+      for (int i = 0; i < 8; ++i) z[i] = all || live[i] ? sc[t][i >> 2][i & 3] : -INFINITY;
+      float most = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))) * c1;
       if (__any(most > peak[t] + kSlack)) {
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
@@ -266,19 +265,17 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
           for (int j = 0; j < C::kTiles; ++j) acc[t][j][i] *= f;
         }
       }
-      const float base = peak[t] == -INFINITY ? 0.0f : peak[t];
+      const float base = peak[t] == -INFINITY ? 0.0f : -peak[t];
       float w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(z[i] - base);
-        total[t] += w[i];
-      }
+      for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], c1, base));
+      if (!all)                                     // (-inf times a scale of 0 is NaN)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = live[i] ? w[i] : 0.0f;
+      total[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       uint32_t h[4], l[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[i] = pack<E>(w[2 * i], w[2 * i + 1]);
-        l[i] = pack<E>(w[2 * i] - unpack<E>(h[i], 0), w[2 * i + 1] - unpack<E>(h[i], 1));
-      }
+      for (int i = 0; i < 4; ++i) parts<E>(w[2 * i], w[2 * i + 1], h[i], l[i]);
       hi[t] = make_uint4(h[0], h[1], h[2], h[3]);
       lo[t] = make_uint4(l[0], l[1], l[2], l[3]);
     }
@@ -321,127 +318,197 @@ __global__ __launch_bounds__(kWaves *kWave) void mx_decode(Decode p) {
     if constexpr (C::kQuarter) columns(C::kRuns - 1, C::kTiles - 2, no, no);
   };
 
-  Step<D> x;
-  int valid[2];
-  unsigned bits;
-  for (int64_t p0 = begin + wave * kStep; p0 < end; p0 += kWaves * kStep) {
-    load(x, p0, valid, bits);
-    fold(x, valid, bits);
+  if constexpr (kUniform) {
+    // The wave's tiles: the first token of each, its page among the job's and its place there.
+    const int ps = p.table.ps, pages_on = W * kStep / ps, places_on = W * kStep - pages_on * ps;
+    int at[2], logical[2], slot[2], raw[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      at[u] = wave * kStep + u * 16;
+      logical[u] = at[u] / ps, slot[u] = at[u] - logical[u] * ps;
+    }
+    const auto look = [&](int u) {                 // the page index of a tile, on its way a step early
+      const int index = index0 + logical[u];
+      raw[u] = at[u] < tokens && index >= 0 && index < p.table.positions ? p.table.indices[index] : -1;
+    };
+    look(0), look(1);
+    // Of this key head, and of this lane's places in a tile.
+    const uint8_t *const k0 = p.k + kh * p.ks[2], *const ke0 = p.ke + kh * p.kes[2];
+    const uint8_t *const v0 = p.v + kh * p.vs[2], *const ve0 = p.ve + kh * p.ves[2];
+    const uint64_t ks0 = p.ks[0], kes0 = p.kes[0], vs0 = p.vs[0], ves0 = p.ves[0];
+    const unsigned ks1 = static_cast<unsigned>(p.ks[1]), kes1 = static_cast<unsigned>(p.kes[1]);
+    const unsigned vs1 = static_cast<unsigned>(p.vs[1]), ves1 = static_cast<unsigned>(p.ves[1]);
+    const unsigned ko = r * ks1, keo = r * kes1;
+    unsigned vo[4], veo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vo[i] = (g * 4 + i) * vs1, veo[i] = (g * 4 + i) * ves1;
+    const auto load = [&](Step<D> &x) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        // A tile without a page reads any 16 rows of the cache: their weights are 0.
+        const bool none = raw[u] < 0 || raw[u] >= p.table.pages;
+        const uint64_t page = static_cast<unsigned>(none ? 0 : raw[u]), in = static_cast<unsigned>(none ? 0 : slot[u]);
+        x.valid[u] = none ? 0 : min(tokens - at[u], 16);
+        at[u] += W * kStep;
+        logical[u] += pages_on, slot[u] += places_on;
+        if (slot[u] >= ps) slot[u] -= ps, ++logical[u];
+        look(u);
+        key(x, u, k0 + (page * ks0 + in * ks1), ke0 + (page * kes0 + in * kes1), ko, keo);
+        const uint8_t *const v = v0 + (page * vs0 + in * vs1), *const ve = ve0 + (page * ves0 + in * ves1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) value(x, u * 4 + i, v, ve, vo[i], veo[i]);
+      }
+    };
+    while (at[0] < tokens) {
+      Step<D> x;
+      load(x);
+      fold(x);
+    }
+  } else {
+    // Any page size: every lane finds its own keys.
+    for (int at = wave * kStep; at < tokens; at += W * kStep) {
+      Step<D> x;
+      x.live = 0;
+      const auto find = [&](int token, int64_t &page, int64_t &in) {
+        const int logical = token / p.table.ps, index = index0 + logical;
+        const int raw = token < tokens && index >= 0 && index < p.table.positions ? p.table.indices[index] : -1;
+        const bool none = raw < 0 || raw >= p.table.pages;
+        page = none ? 0 : raw, in = none ? 0 : token - logical * p.table.ps;
+        return !none;
+      };
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        int64_t page, in;
+        find(at + u * 16 + r, page, in);
+        key(x, u, p.k + page * p.ks[0] + in * p.ks[1] + kh * p.ks[2], p.ke + page * p.kes[0] + in * p.kes[1] + kh * p.kes[2], 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x.live |= static_cast<unsigned>(find(at + u * 16 + g * 4 + i, page, in)) << (u * 4 + i);
+          value(x, u * 4 + i, p.v + page * p.vs[0] + in * p.vs[1] + kh * p.vs[2], p.ve + page * p.ves[0] + in * p.ves[1] + kh * p.ves[2], 0, 0);
+        }
+      }
+      fold(x);
+    }
   }
 
-  // The waves' states: to the common maximum, then added, two waves at a time.
+  // The waves' states, a tile of query heads at a time: brought to the common maximum and added in wave order. Wave w takes
+  // rows 4 g + w % 4 of the tile and, of eight waves, half of their columns.
+  const int q_heads = p.kv_heads * p.group;
+  constexpr int kMine = C::kTiles * 4 / W;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     total[t] += __shfl_xor(total[t], 16);
     total[t] += __shfl_xor(total[t], 32);
-    if (g == 0) peak_s[wave][t * 16 + r] = peak[t], total_s[wave][t * 16 + r] = total[t];
-  }
-  __syncthreads();
-  float whole_peak[QT], whole_total[QT];
+    if (t > 0) __syncthreads();
+    if (g == 0) peak_s[wave][r] = peak[t], total_s[wave][r] = total[t];
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    float m = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, peak_s[w][t * 16 + r]);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float other = peak_s[w][t * 16 + r], part = total_s[w][t * 16 + r];
-      // A wave without a score has no weight; one whose weights are NaN keeps them.
-      sum += other == -INFINITY ? part : part * __builtin_amdgcn_exp2f(other - m);
-    }
-    whole_peak[t] = m, whole_total[t] = sum;
-    const float shrink = peak[t] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(peak[t] - m);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = __shfl(shrink, g * 4 + i);
-#pragma unroll
-      for (int j = 0; j < C::kTiles; ++j) acc[t][j][i] *= f;
-    }
-  }
-#pragma unroll
-  for (int half = kWaves / 2; half >= 1; half /= 2) {
-    if (wave >= half && wave < 2 * half)
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int j = 0; j < C::kTiles; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sums_s[wave - half][(t * C::kTiles + j) * 4 + i][lane] = acc[t][j][i];
+      for (int j = 0; j < C::kTiles; ++j) sums_s[wave][i * C::kTiles + j][lane] = acc[t][j][i];
     __syncthreads();
-    if (wave < half)
+    const int i = wave & 3, j0 = wave / 4 * kMine, in = g * 4 + i, head = t * 16 + in;
+    float whole = -INFINITY, sum = 0.0f, row[kMine] = {};
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
+    for (int w = 0; w < W; ++w) whole = fmaxf(whole, peak_s[w][in]);
 #pragma unroll
-        for (int j = 0; j < C::kTiles; ++j)
+    for (int w = 0; w < W; ++w) {
+      const float own = peak_s[w][in];
+      const float f = own == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(own - whole);      // a wave without a score has sums of 0, or NaN
+      sum += total_s[w][in] * f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][j][i] += sums_s[wave][(t * C::kTiles + j) * 4 + i][lane];
-    __syncthreads();
+      for (int j = 0; j < kMine; ++j) row[j] += sums_s[w][i * C::kTiles + j0 + j][lane] * f;
+    }
+    if (head >= heads) continue;
+    const int64_t state = static_cast<int64_t>(job) * q_heads + head0 + head;
+    if (p.peak != nullptr && r == 0 && j0 == 0) p.peak[state] = whole, p.total[state] = sum;
+    const float share = p.peak != nullptr ? 1.0f : tokens > 0 ? 1.0f / sum : 0.0f;
+    float *const sums = p.sums + state * D;
+    uint16_t *const out = p.out + s * p.outs[0] + (head0 + head) * p.outs[1];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int column = C::column(j0 + j, r);
+      if (p.peak != nullptr)
+        sums[column] = row[j];
+      else
+        out[column] = from_f32<E>(row[j] * share).bits;
+    }
   }
-  if (wave != 0) return;
+}
 
-  const int q_heads = p.kv_heads * p.group;
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    if (p.peak != nullptr && g == 0 && t * 16 + r < heads) {
-      p.peak[static_cast<int64_t>(job) * q_heads + head0 + t * 16 + r] = whole_peak[t];
-      p.total[static_cast<int64_t>(job) * q_heads + head0 + t * 16 + r] = whole_total[t];
+// Output rows from the states of a sequence's jobs: a workgroup per (sequence, query head), its W waves every W-th job each.
+// A lane weighs one job in 64 of its wave's, then the lanes take columns and add the jobs' sums in order, eight on their way
+// at once.
+template <typename E, int D, int W>
+__global__ __launch_bounds__(W *kWave) void mx_decode_merge(Decode p) {
+  constexpr int kColumns = (D + kWave - 1) / kWave, kTogether = 8;
+  __shared__ float sums_s[W][kColumns * kWave], peak_s[W], total_s[W];
+  const int q_heads = p.kv_heads * p.group, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int s = static_cast<int>(blockIdx.x) / q_heads, head = static_cast<int>(blockIdx.x) - s * q_heads;
+  Sequence sequence{s, p.table.offsets[s], 0};
+  sequence.settle(p, p.table.offsets[s + 1], p.lengths[s]);
+  const int64_t size = static_cast<int64_t>(p.job_pages) * p.table.ps;
+  const int first = sequence.first / p.job_pages + s;
+  int jobs = static_cast<int>((sequence.tokens + size - 1) / size);
+  if (first < 0 || static_cast<int64_t>(first) + jobs > p.jobs) jobs = 0;
+  const int mine = (jobs - wave + W - 1) / W;              // jobs wave, wave + W, ..
+  const int64_t row0 = static_cast<int64_t>(first + wave) * q_heads + head, stride = static_cast<int64_t>(W) * q_heads;
+  float peak = -INFINITY;
+  for (int j = lane; j < mine; j += kWave) peak = fmaxf(peak, p.peak[row0 + j * stride]);
+  peak = wave_max(peak);
+  float total = 0.0f, out[kColumns] = {};
+  for (int j0 = 0; j0 < mine; j0 += kWave) {
+    const int count = min(mine - j0, kWave);
+    float weight = 0.0f;
+    if (lane < count) {
+      const float own = p.peak[row0 + (j0 + lane) * stride];
+      weight = own == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(own - peak);        // a job without a score has sums of 0, or NaN
+      total += p.total[row0 + (j0 + lane) * stride] * weight;
     }
+    for (int j = 0; j < count; j += kTogether) {
+      float from[kTogether][kColumns] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int head = t * 16 + g * 4 + i;
-      const float sum = __shfl(whole_total[t], g * 4 + i);
-      if (head >= heads) continue;
-      const float share = end > begin ? 1.0f / sum : 0.0f;
-      float *state = p.sums + (static_cast<int64_t>(job) * q_heads + head0 + head) * D;
-      uint16_t *out = p.out + s * p.outs[0] + (head0 + head) * p.outs[1];
+      for (int i = 0; i < kTogether; ++i)
 #pragma unroll
-      for (int j = 0; j < C::kTiles; ++j) {
-        const int wide = j / 8;
-        const int column = wide < C::kWide ? wide * 128 + r * 8 + j % 8
-                           : C::kHalf && j < C::kWide * 8 + 4 ? C::kWide * 128 + r * 4 + (j - C::kWide * 8)
-                                                              : D - 32 + r * 2 + (j - (C::kTiles - 2));
-        if (p.peak != nullptr)
-          state[column] = acc[t][j][i];
-        else
-          out[column] = from_f32<E>(acc[t][j][i] * share).bits;
+        for (int c = 0; c < kColumns; ++c)
+          if (j + i < count && (D % kWave == 0 || c * kWave + lane < D))
+            from[i][c] = p.sums[(row0 + (j0 + j + i) * stride) * D + c * kWave + lane];
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        const float w = j + i < count ? lane_value(weight, j + i) : 0.0f;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) out[c] += from[i][c] * w;
       }
     }
   }
-}
-
-// Output rows from the states of a sequence's jobs: one wave per (sequence, query head), lanes over columns.
-template <typename E>
-__global__ __launch_bounds__(kWaves *kWave) void mx_decode_merge(Decode p, int d) {
-  const int q_heads = p.kv_heads * p.group, lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-  if (row >= static_cast<int64_t>(p.batch) * q_heads) return;
-  const int s = static_cast<int>(row / q_heads), head = static_cast<int>(row % q_heads);
-  const int64_t tokens = sequence_tokens(p, s), size = static_cast<int64_t>(p.job_pages) * p.table.ps;
-  const int64_t first = static_cast<int64_t>(p.table.offsets[s] / p.job_pages) + s;
-  int64_t jobs = (tokens + size - 1) / size;
-  if (first < 0 || first + jobs > p.jobs) jobs = 0;
-  float peak = -INFINITY, total = 0.0f;
-  for (int64_t j = 0; j < jobs; ++j) peak = fmaxf(peak, p.peak[(first + j) * q_heads + head]);
-  uint16_t *out = p.out + s * p.outs[0] + head * p.outs[1];
-  for (int64_t j = 0; j < jobs; ++j) {
-    const int64_t at = (first + j) * q_heads + head;
-    total += p.peak[at] == -INFINITY ? p.total[at] : p.total[at] * __builtin_amdgcn_exp2f(p.peak[at] - peak);
-  }
-  const float share = jobs > 0 ? 1.0f / total : 0.0f;
-  for (int c = lane; c < d; c += kWave) {
-    float sum = 0.0f;
-    for (int64_t j = 0; j < jobs; ++j) {
-      const int64_t at = (first + j) * q_heads + head;
-      const float f = p.peak[at] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(p.peak[at] - peak);
-      sum += p.sums[at * d + c] * f;
+  total = wave_sum(total);
+  if (lane == 0) peak_s[wave] = peak, total_s[wave] = total;
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) sums_s[wave][c * kWave + lane] = out[c];
+  __syncthreads();
+  float whole = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < W; ++w) whole = fmaxf(whole, peak_s[w]);
+  for (int column = threadIdx.x; column < D; column += W * kWave) {
+    float sum = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = peak_s[w] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(peak_s[w] - whole);
+      sum += total_s[w] * f;
+      value += sums_s[w][column] * f;
     }
-    out[c] = from_f32<E>(sum * share).bits;
+    p.out[s * p.outs[0] + head * p.outs[1] + column] = from_f32<E>(value * (jobs > 0 ? 1.0f / sum : 0.0f)).bits;
   }
 }
 
-// How a call is cut. Jobs of at least 256 tokens, as many as fill the chip a few times over.
+// How a call is cut, from what the host knows: the pages that the table holds for all sequences. Measured with 8 key heads of
+// 128, 4 query heads each, us:
+//   * few tokens in all and per sequence: a workgroup of eight waves takes a whole sequence, and nothing is joined (4
+//     sequences of 300: 7.0, in jobs 10.7; one of 1024 11.2 and 10.3, one of 2048 17.8 and 10.1);
+//   * else jobs of four waves, 6 workgroups a CU where that leaves a job 256 tokens, so that a job's start and end hide behind
+//     others (64 sequences of 8191: 191; 2 a CU 204, 3 210), or 2, which are on the chip at once;
+//   * a job has 128 tokens at least (one sequence of 2048: 10.1; 256 11.4, 512 13.4).
 struct Cut {
-  int job_pages, jobs, head_tiles, qt;
+  int job_pages, jobs, head_tiles, qt, waves;
   bool merge;
   int64_t blocks;
 };
@@ -449,15 +516,18 @@ Cut cut(int64_t batch, int64_t kv_heads, int64_t group, int64_t positions, int64
   Cut c{};
   c.qt = group > 16 ? 2 : 1;
   c.head_tiles = static_cast<int>((group + 16 * c.qt - 1) / (16 * c.qt));
-  const int64_t wanted = 4 * device_cus();
-  int64_t tokens = positions * ps * kv_heads * c.head_tiles / wanted;
-  tokens = tokens < 256 ? 256 : tokens;
+  const int64_t all = positions * ps, heads = kv_heads * c.head_tiles;
+  int64_t tokens = all * heads / (kMany * device_cus());
+  if (tokens < kLong) tokens = all * heads / (kFew * device_cus());
+  tokens = tokens < kLeast ? kLeast : tokens;
   int64_t pages = (tokens + ps - 1) / ps;
-  if (pages >= positions) pages = positions;
+  if ((all <= kWhole && all <= kWholeOne * batch) || pages >= positions) pages = positions;
   c.job_pages = static_cast<int>(pages < 1 ? 1 : pages);
   c.merge = c.job_pages < positions;
-  c.jobs = static_cast<int>(c.merge ? positions / c.job_pages + batch : 0);
-  c.blocks = (positions / c.job_pages + batch) * kv_heads * c.head_tiles;
+  c.waves = !c.merge && c.qt == 1 && ps % 16 == 0 ? 8 : 4;
+  const int64_t jobs = positions / c.job_pages + batch;
+  c.jobs = static_cast<int>(jobs);
+  c.blocks = jobs * heads;
   return c;
 }
 
@@ -468,8 +538,8 @@ int check_extents(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head
   if (head_group < 1 || head_group > INT32_MAX || kv_heads > INT32_MAX || q_heads != kv_heads * head_group)
     return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "query heads (%lld) must equal key heads (%lld) * HEAD_GROUP (%lld)",
                 static_cast<long long>(q_heads), static_cast<long long>(kv_heads), static_cast<long long>(head_group));
-  if (batch > INT32_MAX / 64 || q_heads > INT32_MAX / 64 || ps > INT32_MAX / 64 || positions > INT32_MAX / 64 ||
-      pages > INT32_MAX)
+  if (batch > INT32_MAX / 64 || q_heads > (1 << 20) || ps > INT32_MAX / 64 || positions > INT32_MAX / 64 ||
+      positions * ps > int64_t{1} << 40 || pages > INT32_MAX)
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
   return INTENT_HIP_OK;
 }
@@ -483,18 +553,27 @@ size_t state_bytes(const Cut &c, int64_t q_heads, int64_t d) {
 
 template <typename E, int D>
 void launch(const Decode &p, const Cut &c, bool uniform, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(c.blocks)), block(kWaves * kWave);
+  const dim3 grid(static_cast<unsigned>(c.blocks));
   if (c.qt == 1) {
-    if (uniform)
-      mx_decode<E, D, 1, true><<<grid, block, 0, s>>>(p);
+    if (!uniform)
+      mx_decode<E, D, 1, false, 4><<<grid, 4 * kWave, 0, s>>>(p);
+    else if (c.waves == 4)
+      mx_decode<E, D, 1, true, 4><<<grid, 4 * kWave, 0, s>>>(p);
     else
-      mx_decode<E, D, 1, false><<<grid, block, 0, s>>>(p);
+      mx_decode<E, D, 1, true, 8><<<grid, 8 * kWave, 0, s>>>(p);
   } else {
     if (uniform)
-      mx_decode<E, D, 2, true><<<grid, block, 0, s>>>(p);
+      mx_decode<E, D, 2, true, 4><<<grid, 4 * kWave, 0, s>>>(p);
     else
-      mx_decode<E, D, 2, false><<<grid, block, 0, s>>>(p);
+      mx_decode<E, D, 2, false, 4><<<grid, 4 * kWave, 0, s>>>(p);
   }
+  if (!c.merge) return;
+  // Few rows: four waves share one's jobs.
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.group;
+  if (rows < 4 * device_cus())
+    mx_decode_merge<E, D, 4><<<dim3(static_cast<unsigned>(rows)), 4 * kWave, 0, s>>>(p);
+  else
+    mx_decode_merge<E, D, 1><<<dim3(static_cast<unsigned>(rows)), kWave, 0, s>>>(p);
 }
 
 template <typename E>
@@ -512,23 +591,39 @@ bool width_ok(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 192 || 
 
 }  // namespace
 
-int mx_decode_resources(int dtype, int64_t group, int64_t d, IntentHipKernelResources *out) {
-  const bool half = dtype == INTENT_HIP_F16, two = group > 16;
-#define INTENT_HIP_MX_DECODE(W)                                                                                             \
-  case W:                                                                                                                   \
-    return half ? two ? describe_kernel(reinterpret_cast<const void *>(mx_decode<f16_t, W, 2, true>), "mx_decode<f16," #W ",2>", kWaves * kWave, out)  \
-                      : describe_kernel(reinterpret_cast<const void *>(mx_decode<f16_t, W, 1, true>), "mx_decode<f16," #W ",1>", kWaves * kWave, out)  \
-                : two ? describe_kernel(reinterpret_cast<const void *>(mx_decode<bf16_t, W, 2, true>), "mx_decode<bf16," #W ",2>", kWaves * kWave, out) \
-                      : describe_kernel(reinterpret_cast<const void *>(mx_decode<bf16_t, W, 1, true>), "mx_decode<bf16," #W ",1>", kWaves * kWave, out)
+int mx_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t positions,
+                        IntentHipKernelResources *out) {
+  if (group < 1 || !width_ok(d)) return fail(INTENT_HIP_ERR_UNSUPPORTED, "mx decode has no head width %lld", static_cast<long long>(d));
+  const Cut c = cut(batch, kv_heads, group, positions, ps);
+  const bool uniform = ps % 16 == 0;
+  char name[64];
+  snprintf(name, sizeof(name), "mx_decode<%s,%d,%d,%s,%d>", dtype == INTENT_HIP_F16 ? "f16" : "bf16", static_cast<int>(d), c.qt,
+           uniform ? "true" : "false", uniform ? c.waves : 4);
+  const auto describe = [&](const void *half, const void *brain) {
+    return describe_kernel(dtype == INTENT_HIP_F16 ? half : brain, name, (uniform ? c.waves : 4) * kWave, out);
+  };
+#define INTENT_HIP_MX_DECODE(W)                                                                                          \
+  case W:                                                                                                                \
+    if (c.qt == 2)                                                                                                       \
+      return uniform ? describe(reinterpret_cast<const void *>(mx_decode<f16_t, W, 2, true, 4>),                         \
+                                reinterpret_cast<const void *>(mx_decode<bf16_t, W, 2, true, 4>))                        \
+                     : describe(reinterpret_cast<const void *>(mx_decode<f16_t, W, 2, false, 4>),                        \
+                                reinterpret_cast<const void *>(mx_decode<bf16_t, W, 2, false, 4>));                      \
+    if (!uniform)                                                                                                        \
+      return describe(reinterpret_cast<const void *>(mx_decode<f16_t, W, 1, false, 4>),                                  \
+                      reinterpret_cast<const void *>(mx_decode<bf16_t, W, 1, false, 4>));                                \
+    return c.waves == 4 ? describe(reinterpret_cast<const void *>(mx_decode<f16_t, W, 1, true, 4>),                      \
+                                   reinterpret_cast<const void *>(mx_decode<bf16_t, W, 1, true, 4>))                     \
+                        : describe(reinterpret_cast<const void *>(mx_decode<f16_t, W, 1, true, 8>),                      \
+                                   reinterpret_cast<const void *>(mx_decode<bf16_t, W, 1, true, 8>))
   switch (d) {
     INTENT_HIP_MX_DECODE(64);
     INTENT_HIP_MX_DECODE(96);
     INTENT_HIP_MX_DECODE(128);
     INTENT_HIP_MX_DECODE(192);
-    INTENT_HIP_MX_DECODE(256);
+    default: INTENT_HIP_MX_DECODE(256);
   }
 #undef INTENT_HIP_MX_DECODE
-  return fail(INTENT_HIP_ERR_UNSUPPORTED, "mx decode has no head width %lld", static_cast<long long>(d));
 }
 
 }  // namespace intent_hip
@@ -578,7 +673,7 @@ extern "C" int intent_hip_paged_gqa_decode_mx(int dtype, const void *q, const vo
   if (!aligned(key_cache, 16) || !aligned(value_cache, 16))
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "cache elements must be 16-byte aligned");
   const Cut c = cut(batch, kv_heads, head_group, positions, ps);
-  if (c.blocks > INT32_MAX / 256) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
+  if (c.blocks > INT32_MAX / 512) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
   const size_t bytes = state_bytes(c, q_heads, d);
   if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes || !aligned(workspace, 16)))
     return fail(INTENT_HIP_ERR_WORKSPACE, "mx decode needs %zu workspace bytes, 16-byte aligned", bytes);
@@ -602,17 +697,12 @@ extern "C" int intent_hip_paged_gqa_decode_mx(int dtype, const void *q, const vo
     p.sums = p.total + rounded(rows * 4) / 4;
   }
   hipStream_t s = as_stream(stream);
-  const bool uniform = ps % 16 == 0;
+  // Lane offsets within a tile are 32 bits.
+  const int64_t reach = std::max({strides[4], strides[8], strides[12], strides[16]});
+  const bool uniform = ps % 16 == 0 && reach < INT32_MAX / 32;
   if (dtype == INTENT_HIP_F16)
     launch<f16_t>(p, c, uniform, d, s);
   else
     launch<bf16_t>(p, c, uniform, d, s);
-  if (hipPeekAtLastError() != hipSuccess) return launch_status("mx_decode");
-  if (!c.merge) return INTENT_HIP_OK;
-  const dim3 grid(static_cast<unsigned>((batch * q_heads + kWaves - 1) / kWaves));
-  if (dtype == INTENT_HIP_F16)
-    mx_decode_merge<f16_t><<<grid, kWaves * kWave, 0, s>>>(p, static_cast<int>(d));
-  else
-    mx_decode_merge<bf16_t><<<grid, kWaves * kWave, 0, s>>>(p, static_cast<int>(d));
-  return hipPeekAtLastError() != hipSuccess ? launch_status("mx_decode_merge") : INTENT_HIP_OK;
+  return hipPeekAtLastError() != hipSuccess ? launch_status("mx_decode") : INTENT_HIP_OK;
 }

@@ -2,7 +2,7 @@
 
 Bar. A score in the exponent of two is an f32 sum of D exact products, scaled: off by at most (D + 2) * 2^-24 of the sum of
 their magnitudes, which is bounded from the inputs; a weight is off by that share (times ln 2), once in the numerator and once
-in the denominator. The weights' two parts leave 2^-16 (bf16) of them; the f32 sums run in chains of at most 2^7 steps of 8
+in the denominator. The weights' two parts leave 2^-14 (bf16) of them; the f32 sums run in chains of at most 2^7 steps of 8
 keys, 2^-14 of the sum of weight * |value| with the joins. Then half a step of the output type."""
 import pytest
 import torch
@@ -51,7 +51,7 @@ def check(out, q, keys, values, offsets, indices, lengths, scale, dtype):
     assert not got.isnan().any()
     # the largest sum of magnitudes of a score, in the exponent of two
     magnitude = float(q.double().abs().amax() * keys.abs().nan_to_num().amax()) * q.shape[2] * scale * 1.4427
-    units = 2 * (q.shape[2] + 2) * 2.0 ** -24 * magnitude + 2.0 ** -16 + 2.0 ** -14
+    units = 2 * (q.shape[2] + 2) * 2.0 ** -24 * magnitude + 2.0 ** -14 + 2.0 ** -14
     bound = HALF_STEP[dtype] * want.abs() + units * size + 2.0 ** -25
     worst = (got - want).abs() - bound
     assert (worst <= 0).all(), f"off by {(got - want).abs().flatten()[worst.argmax()]} of {want.flatten()[worst.argmax()]}"
@@ -217,3 +217,38 @@ def test_refusals(device):
     static.run(q, *keys, *values, *table, 1.0)                            # one job: no workspace
     with pytest.raises(intent.CompilationStageError, match="workspace"):
         static.run(q, *keys, *values, table[0], torch.zeros(4000, dtype=torch.int32, device=device), table[2], 1.0)
+
+
+@pytest.mark.parametrize("batch,positions", [(200, 900), (3, 3000), (70, 65)])
+def test_many_sequences_and_jobs(device, batch, positions):
+    """More sequences than a wave has lanes, and long page lists cut into many jobs: each job finds its sequence, also behind
+    sequences without a page; every row is joined from its own states."""
+    announce("mx decode many sequences", batch, positions)
+    g = torch.Generator().manual_seed(batch)
+    ends = torch.randint(0, positions + 1, (batch - 1,), generator=g).sort().values
+    offsets = [0, *ends.tolist(), positions]
+    counts = [b - a for a, b in zip(offsets, offsets[1:])]
+    lengths = [max(0, n * 16 - int(torch.randint(0, 16, (1,), generator=g))) for n in counts]
+    pages = 40                                                     # shared by the sequences, again and again
+    indices = torch.randint(0, pages, (positions,), generator=g).to(torch.int32)
+    keys, plain_keys = filled(g, pages, 16, 1, 64, True, device)
+    values, plain_values = filled(g, pages, 16, 1, 64, True, device)
+    q = torch.randn((batch, 2, 64), generator=g).half()
+    out = kernel("f16", 2).run(q.to(device), *keys, *values, i32(offsets, device), indices.to(device), i32(lengths, device), 0.125)
+    check(out, q, plain_keys, plain_values, offsets, indices, lengths, 0.125, "f16")
+
+
+def test_scale_of_either_sign_and_none(device):
+    announce("mx decode scales")
+    g = torch.Generator().manual_seed(16)
+    keys, plain_keys = filled(g, 4, 16, 1, 64, True, device)
+    values, plain_values = filled(g, 4, 16, 1, 64, True, device)
+    poison(keys, [0, 4], torch.arange(4), [50])
+    poison(values, [0, 4], torch.arange(4), [50])
+    q = torch.randn((1, 3, 64), generator=g).half()
+    table = (i32([0, 4], device), i32([0, 1, 2, 3], device), i32([50], device))
+    for scale in (-0.2, 0.0):
+        out = kernel("f16", 3).run(q.to(device), *keys, *values, *table, scale)
+        want, size = plain64.decode(q, plain_keys, plain_values, [0, 4], [0, 1, 2, 3], [50], scale)
+        assert not out.isnan().any()
+        assert ((out.double().cpu() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -13 * size).all()

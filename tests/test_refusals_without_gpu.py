@@ -103,7 +103,7 @@ def test_decode_mx():
     assert call(b=0) == 0 and call(heads=0, kv=0) == 0
     size = ctypes.c_size_t(0)
     query = lib.fn["paged_gqa_decode_mx_workspace_bytes"]
-    assert query(2, 32, 8, 4, 128, 64, 4, ctypes.byref(size)) == 0 and size.value == 0       # one job of 256 tokens
+    assert query(2, 32, 8, 4, 128, 64, 4, ctypes.byref(size)) == 0 and size.value == 0       # 256 tokens: a job a sequence
     assert query(8, 32, 8, 4, 128, 64, 1000, ctypes.byref(size)) == 0 and size.value > 0
     assert call(b=8, positions=1000, size=size.value) == 5 and b"workspace" in err()
     assert call(b=8, positions=1000, workspace=256, size=size.value - 1) == 5
