@@ -125,6 +125,7 @@ int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int64_t cols,
  *                          (of the kernels of one call the first, not the fold)
  *   PAGED_DECODE_PARTIALS  batch, kv_heads, head_group, d, positions, ps, splits
  *   PAGED_GQA_DECODE_MX    batch, kv_heads, head_group, d, ps, positions (of the two kernels of a joined call the first)
+ *   LINEAR_MXFP4           m, n, k (of the kernels of a call the first, not the fold)
  *   QK_NORM_ROPE, QK_NORM_ROPE_BACKWARD  d, pairs, interleaved, every address and stride in bytes of the rows, weights and
  *                          tables, or-ed */
 int intent_hip_call_resources(int op, int dtype, const int64_t *facts, int count, struct IntentHipKernelResources *out);
@@ -544,9 +545,12 @@ int intent_hip_paged_gqa_decode_mx(int dtype, const void *q, const void *key_cac
 /* y = x W^T with 4-bit weights, no reference counterpart. x [m, k] and y [m, n] in f16 or bf16; weight [n, k / 2] bytes of
  * two e2m1 elements, the even column in the low four bits; exponents u8 [n, k / 32]: W[n, k] = element * 2^(exponent - 127) in
  * the type of x, 255 = NaN. f32 sums, one rounding at the end. k a multiple of 32; rows of x and of the weight 16-byte
- * aligned. ldw and lde are in bytes. */
+ * aligned. ldw and lde are in bytes. Where the product has few tiles, K is divided over workgroups whose f32 sums a second
+ * kernel adds in order through the workspace (intent_hip_linear_mxfp4_workspace_bytes bytes, 16-byte aligned; 0 elsewhere). */
+int intent_hip_linear_mxfp4_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t *bytes);
 int intent_hip_linear_mxfp4(int dtype, const void *x, const uint8_t *weight, const uint8_t *exponents, void *y, int64_t m,
-                            int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t lde, int64_t ldy, void *stream);
+                            int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t lde, int64_t ldy, void *workspace,
+                            size_t workspace_bytes, void *stream);
 
 /* Measurement probe (no counterpart in the reference): the box's own MFMA ceiling, reported by the
  * benchmark beside the published peak, as the measurement protocol asks for an MFMA

@@ -56,7 +56,7 @@ int spmm_resources(int64_t features, IntentHipKernelResources *out);
 int norm_rope_resources(int dtype, int backward, int64_t d, int64_t pairs, int interleaved, uint64_t mix,
                         IntentHipKernelResources *out);
 int paged_cache_resources(int dtype, int reading, int64_t rows, int64_t width, IntentHipKernelResources *out);
-int linear_mxfp4_resources(int dtype, int64_t m, IntentHipKernelResources *out);
+int linear_mxfp4_resources(int dtype, int64_t m, int64_t n, int64_t k, IntentHipKernelResources *out);
 int mx_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t positions,
                         IntentHipKernelResources *out);
 

@@ -118,7 +118,8 @@ SIGNATURES = {
     "intent_hip_paged_cache_read": (_int, (_int, *[_p] * 9, *[_i64] * 8, ctypes.POINTER(_i64), _p)),
     "intent_hip_paged_gqa_decode_mx_workspace_bytes": (_int, (*[_i64] * 7, ctypes.POINTER(_sz))),
     "intent_hip_paged_gqa_decode_mx": (_int, (_int, *[_p] * 9, *[_i64] * 8, ctypes.POINTER(_i64), _f32, _p, _sz, _p)),
-    "intent_hip_linear_mxfp4": (_int, (_int, *[_p] * 4, *[_i64] * 7, _p)),
+    "intent_hip_linear_mxfp4_workspace_bytes": (_int, (_i64, _i64, _i64, ctypes.POINTER(_sz))),
+    "intent_hip_linear_mxfp4": (_int, (_int, *[_p] * 4, *[_i64] * 7, _p, _sz, _p)),
     "intent_hip_mfma_probe": (_int, (_int, _int, _i64, _i64, _p, _p)),
 }
 

@@ -948,6 +948,12 @@ def _csr_spmm(lib, bound, constexprs, device):
                   lambda: lib.kernel_resources(OP_CSR_SPMM_F32, F32, rows, features))
 
 
+def _no_static(name, use):
+    if _static_workspace():
+        raise CompilationStageError("provider_preparation", f"{name} {use} a workspace; backend_options workspace='static' has "
+                                    "none for it, use workspace='prepare'")
+
+
 # ------------------------------------------------------------------------------ norm and rotation of heads
 def _interleaved(constexprs) -> int:
     value = constexprs["INTERLEAVED"]
@@ -1007,10 +1013,7 @@ def _norm_rope_backward(dtype_code):
         (q, k, q_weight, k_weight, positions, cos, sin, grad_q_out, grad_k_out, grad_q, grad_k, grad_q_weight, grad_k_weight,
          eps) = bound.arguments
         interleaved = _interleaved(constexprs)
-        if _static_workspace():
-            raise CompilationStageError(
-                "provider_preparation", "qk_norm_rope_backward sums the weights' gradients through a workspace; "
-                "backend_options workspace='static' has none for it, use workspace='prepare'")
+        _no_static("qk_norm_rope_backward", "sums the weights' gradients through")
         keep, before, after = list(bound.arguments[:13]), [], []
         views, extents = _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, before)
         grads = [_readable(t, keep, before) for t in (grad_q_out, grad_k_out)]
@@ -1162,6 +1165,8 @@ def _decode_mx_signature(element):
 def _linear_mxfp4(dtype_code):
     """linear_mxfp4: x is staged where its layout is not the kernel's; a weight never is."""
     def plan(lib, bound, constexprs, device):
+        import ctypes
+
         x, weight, exponents, out = bound.arguments
         (m, k), n = x.shape, weight.shape[0]
         if k % _MX_BLOCK or weight.shape[1] * 2 != k or exponents.shape[1] * _MX_BLOCK != k:
@@ -1176,8 +1181,16 @@ def _linear_mxfp4(dtype_code):
         fn = lib.fn["linear_mxfp4"]
         args = (dtype_code, xk.data_ptr(), weight.data_ptr(), exponents.data_ptr(), outk.data_ptr(), m, n, k,
                 *(_outer_strides(t)[0] for t in (xk, weight, exponents, outk)))
-        return Launch("intent_hip_linear_mxfp4", lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
-                      (("m", m), ("n", n), ("k", k)), lambda: lib.kernel_resources(OP_LINEAR_MXFP4, dtype_code, m, n))
+        size = ctypes.c_size_t(0)
+        lib.check(lib.fn["linear_mxfp4_workspace_bytes"](m, n, k, ctypes.byref(size)), "provider_preparation")
+        if size.value:
+            _no_static("linear_mxfp4", "divides K of few tiles over workgroups whose sums meet in")
+            run = _workspace_run(fn, args, size.value, device, keep)
+        else:
+            run = lambda stream: fn(*args, None, 0, stream)  # noqa: E731
+        return Launch("intent_hip_linear_mxfp4", run, tuple(keep), tuple(before), tuple(after),
+                      (("m", m), ("n", n), ("k", k), ("workspace_bytes", size.value)),
+                      lambda: lib.call_resources(OP_LINEAR_MXFP4, dtype_code, m, n, k))
     return plan
 
 

@@ -159,3 +159,7 @@ def test_refusals(device):
         run.run(x, weight, torch.zeros((2, 8), dtype=torch.uint8, device=device).t())
     with pytest.raises(ValueError):
         run.run(x, weight, exponents[:7])
+    static = intent.jit(linear_mxfp4.linear_mxfp4_f16, backend="hip", backend_options={"workspace": "static"})
+    static.run(x, weight, exponents)
+    with pytest.raises(intent.CompilationStageError, match="workspace"):
+        static.run(*(a.to(device) for a in case(2, "f16", 100, 64, 4096)))

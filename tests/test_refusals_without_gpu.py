@@ -114,8 +114,9 @@ def test_linear_mxfp4():
     lib = hiplib.library()
     err = lambda: lib.fn["last_error"]()  # noqa: E731
 
-    def call(dtype=F16, x=16, w=16, y=16, m=4, n=8, k=64, ldx=64, ldw=32, lde=2, ldy=8):
-        return lib.fn["linear_mxfp4"](dtype, x, w, 16, y, m, n, k, ldx, ldw, lde, ldy, None)
+    def call(dtype=F16, x=16, w=16, y=16, m=4, n=8, k=64, ldx=64, ldw=32, lde=2, ldy=8, workspace=None,
+             size=0):
+        return lib.fn["linear_mxfp4"](dtype, x, w, 16, y, m, n, k, ldx, ldw, lde, ldy, workspace, size, None)
 
     assert call(dtype=hiplib.F32) == 1 and b"F16 or BF16" in err()
     assert call(m=-1) == 1 and call(ldw=-32) == 1 and b"negative" in err()
@@ -125,3 +126,10 @@ def test_linear_mxfp4():
     assert call(w=24) == 2 and call(ldw=40) == 2 and b"weight rows" in err()
     assert call(m=2 ** 21) == 2 and call(n=2 ** 30) == 2
     assert call(m=0, x=None) == 0 and call(n=0) == 0
+    size = ctypes.c_size_t(0)
+    query = lib.fn["linear_mxfp4_workspace_bytes"]
+    assert query(1, 14336, 4096, ctypes.byref(size)) == 0 and size.value == 0
+    assert query(100, 64, 4096, ctypes.byref(size)) == 0 and size.value % (100 * 64 * 4) == 0 and size.value > 0
+    assert call(m=100, n=64, k=4096, ldx=4096, ldw=2048, lde=128, ldy=64) == 5 and b"workspace" in err()
+    assert call(m=100, n=64, k=4096, ldx=4096, ldw=2048, lde=128, ldy=64, workspace=256, size=size.value - 1) == 5
+    assert query(4, 8, 48, ctypes.byref(size)) == 2 and query(4, 8, 64, None) == 1
