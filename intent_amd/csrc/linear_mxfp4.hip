@@ -6,12 +6,16 @@
 // Design. v_mfma_f32_16x16x32 with 16 weight rows as rows and 16 rows of x as columns. The sum over K may run in any order,
 // so lane (r, g) takes block g of four of weight row r as it lies in memory (16 bytes, one exponent), converts it in four
 // parts, and reads the same 32 values of its row of x. Weights go from memory to registers: no wave needs another's.
-//   * linear_few, up to 16 rows of x: a workgroup's waves take 128 columns of K in turn and add their sums through the LDS.
-//     Bound by the weights' bytes.
+//   * linear_few, up to 16 rows of x: a workgroup's 16 waves take a run of K each and add their sums through the LDS. Bound by
+//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 9.9 us, 3.2 TB/s; without x and the
+//     exponents' loads 6.7; 1 x 4096 x 4096: 5.0, most of it latency: one or two steps a wave).
 //   * linear_tiles: a workgroup's waves share 16 MT rows of x, which pass through the LDS 128 columns at a time (in 16-byte
 //     units, unit u of row r at u ^ r % 16, so that the 16 rows of a read are in different banks), and take 16 NT weight
 //     rows each. A lane's weight rows are NT apart, so its results are 4 NT consecutive columns of y. Where tiles are few, K
-//     is divided over workgroups, whose f32 sums a second kernel adds in order.
+//     is divided over workgroups, whose f32 sums a second kernel adds in order. The small tiles are bound by the latency of a
+//     stage and by x's way to the LDS, so they keep four stages on their way (32 x 4096 x 14336: 22 -> 16.7 us; 256 x 4096 x
+//     4096: 40 -> 23); the large ones by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 107 us, 1120
+//     TFLOP/s; three stages, and so one workgroup a CU, 174).
 #include <stdio.h>
 
 #include <type_traits>
@@ -21,7 +25,7 @@
 namespace intent_hip {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kFewWaves = 16;
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -87,64 +91,105 @@ __device__ __forceinline__ void store(const Linear &p, int m, int n, const float
   }
 }
 
-// Up to 16 rows of x: 16 weight rows a workgroup of W waves.
-template <typename E, int W>
-__global__ __launch_bounds__(W *kWave) void linear_few(Linear p) {
-  constexpr int kAhead = 4;            // steps on their way at once
-  __shared__ float sums[W][4][kWave];
+// Up to 16 rows of x by 16 NT weight rows a workgroup; its 16 waves take a run of K each. The loads of kAhead steps of 128
+// columns are on their way at once, a weight row's exponents for all of them in one. Columns of the product behind the rows of
+// x are never stored, so their lanes read any row.
+template <typename E, int NT>
+__global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
+  constexpr int kAhead = 2, kSums = NT * 4;
+  __shared__ float sums[kFewWaves][kSums][kWave];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = static_cast<int>(blockIdx.x) * 16;
-  const int64_t row = min(n0 + r, p.n - 1);                    // rows behind the last are not stored
-  const uint8_t *w = p.w + row * p.ldw, *e = p.e + row * p.lde;
-  const bool live = r < p.m;
-  const uint16_t *x = p.x + (live ? r : 0) * p.ldx;
-  f32x4_t acc = {0, 0, 0, 0};
-  for (int b0 = wave * 4; b0 < p.blocks; b0 += W * 4 * kAhead) {
-    uint4 raw[kAhead], v[kAhead][4];
-    uint8_t power[kAhead];
+  const int n0 = static_cast<int>(blockIdx.x) * 16 * NT;
+  const uint8_t *w[NT], *e[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t row = min(n0 + r * NT + j, p.n - 1);         // rows behind the last are not stored
+    w[j] = p.w + row * p.ldw + g * 16;
+    e[j] = p.e + row * p.lde;
+  }
+  const uint16_t *x = p.x + min(r, p.m - 1) * p.ldx + g * 32;
+  f32x4_t acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4_t{0, 0, 0, 0};
+  const int first = min(wave * p.stages * 4, p.blocks), last = min(first + p.stages * 4, p.blocks);
+  for (int b0 = first; b0 < last; b0 += kAhead * 4) {
+    uint4 raw[kAhead][NT], v[kAhead][4];
+    uint32_t power[NT][kAhead];        // of step i: word i
+    const bool whole = b0 + kAhead * 4 <= last;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int b = b0 + i * W * 4 + g;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      power[i] = 127;
-      if (b < p.blocks) {
-        raw[i] = *reinterpret_cast<const uint4 *>(w + b * 16);
-        power[i] = e[b];
+      const int b = b0 + i * 4;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        raw[i][j] = make_uint4(0, 0, 0, 0);
+        if (whole || b + g < last) raw[i][j] = *reinterpret_cast<const uint4 *>(w[j] + b * 16);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         v[i][c] = make_uint4(0, 0, 0, 0);
-        if (live && b < p.blocks) v[i][c] = *reinterpret_cast<const uint4 *>(x + b * 32 + c * 8);
+        if (whole || b + g < last) v[i][c] = *reinterpret_cast<const uint4 *>(x + b * 32 + c * 8);
       }
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      const float scale = mx_scale(power[i]);
+    for (int j = 0; j < NT; ++j) {
+      if (whole) {
+        __builtin_memcpy(power[j], e[j] + b0, sizeof(power[j]));
+      } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc = mfma<E>(eight<E>(words[c], scale), v[i][c], acc);
+        for (int i = 0; i < kAhead; ++i) {
+          power[j][i] = 0x7F7F7F7Fu;
+          if (b0 + i * 4 + g < last) power[j][i] = static_cast<uint32_t>(e[j][b0 + i * 4 + g]) << (8 * g);
+        }
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint32_t words[4] = {raw[i][j].x, raw[i][j].y, raw[i][j].z, raw[i][j].w};
+        const float scale = mx_scale(power[j][i] >> (8 * g) & 0xFF);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[j] = mfma<E>(eight<E>(words[c], scale), v[i][c], acc[j]);
+      }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sums[wave][i][lane] = acc[i];
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[wave][i * NT + j][lane] = acc[j][i];
   __syncthreads();
-  if (wave != 0) return;
-  float total[4] = {};
+  if (wave >= kSums || r >= p.m) return;
+  float total = 0.0f;
 #pragma unroll
-  for (int j = 0; j < W; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) total[i] += sums[j][i][lane];
-  store<E>(p, r, n0 + g * 4, total);
+  for (int i = 0; i < kFewWaves; ++i) total += sums[i][wave][lane];
+  const int n = n0 + g * kSums + wave;
+  if (n < p.n) p.y[r * p.ldy + n] = from_f32<E>(total).bits;
 }
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 
-// 16 MT rows of x by 64 NT weight rows a workgroup.
-template <typename E, int MT, int NT>
-__global__ __launch_bounds__(kWaves *kWave) void linear_tiles(Linear p) {
+// s_waitcnt with only the vector-memory counter constrained (vmcnt <= n).
+#define INTENT_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt((((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4) | (0xF << 8)))
+
+// s_barrier with an acquire fence alone: a release fence would wait for every load into the LDS that is on its way.
+__device__ __forceinline__ void stage_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// What is read of x behind K.
+__device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
+
+// 16 MT rows of x by 64 NT weight rows a workgroup; S stages of 128 columns are on their way or in use. Each has an LDS array
+// of its own, and the loop is unrolled by S: the compiler then knows which loads into the LDS a read has to wait for.
+template <typename E, int MT, int NT, int S>
+__global__ __launch_bounds__(kWaves *kWave, 2) void linear_tiles(Linear p) {
   constexpr int kRows = 16 * MT, kUnits = kRows * 16, kLoads = kUnits / (kWaves * kWave);     // 16-byte units of a stage
-  __shared__ uint4 x_s[2 * kUnits];
+  constexpr int kIssued = kLoads + 2 * NT;             // loads of a wave per stage, always as many
+  static_assert(S >= 2 && S <= 4, "one LDS array per stage");
+  __shared__ uint4 x_0[kUnits], x_1[kUnits], x_2[S > 2 ? kUnits : 1], x_3[S > 3 ? kUnits : 1];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = p.m_tiles * p.n_tiles;
@@ -153,33 +198,14 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_tiles(Linear p) {
   const int part = tile / tiles;
   tile -= part * tiles;
   const int m0 = tile % p.m_tiles * kRows, n0 = (tile / p.m_tiles * kWaves + wave) * 16 * NT;
-  const int first = part * p.stages * 4, last = min(p.blocks, first + p.stages * 4);     // blocks of K of this part
-  // Units of x that this thread brings in: unit u of LDS row (u / 16) comes from unit (u % 16) ^ (row % 16) of x's row.
+  const int first = min(part * p.stages * 4, p.blocks), last = min(p.blocks, first + p.stages * 4);     // blocks of K of this part
+  const int stages = (last - first + 3) / 4;
+  // Units of x that this thread brings in: row i * 16 + own, unit `unit` of it into place unit ^ own of its LDS row.
+  const int own_row = wave * 4 + g, unit = r ^ own_row;
   const uint16_t *from[kLoads];
-  int unit[kLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int at = (i * kWaves + wave) * kWave + lane, row = at / 16;
-    unit[i] = (at ^ row) & 15;
-    from[i] = p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx + unit[i] * 8;       // rows behind the last are not stored
-  }
-  const auto bring = [&](int b, int to) {
-    uint4 *stage = x_s + to * kUnits;
-    if (b + 4 <= last) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const uint16_t *src = from[i] + static_cast<int64_t>(b) * 32;
-        __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * kWaves + wave) * kWave), 16, 0, 0);
-      }
-    } else {                           // K ends inside the stage: zeros behind it
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (b + unit[i] / 4 < last) v = *reinterpret_cast<const uint4 *>(from[i] + static_cast<int64_t>(b) * 32);
-        stage[(i * kWaves + wave) * kWave + lane] = v;
-      }
-    }
-  };
+  for (int i = 0; i < kLoads; ++i)                     // rows behind the last are not stored
+    from[i] = p.x + static_cast<int64_t>(min(m0 + i * 16 + own_row, p.m - 1)) * p.ldx + unit * 8;
   const uint8_t *w[NT], *e[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -187,18 +213,31 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_tiles(Linear p) {
     w[j] = p.w + row * p.ldw;
     e[j] = p.e + row * p.lde;
   }
-  uint4 raw[NT];
-  uint8_t power[NT];
-  const auto fetch = [&](int b0) {
-    const int b = b0 + g;
+  uint4 raw[S][NT];
+  uint8_t power[S][NT];
+  const auto array = [&](int u) -> uint4 * { return u == 0 ? x_0 : u == 1 ? x_1 : u == 2 ? x_2 : x_3; };
+  const auto issue = [&](int t, int u) {               // stage t (the last again behind it) into set u
+    const int b0 = first + min(t, stages - 1) * 4;
+    uint4 *stage = array(u);
+    if (b0 + 4 <= last) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint16_t *src = from[i] + static_cast<int64_t>(b0) * 32;
+        __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * kWaves + wave) * kWave), 16, 0, 0);
+      }
+    } else {                                           // K ends inside the stage: zeros behind it
+      const uint16_t *zero = reinterpret_cast<const uint16_t *>(&kZeroUnit);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint16_t *src = b0 + unit / 4 < last ? from[i] + static_cast<int64_t>(b0) * 32 : zero;
+        __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * kWaves + wave) * kWave), 16, 0, 0);
+      }
+    }
+    const int b = min(b0 + g, last - 1);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      raw[j] = make_uint4(0, 0, 0, 0);
-      power[j] = 127;
-      if (b < last) {
-        raw[j] = *reinterpret_cast<const uint4 *>(w[j] + b * 16);
-        power[j] = e[j][b];
-      }
+      raw[u][j] = *reinterpret_cast<const uint4 *>(w[j] + static_cast<int64_t>(b) * 16);
+      power[u][j] = e[j][b];
     }
   };
   f32x4_t acc[MT][NT];
@@ -206,32 +245,39 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_tiles(Linear p) {
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
-  if (first < last) {
-    bring(first, 0);
-    fetch(first);
-  }
-  for (int b0 = first, at = 0; b0 < last; b0 += 4, at ^= 1) {
-    uint4 own[NT];
-    float scale[NT];
-    __syncthreads();                   // this stage has come, and nobody reads the other
+  if (stages > 0) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) own[j] = raw[j], scale[j] = mx_scale(power[j]);
-    if (b0 + 4 < last) {
-      bring(b0 + 4, at ^ 1);
-      fetch(b0 + 4);
+    for (int u = 0; u < S - 1; ++u) issue(u, u);
+    for (int t0 = 0; t0 < stages; t0 += S) {
+#pragma unroll
+      for (int u = 0; u < S; ++u) {
+        if (t0 + u >= stages) break;
+        INTENT_WAIT_VMCNT((S - 2) * kIssued);          // this wave's loads of the stage have come
+        stage_barrier();                               // everybody's have, and nobody reads the set that is filled next
+        issue(t0 + u + S - 1, (u + S - 1) % S);
+        const bool held = first + (t0 + u) * 4 + g < last;
+        uint4 own[NT];
+        float scale[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          own[j] = held ? raw[u][j] : make_uint4(0, 0, 0, 0);
+          scale[j] = mx_scale(held ? power[u][j] : 127);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint4 v[MT], a[NT];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) v[i] = array(u)[(i * 16 + r) * 16 + ((g * 4 + c) ^ r)];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) a[j] = eight<E>(c == 0 ? own[j].x : c == 1 ? own[j].y : c == 2 ? own[j].z : own[j].w, scale[j]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = mfma<E>(a[j], v[i], acc[i][j]);
+        }
+      }
     }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint4 v[MT], a[NT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) v[i] = x_s[at * kUnits + (i * 16 + r) * 16 + ((g * 4 + c) ^ r)];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) a[j] = eight<E>(c == 0 ? own[j].x : c == 1 ? own[j].y : c == 2 ? own[j].z : own[j].w, scale[j]);
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mfma<E>(a[j], v[i], acc[i][j]);
-    }
+    INTENT_WAIT_VMCNT(0);                              // nothing is on its way into the LDS of an ended workgroup
   }
   // A lane's results: row m0 + 16 i + r of y, columns n0 + (4 g + k) NT + j.
 #pragma unroll
@@ -246,87 +292,112 @@ __global__ __launch_bounds__(kWaves *kWave) void linear_tiles(Linear p) {
       store<E>(p, m, n, row);
     } else if (m < p.m) {
       float *to = p.sums + (static_cast<int64_t>(part) * p.m + m) * p.n + n;
+      if (p.wide > 1) {
 #pragma unroll
-      for (int k = 0; k < 4 * NT; ++k)
-        if (n + k < p.n) to[k] = row[k];
+        for (int k = 0; k < 4 * NT; k += 4)
+          if (n + k < p.n) *reinterpret_cast<float4 *>(to + k) = make_float4(row[k], row[k + 1], row[k + 2], row[k + 3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4 * NT; ++k)
+          if (n + k < p.n) to[k] = row[k];
+      }
     }
   }
 }
 
-// y from the parts' sums, in order.
-template <typename E>
+// y from the parts' sums, in order: kCount columns a thread.
+template <typename E, int kCount>
 __global__ __launch_bounds__(256) void linear_fold(Linear p) {
-  const int64_t all = static_cast<int64_t>(p.m) * p.n, at = static_cast<int64_t>(grid_block()) * 256 + threadIdx.x;
+  const int64_t all = static_cast<int64_t>(p.m) * p.n, at = (static_cast<int64_t>(grid_block()) * 256 + threadIdx.x) * kCount;
   if (at >= all) return;
-  float total = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < p.parts; ++i) total += p.sums[i * all + at];
+  typedef float held_t __attribute__((ext_vector_type(kCount)));
+  held_t total = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < p.parts; ++i) total += *reinterpret_cast<const held_t *>(p.sums + i * all + at);
   const int64_t m = at / p.n;
-  p.y[m * p.ldy + (at - m * p.n)] = from_f32<E>(total).bits;
+  uint16_t *y = p.y + m * p.ldy + (at - m * p.n);
+  if constexpr (kCount == 4)
+    *reinterpret_cast<uint2 *>(y) = make_uint2(from_f32<E>(total[0]).bits | static_cast<uint32_t>(from_f32<E>(total[1]).bits) << 16,
+                                               from_f32<E>(total[2]).bits | static_cast<uint32_t>(from_f32<E>(total[3]).bits) << 16);
+  else
+    *y = from_f32<E>(total[0]).bits;
 }
 
 // How a product is cut.
 struct Cut {
-  int mt, nt, waves, parts;            // mt = 0: linear_few with `waves` waves
+  int mt, nt, parts;                   // mt = 0: linear_few
 };
+
+// linear_few for up to 16 rows, NT by the weight rows there are for the workgroups (16 x 14336 x 4096: NT = 1 23.8 us, 2 16.9,
+// 4 12.7; 1 x 4096 x 14336: 10.7, 15.7, 25.8). Where more than eight rows meet a long K and few weight rows, x read once per
+// 16 weight rows costs more than the weights (16 x 4096 x 14336: 19.8 us, in tiles 15.5; 16 x 512 x 7168: 10.3, 7.9).
+// linear_tiles otherwise, by an estimate from what its tiles measured: us a stage takes a workgroup that has a CU for itself,
+// and each of several on a CU, and what writing, reading and adding the parts' sums takes. It is within a fifth of the best of
+// all tiles and parts at M of 17 to 1021 and N x K of 1000 x 4096 to 28672 x 8192.
 Cut cut(int64_t m, int64_t n, int64_t k) {
-  if (m <= 16) return {0, 1, n >= 16 * 16 * device_cus() / 8 ? 4 : n >= 16 * device_cus() ? 8 : 16, 1};
-  const auto tiles = [&](int mt, int nt) { return ((m + 16 * mt - 1) / (16 * mt)) * ((n + 64 * nt - 1) / (64 * nt)); };
-  Cut c{8, 4, 4, 1};
-  if (m <= 32) c.mt = 2, c.nt = 1;
-  else if (m <= 64) c.mt = 4, c.nt = 2;
-  else if (tiles(8, 4) < 3 * device_cus() / 4) c.nt = 2;
-  const int64_t stages = (k + 127) / 128, own = tiles(c.mt, c.nt), wanted = 2 * device_cus() / (own > 0 ? own : 1);
-  c.parts = static_cast<int>(wanted < 1 ? 1 : wanted > stages / 4 ? (stages / 4 < 1 ? 1 : stages / 4) : wanted);
-  return c;
+  const int cus = device_cus();
+  if (m <= 16 && (m <= 8 || n >= 24 * cus || k < 6144)) return {0, n >= 48 * cus ? 4 : n >= 24 * cus ? 2 : 1, 1};
+  constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.47f, 0.32f}, {4, 2, 0.9f, 0.7f}, {8, 2, 1.3f, 0.9f}, {8, 4, 2.1f, 1.67f}};
+  const int64_t stages = (k + 127) / 128;
+  Cut best{};
+  float least = 0.0f;
+  for (const auto &kind : kKinds) {
+    const int64_t tiles = ((m + 16 * kind.mt - 1) / (16 * kind.mt)) * ((n + 64 * kind.nt - 1) / (64 * kind.nt));
+    for (int parts = 1; parts <= 16 && (parts == 1 || parts * 4 <= stages); ++parts) {
+      const float on_one = static_cast<float>((tiles * parts + cus - 1) / cus), shared = kind.shared * on_one;
+      float us = static_cast<float>((stages + parts - 1) / parts) * (kind.alone > shared ? kind.alone : shared);
+      if (parts > 1) us += 3.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(n) * 2.3e-6f;
+      if (best.mt == 0 || us < least) best = {kind.mt, kind.nt, parts}, least = us;
+    }
+  }
+  return best;
+}
+
+// f with the kernel of a cut, its name and its waves.
+template <typename E, typename F>
+int with_kernel(const Cut &c, F f) {
+  if (c.mt == 0)
+    return c.nt == 1   ? f(linear_few<E, 1>, "linear_few", kFewWaves)
+           : c.nt == 2 ? f(linear_few<E, 2>, "linear_few", kFewWaves)
+                       : f(linear_few<E, 4>, "linear_few", kFewWaves);
+  return c.mt == 2   ? f(linear_tiles<E, 2, 1, 4>, "linear_tiles", kWaves)
+         : c.mt == 4 ? f(linear_tiles<E, 4, 2, 4>, "linear_tiles", kWaves)
+         : c.nt == 2 ? f(linear_tiles<E, 8, 2, 2>, "linear_tiles", kWaves)
+                     : f(linear_tiles<E, 8, 4, 2>, "linear_tiles", kWaves);
 }
 
 template <typename E>
 void launch(Linear p, const Cut &c, hipStream_t s) {
-  if (c.mt == 0) {
-    const dim3 grid(static_cast<unsigned>((p.n + 15) / 16));
-    if (c.waves == 4)
-      linear_few<E, 4><<<grid, 4 * kWave, 0, s>>>(p);
-    else if (c.waves == 8)
-      linear_few<E, 8><<<grid, 8 * kWave, 0, s>>>(p);
-    else
-      linear_few<E, 16><<<grid, 16 * kWave, 0, s>>>(p);
-    return;
-  }
-  p.m_tiles = (p.m + 16 * c.mt - 1) / (16 * c.mt), p.n_tiles = (p.n + 64 * c.nt - 1) / (64 * c.nt), p.parts = c.parts;
-  p.stages = ((p.blocks + 3) / 4 + c.parts - 1) / c.parts;
-  const dim3 grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.parts, 1);
-  if (c.mt == 2)
-    linear_tiles<E, 2, 1><<<grid, kWaves * kWave, 0, s>>>(p);
-  else if (c.mt == 4)
-    linear_tiles<E, 4, 2><<<grid, kWaves * kWave, 0, s>>>(p);
-  else if (c.nt == 2)
-    linear_tiles<E, 8, 2><<<grid, kWaves * kWave, 0, s>>>(p);
+  p.parts = c.parts;
+  with_kernel<E>(c, [&](void (*kernel)(Linear), const char *, int waves) {
+    const int runs = c.mt == 0 ? waves : c.parts;
+    p.stages = ((p.blocks + 3) / 4 + runs - 1) / runs;
+    dim3 grid(static_cast<unsigned>((p.n + 16 * c.nt - 1) / (16 * c.nt)));
+    if (c.mt > 0) {
+      p.m_tiles = (p.m + 16 * c.mt - 1) / (16 * c.mt), p.n_tiles = (p.n + 64 * c.nt - 1) / (64 * c.nt);
+      grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.parts, 1);
+    }
+    kernel<<<grid, waves * kWave, 0, s>>>(p);
+    return 0;
+  });
+  if (c.parts == 1) return;
+  const int64_t all = static_cast<int64_t>(p.m) * p.n;
+  if (p.wide > 1)
+    linear_fold<E, 4><<<tile_grid((all / 4 + 255) / 256, 1), 256, 0, s>>>(p);
   else
-    linear_tiles<E, 8, 4><<<grid, kWaves * kWave, 0, s>>>(p);
-  if (c.parts > 1) linear_fold<E><<<tile_grid((static_cast<int64_t>(p.m) * p.n + 255) / 256, 1), 256, 0, s>>>(p);
+    linear_fold<E, 1><<<tile_grid((all + 255) / 256, 1), 256, 0, s>>>(p);
 }
 
 }  // namespace
 
 int linear_mxfp4_resources(int dtype, int64_t m, int64_t n, int64_t k, IntentHipKernelResources *out) {
   const Cut c = cut(m, n, k);
-  char name[64];
-  const auto describe = [&](const void *half, const void *brain, int waves) {
-    return describe_kernel(dtype == INTENT_HIP_F16 ? half : brain, name, waves * kWave, out);
+  const auto describe = [&](void (*kernel)(Linear), const char *which, int waves) {
+    char name[64];
+    snprintf(name, sizeof(name), "%s<%s,%d,%d>", which, dtype == INTENT_HIP_F16 ? "f16" : "bf16", c.mt, c.nt);
+    return describe_kernel(reinterpret_cast<const void *>(kernel), name, waves * kWave, out);
   };
-  const char *const type = dtype == INTENT_HIP_F16 ? "f16" : "bf16";
-  if (c.mt == 0) {
-    snprintf(name, sizeof(name), "linear_few<%s,%d>", type, c.waves);
-    return c.waves == 4   ? describe(reinterpret_cast<const void *>(linear_few<f16_t, 4>), reinterpret_cast<const void *>(linear_few<bf16_t, 4>), 4)
-           : c.waves == 8 ? describe(reinterpret_cast<const void *>(linear_few<f16_t, 8>), reinterpret_cast<const void *>(linear_few<bf16_t, 8>), 8)
-                          : describe(reinterpret_cast<const void *>(linear_few<f16_t, 16>), reinterpret_cast<const void *>(linear_few<bf16_t, 16>), 16);
-  }
-  snprintf(name, sizeof(name), "linear_tiles<%s,%d,%d>", type, c.mt, c.nt);
-  return c.mt == 2   ? describe(reinterpret_cast<const void *>(linear_tiles<f16_t, 2, 1>), reinterpret_cast<const void *>(linear_tiles<bf16_t, 2, 1>), kWaves)
-         : c.mt == 4 ? describe(reinterpret_cast<const void *>(linear_tiles<f16_t, 4, 2>), reinterpret_cast<const void *>(linear_tiles<bf16_t, 4, 2>), kWaves)
-         : c.nt == 2 ? describe(reinterpret_cast<const void *>(linear_tiles<f16_t, 8, 2>), reinterpret_cast<const void *>(linear_tiles<bf16_t, 8, 2>), kWaves)
-                     : describe(reinterpret_cast<const void *>(linear_tiles<f16_t, 8, 4>), reinterpret_cast<const void *>(linear_tiles<bf16_t, 8, 4>), kWaves);
+  return dtype == INTENT_HIP_F16 ? with_kernel<f16_t>(c, describe) : with_kernel<bf16_t>(c, describe);
 }
 
 }  // namespace intent_hip

@@ -50,6 +50,15 @@ def test_matches_plain_form(device, dtype, m, n, k):
     check(kernel(dtype).run(x.to(device), weight.to(device), exponents.to(device)), x, weight, exponents, dtype)
 
 
+@pytest.mark.parametrize("m,n,k", [(9, 70, 6176), (16, 6152, 160), (16, 12296, 96), (40, 8200, 2080), (161, 2058, 6176),
+                                   (250, 4100, 3840), (513, 4128, 96), (1500, 14000, 96), (700, 8190, 1184)])
+def test_every_tile(device, m, n, k):
+    """Sizes that each take another kernel, tile or division of K, whose last stage, row and column tiles are partial."""
+    announce("linear mxfp4 tile", m, n, k)
+    x, weight, exponents = case(m + n + k, "bf16", m, n, k)
+    check(kernel("bf16").run(x.to(device), weight.to(device), exponents.to(device)), x, weight, exponents, "bf16")
+
+
 @pytest.mark.parametrize("m", [1, 40, 150])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_every_element_and_exponent(device, dtype, m):
