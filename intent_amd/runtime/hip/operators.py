@@ -1137,7 +1137,8 @@ def _paged_decode_mx(dtype_code):
         return Launch("intent_hip_paged_gqa_decode_mx", run, tuple(keep), tuple(before), tuple(after),
                       (("batch", batch), ("q_heads", q_heads), ("kv_heads", kv_heads), ("d", d), ("pages", pages), ("ps", ps),
                        ("positions", page_indices.shape[0]), ("workspace_bytes", size.value)),
-                      lambda: lib.kernel_resources(OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4, dtype_code, group, d))
+                      lambda: lib.call_resources(OP_PAGED_GQA_DECODE_MX, dtype_code, batch, kv_heads, group, d, ps,
+                                                 page_indices.shape[0]))
     return plan
 
 
