@@ -76,6 +76,9 @@ class Launch:
     configuration: tuple = ()
     resources: Callable[[], dict | None] = field(default=lambda: None)
     candidates: tuple = ()        # (row, eligible, reasons) of the definition's tuning family, table order
+    # The launch of other arguments of the same layout (shapes, strides, types, alignment to 16 bytes), in declaration order;
+    # holds no tensor. None where a plan has to look at its arguments again.
+    again: Callable[[tuple], "Launch"] | None = None
 
 
 @dataclass(frozen=True)
@@ -258,6 +261,21 @@ def _workspace_run(fn, args, size, device, keep):
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         return fn(*args, workspace.data_ptr(), size, stream)
     return run
+
+
+def _optional_workspace_run(fn, args, size, device, keep):
+    return _workspace_run(fn, args, size, device, keep) if size else lambda stream: fn(*args, None, 0, stream)
+
+
+def _staged(again, values, bound, before, after):
+    """The launch of `values`, which hold staged views where `before` and `after` copy them: such a launch is planned anew for
+    other arguments."""
+    launch = again(values)
+    if before or after:
+        launch.keep, launch.before, launch.after = (*launch.keep, bound.arguments), tuple(before), tuple(after)
+    else:
+        launch.again = again
+    return launch
 
 
 # ------------------------------------------------------------------------------ attention head dimensions
@@ -962,16 +980,22 @@ def _interleaved(constexprs) -> int:
     return int(value)
 
 
-def _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, before):
-    """The views as the kernels read them, and the extents (tokens, q_heads, kv_heads, d, table, pairs)."""
-    tokens, q_heads, d = q.shape
-    table, pairs = cos.shape
+def _norm_rope_staged(arguments, extents, outputs):
+    """(the arguments with the views that the kernels take in place of those they do not, what is copied before and after)"""
+    tokens, _, _, d, table, pairs = extents
     if 2 * pairs > d:
         raise ValueError(f"{pairs} rotated pairs do not fit heads of width {d}")
     if pairs and not table and tokens:
         raise ValueError("the rotation tables hold no position")
-    views = [_readable(t, keep, before) for t in (q, k, q_weight, k_weight, positions, cos, sin)]
-    return views, (tokens, q_heads, k.shape[1], d, table, pairs)
+    keep, before, after = [], [], []
+    last = len(arguments) - 1
+    values = [_readable(t, keep, before) for t in arguments[:last - outputs]]
+    values += [_writable(t, keep, after) for t in arguments[last - outputs:last]]
+    return (*values, arguments[last]), before, after
+
+
+def _norm_rope_extents(q, k, cos) -> tuple:
+    return (q.shape[0], q.shape[1], k.shape[1], q.shape[2], *cos.shape)
 
 
 def _mixed(*views) -> int:
@@ -985,23 +1009,25 @@ def _mixed(*views) -> int:
     return mixed
 
 
+_NORM_ROPE_EXTENTS = ("tokens", "q_heads", "kv_heads", "d", "table", "pairs")
+
+
 def _norm_rope(dtype_code):
     """qk_norm_rope: q and k rows are read through their own strides (a projection's slices), staged only where their
     inner stride is not 1."""
     def plan(lib, bound, constexprs, device):
-        q, k, q_weight, k_weight, positions, cos, sin, q_out, k_out, eps = bound.arguments
         interleaved = _interleaved(constexprs)
-        keep, before, after = list(bound.arguments[:9]), [], []
-        views, extents = _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, before)
-        outs = [_writable(t, keep, after) for t in (q_out, k_out)]
-        strides = _strides(views[0], views[1], views[5], views[6], *outs)
-        keep.append(strides)
-        fn = lib.fn["qk_norm_rope"]
-        args = (dtype_code, *(t.data_ptr() for t in (*views, *outs)), *extents, strides, float(eps), interleaved)
-        return Launch("intent_hip_qk_norm_rope", lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
-                      tuple(zip(("tokens", "q_heads", "kv_heads", "d", "table", "pairs"), extents)),
-                      lambda: lib.call_resources(OP_QK_NORM_ROPE, dtype_code, extents[3], extents[5], interleaved,
-                                                 _mixed(*views[:4], *views[5:], *outs)))
+        extents = _norm_rope_extents(bound.arguments[0], bound.arguments[1], bound.arguments[5])
+        values, before, after = _norm_rope_staged(bound.arguments, extents, 2)
+        strides = _strides(*values[:2], *values[5:9])
+        fn, configuration = lib.fn["qk_norm_rope"], tuple(zip(_NORM_ROPE_EXTENTS, extents))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values[:9]], *extents, strides, float(values[9]), interleaved)
+            return Launch("intent_hip_qk_norm_rope", lambda stream: fn(*args, stream), values, configuration=configuration,
+                          resources=lambda: lib.call_resources(OP_QK_NORM_ROPE, dtype_code, extents[3], extents[5], interleaved,
+                                                               _mixed(*values[:4], *values[5:9])))
+        return _staged(again, values, bound, before, after)
     return plan
 
 
@@ -1010,25 +1036,24 @@ def _norm_rope_backward(dtype_code):
     def plan(lib, bound, constexprs, device):
         import ctypes
 
-        (q, k, q_weight, k_weight, positions, cos, sin, grad_q_out, grad_k_out, grad_q, grad_k, grad_q_weight, grad_k_weight,
-         eps) = bound.arguments
         interleaved = _interleaved(constexprs)
+        extents = _norm_rope_extents(bound.arguments[0], bound.arguments[1], bound.arguments[5])
         _no_static("qk_norm_rope_backward", "sums the weights' gradients through")
-        keep, before, after = list(bound.arguments[:13]), [], []
-        views, extents = _norm_rope_inputs(q, k, q_weight, k_weight, positions, cos, sin, keep, before)
-        grads = [_readable(t, keep, before) for t in (grad_q_out, grad_k_out)]
-        outs = [_writable(t, keep, after) for t in (grad_q, grad_k, grad_q_weight, grad_k_weight)]
-        strides = _strides(views[0], views[1], views[5], views[6], *grads, *outs[:2])
-        keep.append(strides)
+        values, before, after = _norm_rope_staged(bound.arguments, extents, 4)
+        strides = _strides(*values[:2], *values[5:11])
         size = ctypes.c_size_t(0)
         lib.check(lib.fn["qk_norm_rope_backward_workspace_bytes"](*extents[:4], ctypes.byref(size)), "provider_preparation")
-        args = (dtype_code, *(t.data_ptr() for t in (*views, *grads, *outs)), *extents, strides, float(eps), interleaved)
-        run = _workspace_run(lib.fn["qk_norm_rope_backward"], args, size.value, device, keep)
-        return Launch("intent_hip_qk_norm_rope_backward", run, tuple(keep), tuple(before), tuple(after),
-                      tuple(zip(("tokens", "q_heads", "kv_heads", "d", "table", "pairs"), extents))
-                      + (("workspace_bytes", size.value),),
-                      lambda: lib.call_resources(OP_QK_NORM_ROPE_BACKWARD, dtype_code, extents[3], extents[5], interleaved,
-                                                 _mixed(*views[:4], *views[5:], *grads, *outs[:2])))
+        fn, size = lib.fn["qk_norm_rope_backward"], size.value
+        configuration = (*zip(_NORM_ROPE_EXTENTS, extents), ("workspace_bytes", size))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values[:13]], *extents, strides, float(values[13]), interleaved)
+            keep = [values]
+            run = _workspace_run(fn, args, size, device, keep)
+            return Launch("intent_hip_qk_norm_rope_backward", run, tuple(keep), configuration=configuration,
+                          resources=lambda: lib.call_resources(OP_QK_NORM_ROPE_BACKWARD, dtype_code, extents[3], extents[5],
+                                                               interleaved, _mixed(*values[:4], *values[5:11])))
+        return _staged(again, values, bound, before, after)
     return plan
 
 
@@ -1071,7 +1096,6 @@ def _paged_cache(dtype_code, reading: bool):
 
         if reading:
             *cache, cu, page_offsets, page_indices, k, v = bound.arguments
-            lengths = None
         else:
             k, v, *cache, cu, page_offsets, page_indices, lengths = bound.arguments
             if lengths.shape[0] + 1 != cu.shape[0]:
@@ -1079,27 +1103,28 @@ def _paged_cache(dtype_code, reading: bool):
                                  f"entries, got {cu.shape[0]}")
         if cu.shape[0] < 1:
             raise ValueError("cu_seqlens needs an entry per sequence and one more")
-        keep, before, after = list(bound.arguments), [], []
+        keep, before, after = [], [], []
         held = (*_cache_strides("key", *cache[:2]), *_cache_strides("value", *cache[2:]))
         rows = [_writable(t, keep, after, 8) if reading else _readable(t, keep, before, 8) for t in (k, v)]
         if reading and after:      # a staged output starts as the caller's, whose rows behind the last sequence stay
             before += [functools.partial(staged.copy_, out) for staged, out in zip(rows, (k, v)) if staged is not out]
         strides = (ctypes.c_int64 * 22)(*(x for t in rows for x in (*_outer_strides(t), 1)), *held)
         tables = [_readable(t, keep, before) for t in (cu, page_offsets, page_indices)]
-        keep += rows + [strides]
         pages, ps, kv_heads, d = cache[0].shape
         extents = (k.shape[0], cu.shape[0] - 1, kv_heads, d, cache[2].shape[3], pages, ps, page_indices.shape[0])
-        pointers = tuple(t.data_ptr() for t in cache)
+        configuration = tuple(zip(("rows", "sequences", "kv_heads", "d", "dv", "pages", "ps", "positions"), extents))
         if reading:
             fn, entry, op = lib.fn["paged_cache_read"], "intent_hip_paged_cache_read", OP_PAGED_CACHE_READ
-            args = (dtype_code, *pointers, *(t.data_ptr() for t in (*tables, *rows)), *extents, strides)
+            values = (*cache, *tables, *rows)
         else:
             fn, entry, op = lib.fn["paged_cache_append"], "intent_hip_paged_cache_append", OP_PAGED_CACHE_APPEND
-            tables.append(_readable(lengths, keep, before))
-            args = (dtype_code, *(t.data_ptr() for t in rows), *pointers, *(t.data_ptr() for t in tables), *extents, strides)
-        return Launch(entry, lambda stream: fn(*args, stream), tuple(keep), tuple(before), tuple(after),
-                      tuple(zip(("rows", "sequences", "kv_heads", "d", "dv", "pages", "ps", "positions"), extents)),
-                      lambda: lib.kernel_resources(op, dtype_code, extents[0], kv_heads * (d + extents[4])))
+            values = (*rows, *cache, *tables, _readable(lengths, keep, before))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values], *extents, strides)
+            return Launch(entry, lambda stream: fn(*args, stream), values, configuration=configuration,
+                          resources=lambda: lib.kernel_resources(op, dtype_code, extents[0], extents[2] * (extents[3] + extents[4])))
+        return _staged(again, values, bound, before, after)
     return plan
 
 
@@ -1117,28 +1142,29 @@ def _paged_decode_mx(dtype_code):
             raise ValueError(f"query heads ({q_heads}) must equal key/value heads ({kv_heads}) * HEAD_GROUP ({group})")
         if page_offsets.shape[0] != batch + 1:
             raise ValueError(f"page_offsets must hold batch + 1 = {batch + 1} entries, got {page_offsets.shape[0]}")
-        keep, before, after = list(bound.arguments[:9]), [], []
+        keep, before, after = [], [], []
         held = (*_cache_strides("key", *cache[:2]), *_cache_strides("value", *cache[2:]))
-        qk, outk = _readable(q, keep, before, 8), _writable(output, keep, after)
+        q, output = _readable(q, keep, before, 8), _writable(output, keep, after)
         tables = [_readable(t, keep, before) for t in (page_offsets, page_indices, lengths)]
-        strides = (ctypes.c_int64 * 22)(*_outer_strides(qk), 1, *held, *_outer_strides(outk), 1)
-        keep += [qk, outk, strides]
-        size = ctypes.c_size_t(0)
-        lib.check(lib.fn["paged_gqa_decode_mx_workspace_bytes"](batch, q_heads, kv_heads, group, d, ps, page_indices.shape[0],
+        strides = (ctypes.c_int64 * 22)(*_outer_strides(q), 1, *held, *_outer_strides(output), 1)
+        positions, size = page_indices.shape[0], ctypes.c_size_t(0)
+        lib.check(lib.fn["paged_gqa_decode_mx_workspace_bytes"](batch, q_heads, kv_heads, group, d, ps, positions,
                                                                 ctypes.byref(size)), "provider_preparation")
-        fn = lib.fn["paged_gqa_decode_mx"]
-        args = (dtype_code, *(t.data_ptr() for t in (qk, *cache, *tables, outk)), batch, q_heads, kv_heads, group, d, pages, ps,
-                page_indices.shape[0], strides, float(scale))
-        if size.value:
+        fn, size = lib.fn["paged_gqa_decode_mx"], size.value
+        if size:
             _decode_workspace("paged_gqa_decode_mx")
-            run = _workspace_run(fn, args, size.value, device, keep)
-        else:
-            run = lambda stream: fn(*args, None, 0, stream)  # noqa: E731
-        return Launch("intent_hip_paged_gqa_decode_mx", run, tuple(keep), tuple(before), tuple(after),
-                      (("batch", batch), ("q_heads", q_heads), ("kv_heads", kv_heads), ("d", d), ("pages", pages), ("ps", ps),
-                       ("positions", page_indices.shape[0]), ("workspace_bytes", size.value)),
-                      lambda: lib.call_resources(OP_PAGED_GQA_DECODE_MX, dtype_code, batch, kv_heads, group, d, ps,
-                                                 page_indices.shape[0]))
+        configuration = (("batch", batch), ("q_heads", q_heads), ("kv_heads", kv_heads), ("d", d), ("pages", pages), ("ps", ps),
+                         ("positions", positions), ("workspace_bytes", size))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values[:9]], batch, q_heads, kv_heads, group, d, pages, ps, positions,
+                    strides, float(values[9]))
+            keep = [values]
+            return Launch("intent_hip_paged_gqa_decode_mx", _optional_workspace_run(fn, args, size, device, keep), tuple(keep),
+                          configuration=configuration,
+                          resources=lambda: lib.call_resources(OP_PAGED_GQA_DECODE_MX, dtype_code, batch, kv_heads, group, d, ps,
+                                                               positions))
+        return _staged(again, (q, *cache, *tables, output, scale), bound, before, after)
     return plan
 
 
@@ -1177,21 +1203,22 @@ def _linear_mxfp4(dtype_code):
             raise ValueError(f"weights need unit inner stride, rows in multiples of 16 bytes and a 16-byte aligned start, and "
                              f"their exponents unit inner stride; got strides {tuple(weight.stride())} and "
                              f"{tuple(exponents.stride())}")
-        keep, before, after = [x, weight, exponents, out], [], []
-        xk, outk = _readable(x, keep, before, 8), _writable(out, keep, after)
-        fn = lib.fn["linear_mxfp4"]
-        args = (dtype_code, xk.data_ptr(), weight.data_ptr(), exponents.data_ptr(), outk.data_ptr(), m, n, k,
-                *(_outer_strides(t)[0] for t in (xk, weight, exponents, outk)))
+        keep, before, after = [], [], []
+        x, out = _readable(x, keep, before, 8), _writable(out, keep, after)
+        extents = (m, n, k, *(_outer_strides(t)[0] for t in (x, weight, exponents, out)))
         size = ctypes.c_size_t(0)
         lib.check(lib.fn["linear_mxfp4_workspace_bytes"](m, n, k, ctypes.byref(size)), "provider_preparation")
-        if size.value:
+        fn, size = lib.fn["linear_mxfp4"], size.value
+        if size:
             _no_static("linear_mxfp4", "divides K of few tiles over workgroups whose sums meet in")
-            run = _workspace_run(fn, args, size.value, device, keep)
-        else:
-            run = lambda stream: fn(*args, None, 0, stream)  # noqa: E731
-        return Launch("intent_hip_linear_mxfp4", run, tuple(keep), tuple(before), tuple(after),
-                      (("m", m), ("n", n), ("k", k), ("workspace_bytes", size.value)),
-                      lambda: lib.call_resources(OP_LINEAR_MXFP4, dtype_code, m, n, k))
+        configuration = (("m", m), ("n", n), ("k", k), ("workspace_bytes", size))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values], *extents)
+            keep = [values]
+            return Launch("intent_hip_linear_mxfp4", _optional_workspace_run(fn, args, size, device, keep), tuple(keep),
+                          configuration=configuration, resources=lambda: lib.call_resources(OP_LINEAR_MXFP4, dtype_code, m, n, k))
+        return _staged(again, (x, weight, exponents, out), bound, before, after)
     return plan
 
 

@@ -9,13 +9,14 @@ current stream, asynchronously; `result()` does not synchronize.
 """
 from __future__ import annotations
 
+import functools
 import threading
 
 from ...diagnostics import CompilationStageError
 from ..artifact import CompiledArtifact
 from ..diagnostics import ConfigurationAssessment, NativeObservation, NativeResource
 from ..interface import PublicInterface, ViewParameter
-from ..invocation import Binding, bind_arguments
+from ..invocation import Binding, BoundPublicArguments, bind_arguments
 from ..torch_views import allocate_output, observe_view, raw_stream_getter
 from .library import library
 from .operators import OperatorSpec, plan_policies
@@ -41,6 +42,33 @@ def _constexpr_parameters(definition) -> tuple[tuple[str, object], ...]:
         if hasattr(annotation, "value_type") and not hasattr(annotation, "kind"):
             out.append((name, parameter.default))
     return tuple(out)
+
+
+_LAYOUTS_KEPT = 256
+
+
+@functools.lru_cache(maxsize=1)
+def _plain_tensors() -> tuple:
+    import torch
+
+    return torch.Tensor, torch.nn.Parameter
+
+
+class _Layout:
+    """What binding and planning found for the calls whose tensors have the same shapes, strides, types, device and alignment:
+    facts and no tensor, so that nothing outlives a call. A call that finds its layout is bound without looking at them again
+    (qk_norm_rope_backward of 100 tokens, one `run` on the host: 80 us, 30 with it)."""
+
+    __slots__ = ("outputs", "extents", "pairs", "spans", "again")
+
+    def __init__(self, interface, bound, explicit, written_pairs, again):
+        self.outputs = tuple((tuple(v.shape), v.dtype) for v in bound.outputs)
+        self.extents, self.again = bound.extents, again
+        apart = {p.position for p in interface.outputs} if not explicit else set()        # allocated per call
+        apart.update(p.position for p in interface.views if bound.views[p.position].begin == bound.views[p.position].end)
+        self.pairs = tuple((i, j) for i, j, _ in written_pairs if i not in apart and j not in apart)
+        facts = {place: bound.views[place] for pair in self.pairs for place in pair}
+        self.spans = tuple((place, f.begin - f.pointer, f.end - f.pointer) for place, f in facts.items())
 
 
 class HipPreparedCall:
@@ -128,6 +156,10 @@ class HipProgram:
         self._written_pairs = tuple((left.position, right.position, left.writable and right.writable)
                                     for i, left in enumerate(views) for right in views[i + 1:]
                                     if left.writable or right.writable)
+        # What calls of one layout share, of the last layouts seen (prepare_call); None where the plan offers nothing to share.
+        self._layouts: dict | None = None if self._binding.related else {}
+        self._view_places = tuple(tuple(isinstance(p, ViewParameter) for p in parameters)
+                                  for parameters in (interface.inputs, interface.parameters))
         self._last_launch = None
         self._lock = threading.Lock()
         self._closed = False
@@ -165,11 +197,61 @@ class HipProgram:
             raise RuntimeError("hip program is closed")
         if outputs is not None and not isinstance(outputs, tuple):
             raise TypeError("outputs must be a tuple in declared Out order")
+        layouts = self._layouts
+        key = None if layouts is None else self._layout_key(arguments, outputs)
+        if key in (layouts or ()):
+            call = self._prepare_again(layouts[key], arguments, outputs)
+            if call is not None:
+                return call
         bound = self._bind(arguments, outputs)
         self._check_writable_overlap(bound)
         with plan_policies(self.workspace, self.numerics, self.tuning_rows):
             launch = self.spec.plan(self.library, bound, self.constexprs, self.device)
+        if launch.again is not None:
+            if key is not None:
+                if len(layouts) >= _LAYOUTS_KEPT:
+                    layouts = self._layouts = {}
+                layouts[key] = _Layout(self.interface, bound, outputs is not None, self._written_pairs, launch.again)
+        elif not launch.before and not launch.after:
+            self._layouts = None
         return HipPreparedCall(self, bound, launch)
+
+    def _layout_key(self, arguments, outputs):
+        """Everything of a call's tensors that binding and planning look at, their addresses only to 16 bytes; None where a
+        value has to be looked at more closely."""
+        explicit = outputs is not None
+        places = self._view_places[explicit]
+        try:
+            values = self.interface.explicit_arguments(arguments, outputs) if explicit else arguments
+            if len(values) != len(places):
+                return None
+            key = [explicit]
+            for view, value in zip(places, values):
+                if view:
+                    if type(value) not in _plain_tensors():
+                        return None
+                    key.append((value.shape, value.stride(), value.dtype, value.device, value.data_ptr() & 15))
+        except Exception:  # noqa: BLE001 - binding says what is wrong
+            return None
+        return tuple(key)
+
+    def _prepare_again(self, layout, arguments, outputs):
+        """A call whose layout has been bound and planned before; None where views overlap (binding says whether they may)."""
+        import torch
+
+        if outputs is None:
+            outputs = tuple([torch.empty(shape, dtype=dtype, device=self.device) for shape, dtype in layout.outputs])
+        values = self.interface.explicit_arguments(arguments, outputs)
+        if layout.pairs:
+            ranges = {}
+            for place, low, high in layout.spans:
+                pointer = values[place].data_ptr()
+                ranges[place] = (pointer + low, pointer + high)
+            for left, right in layout.pairs:
+                a, b = ranges[left], ranges[right]
+                if a[0] < b[1] and b[0] < a[1]:
+                    return None
+        return HipPreparedCall(self, BoundPublicArguments(values, outputs, (), layout.extents), layout.again(values))
 
     def run(self, *arguments):
         call = self.prepare_call(arguments)
