@@ -14,7 +14,8 @@
 //     rows each. A lane's weight rows are NT apart, so its results are 4 NT consecutive columns of y. Where tiles are few, K
 //     is divided over workgroups, whose f32 sums a second kernel adds in order. The small tiles are bound by the latency of a
 //     stage and by x's way to the LDS, so they keep four stages on their way (32 x 4096 x 14336: 22 -> 16.7 us; 256 x 4096 x
-//     4096: 40 -> 23); the large ones by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 107 us, 1120
+//     4096: 40 -> 23) and the smallest shares its rows of x among eight waves (with four 16.7 and 24.4, with eight 15.8 and
+//     21.0); the large ones by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 107 us, 1120
 //     TFLOP/s; three stages, and so one workgroup a CU, 174).
 #include <stdio.h>
 
@@ -25,7 +26,7 @@
 namespace intent_hip {
 namespace {
 
-constexpr int kWaves = 4, kFewWaves = 16;
+constexpr int kFewWaves = 16;
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -182,11 +183,11 @@ __device__ __forceinline__ void stage_barrier() {
 // What is read of x behind K.
 __device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
 
-// 16 MT rows of x by 64 NT weight rows a workgroup; S stages of 128 columns are on their way or in use. Each has an LDS array
+// 16 MT rows of x by 16 NT weight rows for each of W waves; S stages of 128 columns are on their way or in use. Each has an LDS array
 // of its own, and the loop is unrolled by S: the compiler then knows which loads into the LDS a read has to wait for.
-template <typename E, int MT, int NT, int S>
-__global__ __launch_bounds__(kWaves *kWave, 2) void linear_tiles(Linear p) {
-  constexpr int kRows = 16 * MT, kUnits = kRows * 16, kLoads = kUnits / (kWaves * kWave);     // 16-byte units of a stage
+template <typename E, int MT, int NT, int S, int W>
+__global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
+  constexpr int kRows = 16 * MT, kUnits = kRows * 16, kLoads = kUnits / (W * kWave);     // 16-byte units of a stage
   constexpr int kIssued = kLoads + 2 * NT;             // loads of a wave per stage, always as many
   static_assert(S >= 2 && S <= 4, "one LDS array per stage");
   __shared__ uint4 x_0[kUnits], x_1[kUnits], x_2[S > 2 ? kUnits : 1], x_3[S > 3 ? kUnits : 1];
@@ -197,15 +198,15 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void linear_tiles(Linear p) {
   if (tile < 0) return;
   const int part = tile / tiles;
   tile -= part * tiles;
-  const int m0 = tile % p.m_tiles * kRows, n0 = (tile / p.m_tiles * kWaves + wave) * 16 * NT;
+  const int m0 = tile % p.m_tiles * kRows, n0 = (tile / p.m_tiles * W + wave) * 16 * NT;
   const int first = min(part * p.stages * 4, p.blocks), last = min(p.blocks, first + p.stages * 4);     // blocks of K of this part
   const int stages = (last - first + 3) / 4;
-  // Units of x that this thread brings in: row i * 16 + own, unit `unit` of it into place unit ^ own of its LDS row.
-  const int own_row = wave * 4 + g, unit = r ^ own_row;
+  // Units of x that this thread brings in: row i * 4 W + own_row, its unit `unit` to the place that the thread's load fills.
+  const int own_row = wave * 4 + g, unit = r ^ (own_row & 15);
   const uint16_t *from[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i)                     // rows behind the last are not stored
-    from[i] = p.x + static_cast<int64_t>(min(m0 + i * 16 + own_row, p.m - 1)) * p.ldx + unit * 8;
+    from[i] = p.x + static_cast<int64_t>(min(m0 + i * 4 * W + own_row, p.m - 1)) * p.ldx + unit * 8;
   const uint8_t *w[NT], *e[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -223,14 +224,14 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void linear_tiles(Linear p) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const uint16_t *src = from[i] + static_cast<int64_t>(b0) * 32;
-        __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * kWaves + wave) * kWave), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * W + wave) * kWave), 16, 0, 0);
       }
     } else {                                           // K ends inside the stage: zeros behind it
       const uint16_t *zero = reinterpret_cast<const uint16_t *>(&kZeroUnit);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const uint16_t *src = b0 + unit / 4 < last ? from[i] + static_cast<int64_t>(b0) * 32 : zero;
-        __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * kWaves + wave) * kWave), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * W + wave) * kWave), 16, 0, 0);
       }
     }
     const int b = min(b0 + g, last - 1);
@@ -327,22 +328,24 @@ __global__ __launch_bounds__(256) void linear_fold(Linear p) {
 struct Cut {
   int mt, nt, parts;                   // mt = 0: linear_few
 };
+constexpr int tile_waves(int mt) { return mt == 2 ? 8 : 4; }
 
 // linear_few for up to 16 rows, NT by the weight rows there are for the workgroups (16 x 14336 x 4096: NT = 1 23.8 us, 2 16.9,
 // 4 12.7; 1 x 4096 x 14336: 10.7, 15.7, 25.8). Where more than eight rows meet a long K and few weight rows, x read once per
-// 16 weight rows costs more than the weights (16 x 4096 x 14336: 19.8 us, in tiles 15.5; 16 x 512 x 7168: 10.3, 7.9).
+// 16 weight rows costs more than the weights (16 x 4096 x 14336: 19.8 us, in tiles 15.5).
 // linear_tiles otherwise, by an estimate from what its tiles measured: us a stage takes a workgroup that has a CU for itself,
 // and each of several on a CU, and what writing, reading and adding the parts' sums takes. It is within a fifth of the best of
 // all tiles and parts at M of 17 to 1021 and N x K of 1000 x 4096 to 28672 x 8192.
 Cut cut(int64_t m, int64_t n, int64_t k) {
   const int cus = device_cus();
   if (m <= 16 && (m <= 8 || n >= 24 * cus || k < 6144)) return {0, n >= 48 * cus ? 4 : n >= 24 * cus ? 2 : 1, 1};
-  constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.47f, 0.32f}, {4, 2, 0.9f, 0.7f}, {8, 2, 1.3f, 0.9f}, {8, 4, 2.1f, 1.67f}};
+  constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.59f, 0.56f}, {4, 2, 0.9f, 0.7f}, {8, 2, 1.3f, 0.9f}, {8, 4, 2.1f, 1.67f}};
   const int64_t stages = (k + 127) / 128;
   Cut best{};
   float least = 0.0f;
   for (const auto &kind : kKinds) {
-    const int64_t tiles = ((m + 16 * kind.mt - 1) / (16 * kind.mt)) * ((n + 64 * kind.nt - 1) / (64 * kind.nt));
+    const int64_t per_tile = 16 * tile_waves(kind.mt) * kind.nt;
+    const int64_t tiles = ((m + 16 * kind.mt - 1) / (16 * kind.mt)) * ((n + per_tile - 1) / per_tile);
     for (int parts = 1; parts <= 16 && (parts == 1 || parts * 4 <= stages); ++parts) {
       const float on_one = static_cast<float>((tiles * parts + cus - 1) / cus), shared = kind.shared * on_one;
       float us = static_cast<float>((stages + parts - 1) / parts) * (kind.alone > shared ? kind.alone : shared);
@@ -360,10 +363,10 @@ int with_kernel(const Cut &c, F f) {
     return c.nt == 1   ? f(linear_few<E, 1>, "linear_few", kFewWaves)
            : c.nt == 2 ? f(linear_few<E, 2>, "linear_few", kFewWaves)
                        : f(linear_few<E, 4>, "linear_few", kFewWaves);
-  return c.mt == 2   ? f(linear_tiles<E, 2, 1, 4>, "linear_tiles", kWaves)
-         : c.mt == 4 ? f(linear_tiles<E, 4, 2, 4>, "linear_tiles", kWaves)
-         : c.nt == 2 ? f(linear_tiles<E, 8, 2, 2>, "linear_tiles", kWaves)
-                     : f(linear_tiles<E, 8, 4, 2>, "linear_tiles", kWaves);
+  return c.mt == 2   ? f(linear_tiles<E, 2, 1, 4, tile_waves(2)>, "linear_tiles", tile_waves(2))
+         : c.mt == 4 ? f(linear_tiles<E, 4, 2, 4, tile_waves(4)>, "linear_tiles", tile_waves(4))
+         : c.nt == 2 ? f(linear_tiles<E, 8, 2, 2, tile_waves(8)>, "linear_tiles", tile_waves(8))
+                     : f(linear_tiles<E, 8, 4, 2, tile_waves(8)>, "linear_tiles", tile_waves(8));
 }
 
 template <typename E>
@@ -374,7 +377,7 @@ void launch(Linear p, const Cut &c, hipStream_t s) {
     p.stages = ((p.blocks + 3) / 4 + runs - 1) / runs;
     dim3 grid(static_cast<unsigned>((p.n + 16 * c.nt - 1) / (16 * c.nt)));
     if (c.mt > 0) {
-      p.m_tiles = (p.m + 16 * c.mt - 1) / (16 * c.mt), p.n_tiles = (p.n + 64 * c.nt - 1) / (64 * c.nt);
+      p.m_tiles = (p.m + 16 * c.mt - 1) / (16 * c.mt), p.n_tiles = (p.n + 16 * waves * c.nt - 1) / (16 * waves * c.nt);
       grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.parts, 1);
     }
     kernel<<<grid, waves * kWave, 0, s>>>(p);
