@@ -7,16 +7,19 @@
 // so lane (r, g) takes block g of four of weight row r as it lies in memory (16 bytes, one exponent), converts it in four
 // parts, and reads the same 32 values of its row of x. Weights go from memory to registers: no wave needs another's.
 //   * linear_few, up to 16 rows of x: a workgroup's 16 waves take a run of K each and add their sums through the LDS. Bound by
-//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 9.9 us, 3.2 TB/s; without x and the
+//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 9.7 us, 3.2 TB/s; without x and the
 //     exponents' loads 6.7; 1 x 4096 x 4096: 5.0, most of it latency: one or two steps a wave).
 //   * linear_tiles: a workgroup's waves share 16 MT rows of x, which pass through the LDS 128 columns at a time (in 16-byte
 //     units, unit u of row r at u ^ r % 16, so that the 16 rows of a read are in different banks), and take 16 NT weight
 //     rows each. A lane's weight rows are NT apart, so its results are 4 NT consecutive columns of y. Where tiles are few, K
-//     is divided over workgroups, whose f32 sums a second kernel adds in order. The small tiles are bound by the latency of a
-//     stage and by x's way to the LDS, so they keep four stages on their way (32 x 4096 x 14336: 22 -> 16.7 us; 256 x 4096 x
-//     4096: 40 -> 23) and the smallest shares its rows of x among eight waves (with four 16.7 and 24.4, with eight 15.8 and
-//     21.0); the large ones by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 107 us, 1120
-//     TFLOP/s; three stages, and so one workgroup a CU, 174).
+//     is divided over workgroups, whose f32 sums a second kernel adds in order.
+//     The small tiles are bound by the latency of a stage and by x's way to the LDS. They keep four stages on their way (32 x
+//     4096 x 14336: 22 -> 16.7 us; 256 x 4096 x 4096: 40 -> 24.4), and the smallest shares its rows of x among eight waves
+//     (16.7 -> 15.8, 24.4 -> 21.0). Exponents come four stages at a time, a word a lane, and a lane permutation brings them to
+//     where they are needed: a byte a lane and stage touches as many cache lines as the weights (21.0 -> 19.0; the tiles of
+//     128 x 128 lose up to 4 %).
+//     The large tiles are bound by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 107 us, 1120 TFLOP/s,
+//     the type's own product 90 to 97; three stages, and so one workgroup a CU, 174).
 #include <stdio.h>
 
 #include <type_traits>
@@ -188,9 +191,9 @@ __device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
 template <typename E, int MT, int NT, int S, int W>
 __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
   constexpr int kRows = 16 * MT, kUnits = kRows * 16, kLoads = kUnits / (W * kWave);     // 16-byte units of a stage
-  constexpr int kIssued = kLoads + 2 * NT;             // loads of a wave per stage, always as many
-  static_assert(S >= 2 && S <= 4, "one LDS array per stage");
-  __shared__ uint4 x_0[kUnits], x_1[kUnits], x_2[S > 2 ? kUnits : 1], x_3[S > 3 ? kUnits : 1];
+  constexpr int kIssued = kLoads + NT;                 // loads of a wave per stage, always as many (the exponents' come on top)
+  static_assert(S == 2 || S == 4, "one LDS array per stage, four stages a turn of the loop");
+  __shared__ uint4 x_0[kUnits], x_1[kUnits], x_2[S > 2 ? kUnits : 1], x_3[S > 2 ? kUnits : 1];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = p.m_tiles * p.n_tiles;
@@ -215,7 +218,7 @@ __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
     e[j] = p.e + row * p.lde;
   }
   uint4 raw[S][NT];
-  uint8_t power[S][NT];
+  uint32_t powers[NT], later[NT];      // of four stages: lane (r, g) holds those of stage g
   const auto array = [&](int u) -> uint4 * { return u == 0 ? x_0 : u == 1 ? x_1 : u == 2 ? x_2 : x_3; };
   const auto issue = [&](int t, int u) {               // stage t (the last again behind it) into set u
     const int b0 = first + min(t, stages - 1) * 4;
@@ -236,9 +239,21 @@ __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
     }
     const int b = min(b0 + g, last - 1);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      raw[u][j] = *reinterpret_cast<const uint4 *>(w[j] + static_cast<int64_t>(b) * 16);
-      power[u][j] = e[j][b];
+    for (int j = 0; j < NT; ++j) raw[u][j] = *reinterpret_cast<const uint4 *>(w[j] + static_cast<int64_t>(b) * 16);
+  };
+  const auto fetch = [&](int t) {                      // the exponents of stages t .. t + 3, behind K any
+    const int b = first + (t + g) * 4;
+    if (first + t * 4 + 16 <= p.blocks) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) __builtin_memcpy(&later[j], e[j] + b, 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        uint32_t byte[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) byte[i] = e[j][min(b + i, p.blocks - 1)];
+        later[j] = byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24;
+      }
     }
   };
   f32x4_t acc[MT][NT];
@@ -247,28 +262,35 @@ __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
   if (stages > 0) {
+    fetch(0);
 #pragma unroll
     for (int u = 0; u < S - 1; ++u) issue(u, u);
-    for (int t0 = 0; t0 < stages; t0 += S) {
+    for (int t0 = 0; t0 < stages; t0 += 4) {
 #pragma unroll
-      for (int u = 0; u < S; ++u) {
+      for (int u = 0; u < 4; ++u) {
         if (t0 + u >= stages) break;
         INTENT_WAIT_VMCNT((S - 2) * kIssued);          // this wave's loads of the stage have come
         stage_barrier();                               // everybody's have, and nobody reads the set that is filled next
+        if (u == 0) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) powers[j] = later[j];
+        }
         issue(t0 + u + S - 1, (u + S - 1) % S);
+        if (u + S - 1 == 4 && t0 + 4 < stages) fetch(t0 + 4);
         const bool held = first + (t0 + u) * 4 + g < last;
         uint4 own[NT];
         float scale[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          own[j] = held ? raw[u][j] : make_uint4(0, 0, 0, 0);
-          scale[j] = mx_scale(held ? power[u][j] : 127);
+          const uint32_t word = __builtin_amdgcn_ds_bpermute((u * 16 + r) * 4, static_cast<int>(powers[j]));
+          own[j] = held ? raw[u % S][j] : make_uint4(0, 0, 0, 0);
+          scale[j] = mx_scale(word >> (8 * g) & 0xFF);
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint4 v[MT], a[NT];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) v[i] = array(u)[(i * 16 + r) * 16 + ((g * 4 + c) ^ r)];
+          for (int i = 0; i < MT; ++i) v[i] = array(u % S)[(i * 16 + r) * 16 + ((g * 4 + c) ^ r)];
 #pragma unroll
           for (int j = 0; j < NT; ++j) a[j] = eight<E>(c == 0 ? own[j].x : c == 1 ? own[j].y : c == 2 ? own[j].z : own[j].w, scale[j]);
 #pragma unroll
@@ -339,7 +361,7 @@ constexpr int tile_waves(int mt) { return mt == 2 ? 8 : 4; }
 Cut cut(int64_t m, int64_t n, int64_t k) {
   const int cus = device_cus();
   if (m <= 16 && (m <= 8 || n >= 24 * cus || k < 6144)) return {0, n >= 48 * cus ? 4 : n >= 24 * cus ? 2 : 1, 1};
-  constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.59f, 0.56f}, {4, 2, 0.9f, 0.7f}, {8, 2, 1.3f, 0.9f}, {8, 4, 2.1f, 1.67f}};
+  constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.53f, 0.5f}, {4, 2, 0.9f, 0.7f}, {8, 2, 1.3f, 0.9f}, {8, 4, 2.1f, 1.67f}};
   const int64_t stages = (k + 127) / 128;
   Cut best{};
   float least = 0.0f;
