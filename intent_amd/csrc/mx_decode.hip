@@ -33,6 +33,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStep = 32;              // keys of a wave's step: two tiles of 16
 constexpr float kSlack = 8.0f;
+constexpr float kNoToken = -1.0f;      // the sum of a state without a token (weights are not negative)
 constexpr uint32_t kSigns = 0x80008000u;
 constexpr int kMany = 6, kFew = 2;     // workgroups a CU is given
 constexpr int kLong = 256;            // tokens of a job: from here on it is one of many
@@ -180,6 +181,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
         q[t][c] = make_uint4(q[t][c].x ^ kSigns, q[t][c].y ^ kSigns, q[t][c].z ^ kSigns, q[t][c].w ^ kSigns);
   f32x4_t acc[QT][C::kTiles];
   float peak[QT], total[QT];
+  bool any = false;                    // a token so far
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     peak[t] = -INFINITY;
@@ -362,6 +364,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
     while (at[0] < tokens) {
       Step<D> x;
       load(x);
+      any = any || x.valid[0] > 0 || x.valid[1] > 0;
       fold(x);
     }
   } else {
@@ -387,6 +390,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
           value(x, u * 4 + i, p.v + page * p.vs[0] + in * p.vs[1] + kh * p.vs[2], p.ve + page * p.ves[0] + in * p.ves[1] + kh * p.ves[2], 0, 0);
         }
       }
+      any = any || __any(x.live != 0);
       fold(x);
     }
   }
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
     total[t] += __shfl_xor(total[t], 16);
     total[t] += __shfl_xor(total[t], 32);
     if (t > 0) __syncthreads();
-    if (g == 0) peak_s[wave][r] = peak[t], total_s[wave][r] = total[t];
+    if (g == 0) peak_s[wave][r] = peak[t], total_s[wave][r] = any ? total[t] : kNoToken;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -408,20 +412,23 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
     __syncthreads();
     const int i = wave & 3, j0 = wave / 4 * kMine, in = g * 4 + i, head = t * 16 + in;
     float whole = -INFINITY, sum = 0.0f, row[kMine] = {};
+    bool token = false;
 #pragma unroll
     for (int w = 0; w < W; ++w) whole = fmaxf(whole, peak_s[w][in]);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float own = peak_s[w][in];
       const float f = own == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(own - whole);      // a wave without a score has sums of 0, or NaN
-      sum += total_s[w][in] * f;
+      const bool none = total_s[w][in] < 0.0f;
+      sum += none ? 0.0f : total_s[w][in] * f;
+      token = token || !none;
 #pragma unroll
       for (int j = 0; j < kMine; ++j) row[j] += sums_s[w][i * C::kTiles + j0 + j][lane] * f;
     }
     if (head >= heads) continue;
     const int64_t state = static_cast<int64_t>(job) * q_heads + head0 + head;
-    if (p.peak != nullptr && r == 0 && j0 == 0) p.peak[state] = whole, p.total[state] = sum;
-    const float share = p.peak != nullptr ? 1.0f : tokens > 0 ? 1.0f / sum : 0.0f;
+    if (p.peak != nullptr && r == 0 && j0 == 0) p.peak[state] = whole, p.total[state] = token ? sum : kNoToken;
+    const float share = p.peak != nullptr ? 1.0f : token ? 1.0f / sum : 0.0f;
     float *const sums = p.sums + state * D;
     uint16_t *const out = p.out + s * p.outs[0] + (head0 + head) * p.outs[1];
 #pragma unroll
@@ -456,13 +463,16 @@ __global__ __launch_bounds__(W *kWave) void mx_decode_merge(Decode p) {
   for (int j = lane; j < mine; j += kWave) peak = fmaxf(peak, p.peak[row0 + j * stride]);
   peak = wave_max(peak);
   float total = 0.0f, out[kColumns] = {};
+  bool token = false;
   for (int j0 = 0; j0 < mine; j0 += kWave) {
     const int count = min(mine - j0, kWave);
     float weight = 0.0f;
     if (lane < count) {
       const float own = p.peak[row0 + (j0 + lane) * stride];
       weight = own == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(own - peak);        // a job without a score has sums of 0, or NaN
-      total += p.total[row0 + (j0 + lane) * stride] * weight;
+      const float sum = p.total[row0 + (j0 + lane) * stride];
+      token = token || !(sum < 0.0f);
+      total += sum < 0.0f ? 0.0f : sum * weight;
     }
     for (int j = 0; j < count; j += kTogether) {
       float from[kTogether][kColumns] = {};
@@ -481,7 +491,8 @@ __global__ __launch_bounds__(W *kWave) void mx_decode_merge(Decode p) {
     }
   }
   total = wave_sum(total);
-  if (lane == 0) peak_s[wave] = peak, total_s[wave] = total;
+  token = __any(token);
+  if (lane == 0) peak_s[wave] = peak, total_s[wave] = token ? total : kNoToken;
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) sums_s[wave][c * kWave + lane] = out[c];
   __syncthreads();
@@ -490,13 +501,15 @@ __global__ __launch_bounds__(W *kWave) void mx_decode_merge(Decode p) {
   for (int w = 0; w < W; ++w) whole = fmaxf(whole, peak_s[w]);
   for (int column = threadIdx.x; column < D; column += W * kWave) {
     float sum = 0.0f, value = 0.0f;
+    bool held = false;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float f = peak_s[w] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(peak_s[w] - whole);
-      sum += total_s[w] * f;
+      sum += total_s[w] < 0.0f ? 0.0f : total_s[w] * f;
+      held = held || !(total_s[w] < 0.0f);
       value += sums_s[w][column] * f;
     }
-    p.out[s * p.outs[0] + head * p.outs[1] + column] = from_f32<E>(value * (jobs > 0 ? 1.0f / sum : 0.0f)).bits;
+    p.out[s * p.outs[0] + head * p.outs[1] + column] = from_f32<E>(value * (held ? 1.0f / sum : 0.0f)).bits;
   }
 }
 

@@ -98,6 +98,25 @@ def test_reserved_pages_and_lengths_past_them(device):
     assert (out[3] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("page,held", [(16, [3, 2, 4]), (7, [3, 2, 4]), (16, [400, 90, 3]), (5, [600, 700, 3])])
+def test_sequences_whose_pages_are_all_outside(device, dtype, page, held):
+    """A sequence that has pages, but none in the cache, gives 0, as do jobs of a longer one; its neighbours are not touched."""
+    announce("mx decode with no page inside", dtype, page, held)
+    g = torch.Generator().manual_seed(sum(held) + page)
+    keys, plain_keys = filled(g, 40, page, 2, 64, True, device)
+    values, plain_values = filled(g, 40, page, 2, 64, True, device)
+    offsets = [0, held[0], held[0] + held[1], sum(held)]
+    indices = torch.randint(0, 40, (sum(held),), generator=g, dtype=torch.int32)
+    indices[offsets[0]:offsets[1]] = torch.where(torch.arange(held[0]) % 2 == 0, -1, 40).int()
+    indices[offsets[1]:offsets[1] + held[1] // 2] = 1 << 30
+    lengths = [n * page for n in held]
+    q = torch.randn((3, 8, 64), generator=g).to(TYPES[dtype])
+    out = kernel(dtype, 4).run(q.to(device), *keys, *values, i32(offsets, device), indices.to(device), i32(lengths, device), 0.125)
+    assert (out[0] == 0).all()
+    check(out, q, plain_keys, plain_values, offsets, indices, lengths, 0.125, dtype)
+
+
 def test_caches_without_a_page(device):
     """No page, pages of no token and an empty table give 0, whatever the lengths say."""
     announce("mx decode without pages")
