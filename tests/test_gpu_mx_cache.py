@@ -302,3 +302,23 @@ def test_captured(device):
         assert torch.equal(keys[0].contiguous().float().double().cpu(), want)
         assert torch.equal(keys[1].contiguous().int().cpu(), powers)
         lengths += 1
+
+
+def test_append_as_a_torch_operator(device):
+    """The cache is written in place through the operator's schema; a cache that shares storage with the rows is refused."""
+    announce("cache append as a torch operator")
+    g = torch.Generator().manual_seed(21)
+    append = kernel("paged_cache_append_f16")
+    held = [(*cache(3, 16, 2, 64, True, device), *cache(3, 16, 2, 64, True, device)) for _ in range(2)]
+    k, v = (torch.randn((5, 2, 64), generator=g).half().to(device) for _ in range(2))
+    tables_on = (i32([0, 2, 5], device), i32([0, 1, 2], device), i32([2, 0], device), i32([9, 3], device))
+    append.run(k, v, *held[0], *tables_on)
+    operation = append.as_torch_op("intent_amd_tests::paged_cache_append")
+    assert operation(k, v, *held[1], *tables_on) is None
+    for a, b in zip(*held):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    storage = torch.zeros(3 * 2 * 16 * 64 + 5 * 2 * 64 * 2, dtype=torch.uint8, device=device)
+    shared = storage[:3 * 2 * 16 * 64].view(torch.float8_e4m3fn).view(3, 2, 16, 64).transpose(1, 2)
+    rows = storage[3 * 2 * 16 * 64:].view(torch.float16).view(5, 2, 64)
+    with pytest.raises(NotImplementedError):
+        operation(rows, v, shared, *held[1][1:], *tables_on)

@@ -225,3 +225,42 @@ def test_captured_and_other_stream(device):
         torch.cuda.synchronize()
         for a, b in zip(call.result(), want):
             assert torch.equal(a, b)
+
+
+def test_autograd_registration(device):
+    """Forward and authored backward as torch operators: leaves used by two calls, of which one shares a packed projection,
+    collect the sum of both calls' gradients."""
+    announce("qk_norm_rope autograd")
+    rows, weights, positions, cos, sin, grad_q, grad_k = case(5, "bf16", 12, 4, 2, 64, 32)
+    forward_kernel, backward_kernel = kernel("qk_norm_rope_bf16"), kernel("qk_norm_rope_backward_bf16")
+    packed = rows.to(device).requires_grad_(True)
+    leaves = [w.to(device).requires_grad_(True) for w in weights]
+    tables_on = (positions.to(device), cos.to(device), sin.to(device))
+    grads = (grad_q.to(device), grad_k.to(device))
+    split = lambda t: (t[:, :4], t[:, 4:6])          # noqa: E731
+    forward_kernel.prepare(*split(packed.detach()), *(w.detach() for w in leaves), *tables_on, EPS)
+    backward_kernel.prepare(*split(packed.detach()), *(w.detach() for w in leaves), *tables_on, *grads, EPS)
+    operation = forward_kernel.as_torch_op("intent_amd_tests::qk_norm_rope")
+    backward_operation = backward_kernel.as_torch_op("intent_amd_tests::qk_norm_rope_backward")
+
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(*inputs[:7])
+        ctx.eps = inputs[7]
+
+    def backward_formula(ctx, dq, dk):
+        return (*backward_operation(*ctx.saved_tensors, dq.contiguous(), dk.contiguous(), ctx.eps), None, None, None, None)
+
+    operation.register_autograd(backward_formula, setup_context=setup_context)
+    total = 0
+    for _ in range(2):
+        q, k = operation(*split(packed), *leaves, *tables_on, EPS)
+        total = total + (q.float() * grads[0].float()).sum() + (k.float() * grads[1].float()).sum()
+    total.backward()
+    assert (packed.grad[:, 6:] == 0).all()
+    for i, grad in enumerate((grad_q, grad_k)):
+        x = split(rows)[i]
+        dx, dx_size, dw, dw_size = plain64.norm_rope_backward(x, weights[i], grad, positions, cos, sin, EPS, False)
+        # twice the gradient, each call's and their sum rounded to bf16
+        close(split(packed.grad)[i] / 2, dx, dx_size, "bf16", 2.0 ** -17 + 2 * 2.0 ** -8)
+        bound = 2.0 ** -15 * dw_size + 2.0 ** -23 * dw.abs()
+        assert ((leaves[i].grad.double().cpu() / 2 - dw).abs() <= bound).all()
