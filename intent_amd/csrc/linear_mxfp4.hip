@@ -16,8 +16,8 @@
 //     The small tiles are bound by the latency of a stage and by x's way to the LDS. They keep four stages on their way (32 x
 //     4096 x 14336: 22 -> 16.7 us; 256 x 4096 x 4096: 40 -> 24.4), and the smallest shares its rows of x among eight waves
 //     (16.7 -> 15.8, 24.4 -> 21.0). Exponents come four stages at a time, a word a lane, and a lane permutation brings them to
-//     where they are needed: a byte a lane and stage touches as many cache lines as the weights (21.0 -> 19.0; the tiles of
-//     128 x 128 lose up to 4 %).
+//     where they are needed: a byte a lane and stage touches as many cache lines as the weights (21.0 -> 18.2; the tiles of
+//     128 x 128 lose up to 4 %). Eight stages on their way instead of four are no faster (32 x 4096 x 14336: 16.0, four 15.2).
 //     The large tiles are bound by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 107 us, 1120 TFLOP/s,
 //     the type's own product 90 to 97; three stages, and so one workgroup a CU, 174).
 #include <stdio.h>
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
           for (int j = 0; j < NT; ++j) powers[j] = later[j];
         }
         issue(t0 + u + S - 1, (u + S - 1) % S);
-        if (u + S - 1 == 4 && t0 + 4 < stages) fetch(t0 + 4);
+        if (u == (S == 4 ? 0 : 3) && t0 + 4 < stages) fetch(t0 + 4);       // (S = 2 has no registers to spare before)
         const bool held = first + (t0 + u) * 4 + g < last;
         uint4 own[NT];
         float scale[NT];
