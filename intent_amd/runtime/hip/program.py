@@ -159,7 +159,10 @@ class HipProgram:
         # What calls of one layout share, of the last layouts seen (prepare_call); None where the plan offers nothing to share.
         self._layouts: dict | None = None if self._binding.related else {}
         self._view_places = tuple(tuple(isinstance(p, ViewParameter) for p in parameters)
-                                  for parameters in (interface.inputs, interface.parameters))
+                                  for parameters in (interface.inputs, (*interface.inputs, *interface.outputs)))
+        # Where each parameter stands among the inputs followed by the Out buffers.
+        places = {p.position: at for at, p in enumerate((*interface.inputs, *interface.outputs))}
+        self._order = tuple(places[p.position] for p in interface.parameters)
         self._last_launch = None
         self._lock = threading.Lock()
         self._closed = False
@@ -219,16 +222,15 @@ class HipProgram:
     def _layout_key(self, arguments, outputs):
         """Everything of a call's tensors that binding and planning look at, their addresses only to 16 bytes; None where a
         value has to be looked at more closely."""
-        explicit = outputs is not None
-        places = self._view_places[explicit]
+        values, places = (arguments, self._view_places[0]) if outputs is None else ((*arguments, *outputs), self._view_places[1])
+        if len(values) != len(places) or len(arguments) != len(self._view_places[0]):
+            return None
+        plain = _plain_tensors()
+        key = [len(values)]
         try:
-            values = self.interface.explicit_arguments(arguments, outputs) if explicit else arguments
-            if len(values) != len(places):
-                return None
-            key = [explicit]
             for view, value in zip(places, values):
                 if view:
-                    if type(value) not in _plain_tensors():
+                    if type(value) not in plain:
                         return None
                     key.append((value.shape, value.stride(), value.dtype, value.device, value.data_ptr() & 15))
         except Exception:  # noqa: BLE001 - binding says what is wrong
@@ -241,7 +243,8 @@ class HipProgram:
 
         if outputs is None:
             outputs = tuple([torch.empty(shape, dtype=dtype, device=self.device) for shape, dtype in layout.outputs])
-        values = self.interface.explicit_arguments(arguments, outputs)
+        given = (*arguments, *outputs)
+        values = tuple([given[at] for at in self._order])
         if layout.pairs:
             ranges = {}
             for place, low, high in layout.spans:
