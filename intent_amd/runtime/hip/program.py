@@ -17,7 +17,7 @@ from ..artifact import CompiledArtifact
 from ..diagnostics import ConfigurationAssessment, NativeObservation, NativeResource
 from ..interface import PublicInterface, ViewParameter
 from ..invocation import Binding, BoundPublicArguments, bind_arguments
-from ..torch_views import allocate_output, observe_view, raw_stream_getter
+from ..torch_views import allocate_output, observe_view, raw_device_getter, raw_stream_getter
 from .library import library
 from .operators import OperatorSpec, plan_policies
 from .tuning import FAMILY_OF, SPLIT, TuningConfiguration
@@ -75,13 +75,11 @@ class HipPreparedCall:
     """Bound arguments, allocated outputs/workspace and the native call that uses them."""
 
     def __init__(self, program: "HipProgram", bound, launch):
-        import torch
-
         self._program, self._bound, self._launch = program, bound, launch
         self._index = program.device.index
         self._run = launch.run
         self._before, self._after = launch.before, launch.after
-        self._current_device = torch.cuda.current_device
+        self._current_device = raw_device_getter()
         self._stream = raw_stream_getter()
         self._launched = False
 
@@ -96,14 +94,16 @@ class HipPreparedCall:
 
             torch.cuda.set_device(index)
         try:
-            for step in self._before:
-                step()
+            if self._before:
+                for step in self._before:
+                    step()
             status = self._run(self._stream(index))
             if status != 0:
                 raise CompilationStageError("provider_invocation",
                                             f"{self._launch.entry}: {self._program.library.error(status)}")
-            for step in self._after:
-                step()
+            if self._after:
+                for step in self._after:
+                    step()
         finally:
             if previous != index:
                 import torch

@@ -82,3 +82,11 @@ def raw_stream_getter():
     if raw is not None:
         return raw
     return lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+@functools.lru_cache(maxsize=1)
+def raw_device_getter():
+    """Fast accessor of the current HIP device's index, for callers behind torch's initialisation of the GPU."""
+    import torch
+
+    return getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
