@@ -172,3 +172,18 @@ def test_refusals(device):
     static.run(x, weight, exponents)
     with pytest.raises(intent.CompilationStageError, match="workspace"):
         static.run(*(a.to(device) for a in case(2, "f16", 100, 64, 4096)))
+
+
+@pytest.mark.parametrize("m", [1, 20])
+def test_weights_beyond_32_bits(device, m):
+    announce("linear mxfp4 beyond 32 bits", m)
+    n, k = 2 ** 19 + 70, 16384
+    x, few, powers = case(m, "f16", m, 64, k)
+    weight = torch.zeros((n, k // 2), dtype=torch.uint8, device=device)
+    exponents = torch.full((n, k // 32), 120, dtype=torch.uint8, device=device)
+    assert weight.numel() > 2 ** 32
+    rows = torch.cat((torch.arange(16), torch.arange(n - 48, n)))
+    weight[rows.to(device)], exponents[rows.to(device)] = few.to(device), powers.to(device)
+    out = kernel("f16").run(x.to(device), weight, exponents)
+    check(out[:, rows.to(device)], x, few, powers, "f16")
+    assert (out[:, 16:n - 48] == 0).all()

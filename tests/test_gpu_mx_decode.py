@@ -271,3 +271,34 @@ def test_scale_of_either_sign_and_none(device):
         want, size = plain64.decode(q, plain_keys, plain_values, [0, 4], [0, 1, 2, 3], [50], scale)
         assert not out.isnan().any()
         assert ((out.double().cpu() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -13 * size).all()
+
+
+def test_offsets_beyond_32_bits(device):
+    """Pages behind the first 4 GiB of a cache, and a token stride whose lane offsets would pass 32 bits."""
+    announce("mx decode beyond 32 bits")
+    g = torch.Generator().manual_seed(31)
+    near, plain_near = filled(g, 6, 16, 1, 64, False, device)
+    values, plain_values = filled(g, 6, 16, 1, 64, False, device)
+    pages = 2 ** 32 // (16 * 64) + 7
+    q = torch.randn((2, 4, 64), generator=g).half()
+    offsets, indices, lengths = [0, 4, 6], torch.tensor([5, 0, 3, 1, 2, 4], dtype=torch.int32), [61, 18]
+    far = torch.where(indices % 2 == 0, indices, indices + pages - 6).int()
+    caches = []
+    for elements, exponents in (near, values):
+        wide = torch.zeros((pages, 16, 1, 64), dtype=torch.uint8, device=device)
+        powers = torch.zeros((pages, 16, 1, 2), dtype=torch.uint8, device=device)
+        assert wide.numel() > 2 ** 32
+        for a, b in zip(indices.tolist(), far.tolist()):
+            wide[b], powers[b] = elements[a].view(torch.uint8), exponents[a]
+        caches += [wide.view(torch.float8_e4m3fn), powers]
+    run = lambda held, at: kernel("f16", 4).run(q.to(device), *held, i32(offsets, device), at.to(device), i32(lengths, device), 0.125)  # noqa: E731
+    out = run(caches, far)
+    check(out, q, plain_near, plain_values, offsets, indices, lengths, 0.125, "f16")
+    del caches, wide, powers
+    strided = []
+    for elements, exponents in (near, values):
+        store = torch.zeros(15 * 2 ** 26 + 6 * 64, dtype=torch.uint8, device=device)
+        view = store.as_strided((6, 16, 1, 64), (64, 2 ** 26, 64, 1))
+        view.copy_(elements.view(torch.uint8))
+        strided += [view.view(torch.float8_e4m3fn), exponents]
+    check(run(strided, indices), q, plain_near, plain_values, offsets, indices, lengths, 0.125, "f16")
