@@ -191,6 +191,7 @@ __device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
 template <typename E, int MT, int NT, int S, int W>
 __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
   constexpr int kRows = 16 * MT, kUnits = kRows * 16, kLoads = kUnits / (W * kWave);     // 16-byte units of a stage
+  constexpr int kRead = MT <= 4 ? 4 : 1;               // quarters of a stage read before their products, as registers allow
   constexpr int kIssued = kLoads + NT;                 // loads of a wave per stage, always as many (the exponents' come on top)
   static_assert(S == 2 || S == 4, "one LDS array per stage, four stages a turn of the loop");
   __shared__ uint4 x_0[kUnits], x_1[kUnits], x_2[S > 2 ? kUnits : 1], x_3[S > 2 ? kUnits : 1];
@@ -287,16 +288,22 @@ __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
           scale[j] = mx_scale(word >> (8 * g) & 0xFF);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint4 v[MT], a[NT];
+        for (int c0 = 0; c0 < 4; c0 += kRead) {
+          uint4 v[kRead][MT];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) v[i] = array(u % S)[(i * 16 + r) * 16 + ((g * 4 + c) ^ r)];
+          for (int c = 0; c < kRead; ++c)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) a[j] = eight<E>(c == 0 ? own[j].x : c == 1 ? own[j].y : c == 2 ? own[j].z : own[j].w, scale[j]);
+            for (int i = 0; i < MT; ++i) v[c][i] = array(u % S)[(i * 16 + r) * 16 + ((g * 4 + c0 + c) ^ r)];
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+          for (int c = c0; c < c0 + kRead; ++c) {
+            uint4 a[NT];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = mfma<E>(a[j], v[i], acc[i][j]);
+            for (int j = 0; j < NT; ++j) a[j] = eight<E>(c == 0 ? own[j].x : c == 1 ? own[j].y : c == 2 ? own[j].z : own[j].w, scale[j]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int j = 0; j < NT; ++j) acc[i][j] = mfma<E>(a[j], v[c - c0][i], acc[i][j]);
+          }
         }
       }
     }
