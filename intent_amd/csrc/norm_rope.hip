@@ -5,6 +5,8 @@
 // of g u over rows, through f32 partial sums per workgroup that a second kernel adds in order.
 #include <stdio.h>
 
+#include <algorithm>
+
 #include "common.hpp"
 
 namespace intent_hip {
@@ -618,7 +620,7 @@ extern "C" int intent_hip_qk_norm_rope_backward(int dtype, const void *q, const 
   if (int rc = check(dtype, p, tokens, q_heads, kv_heads, d, table, pairs, strides, 22)) return rc;
   if (d == 0) return INTENT_HIP_OK;
   if (grad_q_weight == nullptr || grad_k_weight == nullptr) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null pointer");
-  const int blocks = backward_blocks(tokens, q_heads, kv_heads);
+  int blocks = backward_blocks(tokens, q_heads, kv_heads);
   const size_t bytes = static_cast<size_t>(blocks) * 2 * d * sizeof(float);
   float *partial = static_cast<float *>(workspace);
   if (blocks > 0) {
@@ -638,6 +640,7 @@ extern "C" int intent_hip_qk_norm_rope_backward(int dtype, const void *q, const 
     p.coss = strides[6], p.sins = strides[8], p.table = table;
     p.tokens = tokens, p.heads[0] = static_cast<int>(q_heads), p.heads[1] = static_cast<int>(kv_heads);
     p.d = static_cast<int>(d), p.pairs = static_cast<int>(pairs), p.interleaved = interleaved != 0, p.eps = eps;
+    if (in_pieces(d, pairs, mixed(p, true))) blocks = static_cast<int>(std::min<int64_t>(blocks, (tokens + kWaves - 1) / kWaves));    // a wave takes a token
     if (dtype == INTENT_HIP_F16)
       launch_backward<f16_t>(p, blocks, partial, as_stream(stream));
     else
