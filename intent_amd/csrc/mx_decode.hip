@@ -581,7 +581,8 @@ void launch(const Decode &p, const Cut &c, bool uniform, hipStream_t s) {
       mx_decode<E, D, 2, false, 4><<<grid, 4 * kWave, 0, s>>>(p);
   }
   if (!c.merge) return;
-  // Few rows: four waves share one's jobs.
+  // Few rows: four waves share one's jobs (one sequence of 8000, 32 heads: 12.4 us in all, one wave a row 15.8; 64 sequences, 64
+  // heads: 135 with one, 142 with four).
   const int64_t rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.group;
   if (rows < 4 * device_cus())
     mx_decode_merge<E, D, 4><<<dim3(static_cast<unsigned>(rows)), 4 * kWave, 0, s>>>(p);

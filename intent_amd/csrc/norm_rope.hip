@@ -3,6 +3,10 @@
 // A row is one (token, head): y = x * rsqrt(mean(x^2) + eps) * w in f32, whose first 2R dimensions are R pairs turned by
 // the token's angles. Backward: g = the gradient turned back; u = x r; grad_x = r (g w - u mean(g w u)); grad_w = the sum
 // of g u over rows, through f32 partial sums per workgroup that a second kernel adds in order.
+//
+// Bound by the rows' bytes, so each is read and written once, in whole 16-byte pieces (bf16, 16384 tokens of 32 + 8 heads of 128:
+// forward 64 us, 5.4 TB/s; backward 102 us and 4 for the sums, 5.0 TB/s); with few tokens by latency and launches (8 tokens: 3.1
+// and 7.2 us). Layouts without such pieces take two bytes a lane (342 and 999 us).
 #include <stdio.h>
 
 #include <algorithm>
@@ -315,9 +319,10 @@ __global__ __launch_bounds__(kWaves * kWave) void norm_rope_rows(NormRope p, int
   }
 }
 
-// The backward of the same; waves walk tokens and keep their share of the weights' gradients in registers.
+// The backward of the same; waves walk tokens (`waves` of them share one's heads) and keep their share of the weights'
+// gradients in registers.
 template <typename E, int G, bool kInterleaved>
-__global__ __launch_bounds__(kWaves * kWave) void norm_rope_backward_rows(NormRope p, float *partial) {
+__global__ __launch_bounds__(kWaves * kWave) void norm_rope_backward_rows(NormRope p, float *partial, int waves) {
   constexpr int kRows = kWave / G;
   __shared__ float sums[kWaves][2][16 * G];
   const int lane = threadIdx.x & 63, c = lane % G, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -346,15 +351,17 @@ __global__ __launch_bounds__(kWaves * kWave) void norm_rope_backward_rows(NormRo
     }
     return x;
   };
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWaves;
-  for (int64_t token = static_cast<int64_t>(blockIdx.x) * kWaves + wave; token < p.tokens; token += stride) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWaves, jobs = p.tokens * waves;
+  for (int64_t job = static_cast<int64_t>(blockIdx.x) * kWaves + wave; job < jobs; job += stride) {
+    const int64_t token = waves == 1 ? job : job / waves;
     float cs[8], sn[8];
-    Row next = load(token, lane / G);
+    int f0 = static_cast<int>(job - token * waves) * kRows;
+    Row next = load(token, f0 + lane / G);
     angles(p, at, c, token, cs, sn);
-    for (int f0 = 0; f0 < heads; f0 += kRows) {
+    for (; f0 < heads; f0 += waves * kRows) {
       const int f = f0 + lane / G, which = f >= p.heads[0];
       const Row x = next;
-      if (f0 + kRows < heads) next = load(token, f + kRows);
+      if (f0 + waves * kRows < heads) next = load(token, f + waves * kRows);
       float u[8], v[8], first[8], second[8], ga[8], gb[8], sum = 0.0f, along = 0.0f;
       widen<E>(x.a, u);
       widen<E>(x.b, v);
@@ -412,7 +419,8 @@ __global__ __launch_bounds__(kWaves * kWave) void norm_rope_backward_rows(NormRo
   }
 }
 
-// Workgroups of the backward pass: as many as the chip holds at once, fewer where a wave would have no token (or no row).
+// Workgroups of the backward pass: as many as the chip holds at once (16384 tokens: 106 us; half as many 145, twice as many
+// 107), fewer where a wave would have no row.
 int backward_blocks(int64_t tokens, int64_t q_heads, int64_t kv_heads) {
   const int64_t rows = tokens * (q_heads + kv_heads), wanted = (rows + kWaves - 1) / kWaves, most = 2 * device_cus();
   return static_cast<int>(wanted < most ? wanted : most);
@@ -469,11 +477,17 @@ int row_lanes(int d) {
   return g;
 }
 
+// Waves of a token: more than one where tokens alone leave CUs idle (forward, 40 heads of 128: 8 tokens 3.1 us, a wave each 5.6;
+// 512 tokens 4.8 and 6.4; backward with its second kernel 7.2 and 11.1, 10.4 and 12.3).
+int token_waves(const NormRope &p) {
+  const int rows = kWave / row_lanes(p.d), steps = (p.heads[0] + p.heads[1] + rows - 1) / rows;
+  const int64_t spare = (8 * static_cast<int64_t>(device_cus()) + p.tokens - 1) / p.tokens;
+  return static_cast<int>(spare < steps ? spare : steps);
+}
+
 template <typename E, int G>
 void launch_rows(const NormRope &p, hipStream_t s) {
-  const int steps = (p.heads[0] + p.heads[1] + kWave / G - 1) / (kWave / G);
-  const int64_t spare = (8 * static_cast<int64_t>(device_cus()) + p.tokens - 1) / p.tokens;
-  const int waves = static_cast<int>(spare < steps ? spare : steps);     // of a token, where tokens alone leave CUs idle
+  const int waves = token_waves(p);
   const dim3 grid = tile_grid((p.tokens * waves + kWaves - 1) / kWaves, 1);
   if (p.interleaved)
     norm_rope_rows<E, G, true><<<grid, kWaves * kWave, 0, s>>>(p, waves);
@@ -484,9 +498,9 @@ void launch_rows(const NormRope &p, hipStream_t s) {
 template <typename E, int G>
 void launch_backward_rows(const NormRope &p, int blocks, float *partial, hipStream_t s) {
   if (p.interleaved)
-    norm_rope_backward_rows<E, G, true><<<blocks, kWaves * kWave, 0, s>>>(p, partial);
+    norm_rope_backward_rows<E, G, true><<<blocks, kWaves * kWave, 0, s>>>(p, partial, token_waves(p));
   else
-    norm_rope_backward_rows<E, G, false><<<blocks, kWaves * kWave, 0, s>>>(p, partial);
+    norm_rope_backward_rows<E, G, false><<<blocks, kWaves * kWave, 0, s>>>(p, partial, token_waves(p));
 }
 
 template <typename E>
@@ -640,7 +654,8 @@ extern "C" int intent_hip_qk_norm_rope_backward(int dtype, const void *q, const 
     p.coss = strides[6], p.sins = strides[8], p.table = table;
     p.tokens = tokens, p.heads[0] = static_cast<int>(q_heads), p.heads[1] = static_cast<int>(kv_heads);
     p.d = static_cast<int>(d), p.pairs = static_cast<int>(pairs), p.interleaved = interleaved != 0, p.eps = eps;
-    if (in_pieces(d, pairs, mixed(p, true))) blocks = static_cast<int>(std::min<int64_t>(blocks, (tokens + kWaves - 1) / kWaves));    // a wave takes a token
+    if (in_pieces(d, pairs, mixed(p, true)))
+      blocks = static_cast<int>(std::min<int64_t>(blocks, (tokens * token_waves(p) + kWaves - 1) / kWaves));      // none without a job
     if (dtype == INTENT_HIP_F16)
       launch_backward<f16_t>(p, blocks, partial, as_stream(stream));
     else
