@@ -16,6 +16,8 @@
 //   * weights: the result leaves keys 4 g .. 4 g + 3 of head r in lane (r, g), which is where the second product wants
 //     them: heads as rows, 32 keys (4 of each 16 per lane) summed over.
 //   * values: lane (c, g) loads its columns of its own 8 keys and pairs them with v_perm, for 16 columns a product.
+//     Their exponents come a key a lane and go to the lanes that use them by a permutation (8 sequences of 8191: 34.9 us with a
+//     byte a lane and key, 33.9 so).
 //   * the running maximum is raised (and the sums scaled down) only when a score passes it by 2^8, so most steps have no
 //     cross-lane move at all; weights up to 2^8 are far inside either type.
 // Bound by the cache's bytes once there are many jobs (64 sequences of 8191, 8 key heads of 128: 191 us, 5.1 TB/s; the loads
@@ -135,7 +137,8 @@ struct Step {                                     // what a lane loads for 32 ke
   uint2 k[2][D / 32];                             // [tile][8 dimensions]
   uint8_t ke[2][D / 32];
   uint2 v[8][Columns<D>::kRuns];                  // [key][run]
-  uint8_t ve[8][Columns<D>::kRuns];
+  uint8_t ve[8][Columns<D>::kRuns];               // its block's exponent; with kUniform instead:
+  uint32_t powers[2][Columns<D>::kRuns];          // [tile][run]: all exponents of key r of the tile
   int valid[2];                                   // kUniform: how many keys of a tile have a token
   unsigned live;                                  // else: a bit for each of the lane's keys of the values
 };
@@ -198,20 +201,29 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
       x.ke[u][c] = ke[keo + (g * (D / 4) + c * 8) / 32];
     }
   };
-  const auto value = [&](Step<D> &x, int i, const uint8_t *v, const uint8_t *ve, unsigned vo, unsigned veo) {
+  const auto value = [&](Step<D> &x, int i, const uint8_t *v, unsigned vo) {
 #pragma unroll
-    for (int w = 0; w < C::kWide; ++w) {
-      x.v[i][w] = *reinterpret_cast<const uint2 *>(v + vo + w * 128 + r * 8);
-      x.ve[i][w] = ve[veo + w * 4 + r / 4];
-    }
+    for (int w = 0; w < C::kWide; ++w) x.v[i][w] = *reinterpret_cast<const uint2 *>(v + vo + w * 128 + r * 8);
+    if constexpr (C::kHalf) x.v[i][C::kWide].x = *reinterpret_cast<const uint32_t *>(v + vo + C::kWide * 128 + r * 4);
+    if constexpr (C::kQuarter) x.v[i][C::kRuns - 1].x = *reinterpret_cast<const uint16_t *>(v + vo + D - 32 + r * 2);
+  };
+  const auto value_power = [&](Step<D> &x, int i, const uint8_t *ve) {
+#pragma unroll
+    for (int w = 0; w < C::kWide; ++w) x.ve[i][w] = ve[w * 4 + r / 4];
+    if constexpr (C::kHalf) x.ve[i][C::kWide] = ve[C::kWide * 4 + r / 8];
+    if constexpr (C::kQuarter) x.ve[i][C::kRuns - 1] = ve[D / 32 - 1];
+  };
+  // A tile's value exponents, key r's in lane (r, g): a load a run, where the lanes that use them would take one a key, and
+  // each touch as many lines.
+  const auto value_powers = [&](Step<D> &x, int u, const uint8_t *ve) {
+#pragma unroll
+    for (int w = 0; w < C::kWide; ++w) __builtin_memcpy(&x.powers[u][w], ve + w * 4, 4);
     if constexpr (C::kHalf) {
-      x.v[i][C::kWide].x = *reinterpret_cast<const uint32_t *>(v + vo + C::kWide * 128 + r * 4);
-      x.ve[i][C::kWide] = ve[veo + C::kWide * 4 + r / 8];
+      uint16_t two;
+      __builtin_memcpy(&two, ve + C::kWide * 4, 2);
+      x.powers[u][C::kWide] = two;
     }
-    if constexpr (C::kQuarter) {
-      x.v[i][C::kRuns - 1].x = *reinterpret_cast<const uint16_t *>(v + vo + D - 32 + r * 2);
-      x.ve[i][C::kRuns - 1] = ve[veo + D / 32 - 1];
-    }
+    if constexpr (C::kQuarter) x.powers[u][C::kRuns - 1] = ve[D / 32 - 1];
   };
 
   const auto fold = [&](Step<D> &x) {
@@ -238,13 +250,25 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
       whole = whole && live[i];
     }
     const bool all = kUniform ? x.valid[0] == 16 && x.valid[1] == 16 : __all(whole);
+    float vs[8][C::kRuns];                          // scales of the lane's columns of its keys
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int w = 0; w < C::kRuns; ++w) {
+        if constexpr (kUniform) {
+          const uint32_t word = __builtin_amdgcn_ds_bpermute((g * 4 + (i & 3)) * 4, static_cast<int>(x.powers[i >> 2][w]));
+          vs[i][w] = mx_scale(word >> (w < C::kWide ? r / 4 * 8 : C::kHalf && w == C::kWide ? r / 8 * 8 : 0) & 0xFF);
+        } else {
+          vs[i][w] = mx_scale(x.ve[i][w]);
+        }
+      }
     if (!all) {
       // What lies in places without a token has no weight, and must not turn a zero weight into NaN.
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int w = 0; w < C::kRuns; ++w)
-          if (!live[i]) x.v[i][w] = make_uint2(0, 0), x.ve[i][w] = 127;
+          if (!live[i]) x.v[i][w] = make_uint2(0, 0), vs[i][w] = 1.0f;
     }
     uint4 hi[QT], lo[QT];
 #pragma unroll
@@ -286,8 +310,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
       uint32_t pair[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float vs = mx_scale(x.ve[i][run]);
-        pair[i] = mx_pair_e4m3<E, half.value>(upper.value ? x.v[i][run].y : x.v[i][run].x, vs);
+        pair[i] = mx_pair_e4m3<E, half.value>(upper.value ? x.v[i][run].y : x.v[i][run].x, vs[i][run]);
       }
       uint32_t even[4], odd[4];
 #pragma unroll
@@ -341,9 +364,10 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
     const unsigned ks1 = static_cast<unsigned>(p.ks[1]), kes1 = static_cast<unsigned>(p.kes[1]);
     const unsigned vs1 = static_cast<unsigned>(p.vs[1]), ves1 = static_cast<unsigned>(p.ves[1]);
     const unsigned ko = r * ks1, keo = r * kes1;
-    unsigned vo[4], veo[4];
+    const unsigned veo = r * ves1;
+    unsigned vo[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vo[i] = (g * 4 + i) * vs1, veo[i] = (g * 4 + i) * ves1;
+    for (int i = 0; i < 4; ++i) vo[i] = (g * 4 + i) * vs1;
     const auto load = [&](Step<D> &x) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -357,8 +381,9 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
         look(u);
         key(x, u, k0 + (page * ks0 + in * ks1), ke0 + (page * kes0 + in * kes1), ko, keo);
         const uint8_t *const v = v0 + (page * vs0 + in * vs1), *const ve = ve0 + (page * ves0 + in * ves1);
+        value_powers(x, u, ve + veo);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) value(x, u * 4 + i, v, ve, vo[i], veo[i]);
+        for (int i = 0; i < 4; ++i) value(x, u * 4 + i, v, vo[i]);
       }
     };
     while (at[0] < tokens) {
@@ -387,7 +412,8 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x.live |= static_cast<unsigned>(find(at + u * 16 + g * 4 + i, page, in)) << (u * 4 + i);
-          value(x, u * 4 + i, p.v + page * p.vs[0] + in * p.vs[1] + kh * p.vs[2], p.ve + page * p.ves[0] + in * p.ves[1] + kh * p.ves[2], 0, 0);
+          value(x, u * 4 + i, p.v + page * p.vs[0] + in * p.vs[1] + kh * p.vs[2], 0);
+          value_power(x, u * 4 + i, p.ve + page * p.ves[0] + in * p.ves[1] + kh * p.ves[2]);
         }
       }
       any = any || __any(x.live != 0);
