@@ -89,6 +89,7 @@ class OperatorSpec:
     plan: Callable
     inplace_safe: bool = False    # an Out may be exactly one of the inputs (same address and strides)
     derived: tuple = ()           # (symbol, source symbol, offset): extent(symbol) = extent(source) + offset
+    repeats: bool = False         # its launches can be made again for other arguments of their layout (Launch.again)
 
     @property
     def entry_point(self) -> str:
@@ -1222,6 +1223,7 @@ def _linear_mxfp4(dtype_code):
     return plan
 
 
+_repeated = functools.partial(OperatorSpec, repeats=True)
 _SPECS = (
     OperatorSpec("stable_softmax", (_view(IN, "f32", 2), _view(OUT, "f32", 2)), (), _softmax_fwd(F32), True),
     OperatorSpec("stable_softmax_f16", (_view(IN, "f16", 2), _view(OUT, "f16", 2)), (), _softmax_fwd(F16), True),
@@ -1297,21 +1299,21 @@ _SPECS = (
                               _view(OUT, "f32", 2)), (), _csr_spmm, derived=(("R", "R1", -1),)),
     OperatorSpec("csr_spmv", (_view(IN, "i32", 1), _view(IN, "i32", 1), _view(IN, "f32", 1), _view(IN, "f32", 1),
                               _view(OUT, "f32", 1)), (), _csr_spmv, derived=(("R", "R1", -1),)),
-    OperatorSpec("qk_norm_rope_f16", _norm_rope_signature("f16", False), ("INTERLEAVED",), _norm_rope(F16)),
-    OperatorSpec("qk_norm_rope_bf16", _norm_rope_signature("bf16", False), ("INTERLEAVED",), _norm_rope(BF16)),
-    OperatorSpec("qk_norm_rope_backward_f16", _norm_rope_signature("f16", True), ("INTERLEAVED",), _norm_rope_backward(F16)),
-    OperatorSpec("qk_norm_rope_backward_bf16", _norm_rope_signature("bf16", True), ("INTERLEAVED",),
-                 _norm_rope_backward(BF16)),
-    OperatorSpec("paged_cache_append_f16", _append_signature("f16"), (), _paged_cache(F16, False)),
-    OperatorSpec("paged_cache_append_bf16", _append_signature("bf16"), (), _paged_cache(BF16, False)),
-    OperatorSpec("paged_cache_read_f16", _read_signature("f16"), (), _paged_cache(F16, True)),
-    OperatorSpec("paged_cache_read_bf16", _read_signature("bf16"), (), _paged_cache(BF16, True)),
-    OperatorSpec("paged_gqa_decode_mx_f16", _decode_mx_signature("f16"), ("HEAD_GROUP",), _paged_decode_mx(F16)),
-    OperatorSpec("paged_gqa_decode_mx_bf16", _decode_mx_signature("bf16"), ("HEAD_GROUP",), _paged_decode_mx(BF16)),
-    OperatorSpec("linear_mxfp4_f16", (_view(IN, "f16", 2), _view(IN, "u8", 2), _view(IN, "u8", 2), _view(OUT, "f16", 2)), (),
-                 _linear_mxfp4(F16)),
-    OperatorSpec("linear_mxfp4_bf16", (_view(IN, "bf16", 2), _view(IN, "u8", 2), _view(IN, "u8", 2), _view(OUT, "bf16", 2)), (),
-                 _linear_mxfp4(BF16)),
+    _repeated("qk_norm_rope_f16", _norm_rope_signature("f16", False), ("INTERLEAVED",), _norm_rope(F16)),
+    _repeated("qk_norm_rope_bf16", _norm_rope_signature("bf16", False), ("INTERLEAVED",), _norm_rope(BF16)),
+    _repeated("qk_norm_rope_backward_f16", _norm_rope_signature("f16", True), ("INTERLEAVED",), _norm_rope_backward(F16)),
+    _repeated("qk_norm_rope_backward_bf16", _norm_rope_signature("bf16", True), ("INTERLEAVED",),
+              _norm_rope_backward(BF16)),
+    _repeated("paged_cache_append_f16", _append_signature("f16"), (), _paged_cache(F16, False)),
+    _repeated("paged_cache_append_bf16", _append_signature("bf16"), (), _paged_cache(BF16, False)),
+    _repeated("paged_cache_read_f16", _read_signature("f16"), (), _paged_cache(F16, True)),
+    _repeated("paged_cache_read_bf16", _read_signature("bf16"), (), _paged_cache(BF16, True)),
+    _repeated("paged_gqa_decode_mx_f16", _decode_mx_signature("f16"), ("HEAD_GROUP",), _paged_decode_mx(F16)),
+    _repeated("paged_gqa_decode_mx_bf16", _decode_mx_signature("bf16"), ("HEAD_GROUP",), _paged_decode_mx(BF16)),
+    _repeated("linear_mxfp4_f16", (_view(IN, "f16", 2), _view(IN, "u8", 2), _view(IN, "u8", 2), _view(OUT, "f16", 2)), (),
+              _linear_mxfp4(F16)),
+    _repeated("linear_mxfp4_bf16", (_view(IN, "bf16", 2), _view(IN, "u8", 2), _view(IN, "u8", 2), _view(OUT, "bf16", 2)), (),
+              _linear_mxfp4(BF16)),
 )
 
 SPECS = {spec.name: spec for spec in _SPECS}

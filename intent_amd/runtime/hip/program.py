@@ -157,7 +157,7 @@ class HipProgram:
                                     for i, left in enumerate(views) for right in views[i + 1:]
                                     if left.writable or right.writable)
         # What calls of one layout share, of the last layouts seen (prepare_call); None where the plan offers nothing to share.
-        self._layouts: dict | None = None if self._binding.related else {}
+        self._layouts: dict | None = {} if spec.repeats and not self._binding.related else None
         self._view_places = tuple(tuple(isinstance(p, ViewParameter) for p in parameters)
                                   for parameters in (interface.inputs, (*interface.inputs, *interface.outputs)))
         # Where each parameter stands among the inputs followed by the Out buffers.
@@ -210,13 +210,10 @@ class HipProgram:
         self._check_writable_overlap(bound)
         with plan_policies(self.workspace, self.numerics, self.tuning_rows):
             launch = self.spec.plan(self.library, bound, self.constexprs, self.device)
-        if launch.again is not None:
-            if key is not None:
-                if len(layouts) >= _LAYOUTS_KEPT:
-                    layouts = self._layouts = {}
-                layouts[key] = _Layout(self.interface, bound, outputs is not None, self._written_pairs, launch.again)
-        elif not launch.before and not launch.after:
-            self._layouts = None
+        if key is not None and launch.again is not None:
+            if len(layouts) >= _LAYOUTS_KEPT:
+                layouts = self._layouts = {}
+            layouts[key] = _Layout(self.interface, bound, outputs is not None, self._written_pairs, launch.again)
         return HipPreparedCall(self, bound, launch)
 
     def _layout_key(self, arguments, outputs):
