@@ -420,9 +420,17 @@ void launch(Linear p, const Cut &c, hipStream_t s) {
     linear_fold<E, 1><<<tile_grid((all + 255) / 256, 1), 256, 0, s>>>(p);
 }
 
+int check(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 0 || k < 0) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "negative extent");
+  if (k % kMxBlock)
+    return fail(INTENT_HIP_ERR_UNSUPPORTED, "weights are blocks of %d elements (got K = %lld)", kMxBlock, static_cast<long long>(k));
+  if (m > (1 << 20) || n > (1 << 24) || k > INT32_MAX / 64) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
+  return INTENT_HIP_OK;
+}
 }  // namespace
 
 int linear_mxfp4_resources(int dtype, int64_t m, int64_t n, int64_t k, IntentHipKernelResources *out) {
+  if (int rc = check(m, n, k)) return rc;
   const Cut c = cut(m, n, k);
   const auto describe = [&](void (*kernel)(Linear), const char *which, int waves) {
     char name[64];
@@ -435,16 +443,6 @@ int linear_mxfp4_resources(int dtype, int64_t m, int64_t n, int64_t k, IntentHip
 }  // namespace intent_hip
 
 using namespace intent_hip;
-
-namespace {
-int check(int64_t m, int64_t n, int64_t k) {
-  if (m < 0 || n < 0 || k < 0) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "negative extent");
-  if (k % kMxBlock)
-    return fail(INTENT_HIP_ERR_UNSUPPORTED, "weights are blocks of %d elements (got K = %lld)", kMxBlock, static_cast<long long>(k));
-  if (m > (1 << 20) || n > (1 << 24) || k > INT32_MAX / 64) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
-  return INTENT_HIP_OK;
-}
-}  // namespace
 
 extern "C" int intent_hip_linear_mxfp4_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t *bytes) {
   if (bytes == nullptr) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null output");

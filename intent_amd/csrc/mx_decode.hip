@@ -634,6 +634,8 @@ bool width_ok(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 192 || 
 int mx_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t positions,
                         IntentHipKernelResources *out) {
   if (group < 1 || !width_ok(d)) return fail(INTENT_HIP_ERR_UNSUPPORTED, "mx decode has no head width %lld", static_cast<long long>(d));
+  if (int rc = check_extents(batch, kv_heads * group, kv_heads, group, d, 0, ps, positions)) return rc;
+  if (ps == 0) ps = 1;                             // a cache without a token
   const Cut c = cut(batch, kv_heads, group, positions, ps);
   const bool uniform = ps % 16 == 0;
   char name[64];

@@ -538,6 +538,7 @@ void launch_backward(const NormRope &p, int blocks, float *partial, hipStream_t 
 
 int norm_rope_resources(int dtype, int backward, int64_t d, int64_t pairs, int interleaved, uint64_t mix,
                         IntentHipKernelResources *out) {
+  if (d < 0 || d > kMaxWidth) return fail(INTENT_HIP_ERR_UNSUPPORTED, "qk_norm_rope takes heads of up to %d dimensions", kMaxWidth);
   const char *const type = dtype == INTENT_HIP_F16 ? "f16" : "bf16";
   char name[64];
   const auto describe = [&](const void *half, const void *brain) {

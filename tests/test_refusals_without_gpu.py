@@ -133,3 +133,20 @@ def test_linear_mxfp4():
     assert call(m=100, n=64, k=4096, ldx=4096, ldw=2048, lde=128, ldy=64) == 5 and b"workspace" in err()
     assert call(m=100, n=64, k=4096, ldx=4096, ldw=2048, lde=128, ldy=64, workspace=256, size=size.value - 1) == 5
     assert query(4, 8, 48, ctypes.byref(size)) == 2 and query(4, 8, 64, None) == 1
+
+
+def test_facts_of_odd_calls():
+    """The resource entry points take any sizes: an answer (where there is a GPU) or an error, never the end of the process."""
+    lib = hiplib.library()
+    out = hiplib.KernelResources()
+    ask = lambda op, *f: lib.fn["call_resources"](op, BF16, (ctypes.c_int64 * len(f))(*f), len(f), ctypes.byref(out))  # noqa: E731
+    for op, calls in ((hiplib.OP_PAGED_GQA_DECODE_MX, ((4, 2, 4, 128, 0, 9), (0, 0, 1, 64, 16, 0), (1, 1, 0, 64, 16, 1), (4, 2, 4, 100, 16, 9),
+                                                       (-1, 2, 4, 128, 16, 9), (4, 2, 4, 128, 2 ** 40, 2 ** 40), (1, 1, 1, 64, -16, 1))),
+                      (hiplib.OP_LINEAR_MXFP4, ((0, 0, 0), (-1, 4, 32), (2 ** 40, 2 ** 40, 32), (1, 1, 33))),
+                      (hiplib.OP_QK_NORM_ROPE, ((2 ** 31 - 16, 8, 0, 0), (2 ** 40, 8, 0, 0), (-16, 0, 0, 0), (0, 0, 0, 0), (1025, 0, 0, 1)))):
+        for f in calls:
+            ask(op, *f)
+            assert ask(op, *f[:-1]) == 1
+    for f in ((1, 1, 0, 64, 16, 1), (-1, 2, 4, 128, 16, 9), (4, 2, 4, 128, 2 ** 40, 2 ** 40), (1, 1, 1, 64, -16, 1)):
+        assert ask(hiplib.OP_PAGED_GQA_DECODE_MX, *f) in (1, 2)
+    assert ask(hiplib.OP_QK_NORM_ROPE, 2 ** 31 - 16, 8, 0, 0) == 2 and ask(hiplib.OP_LINEAR_MXFP4, 1, 1, 33) == 2
