@@ -12,7 +12,7 @@
 // A wave takes a piece of 512 elements of up to 4 consecutive rows, all on their way at once: where its lanes' elements lie in
 // a row is found once, and the tables are asked again only where a sequence or a page ends. Consecutive rows stay on one XCD,
 // so the exponents of a page's tokens, which share lines, leave its L2 together. Bound by bytes (8 prompts of up to 8191, 8 key
-// heads of 128: appended in 33.5 us, 4.4 TB/s; read in 31, 4.7 TB/s); a token for each of 32 sequences by latency, 3.3 us.
+// heads of 128: appended in 28.9 us, 5.1 TB/s; read in 31, 4.7 TB/s); a token for each of 32 sequences by latency, 3.3 us.
 #include <stdio.h>
 
 #include "mx.hpp"
@@ -21,6 +21,8 @@ namespace intent_hip {
 namespace {
 
 constexpr int kWaves = 4;
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 struct Rows {
   uint16_t *rows[2];                 // keys, values
@@ -101,7 +103,10 @@ __device__ __forceinline__ uint32_t dpp_bits(uint32_t v) {
   return __builtin_amdgcn_update_dpp(0, v, kCtrl, 0xF, 0xF, false);
 }
 
-// R: consecutive rows that a wave holds at once.
+// R: consecutive rows that a wave holds at once. The elements of many rows (R > 1) are more than the L2s hold and pass them by
+// (33.6 -> 28.9 us; with a reader of the rows behind it 65.2 -> 60.3). Not the exponents, whose bytes would reach memory one by
+// one (35), nor what cache_read writes: alone it would take 23.6 us instead of 34.8, with the reader of its rows, who then finds
+// none of them on the chip, 66.0 instead of 62.5.
 template <typename E, int R>
 __global__ __launch_bounds__(kWaves * kWave) void cache_append(Rows p) {
   constexpr uint32_t kMagnitude = 0x7FFF7FFFu, kInfinity = __is_same(E, f16_t) ? 0x7C00u : 0x7F80u;
@@ -146,7 +151,11 @@ __global__ __launch_bounds__(kWaves * kWave) void cache_append(Rows p) {
     const float scale = mx_scale(exponent);
     const uint2 out = make_uint2(mx_quad_e4m3<E>(words[0], words[1], scale), mx_quad_e4m3<E>(words[2], words[3], scale));
     if (!at.live) continue;
-    *reinterpret_cast<uint2 *>(at.cache + page[i] * at.page_stride + slot[i] * at.slot_stride) = out;
+    uint8_t *const to = at.cache + page[i] * at.page_stride + slot[i] * at.slot_stride;
+    if constexpr (R > 1)
+      __builtin_nontemporal_store(u32x2_t{out.x, out.y}, reinterpret_cast<u32x2_t *>(to));
+    else
+      *reinterpret_cast<uint2 *>(to) = out;
     if (at.first) at.exponents[page[i] * at.page_exponents + slot[i] * at.slot_exponents] = static_cast<uint8_t>(exponent);
   }
 }
@@ -185,8 +194,8 @@ __global__ __launch_bounds__(kWaves * kWave) void cache_read(Rows p) {
   }
 }
 
-// Rows of a wave: four where that still leaves every CU its 32 waves (23585 rows of 8 + 8 heads of 128: appended in 33.7 us, one
-// row a wave 43.5; read in 34.9 and 54.3), else one (32 rows: 4.4 us with the launch, four 5.7).
+// Rows of a wave: four where that still leaves every CU its 32 waves (23585 rows of 8 + 8 heads of 128: appended in 33.7 us before
+// its stores passed the L2s by, one row a wave 43.5; read in 34.9 and 54.3), else one (32 rows: 4.4 us with the launch, four 5.7).
 int together(int64_t rows, int64_t pieces) { return rows * pieces < 128 * device_cus() ? 1 : 4; }
 
 // strides: k[3], v[3], then per cache its elements [4] and exponents [4].
