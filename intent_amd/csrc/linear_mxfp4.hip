@@ -7,7 +7,7 @@
 // so lane (r, g) takes block g of four of weight row r as it lies in memory (16 bytes, one exponent), converts it in four
 // parts, and reads the same 32 values of its row of x. Weights go from memory to registers: no wave needs another's.
 //   * linear_few, up to 16 rows of x: a workgroup's 16 waves take a run of K each and add their sums through the LDS. Bound by
-//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 9.7 us, 3.2 TB/s; without x and the
+//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 9.2 us, 3.4 TB/s; without x and the
 //     exponents' loads 6.7; 1 x 4096 x 4096: 5.0, most of it latency: one or two steps a wave).
 //   * linear_tiles: a workgroup's waves share 16 MT rows of x, which pass through the LDS 128 columns at a time (in 16-byte
 //     units, unit u of row r at u ^ r % 16, so that the 16 rows of a read are in different banks), and take 16 NT weight
@@ -96,8 +96,9 @@ __device__ __forceinline__ void store(const Linear &p, int m, int n, const float
 }
 
 // Up to 16 rows of x by 16 NT weight rows a workgroup; its 16 waves take a run of K each. The loads of kAhead steps of 128
-// columns are on their way at once, a weight row's exponents for all of them in one. Columns of the product behind the rows of
-// x are never stored, so their lanes read any row.
+// columns are on their way at once, the exponents of all weight rows in one, which a lane permutation brings to where they are
+// needed (1 x 14336 x 4096: 10.0 us with a load a weight row, 9.2 so; 16 x 14336 x 4096: 12.8 and 12.2). Columns of the product
+// behind the rows of x are never stored, so their lanes read any row.
 template <typename E, int NT>
 __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
   constexpr int kAhead = 2, kSums = NT * 4;
@@ -105,13 +106,11 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = static_cast<int>(blockIdx.x) * 16 * NT;
-  const uint8_t *w[NT], *e[NT];
+  const uint8_t *w[NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int64_t row = min(n0 + r * NT + j, p.n - 1);         // rows behind the last are not stored
-    w[j] = p.w + row * p.ldw + g * 16;
-    e[j] = p.e + row * p.lde;
-  }
+  for (int j = 0; j < NT; ++j)         // rows behind the last are not stored
+    w[j] = p.w + static_cast<int64_t>(min(n0 + r * NT + j, p.n - 1)) * p.ldw + g * 16;
+  const uint8_t *const e = p.e + static_cast<int64_t>(min(n0 + r * NT + g % NT, p.n - 1)) * p.lde;
   const uint16_t *x = p.x + min(r, p.m - 1) * p.ldx + g * 32;
   f32x4_t acc[NT];
 #pragma unroll
@@ -119,8 +118,19 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
   const int first = min(wave * p.stages * 4, p.blocks), last = min(first + p.stages * 4, p.blocks);
   for (int b0 = first; b0 < last; b0 += kAhead * 4) {
     uint4 raw[kAhead][NT], v[kAhead][4];
-    uint32_t power[NT][kAhead];        // of step i: word i
+    uint32_t power[kAhead];            // of step i: word i, of weight row r NT + g in lane (r, g)
     const bool whole = b0 + kAhead * 4 <= last;
+    if (b0 + kAhead * 4 <= p.blocks) {
+      if (g < NT) __builtin_memcpy(power, e + b0, sizeof(power));
+    } else {                           // behind K any
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        uint32_t byte[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) byte[t] = e[min(b0 + i * 4 + t, p.blocks - 1)];
+        power[i] = byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int b = b0 + i * 4;
@@ -136,23 +146,12 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
       }
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if (whole) {
-        __builtin_memcpy(power[j], e[j] + b0, sizeof(power[j]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          power[j][i] = 0x7F7F7F7Fu;
-          if (b0 + i * 4 + g < last) power[j][i] = static_cast<uint32_t>(e[j][b0 + i * 4 + g]) << (8 * g);
-        }
-      }
-    }
-#pragma unroll
     for (int i = 0; i < kAhead; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const uint32_t words[4] = {raw[i][j].x, raw[i][j].y, raw[i][j].z, raw[i][j].w};
-        const float scale = mx_scale(power[j][i] >> (8 * g) & 0xFF);
+        const uint32_t word = __builtin_amdgcn_ds_bpermute((j * 16 + r) * 4, static_cast<int>(power[i]));
+        const float scale = mx_scale(whole || b0 + i * 4 + g < last ? word >> (8 * g) & 0xFF : 127);
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[j] = mfma<E>(eight<E>(words[c], scale), v[i][c], acc[j]);
       }
