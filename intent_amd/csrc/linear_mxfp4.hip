@@ -7,8 +7,8 @@
 // so lane (r, g) takes block g of four of weight row r as it lies in memory (16 bytes, one exponent), converts it in four
 // parts, and reads the same 32 values of its row of x. Weights go from memory to registers: no wave needs another's.
 //   * linear_few, up to 16 rows of x: a workgroup's 16 waves take a run of K each and add their sums through the LDS. Bound by
-//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 9.2 us, 3.4 TB/s; without x and the
-//     exponents' loads 6.7; 1 x 4096 x 4096: 5.0, most of it latency: one or two steps a wave).
+//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 7.9 us, 4.0 TB/s; 16 x 14336 x 4096:
+//     12.2; 1 x 4096 x 4096: 3.7, most of it latency: one or two steps a wave).
 //   * linear_tiles: a workgroup's waves share 16 MT rows of x, which pass through the LDS 128 columns at a time (in 16-byte
 //     units, unit u of row r at u ^ r % 16, so that the 16 rows of a read are in different banks), and take 16 NT weight
 //     rows each. A lane's weight rows are NT apart, so its results are 4 NT consecutive columns of y. Where tiles are few, K
@@ -99,7 +99,18 @@ __device__ __forceinline__ void store(const Linear &p, int m, int n, const float
 // columns are on their way at once, the exponents of all weight rows in one, which a lane permutation brings to where they are
 // needed (1 x 14336 x 4096: 10.0 us with a load a weight row, 9.2 so; 16 x 14336 x 4096: 12.8 and 12.2). Columns of the product
 // behind the rows of x are never stored, so their lanes read any row.
-template <typename E, int NT>
+//
+// kOne: x is one row. Its 128 columns of a step are a word a lane, and every lane takes the 16 words of its block from the lanes
+// of its row of 16: loads of 16 bytes a lane, 16 times each value, hold up the weights' (1 x 4096 x 14336: 10.5 and 8.6 us; 1 x 14336 x
+// 4096: 9.2 and 7.9; 1 x 128256 x 4096: 53.6, 5.2 TB/s).
+template <int kFirst>
+__device__ __forceinline__ uint4 words_of_row(uint32_t own) {
+  const int v = static_cast<int>(own);
+  return make_uint4(__builtin_amdgcn_update_dpp(0, v, 0x150 + kFirst, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, v, 0x151 + kFirst, 0xF, 0xF, false),
+                    __builtin_amdgcn_update_dpp(0, v, 0x152 + kFirst, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, v, 0x153 + kFirst, 0xF, 0xF, false));
+}
+
+template <typename E, int NT, bool kOne>
 __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
   constexpr int kAhead = 2, kSums = NT * 4;
   __shared__ float sums[kFewWaves][kSums][kWave];
@@ -111,13 +122,14 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
   for (int j = 0; j < NT; ++j)         // rows behind the last are not stored
     w[j] = p.w + static_cast<int64_t>(min(n0 + r * NT + j, p.n - 1)) * p.ldw + g * 16;
   const uint8_t *const e = p.e + static_cast<int64_t>(min(n0 + r * NT + g % NT, p.n - 1)) * p.lde;
-  const uint16_t *x = p.x + min(r, p.m - 1) * p.ldx + g * 32;
+  const uint16_t *x = kOne ? p.x + g * 32 + r * 2 : p.x + min(r, p.m - 1) * p.ldx + g * 32;
   f32x4_t acc[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j] = f32x4_t{0, 0, 0, 0};
   const int first = min(wave * p.stages * 4, p.blocks), last = min(first + p.stages * 4, p.blocks);
   for (int b0 = first; b0 < last; b0 += kAhead * 4) {
     uint4 raw[kAhead][NT], v[kAhead][4];
+    uint32_t one[kAhead];
     uint32_t power[kAhead];            // of step i: word i, of weight row r NT + g in lane (r, g)
     const bool whole = b0 + kAhead * 4 <= last;
     if (b0 + kAhead * 4 <= p.blocks) {
@@ -139,14 +151,23 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
         raw[i][j] = make_uint4(0, 0, 0, 0);
         if (whole || b + g < last) raw[i][j] = *reinterpret_cast<const uint4 *>(w[j] + b * 16);
       }
+      if constexpr (kOne) {
+        one[i] = 0;
+        if (whole || b + g < last) one[i] = *reinterpret_cast<const uint32_t *>(x + b * 32);
+      } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        v[i][c] = make_uint4(0, 0, 0, 0);
-        if (whole || b + g < last) v[i][c] = *reinterpret_cast<const uint4 *>(x + b * 32 + c * 8);
+        for (int c = 0; c < 4; ++c) {
+          v[i][c] = make_uint4(0, 0, 0, 0);
+          if (whole || b + g < last) v[i][c] = *reinterpret_cast<const uint4 *>(x + b * 32 + c * 8);
+        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
+    for (int i = 0; i < kAhead; ++i) {
+      if constexpr (kOne) {
+        v[i][0] = words_of_row<0>(one[i]), v[i][1] = words_of_row<4>(one[i]);
+        v[i][2] = words_of_row<8>(one[i]), v[i][3] = words_of_row<12>(one[i]);
+      }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const uint32_t words[4] = {raw[i][j].x, raw[i][j].y, raw[i][j].z, raw[i][j].w};
@@ -155,6 +176,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[j] = mfma<E>(eight<E>(words[c], scale), v[i][c], acc[j]);
       }
+    }
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -354,18 +376,19 @@ __global__ __launch_bounds__(256) void linear_fold(Linear p) {
 
 // How a product is cut.
 struct Cut {
-  int mt, nt, parts;                   // mt = 0: linear_few
+  int mt, nt, parts;                   // mt = 0: linear_few; 1: of one row
 };
 constexpr int tile_waves(int mt) { return mt == 2 ? 8 : 4; }
 
 // linear_few for up to 16 rows, NT by the weight rows there are for the workgroups (16 x 14336 x 4096: NT = 1 23.8 us, 2 16.9,
-// 4 12.7; 1 x 4096 x 14336: 10.7, 15.7, 25.8). Where more than eight rows meet a long K and few weight rows, x read once per
+// 4 12.7; 2 x 4096 x 14336: 11.3, 16.4, 26.7; one row of 14336 x 4096: 8.7, 7.8, 8.7, of 4096 x 4096: 3.6, 4.7, 6.9). Where more than eight rows meet a long K and few weight rows, x read once per
 // 16 weight rows costs more than the weights (16 x 4096 x 14336: 19.8 us, in tiles 15.5).
 // linear_tiles otherwise, by an estimate from what its tiles measured: us a stage takes a workgroup that has a CU for itself,
 // and each of several on a CU, and what writing, reading and adding the parts' sums takes. It is within a fifth of the best of
 // all tiles and parts at M of 17 to 1021 and N x K of 1000 x 4096 to 28672 x 8192.
 Cut cut(int64_t m, int64_t n, int64_t k) {
   const int cus = device_cus();
+  if (m == 1) return {1, n >= 24 * cus ? 2 : 1, 1};
   if (m <= 16 && (m <= 8 || n >= 24 * cus || k < 6144)) return {0, n >= 48 * cus ? 4 : n >= 24 * cus ? 2 : 1, 1};
   constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.53f, 0.5f}, {4, 2, 0.9f, 0.7f}, {8, 2, 1.3f, 0.9f}, {8, 4, 2.1f, 1.67f}};
   const int64_t stages = (k + 127) / 128;
@@ -378,7 +401,7 @@ Cut cut(int64_t m, int64_t n, int64_t k) {
       const float on_one = static_cast<float>((tiles * parts + cus - 1) / cus), shared = kind.shared * on_one;
       float us = static_cast<float>((stages + parts - 1) / parts) * (kind.alone > shared ? kind.alone : shared);
       if (parts > 1) us += 3.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(n) * 2.3e-6f;
-      if (best.mt == 0 || us < least) best = {kind.mt, kind.nt, parts}, least = us;
+      if (best.parts == 0 || us < least) best = {kind.mt, kind.nt, parts}, least = us;
     }
   }
   return best;
@@ -388,9 +411,10 @@ Cut cut(int64_t m, int64_t n, int64_t k) {
 template <typename E, typename F>
 int with_kernel(const Cut &c, F f) {
   if (c.mt == 0)
-    return c.nt == 1   ? f(linear_few<E, 1>, "linear_few", kFewWaves)
-           : c.nt == 2 ? f(linear_few<E, 2>, "linear_few", kFewWaves)
-                       : f(linear_few<E, 4>, "linear_few", kFewWaves);
+    return c.nt == 1   ? f(linear_few<E, 1, false>, "linear_few", kFewWaves)
+           : c.nt == 2 ? f(linear_few<E, 2, false>, "linear_few", kFewWaves)
+                       : f(linear_few<E, 4, false>, "linear_few", kFewWaves);
+  if (c.mt == 1) return c.nt == 1 ? f(linear_few<E, 1, true>, "linear_few", kFewWaves) : f(linear_few<E, 2, true>, "linear_few", kFewWaves);
   return c.mt == 2   ? f(linear_tiles<E, 2, 1, 4, tile_waves(2)>, "linear_tiles", tile_waves(2))
          : c.mt == 4 ? f(linear_tiles<E, 4, 2, 4, tile_waves(4)>, "linear_tiles", tile_waves(4))
          : c.nt == 2 ? f(linear_tiles<E, 8, 2, 2, tile_waves(8)>, "linear_tiles", tile_waves(8))
@@ -401,10 +425,10 @@ template <typename E>
 void launch(Linear p, const Cut &c, hipStream_t s) {
   p.parts = c.parts;
   with_kernel<E>(c, [&](void (*kernel)(Linear), const char *, int waves) {
-    const int runs = c.mt == 0 ? waves : c.parts;
+    const int runs = c.mt <= 1 ? waves : c.parts;
     p.stages = ((p.blocks + 3) / 4 + runs - 1) / runs;
     dim3 grid(static_cast<unsigned>((p.n + 16 * c.nt - 1) / (16 * c.nt)));
-    if (c.mt > 0) {
+    if (c.mt > 1) {
       p.m_tiles = (p.m + 16 * c.mt - 1) / (16 * c.mt), p.n_tiles = (p.n + 16 * waves * c.nt - 1) / (16 * waves * c.nt);
       grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.parts, 1);
     }

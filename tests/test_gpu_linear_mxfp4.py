@@ -174,6 +174,15 @@ def test_refusals(device):
         static.run(*(a.to(device) for a in case(2, "f16", 100, 64, 4096)))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,k", [(1, 32), (6143, 96), (6145, 96), (6150, 4128), (33, 8224), (100, 4064), (7000, 64)])
+def test_one_row(device, dtype, n, k):
+    """A single row of x: both sizes of its kernel, runs of K that end inside a step, weight rows behind the last."""
+    announce("linear mxfp4 one row", dtype, n, k)
+    x, weight, exponents = case(n + k, dtype, 1, n, k)
+    check(kernel(dtype).run(x.to(device), weight.to(device), exponents.to(device)), x, weight, exponents, dtype)
+
+
 @pytest.mark.parametrize("m", [1, 20])
 def test_weights_beyond_32_bits(device, m):
     announce("linear mxfp4 beyond 32 bits", m)
