@@ -3,8 +3,11 @@
 //
 // For query head h of sequence s, over the positions j below lengths[s] that the tables have a page for:
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = exp2(scale * log2(e) * (q . k_j) - peak)        0 where there is none
-// Keys and values are taken in the query's type (element * 2^e, one rounding), products are summed in f32, weights enter
-// the second product in two parts (the 16-bit rounding of w and of what it left), so its rounding is below f32's.
+// Keys and values are taken in the query's type (element * 2^e, one rounding) and products are summed in f32. Weights are f32
+// and enter the second product whole, as three bf16 numbers of 8 bits each: f16 numbers end at 2^-24, and the sum that the
+// products are divided by holds the weights below. Two bf16 numbers would leave out 2^-16 of a weight; the third costs up to 4 %
+// where jobs are few (8 sequences of 8191, f16: 35.2 us, 34.2 with two f16 numbers) and nothing where they are many (64 ragged
+// sequences up to 8191, bf16: 135.2 and 135.2). The values are bf16 numbers exactly: e4m3 has four bits.
 //
 // Design. The page range of a sequence is cut into jobs of `job_pages` pages; job j of the flat list belongs to the last
 // sequence s with page_offsets[s] / job_pages + s <= j, which every wave finds by itself, so no table of work is made and
@@ -33,6 +36,7 @@ namespace intent_hip {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kParts = 3;              // bf16 numbers of a weight
 constexpr int kStep = 32;              // keys of a wave's step: two tiles of 16
 constexpr float kSlack = 8.0f;
 constexpr float kNoToken = -1.0f;      // the sum of a state without a token (weights are not negative)
@@ -42,6 +46,7 @@ constexpr int kLong = 256;            // tokens of a job: from here on it is one
 constexpr int kLeast = 128;
 constexpr int kWhole = 2048, kWholeOne = 768;   // tokens of all sequences and of one, up to here each is one job
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -66,19 +71,19 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// Two non-negative weights in two parts of type E each: `high` cut off to its bits, `low` what that left, cut off too; 2^-20
-// (f16) and 2^-14 (bf16) of a weight are left out.
-template <typename E>
-__device__ __forceinline__ void parts(float a, float b, uint32_t &high, uint32_t &low) {
-  if constexpr (std::is_same_v<E, f16_t>) {
-    const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-    high = __builtin_bit_cast(uint32_t, h);
-    low = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(h[0]), b - static_cast<float>(h[1])));
-  } else {
+// Two f32 in bf16, rounded to nearest even.
+__device__ __forceinline__ uint32_t in_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bfloat2_t));
+}
+
+// Two weights as sums of kParts bf16 numbers each: 8 bits of what the numbers before leave, cut off, so that three hold all 24
+// and none is negative.
+__device__ __forceinline__ void parts(float a, float b, uint32_t (&part)[kParts]) {
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
     const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
-    high = __builtin_amdgcn_perm(v, u, 0x07060302);
-    low = __builtin_amdgcn_perm(__float_as_uint(b - __uint_as_float(v & 0xFFFF0000u)), __float_as_uint(a - __uint_as_float(u & 0xFFFF0000u)),
-                                0x07060302);
+    part[i] = __builtin_amdgcn_perm(v, u, 0x07060302);
+    a -= __uint_as_float(u & 0xFFFF0000u), b -= __uint_as_float(v & 0xFFFF0000u);
   }
 }
 
@@ -262,6 +267,22 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
           vs[i][w] = mx_scale(x.ve[i][w]);
         }
       }
+    // f16: whether a value may be one that it rounds or holds as infinity: exponents outside -15 .. 7, asked of all exponents in a
+    // few comparisons of bits, which take -15 .. 0 as certain.
+    constexpr bool kF16 = std::is_same_v<E, f16_t>;
+    constexpr uint32_t kSure = 0x70707070u, kAsked = kF16 ? 0xF0F0F0F0u : 0u;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int w = 0; w < C::kRuns; ++w) {
+      if constexpr (kUniform) {
+        const uint32_t bytes = w < C::kWide ? ~0u : C::kHalf && w == C::kWide ? 0xFFFFu : 0xFFu;
+        odd |= ((x.powers[0][w] ^ kSure) | (x.powers[1][w] ^ kSure)) & bytes;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) odd |= x.ve[i][w] ^ (kSure & 0xFFu);
+      }
+    }
+    const bool extreme = __any((odd & kAsked) != 0);
     if (!all) {
       // What lies in places without a token has no weight, and must not turn a zero weight into NaN.
 #pragma unroll
@@ -270,7 +291,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
         for (int w = 0; w < C::kRuns; ++w)
           if (!live[i]) x.v[i][w] = make_uint2(0, 0), vs[i][w] = 1.0f;
     }
-    uint4 hi[QT], lo[QT];
+    uint4 wp[QT][kParts];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       float z[8];
@@ -299,19 +320,28 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = live[i] ? w[i] : 0.0f;
       total[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-      uint32_t h[4], l[4];
+      uint32_t part[4][kParts];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) parts<E>(w[2 * i], w[2 * i + 1], h[i], l[i]);
-      hi[t] = make_uint4(h[0], h[1], h[2], h[3]);
-      lo[t] = make_uint4(l[0], l[1], l[2], l[3]);
+      for (int i = 0; i < 4; ++i) parts(w[2 * i], w[2 * i + 1], part[i]);
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) wp[t][i] = make_uint4(part[0][i], part[1][i], part[2][i], part[3][i]);
     }
     // Values: pairs of columns of each key, paired again over the keys.
     const auto columns = [&](int run, int tile, auto upper, auto half) {
       uint32_t pair[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        pair[i] = mx_pair_e4m3<E, half.value>(upper.value ? x.v[i][run].y : x.v[i][run].x, vs[i][run]);
+        const uint32_t word = upper.value ? x.v[i][run].y : x.v[i][run].x;
+        pair[i] = mx_pair_e4m3<bf16_t, half.value>(word, vs[i][run]);
       }
+      if constexpr (kF16)
+        if (__builtin_expect(extreme, 0))           // by way of f16
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t word = upper.value ? x.v[i][run].y : x.v[i][run].x;
+            const half2_t h = __builtin_bit_cast(half2_t, mx_pair_e4m3<f16_t, half.value>(word, vs[i][run]));
+            pair[i] = in_bf16(static_cast<float>(h[0]), static_cast<float>(h[1]));
+          }
       uint32_t even[4], odd[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -320,12 +350,12 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
       }
       const uint4 v0 = make_uint4(even[0], even[1], even[2], even[3]), v1 = make_uint4(odd[0], odd[1], odd[2], odd[3]);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        acc[t][tile] = mfma<E>(hi[t], v0, acc[t][tile]);
-        acc[t][tile + 1] = mfma<E>(hi[t], v1, acc[t][tile + 1]);
-        acc[t][tile] = mfma<E>(lo[t], v0, acc[t][tile]);
-        acc[t][tile + 1] = mfma<E>(lo[t], v1, acc[t][tile + 1]);
-      }
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          acc[t][tile] = mfma<bf16_t>(wp[t][i], v0, acc[t][tile]);
+          acc[t][tile + 1] = mfma<bf16_t>(wp[t][i], v1, acc[t][tile + 1]);
+        }
     };
     constexpr std::integral_constant<bool, false> no{};
     constexpr std::integral_constant<bool, true> yes{};
