@@ -57,9 +57,13 @@ __device__ __forceinline__ uint32_t mx_settled(uint32_t pair) {
   return one(pair & 0xFFFFu) | one(pair >> 16) << 16;
 }
 
-// The larger of each half of two pairs of 16-bit magnitudes (sign bits clear: they order as whole numbers).
+// The larger (smaller) of each half of two pairs of 16-bit magnitudes (sign bits clear: they order as whole numbers).
 __device__ __forceinline__ uint32_t mx_larger(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
+}
+
+__device__ __forceinline__ uint32_t mx_smaller(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
 }
 
 // The sequence of packed row `row`: the number of sequences among the first `sequences` that end at or before it, found 64

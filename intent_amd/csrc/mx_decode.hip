@@ -41,6 +41,7 @@ constexpr int kStep = 32;              // keys of a wave's step: two tiles of 16
 constexpr float kSlack = 8.0f;
 constexpr float kNoToken = -1.0f;      // the sum of a state without a token (weights are not negative)
 constexpr uint32_t kSigns = 0x80008000u;
+constexpr uint32_t kTiny = 0x00800080u;          // 2^-126 in bf16, twice
 constexpr int kMany = 6, kFew = 2;     // workgroups a CU is given
 constexpr int kLong = 256;            // tokens of a job: from here on it is one of many
 constexpr int kLeast = 128;
@@ -267,10 +268,10 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
           vs[i][w] = mx_scale(x.ve[i][w]);
         }
       }
-    // f16: whether a value may be one that it rounds or holds as infinity: exponents outside -15 .. 7, asked of all exponents in a
-    // few comparisons of bits, which take -15 .. 0 as certain.
+    // Whether a value may be one that its type rounds or holds as infinity: exponents outside -15 .. 7 (f16) or above 119 (bf16);
+    // asked of all exponents in a few comparisons of bits, which take -15 .. 0 and up to 0 as certain.
     constexpr bool kF16 = std::is_same_v<E, f16_t>;
-    constexpr uint32_t kSure = 0x70707070u, kAsked = kF16 ? 0xF0F0F0F0u : 0u;
+    constexpr uint32_t kSure = kF16 ? 0x70707070u : 0u, kAsked = kF16 ? 0xF0F0F0F0u : 0x80808080u;
     uint32_t odd = 0;
 #pragma unroll
     for (int w = 0; w < C::kRuns; ++w) {
@@ -323,6 +324,11 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(waves_
       uint32_t part[4][kParts];
 #pragma unroll
       for (int i = 0; i < 4; ++i) parts(w[2 * i], w[2 * i + 1], part[i]);
+      if (__builtin_expect(extreme, 0))             // infinity by a number of 0 is NaN; none is 0 where the first is not
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 1; j < kParts; ++j) part[i][j] = mx_larger(part[i][j], mx_smaller(part[i][0], kTiny));
 #pragma unroll
       for (int i = 0; i < kParts; ++i) wp[t][i] = make_uint4(part[0][i], part[1][i], part[2][i], part[3][i]);
     }
