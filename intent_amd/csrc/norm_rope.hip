@@ -371,7 +371,8 @@ __global__ __launch_bounds__(kWaves * kWave) void norm_rope_backward_rows(NormRo
       apart<kInterleaved>(u, v, ga, gb);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += first[j] * first[j] + second[j] * second[j];
-      const float r = rsqrtf(row_sum<G>(sum) / p.d + p.eps);
+      // A place without a row adds nothing, also where the rows need no eps.
+      const float mean = row_sum<G>(sum) / p.d, r = f < heads ? rsqrtf(mean + p.eps) : 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float a = at.turned ? ga[j] * cs[j] + gb[j] * sn[j] : ga[j], b = at.turned ? gb[j] * cs[j] - ga[j] * sn[j] : gb[j];
