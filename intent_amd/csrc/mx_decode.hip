@@ -734,7 +734,7 @@ extern "C" int intent_hip_paged_gqa_decode_mx(int dtype, const void *q, const vo
   if (!width_ok(d))
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "mx decode takes head widths of 64, 96, 128, 192 and 256 (got %lld)",
                 static_cast<long long>(d));
-  if (pages == 0 || ps == 0) pages = 0, ps = 1;
+  if (ps == 0) pages = 0, ps = 1;                  // as the workspace's size has it; without a page no sequence has a token
   if (q == nullptr || page_offsets == nullptr || lengths == nullptr || output == nullptr || strides == nullptr ||
       (positions > 0 && page_indices == nullptr) ||
       (pages > 0 && (key_cache == nullptr || key_exponents == nullptr || value_cache == nullptr || value_exponents == nullptr)))

@@ -100,3 +100,15 @@ def test_infinite_values(device, dtype, page):
     out, _ = run(q, keys, values, page, 0.1, dtype, device, exact=False)       # beside 2^128, a block's ones are 0
     assert out[0, 2:, 40].isposinf().all() and out[0, :2, 3].isneginf().all()
     assert out.isfinite().sum() == out.numel() - 4
+
+
+def test_long_table_without_a_page(device):
+    """A table too long for one job over a cache that has no page: 0 from every job."""
+    announce("mx decode long table, no page")
+    held = [torch.zeros((0, 64, 8, w), dtype=torch.uint8, device=device) for w in (64, 2, 64, 2)]
+    held[0], held[2] = held[0].view(torch.float8_e4m3fn), held[2].view(torch.float8_e4m3fn)
+    q = torch.ones((4, 32, 64), dtype=torch.float16, device=device)
+    out = torch.full_like(q, 7.0)
+    kernel("f16", 4)(q, *held, i32([0, 10, 20000, 20000, 50001], device), torch.zeros(50001, dtype=torch.int32, device=device),
+                     i32([640, 10 ** 6, 5, 2 * 10 ** 6], device), out, 1.0)
+    assert (out == 0).all()
