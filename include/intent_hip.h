@@ -124,7 +124,8 @@ int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int64_t cols,
  *   ATTENTION_BWD_DKDV     batch, q_heads, head_group, sq, sk, d, causal, whether it has a workspace of the size it names
  *                          (of the kernels of one call the first, not the fold)
  *   PAGED_DECODE_PARTIALS  batch, kv_heads, head_group, d, positions, ps, splits
- *   PAGED_GQA_DECODE_MX    batch, kv_heads, head_group, d, ps, positions (of the two kernels of a joined call the first)
+ *   PAGED_GQA_DECODE_MX    batch, kv_heads, head_group, d, ps, positions and, if not left out, the largest stride of a token
+ *                          among the cache's four arrays (of the two kernels of a joined call the first)
  *   LINEAR_MXFP4           m, n, k (of the kernels of a call the first, not the fold)
  *   QK_NORM_ROPE, QK_NORM_ROPE_BACKWARD  d, pairs, interleaved, every address and stride in bytes of the rows, weights and
  *                          tables, or-ed */

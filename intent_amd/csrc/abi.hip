@@ -159,7 +159,7 @@ extern "C" int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int6
     case INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD: return norm_rope_resources(dtype, 1, cols, 0, 0, 0, out);
     case INTENT_HIP_OP_PAGED_CACHE_APPEND: return paged_cache_resources(dtype, 0, rows, cols, out);
     case INTENT_HIP_OP_PAGED_CACHE_READ: return paged_cache_resources(dtype, 1, rows, cols, out);
-    case INTENT_HIP_OP_PAGED_GQA_DECODE_MX: return mx_decode_resources(dtype, 1, 1, rows, cols, 16, 1 << 20, out);   // a long cache of 16-token pages
+    case INTENT_HIP_OP_PAGED_GQA_DECODE_MX: return mx_decode_resources(dtype, 1, 1, rows, cols, 16, 1 << 20, 0, out);   // a long cache of 16-token pages
     case INTENT_HIP_OP_LINEAR_MXFP4: return linear_mxfp4_resources(dtype, rows, cols, 4096, out);
     case INTENT_HIP_OP_GEMM_I8: return gemm_i8_resources(rows, cols, out);
     case INTENT_HIP_OP_QUANTIZED_GEMM:
@@ -206,8 +206,8 @@ extern "C" int intent_hip_call_resources(int op, int dtype, const int64_t *facts
       if (const int rc = takes(7)) return rc;
       return paged_decode_resources(f[0], f[1], f[2], f[3], f[4], f[5], f[6], out);
     case INTENT_HIP_OP_PAGED_GQA_DECODE_MX:
-      if (const int rc = takes(6)) return rc;
-      return mx_decode_resources(dtype, f[0], f[1], f[2], f[3], f[4], f[5], out);
+      if (const int rc = count == 7 ? INTENT_HIP_OK : takes(6)) return rc;
+      return mx_decode_resources(dtype, f[0], f[1], f[2], f[3], f[4], f[5], count == 7 ? f[6] : 0, out);
     case INTENT_HIP_OP_LINEAR_MXFP4:
       if (const int rc = takes(3)) return rc;
       return linear_mxfp4_resources(dtype, f[0], f[1], f[2], out);

@@ -58,7 +58,7 @@ int norm_rope_resources(int dtype, int backward, int64_t d, int64_t pairs, int i
 int paged_cache_resources(int dtype, int reading, int64_t rows, int64_t width, IntentHipKernelResources *out);
 int linear_mxfp4_resources(int dtype, int64_t m, int64_t n, int64_t k, IntentHipKernelResources *out);
 int mx_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t positions,
-                        IntentHipKernelResources *out);
+                        int64_t reach, IntentHipKernelResources *out);
 
 // f32 products of few output tiles (gemm_f32_few.hip); `workspace` may be null (one workgroup per tile).
 bool gemm_f32_few_applies(int64_t m, int64_t n, int64_t k);

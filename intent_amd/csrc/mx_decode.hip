@@ -663,17 +663,20 @@ void launch(const Decode &p, const Cut &c, bool uniform, int64_t d, hipStream_t 
   }
 }
 
+// Whether a tile of 16 keys lies in one page and a lane's place in it within 32 bits; reach: the largest stride of a token.
+bool is_uniform(int64_t ps, int64_t reach) { return ps % 16 == 0 && reach < INT32_MAX / 32; }
+
 bool width_ok(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 
 }  // namespace
 
 int mx_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t positions,
-                        IntentHipKernelResources *out) {
+                        int64_t reach, IntentHipKernelResources *out) {
   if (group < 1 || !width_ok(d)) return fail(INTENT_HIP_ERR_UNSUPPORTED, "mx decode has no head width %lld", static_cast<long long>(d));
   if (int rc = check_extents(batch, kv_heads * group, kv_heads, group, d, 0, ps, positions)) return rc;
   if (ps == 0) ps = 1;                             // a cache without a token
   const Cut c = cut(batch, kv_heads, group, positions, ps);
-  const bool uniform = ps % 16 == 0;
+  const bool uniform = is_uniform(ps, reach);
   char name[64];
   snprintf(name, sizeof(name), "mx_decode<%s,%d,%d,%s,%d>", dtype == INTENT_HIP_F16 ? "f16" : "bf16", static_cast<int>(d), c.qt,
            uniform ? "true" : "false", uniform ? c.waves : 4);
@@ -775,9 +778,7 @@ extern "C" int intent_hip_paged_gqa_decode_mx(int dtype, const void *q, const vo
     p.sums = p.total + rounded(rows * 4) / 4;
   }
   hipStream_t s = as_stream(stream);
-  // Lane offsets within a tile are 32 bits.
-  const int64_t reach = std::max({strides[4], strides[8], strides[12], strides[16]});
-  const bool uniform = ps % 16 == 0 && reach < INT32_MAX / 32;
+  const bool uniform = is_uniform(ps, std::max({strides[4], strides[8], strides[12], strides[16]}));
   if (dtype == INTENT_HIP_F16)
     launch<f16_t>(p, c, uniform, d, s);
   else

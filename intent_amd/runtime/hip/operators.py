@@ -1148,6 +1148,7 @@ def _paged_decode_mx(dtype_code):
         q, output = _readable(q, keep, before, 8), _writable(output, keep, after)
         tables = [_readable(t, keep, before) for t in (page_offsets, page_indices, lengths)]
         strides = (ctypes.c_int64 * 22)(*_outer_strides(q), 1, *held, *_outer_strides(output), 1)
+        reach = max(held[1], held[5], held[9], held[13])         # the tokens' strides
         positions, size = page_indices.shape[0], ctypes.c_size_t(0)
         lib.check(lib.fn["paged_gqa_decode_mx_workspace_bytes"](batch, q_heads, kv_heads, group, d, ps, positions,
                                                                 ctypes.byref(size)), "provider_preparation")
@@ -1164,7 +1165,7 @@ def _paged_decode_mx(dtype_code):
             return Launch("intent_hip_paged_gqa_decode_mx", _optional_workspace_run(fn, args, size, device, keep), tuple(keep),
                           configuration=configuration,
                           resources=lambda: lib.call_resources(OP_PAGED_GQA_DECODE_MX, dtype_code, batch, kv_heads, group, d, ps,
-                                                               positions))
+                                                               positions, reach))
         return _staged(again, (q, *cache, *tables, output, scale), bound, before, after)
     return plan
 
