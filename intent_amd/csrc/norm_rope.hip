@@ -19,6 +19,7 @@ namespace {
 constexpr int kMaxWidth = 1024;       // head width: a wave holds a row in 16 registers a lane
 constexpr int kRowRegisters = kMaxWidth / kWave;
 constexpr int kWaves = 4;
+constexpr int kMaxHeads = INT32_MAX / 4;        // of queries, of keys: a walk over both, and a step past its end, stay within 32 bits
 
 struct NormRope {
   const uint16_t *x[2], *dy[2];       // queries, keys
@@ -439,7 +440,7 @@ int check(int dtype, const NormRope &p, int64_t tokens, int64_t q_heads, int64_t
   if (d > kMaxWidth)
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "qk_norm_rope takes heads of up to %d dimensions, got %lld", kMaxWidth,
                 static_cast<long long>(d));
-  if (q_heads > INT32_MAX / 2 || kv_heads > INT32_MAX / 2) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
+  if (q_heads > kMaxHeads || kv_heads > kMaxHeads) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
   if (q_heads + kv_heads > 0 && tokens > (int64_t{1} << 32) / (q_heads + kv_heads))
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
   if (tokens == 0 || d == 0 || q_heads + kv_heads == 0) return INTENT_HIP_OK;
@@ -613,7 +614,7 @@ extern "C" int intent_hip_qk_norm_rope_backward_workspace_bytes(int64_t tokens, 
   if (bytes == nullptr) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null output");
   *bytes = 0;
   if (tokens < 0 || q_heads < 0 || kv_heads < 0 || d < 0) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "negative extent");
-  if (q_heads > INT32_MAX / 2 || kv_heads > INT32_MAX / 2 || d > kMaxWidth ||
+  if (q_heads > kMaxHeads || kv_heads > kMaxHeads || d > kMaxWidth ||
       (q_heads + kv_heads > 0 && tokens > (int64_t{1} << 32) / (q_heads + kv_heads)))
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
   *bytes = static_cast<size_t>(backward_blocks(tokens, q_heads, kv_heads)) * 2 * d * sizeof(float);

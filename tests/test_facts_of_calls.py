@@ -18,3 +18,16 @@ def test_decode_workspace_of_any_cache(pages, ps, batch, positions):
     assert lib.fn["paged_gqa_decode_mx"](hiplib.F16, *[256] * 9, batch, 32, 8, 4, 128, pages, ps, positions, strides, 0.1, 256,
                                          size.value - 1, None) == 5
     assert int(re.search(rb"needs (\d+) workspace", lib.fn["last_error"]()).group(1)) == size.value
+
+
+def test_norm_rope_of_too_many_heads():
+    """Numbers of heads whose walk would leave 32 bits are refused before any launch, and by the query."""
+    lib, size = hiplib.library(), ctypes.c_size_t(0)
+    strides = (ctypes.c_int64 * 22)(*(2 ** 34, 16, 1) * 2, 8, 1, 8, 1, *(2 ** 34, 16, 1) * 4)
+    for q_heads, kv_heads in ((2 ** 30 - 1, 2 ** 30 - 1), (2 ** 30 - 1, 1), (1, 2 ** 30 - 1)):
+        assert lib.fn["qk_norm_rope"](hiplib.F16, *[256] * 9, 2, q_heads, kv_heads, 16, 9, 8, strides, 0.0, 0, None) == 2
+        assert b"too large" in lib.fn["last_error"]()
+        assert lib.fn["qk_norm_rope_backward"](hiplib.F16, *[256] * 13, 2, q_heads, kv_heads, 16, 9, 8, strides, 0.0, 0, 256, 2 ** 40,
+                                               None) == 2
+        assert lib.fn["qk_norm_rope_backward_workspace_bytes"](2, q_heads, kv_heads, 16, ctypes.byref(size)) == 2
+    assert lib.fn["qk_norm_rope_backward_workspace_bytes"](2, 2 ** 29 - 1, 2 ** 29 - 1, 16, ctypes.byref(size)) == 0
