@@ -4,7 +4,8 @@ No reference counterpart; the tables are those of `paged_gqa_decode_partials` (s
 
 Cache. Elements f8e4m3fn [P, PS, HK, D] and exponents u8 [P, PS, HK, D / 32]: element i of a row stands for
 element * 2^(exponent[i / 32] - 127); exponent 255 stands for NaN. Any order of the page, token and head axes may lie in
-memory (a [P, HK, PS, D] allocation seen through a transpose keeps a head's page together). Sequence s holds the logical
+memory (a [P, HK, PS, D] allocation seen through a transpose keeps a head's page together), and keys and values may be slices
+of one allocation ([P, 2, PS, HK, D]). Sequence s holds the logical
 pages page_offsets[s] .. page_offsets[s + 1] of page_indices; its position p is place p % PS of logical page p / PS. A page
 that several sequences name may be read by all and appended to by one.
 

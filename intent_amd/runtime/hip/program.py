@@ -17,7 +17,7 @@ from ..artifact import CompiledArtifact
 from ..diagnostics import ConfigurationAssessment, NativeObservation, NativeResource
 from ..interface import PublicInterface, ViewParameter
 from ..invocation import Binding, BoundPublicArguments, bind_arguments
-from ..torch_views import allocate_output, observe_view, raw_device_getter, raw_stream_getter
+from ..torch_views import allocate_output, observe_view, raw_device_getter, raw_stream_getter, share_no_byte
 from .library import library
 from .operators import OperatorSpec, plan_policies
 from .tuning import FAMILY_OF, SPLIT, TuningConfiguration
@@ -183,13 +183,14 @@ class HipProgram:
 
     def _check_writable_overlap(self, bound) -> None:
         """Writable views may not overlap another view, except an exact in-place alias that the
-        kernel supports (same address and strides; each element is read before it is written)."""
+        kernel supports (same address and strides; each element is read before it is written). Slices of
+        one packed buffer, whose elements lie between each other's, do not."""
         for i, j, both in self._written_pairs:
             lf, rf = bound.views[i], bound.views[j]
             if not (lf.begin < lf.end and rf.begin < rf.end and lf.begin < rf.end and rf.begin < lf.end):
                 continue
             exact = (lf.pointer == rf.pointer and lf.shape == rf.shape and lf.strides == rf.strides)
-            if exact and self.spec.inplace_safe and not both:
+            if (exact and self.spec.inplace_safe and not both) or share_no_byte(lf, rf):
                 continue
             left, right = self.interface.parameters[i], self.interface.parameters[j]
             raise ValueError(f"{left.name} and {right.name} overlap; the hip kernel for "
@@ -235,7 +236,7 @@ class HipProgram:
         return tuple(key)
 
     def _prepare_again(self, layout, arguments, outputs):
-        """A call whose layout has been bound and planned before; None where views overlap (binding says whether they may)."""
+        """A call whose layout has been bound and planned before; None where views' ranges cross (binding says whether they may)."""
         import torch
 
         if outputs is None:

@@ -8,9 +8,9 @@ call's device.
 A tensor's facts are its shape and strides, plus its address range for alias checks. The range
 runs from the first to one past the last byte that its elements reach. `byte_span` accepts
 strides of either sign; torch strides are never negative, so for a tensor the range starts at
-`data_ptr()`. An allocation is identified by its device and
-base address. A storage of zero bytes holds nothing two views could disagree about, so every
-empty storage counts as one allocation. Abstract binding (fake tensors, `torch.compile` tracing)
+`data_ptr()`. Ranges that cross need not share a byte (`share_no_byte`). An allocation is
+identified by its device and base address. A storage of zero bytes holds nothing two views could
+disagree about, so every empty storage counts as one allocation. Abstract binding (fake tensors, `torch.compile` tracing)
 records shape, strides and dtype only.
 """
 from __future__ import annotations
@@ -32,6 +32,18 @@ def byte_span(pointer: int, shape: tuple, strides: tuple, itemsize: int) -> tupl
         else:
             below += (extent - 1) * stride
     return pointer + below * itemsize, pointer + (above + 1) * itemsize
+
+
+def share_no_byte(left: ViewFacts, right: ViewFacts) -> bool:
+    """Whether two views whose byte ranges cross are shown to be interleaved, as slices of one packed buffer are: modulo some
+    stride of theirs, each lies within an interval (of the axes whose strides are not its multiples), and the two are apart."""
+    views = [(v.pointer, v.dtype.itemsize, [(n - 1, st * v.dtype.itemsize) for n, st in zip(v.shape, v.strides) if n > 1])
+             for v in (left, right)]
+    for period in {st for _, _, axes in views for _, st in axes if st > 0}:
+        (a, reach_a), (b, reach_b) = ((at, size + sum(n * st for n, st in axes if st % period)) for at, size, axes in views)
+        if (b - a) % period >= reach_a and (a - b) % period >= reach_b:
+            return True
+    return False
 
 
 def _check(parameter: ViewParameter, value, device):
