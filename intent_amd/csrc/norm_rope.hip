@@ -592,15 +592,15 @@ extern "C" int intent_hip_qk_norm_rope(int dtype, const void *q, const void *k, 
   p.positions = positions, p.cos = cos, p.sin = sin;
   if (int rc = check(dtype, p, tokens, q_heads, kv_heads, d, table, pairs, strides, 16)) return rc;
   if (tokens == 0 || d == 0 || q_heads + kv_heads == 0) return INTENT_HIP_OK;
+  p.tokens = tokens, p.heads[0] = static_cast<int>(q_heads), p.heads[1] = static_cast<int>(kv_heads);
   for (int i = 0; i < 2; ++i) {
     p.xs[i][0] = strides[3 * i], p.xs[i][1] = strides[3 * i + 1];
     p.outs[i][0] = strides[10 + 3 * i], p.outs[i][1] = strides[11 + 3 * i];
-    if (d > 1 && (strides[3 * i + 2] != 1 || strides[12 + 3 * i] != 1))
+    if (p.heads[i] > 0 && d > 1 && (strides[3 * i + 2] != 1 || strides[12 + 3 * i] != 1))
       return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "rows need unit inner stride");
   }
   if (pairs > 1 && (strides[7] != 1 || strides[9] != 1)) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "tables need unit inner stride");
   p.coss = strides[6], p.sins = strides[8], p.table = table;
-  p.tokens = tokens, p.heads[0] = static_cast<int>(q_heads), p.heads[1] = static_cast<int>(kv_heads);
   p.d = static_cast<int>(d), p.pairs = static_cast<int>(pairs), p.interleaved = interleaved != 0, p.eps = eps;
   if (dtype == INTENT_HIP_F16)
     launch_forward<f16_t>(p, as_stream(stream));
@@ -645,17 +645,17 @@ extern "C" int intent_hip_qk_norm_rope_backward(int dtype, const void *q, const 
       return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null pointer");
     if (workspace == nullptr || workspace_bytes < bytes || !aligned(workspace, 16))
       return fail(INTENT_HIP_ERR_WORKSPACE, "qk_norm_rope_backward needs %zu workspace bytes, 16-byte aligned", bytes);
+    p.tokens = tokens, p.heads[0] = static_cast<int>(q_heads), p.heads[1] = static_cast<int>(kv_heads);
     for (int i = 0; i < 2; ++i) {
       p.xs[i][0] = strides[3 * i], p.xs[i][1] = strides[3 * i + 1];
       p.dys[i][0] = strides[10 + 3 * i], p.dys[i][1] = strides[11 + 3 * i];
       p.outs[i][0] = strides[16 + 3 * i], p.outs[i][1] = strides[17 + 3 * i];
-      if (d > 1 && (strides[3 * i + 2] != 1 || strides[12 + 3 * i] != 1 || strides[18 + 3 * i] != 1))
+      if (p.heads[i] > 0 && d > 1 && (strides[3 * i + 2] != 1 || strides[12 + 3 * i] != 1 || strides[18 + 3 * i] != 1))
         return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "rows need unit inner stride");
     }
     if (pairs > 1 && (strides[7] != 1 || strides[9] != 1))
       return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "tables need unit inner stride");
     p.coss = strides[6], p.sins = strides[8], p.table = table;
-    p.tokens = tokens, p.heads[0] = static_cast<int>(q_heads), p.heads[1] = static_cast<int>(kv_heads);
     p.d = static_cast<int>(d), p.pairs = static_cast<int>(pairs), p.interleaved = interleaved != 0, p.eps = eps;
     if (in_pieces(d, pairs, mixed(p, true)))
       blocks = static_cast<int>(std::min<int64_t>(blocks, (tokens * token_waves(p) + kWaves - 1) / kWaves));      // none without a job

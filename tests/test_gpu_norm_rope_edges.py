@@ -32,3 +32,21 @@ def test_without_eps(device, dtype, tokens, q_heads, kv_heads, d, pairs, interle
             assert ((got[2 + i].double().cpu() - dw).abs() <= 2.0 ** -15 * dw_size + 1e-37).all()
         else:
             assert (got[2 + i] == 0).all()
+
+
+@pytest.mark.parametrize("absent", [0, 1])
+def test_absent_heads_of_any_layout(device, absent):
+    """The heads that are not there have no layout to refuse."""
+    announce("qk_norm_rope absent heads", absent)
+    rows, weights, positions, cos, sin, grad, _ = (t.to(device) for t in case(7, "bf16", 5, 3, 1, 64, 32))
+    x, nothing = rows[:, :3], torch.empty((5, 0, 64, 2), dtype=torch.bfloat16, device=device)[..., 0]
+    both = lambda a: (nothing, a) if absent == 0 else (a, nothing)          # noqa: E731
+    common = (*both(x), *weights, positions, cos, sin)
+    plain = (*both(x.contiguous()), *weights, positions, cos, sin)
+    out = kernel("qk_norm_rope_bf16").run(*common, 1e-6)
+    none = torch.empty((5, 0, 64), dtype=torch.bfloat16, device=device)
+    want = kernel("qk_norm_rope_bf16").run(*[none if t is nothing else t for t in plain], 1e-6)
+    assert torch.equal(out[1 - absent], want[1 - absent]) and out[absent].shape == (5, 0, 64)
+    got = kernel("qk_norm_rope_backward_bf16").run(*common, *both(grad), 1e-6)
+    sizes = [t.abs().sum().item() for t in got[2:]]
+    assert sizes[absent] == 0 and sizes[1 - absent] > 0 and got[1 - absent].isfinite().all()
