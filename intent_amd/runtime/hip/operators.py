@@ -995,6 +995,12 @@ def _norm_rope_staged(arguments, extents, outputs):
     return (*values, arguments[last]), before, after
 
 
+def _norm_rope_mixed(values, last) -> int:
+    """`_mixed` of the rows, of the weights of the heads there are, and of the tables; `last`: the last view of rows."""
+    weights = [w for x, w in zip(values[:2], values[2:4]) if x.numel()]
+    return _mixed(*values[:2], *weights, *values[5:last + 1])
+
+
 def _norm_rope_extents(q, k, cos) -> tuple:
     return (q.shape[0], q.shape[1], k.shape[1], q.shape[2], *cos.shape)
 
@@ -1027,7 +1033,7 @@ def _norm_rope(dtype_code):
             args = (dtype_code, *[t.data_ptr() for t in values[:9]], *extents, strides, float(values[9]), interleaved)
             return Launch("intent_hip_qk_norm_rope", lambda stream: fn(*args, stream), values, configuration=configuration,
                           resources=lambda: lib.call_resources(OP_QK_NORM_ROPE, dtype_code, extents[3], extents[5], interleaved,
-                                                               _mixed(*values[:4], *values[5:9])))
+                                                               _norm_rope_mixed(values, 8)))
         return _staged(again, values, bound, before, after)
     return plan
 
@@ -1053,7 +1059,7 @@ def _norm_rope_backward(dtype_code):
             run = _workspace_run(fn, args, size, device, keep)
             return Launch("intent_hip_qk_norm_rope_backward", run, tuple(keep), configuration=configuration,
                           resources=lambda: lib.call_resources(OP_QK_NORM_ROPE_BACKWARD, dtype_code, extents[3], extents[5],
-                                                               interleaved, _mixed(*values[:4], *values[5:11])))
+                                                               interleaved, _norm_rope_mixed(values, 10)))
         return _staged(again, values, bound, before, after)
     return plan
 

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from tests import test_gpu_norm_rope as norm
 from tests.gpu_util import announce
 from tests.test_gpu_mx_cache import cache, i32
 from tests.test_gpu_mx_decode import kernel
@@ -22,3 +23,18 @@ def test_decode_of_far_tokens(device, stride, walk):
         call = kernel("f16", 4).prepare(q, *held, *tables, 1.0)
         call.launch()
         assert f",1,{walk}," in call.observation.kernel, call.observation.kernel
+
+
+@pytest.mark.parametrize("absent", [0, 1])
+def test_norm_of_absent_heads(device, absent):
+    """The weight of heads that are not there says nothing about the kernel, however it lies."""
+    announce("observed norm", absent)
+    rows, weights, positions, cos, sin, grad, _ = (t.to(device) for t in norm.case(7, "bf16", 5, 3, 1, 64, 32))
+    odd = torch.ones(65, device=device)[1:]
+    both = lambda a, b: (b, a) if absent == 0 else (a, b)          # noqa: E731
+    none = torch.empty((5, 0, 64), dtype=torch.bfloat16, device=device)
+    common = (*both(rows[:, :3], none), *both(weights[0], odd), positions, cos, sin)
+    for name, grads in (("qk_norm_rope_bf16", ()), ("qk_norm_rope_backward_bf16", both(grad, none))):
+        call = norm.kernel(name).prepare(*common, *grads, 1e-6)
+        call.launch()
+        assert "_rows<" in call.observation.kernel, call.observation.kernel
