@@ -7,8 +7,8 @@
 // so lane (r, g) takes block g of four of weight row r as it lies in memory (16 bytes, one exponent), converts it in four
 // parts, and reads the same 32 values of its row of x. Weights go from memory to registers: no wave needs another's.
 //   * linear_few, up to 16 rows of x: a workgroup's 16 waves take a run of K each and add their sums through the LDS. Bound by
-//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 7.9 us, 4.0 TB/s; 16 x 14336 x 4096:
-//     12.2; 1 x 4096 x 4096: 3.7, most of it latency: one or two steps a wave).
+//     the weights' bytes and by x, which every workgroup reads (1 x 14336 x 4096: 7.7 us, 4.1 TB/s; 8 rows 10.7, 16
+//     rows 12.6; 1 x 4096 x 4096: 3.7, most of it latency: one or two steps a wave; 1 x 128256 x 4096: 59.5, 4.7 TB/s).
 //   * linear_tiles: a workgroup's waves share 16 MT rows of x, which pass through the LDS 128 columns at a time (in 16-byte
 //     units, unit u of row r at u ^ r % 16, so that the 16 rows of a read are in different banks), and take 16 NT weight
 //     rows each. A lane's weight rows are NT apart, so its results are 4 NT consecutive columns of y. Where tiles are few, K
@@ -18,8 +18,9 @@
 //     (16.7 -> 15.8, 24.4 -> 21.0). Exponents come four stages at a time, a word a lane, and a lane permutation brings them to
 //     where they are needed: a byte a lane and stage touches as many cache lines as the weights (21.0 -> 18.2; the tiles of
 //     128 x 128 lose up to 4 %). Eight stages on their way instead of four are no faster (32 x 4096 x 14336: 16.0, four 15.2).
-//     The large tiles are bound by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 107 us, 1120 TFLOP/s,
-//     the type's own product 90 to 97; three stages, and so one workgroup a CU, 174).
+//     The large tiles are bound by the matrix pipe and the conversions beside it (1021 x 14336 x 4096: 103 us, 1160
+//     TFLOP/s, among other calls, 111 behind others of its kind; the type's own product 90 to 97; three stages, and so one
+//     workgroup a CU, 174).
 #include <stdio.h>
 
 #include <type_traits>
@@ -97,12 +98,12 @@ __device__ __forceinline__ void store(const Linear &p, int m, int n, const float
 
 // Up to 16 rows of x by 16 NT weight rows a workgroup; its 16 waves take a run of K each. The loads of kAhead steps of 128
 // columns are on their way at once, the exponents of all weight rows in one, which a lane permutation brings to where they are
-// needed (1 x 14336 x 4096: 10.0 us with a load a weight row, 9.2 so; 16 x 14336 x 4096: 12.8 and 12.2). Columns of the product
-// behind the rows of x are never stored, so their lanes read any row.
+// needed (16 x 14336 x 4096: 12.8 us with a load a weight row, 12.2 so). Columns of the product behind the rows of x are never
+// stored, so their lanes read any row.
 //
 // kOne: x is one row. Its 128 columns of a step are a word a lane, and every lane takes the 16 words of its block from the lanes
-// of its row of 16: loads of 16 bytes a lane, 16 times each value, hold up the weights' (1 x 4096 x 14336: 10.5 and 8.6 us; 1 x 14336 x
-// 4096: 9.2 and 7.9; 1 x 128256 x 4096: 53.6, 5.2 TB/s).
+// of its row of 16: loads of 16 bytes a lane, 16 times each value, hold up the weights' (1 x 4096 x 14336: 10.5 us, so 8.6; 1 x
+// 14336 x 4096: 8.9 and 7.8).
 template <int kFirst>
 __device__ __forceinline__ uint4 words_of_row(uint32_t own) {
   const int v = static_cast<int>(own);

@@ -12,7 +12,7 @@
 // A wave takes a piece of 512 elements of up to 4 consecutive rows, all on their way at once: where its lanes' elements lie in
 // a row is found once, and the tables are asked again only where a sequence or a page ends. Consecutive rows stay on one XCD,
 // so the exponents of a page's tokens, which share lines, leave its L2 together. Bound by bytes (8 prompts of up to 8191, 8 key
-// heads of 128: appended in 28.9 us, 5.1 TB/s; read in 31, 4.7 TB/s); a token for each of 32 sequences by latency, 3.3 us.
+// heads of 128: appended in 28.5 us, 5.1 TB/s; read in 30.5, 4.8 TB/s); a token for each of 32 sequences by latency, 3.3 us.
 #include <stdio.h>
 
 #include "mx.hpp"

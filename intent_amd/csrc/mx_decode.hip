@@ -6,8 +6,8 @@
 // Keys and values are taken in the query's type (element * 2^e, one rounding) and products are summed in f32. Weights are f32
 // and enter the second product whole, as three bf16 numbers of 8 bits each: f16 numbers end at 2^-24, and the sum that the
 // products are divided by holds the weights below. Two bf16 numbers would leave out 2^-16 of a weight; the third costs up to 4 %
-// where jobs are few (8 sequences of 8191, f16: 35.2 us, 34.2 with two f16 numbers) and nothing where they are many (64 ragged
-// sequences up to 8191, bf16: 135.2 and 135.2). The values are bf16 numbers exactly: e4m3 has four bits.
+// where jobs are few (one sequence of 512, f16: 8.1 us, two 7.8; 8 of 8191: 34.5 and 34.3) and nothing where they are many (64
+// ragged sequences up to 8191, bf16: 135.2 and 135.4). The values are bf16 numbers exactly: e4m3 has four bits.
 //
 // Design. The page range of a sequence is cut into jobs of `job_pages` pages; job j of the flat list belongs to the last
 // sequence s with page_offsets[s] / job_pages + s <= j, which every wave finds by itself, so no table of work is made and
@@ -22,9 +22,11 @@
 //     Their exponents come a key a lane and go to the lanes that use them by a permutation (8 sequences of 8191: 34.9 us with a
 //     byte a lane and key, 33.9 so).
 //   * the running maximum is raised (and the sums scaled down) only when a score passes it by 2^8, so most steps have no
-//     cross-lane move at all; weights up to 2^8 are far inside either type.
+//     cross-lane move at all; weights up to 2^8 are far inside bf16.
 // Bound by the cache's bytes once there are many jobs (64 sequences of 8191, 8 key heads of 128: 191 us, 5.1 TB/s; the loads
-// alone take as long); with few jobs by a step's chain of instructions, about 430 of a wave (1.2 us where it runs alone).
+// alone take as long); with few jobs by a step's chain of instructions, about 470 of a wave. Where a tile of 16 keys may cross pages
+// (PS no multiple of 16) every lane looks up the pages of its own keys: 8 sequences of 8191 take 82 us with pages of 1, 80 with 8,
+// 39 with 16, 35 with 64.
 #include <stdio.h>
 
 #include <algorithm>

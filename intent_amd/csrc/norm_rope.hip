@@ -5,8 +5,9 @@
 // of g u over rows, through f32 partial sums per workgroup that a second kernel adds in order.
 //
 // Bound by the rows' bytes, so each is read and written once, in whole 16-byte pieces (bf16, 16384 tokens of 32 + 8 heads of 128:
-// forward 64 us, 5.4 TB/s; backward 102 us and 4 for the sums, 5.0 TB/s); with few tokens by latency and launches (8 tokens: 3.1
-// and 7.2 us). Layouts without such pieces take two bytes a lane (342 and 999 us).
+// forward 67 us, 5.1 TB/s; backward 102 us, 5.0 TB/s, and 4 for the sums); with few tokens by latency and launches (8 tokens: 3.1
+// and 7.2 us). Layouts without such pieces (D no multiple of 16, R no multiple of 8, odd strides) take two bytes a lane: 342 and
+// 999 us; heads of 80 with 10 pairs turned 276 and 916, all 40 turned 55 and 95.
 #include <stdio.h>
 
 #include <algorithm>
