@@ -482,7 +482,8 @@ int intent_hip_csr_spmm_f32(const int32_t *row_offsets, const int32_t *column_in
                             void *stream);
 
 /* Root-mean-square norm of every query and key head and the rotation of its token's position, no reference counterpart.
- * q [tokens, q_heads, d], k [tokens, kv_heads, d] and the outputs of the same shapes in f16 or bf16 (d at most 1024);
+ * q [tokens, q_heads, d], k [tokens, kv_heads, d] and the outputs of the same shapes in f16 or bf16 (d at most 1024, fewer
+ * than 2^29 heads of either kind);
  * weights f32 [d]; positions i32 [tokens] (clamped into the tables); cos, sin f32 [table, pairs], 2 * pairs <= d. A head's
  * row x gives y = x * rsqrt(mean(x^2) + eps) * weight in f32, of which the pairs (i, i + pairs), or (2i, 2i + 1) when
  * `interleaved`, are turned by the position's angles; one rounding at the end. Outputs may not overlap inputs.

@@ -8,6 +8,7 @@
 // products are divided by holds the weights below. Two bf16 numbers would leave out 2^-16 of a weight; the third costs up to 4 %
 // where jobs are few (one sequence of 512, f16: 8.1 us, two 7.8; 8 of 8191: 34.5 and 34.3) and nothing where they are many (64
 // ragged sequences up to 8191, bf16: 135.2 and 135.4). The values are bf16 numbers exactly: e4m3 has four bits.
+// Where their exponents are such that f16 rounds or does not reach them, f16 calls convert them by way of f16 (35.9 -> 37.8).
 //
 // Design. The page range of a sequence is cut into jobs of `job_pages` pages; job j of the flat list belongs to the last
 // sequence s with page_offsets[s] / job_pages + s <= j, which every wave finds by itself, so no table of work is made and

@@ -71,7 +71,7 @@ def test_values_at_the_ends_of_f16(device, d, page):
     g = torch.Generator().manual_seed(d + page)
     keys = torch.zeros((40, 1, d), dtype=torch.float64)
     values = torch.randint(1, 16, (40, 1, d), generator=g).double() / 8
-    values[..., :32] *= 2.0 ** 14                     # up to 30720
+    values[..., :32] *= 2.0 ** 14                     # up to 1.875 * 2^14
     values[..., 32:64] *= 2.0 ** -25                  # multiples of 2^-28
     for dtype in ("f16", "bf16"):
         q = torch.ones((1, 2, d), dtype=TYPES[dtype])
