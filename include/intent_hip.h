@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define INTENT_HIP_ABI_VERSION 21
+#define INTENT_HIP_ABI_VERSION 22
 
 enum IntentHipStatus {
   INTENT_HIP_OK = 0,
@@ -71,7 +71,14 @@ enum IntentHipOperator {
   INTENT_HIP_OP_PAGED_CACHE_APPEND = 25,  /* dtype F16 or BF16; rows, cols = kv_heads * (d + dv), for both */
   INTENT_HIP_OP_PAGED_CACHE_READ = 26,
   INTENT_HIP_OP_PAGED_GQA_DECODE_MX = 27, /* dtype F16 or BF16; rows = HEAD_GROUP, cols = head width */
-  INTENT_HIP_OP_LINEAR_MXFP4 = 28         /* dtype F16 or BF16; rows = m, cols = n */
+  INTENT_HIP_OP_LINEAR_MXFP4 = 28,        /* dtype F16 or BF16; rows = m, cols = n */
+  INTENT_HIP_OP_RESIDUAL_NORM = 29,       /* dtype F16 or BF16; rows = tokens, cols = d, for the three */
+  INTENT_HIP_OP_RESIDUAL_NORM_I8 = 30,
+  INTENT_HIP_OP_RESIDUAL_NORM_BACKWARD = 31,
+  INTENT_HIP_OP_QUANTIZE_ROWS = 32,       /* dtype F16 or BF16; rows, cols = d, for both */
+  INTENT_HIP_OP_SWIGLU_QUANTIZE_ROWS = 33,
+  INTENT_HIP_OP_LINEAR_I8 = 34,           /* dtype F16 or BF16; rows = m, cols = n */
+  INTENT_HIP_OP_PAGED_GQA_DECODE_PREFIX = 35 /* dtype F16 or BF16; rows = HEAD_GROUP, cols = head width */
 };
 
 /* Epilogue activations of intent_hip_gemm (the Activation enum of contraction/gemm.py:10-12). */
@@ -126,7 +133,11 @@ int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int64_t cols,
  *   PAGED_DECODE_PARTIALS  batch, kv_heads, head_group, d, positions, ps, splits
  *   PAGED_GQA_DECODE_MX    batch, kv_heads, head_group, d, ps, positions and, if not left out, the largest stride of a token
  *                          among the cache's four arrays (of the two kernels of a joined call the first)
- *   LINEAR_MXFP4           m, n, k (of the kernels of a call the first, not the fold)
+ *   LINEAR_MXFP4, LINEAR_I8  m, n, k (of the kernels of a call the first, not the fold)
+ *   PAGED_GQA_DECODE_PREFIX  batch, kv_heads, head_group, d, ps, prefix_positions, positions (the first, not the join)
+ *   RESIDUAL_NORM, RESIDUAL_NORM_I8, RESIDUAL_NORM_BACKWARD  d, post, every address and stride in bytes of the rows and weights,
+ *                          or-ed, those of the 8-bit rows doubled (of the kernels of a call the first, not the fold)
+ *   QUANTIZE_ROWS, SWIGLU_QUANTIZE_ROWS  d, the same
  *   QK_NORM_ROPE, QK_NORM_ROPE_BACKWARD  d, pairs, interleaved, every address and stride in bytes of the rows, weights and
  *                          tables, or-ed */
 int intent_hip_call_resources(int op, int dtype, const int64_t *facts, int count, struct IntentHipKernelResources *out);
@@ -553,6 +564,72 @@ int intent_hip_linear_mxfp4_workspace_bytes(int64_t m, int64_t n, int64_t k, siz
 int intent_hip_linear_mxfp4(int dtype, const void *x, const uint8_t *weight, const uint8_t *exponents, void *y, int64_t m,
                             int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t lde, int64_t ldy, void *workspace,
                             size_t workspace_bytes, void *stream);
+
+/* The residual stream after a block's output has joined it, and its norm; no reference counterpart. block, residual, sum [tokens, d] in
+ * f16 or bf16 (d at most 16384); gate f32 [gates], gates = tokens, or 0 for a gate of 1; post_weight f32 [post], post = d, or 0 for a
+ * block without a norm of its own; weight f32 [d]. In f32, each stored with one rounding:
+ *   u = block * rsqrt(mean(block^2) + eps) * post_weight (block itself without), sum = residual_scale * residual + block_scale * gate * u,
+ *   output = sum * rsqrt(mean(sum^2) + eps) * weight, from the sum before its rounding.
+ * residual_norm writes output [tokens, d] in the rows' type, residual_norm_i8 as round(127 output / max|output|) (halves to even) with
+ * scales f32 [tokens] = max|output| / 127; a row that is not finite has a scale of NaN and elements of 0. sum and output (of
+ * residual_norm) may be block or residual itself, element for element. Strides of a token, strides[5]: block, residual, gate, sum,
+ * output. */
+int intent_hip_residual_norm(int dtype, const void *block, const void *residual, const float *gate, const float *post_weight,
+                             const float *weight, void *sum, void *output, int64_t tokens, int64_t d, int64_t gates, int64_t post,
+                             const int64_t strides[5], float residual_scale, float block_scale, float eps, void *stream);
+int intent_hip_residual_norm_i8(int dtype, const void *block, const void *residual, const float *gate, const float *post_weight,
+                                const float *weight, void *sum, int8_t *output, float *scales, int64_t tokens, int64_t d, int64_t gates,
+                                int64_t post, const int64_t strides[5], float residual_scale, float block_scale, float eps, void *stream);
+
+/* Its gradients, from block and the stored sum and the gradients that reach sum and output: grad_block, grad_residual in the rows' type,
+ * grad_gate f32 [gates], grad_post_weight f32 [post], grad_weight f32 [d], the last two sums over tokens in a fixed order through the
+ * workspace (intent_hip_residual_norm_backward_workspace_bytes bytes, 16-byte aligned). A gradient of rows may be any of the rows that
+ * are read, element for element. Strides of a token, strides[8]: block, sum, gate, grad_sum, grad_output, grad_block, grad_residual,
+ * grad_gate. */
+int intent_hip_residual_norm_backward_workspace_bytes(int64_t tokens, int64_t d, int64_t post, size_t *bytes);
+int intent_hip_residual_norm_backward(int dtype, const void *block, const void *sum, const float *gate, const float *post_weight,
+                                      const float *weight, const void *grad_sum, const void *grad_output, void *grad_block,
+                                      void *grad_residual, float *grad_gate, float *grad_post_weight, float *grad_weight, int64_t tokens,
+                                      int64_t d, int64_t gates, int64_t post, const int64_t strides[8], float residual_scale,
+                                      float block_scale, float eps, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Rows made 8-bit integers with a scale each; no reference counterpart. a = x, or gate / (1 + e^-gate) * up in f32, [rows, d] in f16 or
+ * bf16 (d at most 32768): scales f32 [rows] = max|a| / 127, output int8 [rows, d] = round(127 a / max|a|), halves to even. A row of zeros
+ * has a scale of 0; one that holds an infinity or NaN a scale of NaN and elements of 0. ldx, ldg, ldu, ldo: strides of a row. */
+int intent_hip_quantize_rows(int dtype, const void *x, int8_t *output, float *scales, int64_t rows, int64_t d, int64_t ldx, int64_t ldo,
+                             void *stream);
+int intent_hip_swiglu_quantize_rows(int dtype, const void *gate, const void *up, int8_t *output, float *scales, int64_t rows, int64_t d,
+                                    int64_t ldg, int64_t ldu, int64_t ldo, void *stream);
+
+/* y[m, n] = (sum_k x[m, k] weight[n, k]) * x_scales[m] * weight_scales[n] + bias[n]; no reference counterpart. x int8 [m, k], weight int8
+ * [n, k], scales and bias f32 (bias null for none), y in f16 or bf16. Sums are int32 and exact (k below 131072), the rest is f32, one
+ * rounding at the end. k a multiple of 16; rows of x and of the weight 16-byte aligned. Where the product has few tiles, K is divided over
+ * workgroups whose sums a second kernel adds through the workspace (intent_hip_linear_i8_workspace_bytes bytes, 16-byte aligned; 0
+ * elsewhere). */
+int intent_hip_linear_i8_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t *bytes);
+int intent_hip_linear_i8(int dtype, const int8_t *x, const int8_t *weight, const float *x_scales, const float *weight_scales,
+                         const float *bias, void *y, int64_t m, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t ldy,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* Attention of one new token per sequence over a prefix that all sequences share, read once for all, and over each sequence's own tokens;
+ * no reference counterpart. q and output [batch, q_heads, d], caches [pages, ps, kv_heads, d] in f16 or bf16, d 64 or 128, q_heads =
+ * kv_heads * head_group; query head h uses key head h / head_group. The prefix is the first prefix_length[0] tokens of the pages
+ * prefix_indices [prefix_positions]; sequence s adds the first lengths[s] tokens of the pages page_offsets[s] .. page_offsets[s + 1] of
+ * page_indices [positions], lengths[s] not counting the prefix; no more than the tables hold; output is 0 where there is no token.
+ * page_offsets [batch + 1] start at 0 or above and do not decrease; entries and pages outside their arrays read the nearest. Products are
+ * summed in f32; weights enter the second product as f16 numbers or as two bf16 numbers each, and the sum that divides is of these; one
+ * rounding at the end. Nothing depends on the host's knowledge of lengths and offsets, so they may change under a captured graph. Rows of
+ * q and of the caches 16-byte aligned, their strides multiples of 8. The states of jobs meet in the workspace
+ * (intent_hip_paged_gqa_decode_prefix_workspace_bytes bytes, 16-byte aligned).
+ * strides[14]: q[3], key_cache[4], value_cache[4], output[3]. */
+int intent_hip_paged_gqa_decode_prefix_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_group, int64_t d,
+                                                       int64_t ps, int64_t prefix_positions, int64_t positions, size_t *bytes);
+int intent_hip_paged_gqa_decode_prefix(int dtype, const void *q, const void *key_cache, const void *value_cache,
+                                       const int32_t *prefix_indices, const int32_t *prefix_length, const int32_t *page_offsets,
+                                       const int32_t *page_indices, const int32_t *lengths, void *output, int64_t batch, int64_t q_heads,
+                                       int64_t kv_heads, int64_t head_group, int64_t d, int64_t pages, int64_t ps,
+                                       int64_t prefix_positions, int64_t positions, const int64_t strides[14], float scale,
+                                       void *workspace, size_t workspace_bytes, void *stream);
 
 /* Measurement probe (no counterpart in the reference): the box's own MFMA ceiling, reported by the
  * benchmark beside the published peak, as the measurement protocol asks for an MFMA

@@ -98,7 +98,7 @@ def read_hip_facts(metadata: dict) -> HipFacts:
                     hip["entry_point"], hip["abi_version"], table_from_metadata(hip.get("tuning")))
 
 
-def _native_section(interface, inplace_safe: bool) -> dict:
+def _native_section(interface, may_be_one) -> dict:
     from ..runtime.interface import ViewParameter
 
     slots, views, disjoint = [], [], []
@@ -120,7 +120,7 @@ def _native_section(interface, inplace_safe: bool) -> dict:
         for right in view_params[i + 1:]:
             if not (left.writable or right.writable):
                 continue
-            if inplace_safe and left.writable != right.writable:
+            if may_be_one(left.position, right.position) and left.writable != right.writable:
                 continue                      # the exact in-place alias is allowed; other overlaps are refused
             disjoint.append({"left": left.position, "right": right.position})
     return {"slots": slots, "workspaces": [], "requirements": {"views": views, "disjoint": disjoint}}
@@ -415,7 +415,7 @@ def generate(definition, *, target, compiler=None, constexprs: dict | None = Non
         "target": compilation.metadata(),
         "compile_options": policy.metadata(),
         "interface": interface.to_json(),
-        "native": _native_section(interface, spec.inplace_safe),
+        "native": _native_section(interface, spec.may_be_one),
         "hip": {"format": FORMAT, "definition": spec.name,
                 "signature": [list(item) for item in signature_of(interface)],
                 "constexprs": {name: _encode_constexpr(value) for name, value in values.items()},

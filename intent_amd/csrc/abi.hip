@@ -161,6 +161,13 @@ extern "C" int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int6
     case INTENT_HIP_OP_PAGED_CACHE_READ: return paged_cache_resources(dtype, 1, rows, cols, out);
     case INTENT_HIP_OP_PAGED_GQA_DECODE_MX: return mx_decode_resources(dtype, 1, 1, rows, cols, 16, 1 << 20, 0, out);   // a long cache of 16-token pages
     case INTENT_HIP_OP_LINEAR_MXFP4: return linear_mxfp4_resources(dtype, rows, cols, 4096, out);
+    case INTENT_HIP_OP_RESIDUAL_NORM: return residual_norm_resources(dtype, 0, cols, 0, 0, out);   // aligned rows, no norm of the block
+    case INTENT_HIP_OP_RESIDUAL_NORM_I8: return residual_norm_resources(dtype, 1, cols, 0, 0, out);
+    case INTENT_HIP_OP_RESIDUAL_NORM_BACKWARD: return residual_norm_resources(dtype, 2, cols, 0, 0, out);
+    case INTENT_HIP_OP_QUANTIZE_ROWS: return quantize_rows_resources(dtype, 0, cols, 0, out);
+    case INTENT_HIP_OP_SWIGLU_QUANTIZE_ROWS: return quantize_rows_resources(dtype, 1, cols, 0, out);
+    case INTENT_HIP_OP_LINEAR_I8: return linear_i8_resources(dtype, rows, cols, 4096, out);
+    case INTENT_HIP_OP_PAGED_GQA_DECODE_PREFIX: return prefix_decode_resources(dtype, 16, 1, rows, cols, 16, 1024, 1024, out);
     case INTENT_HIP_OP_GEMM_I8: return gemm_i8_resources(rows, cols, out);
     case INTENT_HIP_OP_QUANTIZED_GEMM:
       return quantized_gemm_resources(nullptr, nullptr, nullptr, nullptr, rows, (cols + 7) / 8 * 8, 64, 64, 64, 64, 64, out);
@@ -211,6 +218,18 @@ extern "C" int intent_hip_call_resources(int op, int dtype, const int64_t *facts
     case INTENT_HIP_OP_LINEAR_MXFP4:
       if (const int rc = takes(3)) return rc;
       return linear_mxfp4_resources(dtype, f[0], f[1], f[2], out);
+    case INTENT_HIP_OP_LINEAR_I8:
+      if (const int rc = takes(3)) return rc;
+      return linear_i8_resources(dtype, f[0], f[1], f[2], out);
+    case INTENT_HIP_OP_PAGED_GQA_DECODE_PREFIX:
+      if (const int rc = takes(7)) return rc;
+      return prefix_decode_resources(dtype, f[0], f[1], f[2], f[3], f[4], f[5], f[6], out);
+    case INTENT_HIP_OP_RESIDUAL_NORM: case INTENT_HIP_OP_RESIDUAL_NORM_I8: case INTENT_HIP_OP_RESIDUAL_NORM_BACKWARD:
+      if (const int rc = takes(3)) return rc;
+      return residual_norm_resources(dtype, op - INTENT_HIP_OP_RESIDUAL_NORM, f[0], f[1], static_cast<uint64_t>(f[2]), out);
+    case INTENT_HIP_OP_QUANTIZE_ROWS: case INTENT_HIP_OP_SWIGLU_QUANTIZE_ROWS:
+      if (const int rc = takes(2)) return rc;
+      return quantize_rows_resources(dtype, op == INTENT_HIP_OP_SWIGLU_QUANTIZE_ROWS, f[0], static_cast<uint64_t>(f[1]), out);
     case INTENT_HIP_OP_QK_NORM_ROPE: case INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD:
       if (const int rc = takes(4)) return rc;
       return norm_rope_resources(dtype, op == INTENT_HIP_OP_QK_NORM_ROPE_BACKWARD, f[0], f[1], f[2] != 0,

@@ -1,0 +1,515 @@
+// Products of 8-bit integers with a scale for each row of x and each row of the weight, for gfx950. No reference counterpart.
+//
+//   y[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] + bias[n]
+// The sums are int32 and exact (K below 2^17, so they cannot leave 32 bits): no order, cut or tile changes them, and a result is rounded
+// once to f32 by each factor and the bias, and once to its type.
+//
+// Design. x [M, K] and w [N, K] both lie along K, as the matrix instructions take them. Products are formed transposed, weight rows as
+// rows, so that a lane ends with consecutive columns of one row of y.
+#include <stdio.h>
+
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace intent_hip {
+namespace {
+
+constexpr int kUnit = 16;              // bytes of a lane's load; K is a multiple of it
+constexpr int kFewWaves = 16;
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+struct Linear {
+  const int8_t *x, *w;
+  const float *xs, *ws, *bias;         // bias: null for none
+  uint16_t *y;
+  int32_t *sums;                       // [parts][m][n] where K is divided
+  int64_t ldx, ldw, ldy;
+  int m, n, units;                     // units: K / 16
+  int m_tiles, n_tiles, parts, stages; // tiles; stages of a part (or of a wave)
+  int wide;                            // y takes stores of so many elements (1, 4 or 8)
+};
+
+// s_waitcnt with only the vector-memory counter constrained (vmcnt <= n).
+#define INTENT_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt((((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4) | (0xF << 8)))
+#define INTENT_WAIT_LGKMCNT0() __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4))
+
+// s_barrier with an acquire fence alone: a release fence would wait for every load into the LDS that is on its way.
+__device__ __forceinline__ void stage_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// What is read behind K.
+__device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
+
+__device__ __forceinline__ i32x4_t mfma(uint4 a, uint4 b, i32x4_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float scaled(const Linear &p, int sum, float xs, int n) {
+  const float y = static_cast<float>(sum) * xs * p.ws[n];
+  return p.bias != nullptr ? y + p.bias[n] : y;
+}
+
+// kCount consecutive results of one row of y, from column n on.
+template <typename E, int kCount>
+__device__ __forceinline__ void store(const Linear &p, int m, int n, const int (&sum)[kCount]) {
+  if (m >= p.m || n >= p.n) return;
+  uint16_t *y = p.y + m * p.ldy + n;
+  const float xs = p.xs[m];
+  if (p.wide >= 4) {
+#pragma unroll
+    for (int i = 0; i < kCount; i += 4) {
+      if (n + i >= p.n) break;
+      uint32_t words[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        words[j] = from_f32<E>(scaled(p, sum[i + 2 * j], xs, n + i + 2 * j)).bits |
+                   static_cast<uint32_t>(from_f32<E>(scaled(p, sum[i + 2 * j + 1], xs, n + i + 2 * j + 1)).bits) << 16;
+      *reinterpret_cast<uint2 *>(y + i) = make_uint2(words[0], words[1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i)
+      if (n + i < p.n) y[i] = from_f32<E>(scaled(p, sum[i], xs, n + i)).bits;
+  }
+}
+
+// ---------------------------------------------------------------- few rows of x
+// A wave's word of its row of 16 lanes, from lane kFirst on: four of them.
+template <int kFirst>
+__device__ __forceinline__ uint4 words_of_row(uint32_t own) {
+  const int v = static_cast<int>(own);
+  return make_uint4(__builtin_amdgcn_update_dpp(0, v, 0x150 + kFirst, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, v, 0x151 + kFirst, 0xF, 0xF, false),
+                    __builtin_amdgcn_update_dpp(0, v, 0x152 + kFirst, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, v, 0x153 + kFirst, 0xF, 0xF, false));
+}
+
+// Up to 16 rows of x by 16 NT weight rows a workgroup; its 16 waves take a run of K each and add their sums through the LDS. A step is
+// 128 bytes of K, of which lane (r, g) takes 32 of weight row r and, of its row of x, the same; kAhead steps are on their way at once.
+// Columns of the product behind the rows of x are never stored, so their lanes read any row. kOne: x is one row, whose 32 bytes of a
+// lane are spread over the 16 lanes that want them, eight words of which every lane takes by moves within its row of lanes.
+template <typename E, int NT, bool kOne>
+__global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
+  constexpr int kAhead = NT == 1 ? 4 : 2, kSums = NT * 4;
+  __shared__ int sums[kFewWaves][kSums][kWave];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = grid_block() * 16 * NT;
+  if (n0 >= p.n) return;
+  const int8_t *w[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)         // rows behind the last are not stored
+    w[j] = p.w + static_cast<int64_t>(min(n0 + r * NT + j, p.n - 1)) * p.ldw + g * 32;
+  const int8_t *x = kOne ? p.x + g * 32 + (r & 7) * 4 : p.x + min(r, p.m - 1) * p.ldx + g * 32;
+  i32x4_t acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = i32x4_t{0, 0, 0, 0};
+  const int first = min(wave * p.stages * 8, p.units), last = min(first + p.stages * 8, p.units);
+  for (int u0 = first; u0 < last; u0 += kAhead * 8) {
+    uint4 raw[kAhead][NT][2], v[kAhead][2];
+    uint32_t one[kAhead];
+    const bool whole = u0 + kAhead * 8 <= last;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int u = u0 + i * 8 + g * 2;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          raw[i][j][c] = make_uint4(0, 0, 0, 0);
+          if (whole || u + c < last) raw[i][j][c] = *reinterpret_cast<const uint4 *>(w[j] + (u0 + i * 8) * kUnit + c * kUnit);
+        }
+      if constexpr (kOne) {
+        one[i] = 0;
+        if (whole || u + ((r >> 2) & 1) < last) one[i] = *reinterpret_cast<const uint32_t *>(x + (u0 + i * 8) * kUnit);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          v[i][c] = make_uint4(0, 0, 0, 0);
+          if (whole || u + c < last) v[i][c] = *reinterpret_cast<const uint4 *>(x + (u0 + i * 8) * kUnit + c * kUnit);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if constexpr (kOne) v[i][0] = words_of_row<0>(one[i]), v[i][1] = words_of_row<4>(one[i]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = mfma(raw[i][j][c], v[i][c], acc[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[wave][i * NT + j][lane] = acc[j][i];
+  __syncthreads();
+  if (wave >= kSums || r >= p.m) return;
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) total += sums[i][wave][lane];
+  const int n = n0 + g * kSums + wave;
+  if (n < p.n) p.y[r * p.ldy + n] = from_f32<E>(scaled(p, total, p.xs[r], n)).bits;
+}
+
+// ---------------------------------------------------------------- tiles whose weights go to registers
+// 16 MT rows of x by 16 NT weight rows for each of W waves; S stages of B bytes of K are on their way or in use. x passes through the
+// LDS (unit u of row r at another place for each of 16 rows, so that a read's rows lie in different banks), weights go straight to
+// registers: no wave needs another's. Each stage has an LDS array of its own, and the loop is unrolled by S: the compiler then knows
+// which loads into the LDS a read has to wait for.
+template <typename E, int MT, int NT, int S, int W, int B>
+__global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
+  constexpr int kRows = 16 * MT, kRowUnits = B / kUnit, kUnits = kRows * kRowUnits, kLoads = kUnits / (W * kWave);
+  constexpr int kOwn = kRowUnits / 4;                  // units of a stage that a lane multiplies
+  constexpr int kIssued = kLoads + NT * kOwn;          // loads of a wave per stage, always as many
+  static_assert(S == 4 && kLoads >= 1, "one LDS array per stage");
+  __shared__ uint4 x_0[kUnits], x_1[kUnits], x_2[kUnits], x_3[kUnits];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = p.m_tiles * p.n_tiles;
+  int tile = xcd_tile(grid_block(), tiles * p.parts);
+  if (tile < 0) return;
+  const int part = tile / tiles;
+  tile -= part * tiles;
+  const int m0 = tile % p.m_tiles * kRows, n0 = (tile / p.m_tiles * W + wave) * 16 * NT;
+  const int first = min(part * p.stages * kRowUnits, p.units), last = min(p.units, first + p.stages * kRowUnits);     // units of this part
+  const int stages = (last - first + kRowUnits - 1) / kRowUnits;
+  const auto place = [](int row) { return kRowUnits == 16 ? row & 15 : (row >> 1) & 7; };
+  const int8_t *from[kLoads];
+  int unit[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int slot = (i * W + wave) * kWave + lane, row = slot / kRowUnits;
+    unit[i] = slot % kRowUnits ^ place(row);
+    from[i] = p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx + unit[i] * kUnit;      // rows behind the last are not stored
+  }
+  const int8_t *w[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) w[j] = p.w + static_cast<int64_t>(min(n0 + r * NT + j, p.n - 1)) * p.ldw;
+  uint4 raw[S][NT][kOwn];
+  const auto array = [&](int u) -> uint4 * { return u == 0 ? x_0 : u == 1 ? x_1 : u == 2 ? x_2 : x_3; };
+  const auto issue = [&](int t, int set) {             // stage t (the last again behind it) into a set
+    const int u0 = first + min(t, stages - 1) * kRowUnits;
+    const bool whole = u0 + kRowUnits <= last;
+    uint4 *stage = array(set);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int8_t *src = whole || u0 + unit[i] < last ? from[i] + static_cast<int64_t>(u0) * kUnit : reinterpret_cast<const int8_t *>(&kZeroUnit);
+      __builtin_amdgcn_global_load_lds(src, (lds_void_t *)(stage + (i * W + wave) * kWave), 16, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < kOwn; ++c)                   // behind K any: x is 0 there
+        raw[set][j][c] = *reinterpret_cast<const uint4 *>(w[j] + static_cast<int64_t>(min(u0 + g * kOwn + c, last - 1)) * kUnit);
+  };
+  i32x4_t acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+  if (stages > 0) {
+#pragma unroll
+    for (int u = 0; u < S - 1; ++u) issue(u, u);
+    for (int t0 = 0; t0 < stages; t0 += S) {
+#pragma unroll
+      for (int u = 0; u < S; ++u) {
+        if (t0 + u >= stages) break;
+        INTENT_WAIT_VMCNT((S - 2) * kIssued);          // this wave's loads of the stage have come
+        stage_barrier();                               // everybody's have, and nobody reads the set that is filled next
+        issue(t0 + u + S - 1, (u + S - 1) % S);
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) {
+          uint4 v[MT];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) v[i] = array(u)[(i * 16 + r) * kRowUnits + ((g * kOwn + c) ^ place(r))];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = mfma(raw[u][j][c], v[i], acc[i][j]);
+        }
+      }
+    }
+    INTENT_WAIT_VMCNT(0);                              // nothing is on its way into the LDS of an ended workgroup
+  }
+  // A lane's results: row m0 + 16 i + r of y, columns n0 + (4 g + k) NT + j.
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    int row[4 * NT];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) row[k * NT + j] = acc[i][j][k];
+    const int m = m0 + i * 16 + r, n = n0 + g * 4 * NT;
+    if (p.parts == 1) {
+      store<E>(p, m, n, row);
+    } else if (m < p.m) {
+      int32_t *to = p.sums + (static_cast<int64_t>(part) * p.m + m) * p.n + n;
+      if (p.wide >= 4) {
+#pragma unroll
+        for (int k = 0; k < 4 * NT; k += 4)
+          if (n + k < p.n) *reinterpret_cast<i32x4_t *>(to + k) = i32x4_t{row[k], row[k + 1], row[k + 2], row[k + 3]};
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4 * NT; ++k)
+          if (n + k < p.n) to[k] = row[k];
+      }
+    }
+  }
+}
+
+// y from the parts' sums: kCount columns a thread.
+template <typename E, int kCount>
+__global__ __launch_bounds__(256) void linear_fold(Linear p) {
+  const int64_t all = static_cast<int64_t>(p.m) * p.n, at = (static_cast<int64_t>(grid_block()) * 256 + threadIdx.x) * kCount;
+  if (at >= all) return;
+  typedef int held_t __attribute__((ext_vector_type(kCount)));
+  held_t total = 0;
+#pragma unroll 8
+  for (int i = 0; i < p.parts; ++i) total += *reinterpret_cast<const held_t *>(p.sums + i * all + at);
+  const int m = static_cast<int>(at / p.n), n = static_cast<int>(at - static_cast<int64_t>(m) * p.n);
+  int sum[kCount];
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) sum[i] = total[i];
+  store<E>(p, m, n, sum);
+}
+
+// ---------------------------------------------------------------- large tiles, both operands through the LDS
+// 256 rows of x by 256 weight rows, 8 waves in 2 x 4 of 128 x 64 = 4 x 2 products of 32 x 32 x 32. A stage is 64 bytes of K of both, 32
+// KB; five of them arrive by loads into the LDS, and the two waves of a SIMD alternate, one barrier apart, between their matrix
+// products and their reads and loads.
+constexpr int kBM = 256, kBN = 256, kBK = 64, kBigThreads = 512, kBigStages = 5;
+constexpr int kHalf = kBM * kBK / kUnit, kStageUnits = 2 * kHalf;
+
+template <typename E>
+__global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
+  __shared__ uint4 lds[kBigStages * kStageUnits];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const int tile = xcd_tile(grid_block(), p.m_tiles * p.n_tiles);
+  if (tile < 0) return;
+  const int m0 = tile % p.m_tiles * kBM, n0 = tile / p.m_tiles * kBN;
+  // Each wave moves 2 KB of x and 2 KB of the weight a stage. Unit c of row r lies at place c ^ (r / 4) % 4 of its four.
+  const int8_t *x_src[2], *w_src[2];
+  int unit[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int slot = (wave * 2 + i) * kWave + lane, row = slot >> 2;
+    unit[i] = (slot & 3) ^ ((row >> 2) & 3);
+    x_src[i] = p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx + unit[i] * kUnit;
+    w_src[i] = p.w + static_cast<int64_t>(min(n0 + row, p.n - 1)) * p.ldw + unit[i] * kUnit;
+  }
+  const int stages = (p.units + 3) / 4;
+  const auto issue = [&](int t) {
+    uint4 *stage = lds + (t % kBigStages) * kStageUnits;
+    const int64_t k0 = static_cast<int64_t>(t) * kBK;
+    const bool whole = t * 4 + 4 <= p.units;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool held = whole || t * 4 + unit[i] < p.units;
+      const int8_t *zero = reinterpret_cast<const int8_t *>(&kZeroUnit);
+      __builtin_amdgcn_global_load_lds(held ? x_src[i] + k0 : zero, (lds_void_t *)(stage + (wave * 2 + i) * kWave), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(held ? w_src[i] + k0 : zero, (lds_void_t *)(stage + kHalf + (wave * 2 + i) * kWave), 16, 0, 0);
+    }
+  };
+  i32x16_t acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  const int row = lane & 31, half = lane >> 5, turn = (row >> 2) & 3;
+  const bool lag = wave >= 4;
+#pragma unroll
+  for (int t = 0; t < kBigStages - 1; ++t)
+    if (t < stages) issue(t);
+  const auto wait_stage = [&](int t) {                 // this wave's loads of stage t have come; later ones may be on their way
+    const int later = min(stages - 1 - t, kBigStages - 2);
+    if (later >= 3) INTENT_WAIT_VMCNT(12);
+    else if (later == 2) INTENT_WAIT_VMCNT(8);
+    else if (later == 1) INTENT_WAIT_VMCNT(4);
+    else INTENT_WAIT_VMCNT(0);
+  };
+  wait_stage(0);
+  stage_barrier();
+  if (lag) stage_barrier();
+  i32x4_t xf[2][4], wf[2][2];
+  for (int t = 0; t < stages; ++t) {
+    const uint4 *sx = lds + (t % kBigStages) * kStageUnits, *sw = sx + kHalf;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xf[k][i] = __builtin_bit_cast(i32x4_t, sx[(wm * 128 + i * 32 + row) * 4 + ((k * 2 + half) ^ turn)]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) wf[k][j] = __builtin_bit_cast(i32x4_t, sw[(wn * 64 + j * 32 + row) * 4 + ((k * 2 + half) ^ turn)]);
+    }
+    if (t + kBigStages - 1 < stages) issue(t + kBigStages - 1);
+    if (lag) wait_stage(t + 1);
+    INTENT_WAIT_LGKMCNT0();
+    stage_barrier();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k][j], xf[k][i], acc[i][j], 0, 0, 0);
+    if (!lag) wait_stage(t + 1);
+    stage_barrier();
+  }
+  if (!lag) stage_barrier();
+  // acc[i][j][4 q + e] is row 32 i + (lane % 32) of x with weight row 32 j + 8 q + 4 half + e.
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int sum[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        store<E>(p, m0 + wm * 128 + i * 32 + row, n0 + wn * 64 + j * 32 + 8 * q + 4 * half, sum);
+      }
+}
+
+// ---------------------------------------------------------------- which kernel
+// How a product is cut. mt = 0: linear_few; 1: of one row; 16: linear_big.
+struct Cut {
+  int mt, nt, parts;
+};
+constexpr int tile_waves(int mt) { return mt == 2 ? 8 : 4; }
+constexpr int stage_bytes(int mt) { return mt == 2 ? 256 : 128; }
+
+Cut cut(int64_t m, int64_t n, int64_t k) {
+  const int cus = device_cus();
+  if (m == 1) return {1, n >= 24 * cus ? 2 : 1, 1};
+  if (m <= 16) return {0, n >= 24 * cus ? 2 : 1, 1};
+  constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.53f, 0.5f}, {4, 2, 0.55f, 0.45f}, {8, 2, 0.8f, 0.65f}, {16, 16, 0.62f, 0.62f}};
+  Cut best{};
+  float least = 0.0f;
+  for (const auto &kind : kKinds) {
+    const int64_t per_tile = kind.mt == 16 ? kBN : 16 * tile_waves(kind.mt) * kind.nt;
+    const int64_t tiles = ((m + 16 * kind.mt - 1) / (16 * kind.mt)) * ((n + per_tile - 1) / per_tile);
+    const int64_t bytes = kind.mt == 16 ? kBK : stage_bytes(kind.mt), stages = (k + bytes - 1) / bytes;
+    for (int parts = 1; parts <= (kind.mt == 16 ? 1 : 16) && (parts == 1 || parts * 4 <= stages); ++parts) {
+      const float on_one = static_cast<float>((tiles * parts + cus - 1) / cus), shared = kind.shared * on_one;
+      float us = static_cast<float>((stages + parts - 1) / parts) * (kind.alone > shared ? kind.alone : shared);
+      if (parts > 1) us += 3.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(n) * 2.3e-6f;
+      if (best.parts == 0 || us < least) best = {kind.mt, kind.nt, parts}, least = us;
+    }
+  }
+  return best;
+}
+
+// f with the kernel of a cut, its name and its waves.
+template <typename E, typename F>
+int with_kernel(const Cut &c, F f) {
+  if (c.mt == 0) return c.nt == 1 ? f(linear_few<E, 1, false>, "linear_few", kFewWaves) : f(linear_few<E, 2, false>, "linear_few", kFewWaves);
+  if (c.mt == 1) return c.nt == 1 ? f(linear_few<E, 1, true>, "linear_few", kFewWaves) : f(linear_few<E, 2, true>, "linear_few", kFewWaves);
+  if (c.mt == 16) return f(linear_big<E>, "linear_big", kBigThreads / kWave);
+  return c.mt == 2   ? f(linear_tiles<E, 2, 1, 4, tile_waves(2), stage_bytes(2)>, "linear_tiles", tile_waves(2))
+         : c.mt == 4 ? f(linear_tiles<E, 4, 2, 4, tile_waves(4), stage_bytes(4)>, "linear_tiles", tile_waves(4))
+                     : f(linear_tiles<E, 8, 2, 4, tile_waves(8), stage_bytes(8)>, "linear_tiles", tile_waves(8));
+}
+
+template <typename E>
+void launch(Linear p, const Cut &c, hipStream_t s) {
+  p.parts = c.parts;
+  with_kernel<E>(c, [&](void (*kernel)(Linear), const char *, int waves) {
+    dim3 grid;
+    if (c.mt <= 1) {
+      p.stages = ((p.units + 7) / 8 + waves - 1) / waves;
+      grid = tile_grid((p.n + 16 * c.nt - 1) / (16 * c.nt), 1);
+    } else if (c.mt == 16) {
+      p.m_tiles = (p.m + kBM - 1) / kBM, p.n_tiles = (p.n + kBN - 1) / kBN;
+      grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles, 1);
+    } else {
+      const int of_stage = stage_bytes(c.mt) / kUnit;
+      p.stages = ((p.units + of_stage - 1) / of_stage + c.parts - 1) / c.parts;
+      p.m_tiles = (p.m + 16 * c.mt - 1) / (16 * c.mt), p.n_tiles = (p.n + 16 * waves * c.nt - 1) / (16 * waves * c.nt);
+      grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.parts, 1);
+    }
+    kernel<<<grid, waves * kWave, 0, s>>>(p);
+    return 0;
+  });
+  if (c.parts == 1) return;
+  const int64_t all = static_cast<int64_t>(p.m) * p.n;
+  if (p.wide >= 4)
+    linear_fold<E, 4><<<tile_grid((all / 4 + 255) / 256, 1), 256, 0, s>>>(p);
+  else
+    linear_fold<E, 1><<<tile_grid((all + 255) / 256, 1), 256, 0, s>>>(p);
+}
+
+int check(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 0 || k < 0) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "negative extent");
+  if (k % kUnit) return fail(INTENT_HIP_ERR_UNSUPPORTED, "linear_i8 takes K in multiples of %d (got %lld)", kUnit, static_cast<long long>(k));
+  if (k >= 1 << 17) return fail(INTENT_HIP_ERR_UNSUPPORTED, "linear_i8 sums K below 131072 in 32 bits (got %lld)", static_cast<long long>(k));
+  if (m > (1 << 20) || n > (1 << 24) || m * n > (int64_t{1} << 40)) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
+  return INTENT_HIP_OK;
+}
+
+}  // namespace
+
+int linear_i8_resources(int dtype, int64_t m, int64_t n, int64_t k, IntentHipKernelResources *out) {
+  if (int rc = check(m, n, k)) return rc;
+  const Cut c = cut(m, n, k);
+  const auto describe = [&](void (*kernel)(Linear), const char *which, int waves) {
+    char name[64];
+    snprintf(name, sizeof(name), "linear_i8 %s<%s,%d,%d>", which, dtype == INTENT_HIP_F16 ? "f16" : "bf16", c.mt, c.nt);
+    return describe_kernel(reinterpret_cast<const void *>(kernel), name, waves * kWave, out);
+  };
+  return dtype == INTENT_HIP_F16 ? with_kernel<f16_t>(c, describe) : with_kernel<bf16_t>(c, describe);
+}
+
+}  // namespace intent_hip
+
+using namespace intent_hip;
+
+extern "C" int intent_hip_linear_i8_workspace_bytes(int64_t m, int64_t n, int64_t k, size_t *bytes) {
+  if (bytes == nullptr) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null output");
+  *bytes = 0;
+  if (int rc = check(m, n, k)) return rc;
+  if (m == 0 || n == 0) return INTENT_HIP_OK;
+  const Cut c = cut(m, n, k);
+  if (c.parts > 1) *bytes = static_cast<size_t>(c.parts) * m * n * sizeof(int32_t);
+  return INTENT_HIP_OK;
+}
+
+extern "C" int intent_hip_linear_i8(int dtype, const int8_t *x, const int8_t *weight, const float *x_scales, const float *weight_scales,
+                                    const float *bias, void *y, int64_t m, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t ldy,
+                                    void *workspace, size_t workspace_bytes, void *stream) {
+  if (dtype != INTENT_HIP_F16 && dtype != INTENT_HIP_BF16)
+    return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "linear_i8 dtype must be F16 or BF16, got %d", dtype);
+  if (ldx < 0 || ldw < 0 || ldy < 0) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "negative stride");
+  if (int rc = check(m, n, k)) return rc;
+  if (m == 0 || n == 0) return INTENT_HIP_OK;
+  if (y == nullptr || x_scales == nullptr || weight_scales == nullptr || (k > 0 && (x == nullptr || weight == nullptr)))
+    return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null pointer");
+  if (k > 0 && (ldx % kUnit || !aligned(x, kUnit)))
+    return fail(INTENT_HIP_ERR_UNSUPPORTED, "rows of x must be 16-byte aligned, their stride a multiple of 16");
+  if (k > 0 && (ldw % kUnit || !aligned(weight, kUnit)))
+    return fail(INTENT_HIP_ERR_UNSUPPORTED, "weight rows must be 16-byte aligned, their stride a multiple of 16");
+  if (!aligned(y, 2)) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "y is not aligned to its type");
+  Linear p{};
+  p.x = x, p.w = weight, p.xs = x_scales, p.ws = weight_scales, p.bias = bias, p.y = static_cast<uint16_t *>(y);
+  p.ldx = ldx, p.ldw = ldw, p.ldy = ldy;
+  p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.units = static_cast<int>(k / kUnit);
+  p.wide = n % 8 == 0 && ldy % 8 == 0 && aligned(y, 16) ? 8 : n % 4 == 0 && ldy % 4 == 0 && aligned(y, 8) ? 4 : 1;
+  const Cut c = cut(m, n, k);
+  if (c.parts > 1) {
+    const size_t bytes = static_cast<size_t>(c.parts) * m * n * sizeof(int32_t);
+    if (workspace == nullptr || workspace_bytes < bytes || !aligned(workspace, 16))
+      return fail(INTENT_HIP_ERR_WORKSPACE, "linear_i8 needs %zu workspace bytes, 16-byte aligned", bytes);
+    p.sums = static_cast<int32_t *>(workspace);
+  }
+  if (dtype == INTENT_HIP_F16)
+    launch<f16_t>(p, c, as_stream(stream));
+  else
+    launch<bf16_t>(p, c, as_stream(stream));
+  return hipPeekAtLastError() != hipSuccess ? launch_status("linear_i8") : INTENT_HIP_OK;
+}

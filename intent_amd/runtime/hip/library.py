@@ -11,7 +11,7 @@ from pathlib import Path
 
 from ...diagnostics import CompilationStageError
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 # INTENT_HIP_STATIC_SCRATCH_BYTES: the static scratch of intent_hip_csr_spmv_f32_static.
 STATIC_SCRATCH_BYTES = 32 << 20
 LIBRARY_NAME = "libintent_hip.so"
@@ -23,7 +23,8 @@ F32, F16, BF16 = 0, 1, 2
  OP_SPLITK_REDUCE, OP_CSR_SPMM_F32, OP_ATTENTION_VARLEN, OP_GEMM_I8, OP_QUANTIZED_GEMM,
  OP_ATTENTION_BIAS, OP_GROUPED_DECODE_PARTIALS, OP_CONTINUOUS_DECODE, OP_VARLEN_DECODE, OP_DECODE_MERGE,
  OP_MLA_PREFILL, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ,
- OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4) = range(29)
+ OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4, OP_RESIDUAL_NORM, OP_RESIDUAL_NORM_I8, OP_RESIDUAL_NORM_BACKWARD,
+ OP_QUANTIZE_ROWS, OP_SWIGLU_QUANTIZE_ROWS, OP_LINEAR_I8, OP_PAGED_GQA_DECODE_PREFIX) = range(36)
 ACT_NONE, ACT_RELU = 0, 1
 
 _i64, _int, _p, _f32, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_size_t
@@ -120,6 +121,17 @@ SIGNATURES = {
     "intent_hip_paged_gqa_decode_mx": (_int, (_int, *[_p] * 9, *[_i64] * 8, ctypes.POINTER(_i64), _f32, _p, _sz, _p)),
     "intent_hip_linear_mxfp4_workspace_bytes": (_int, (_i64, _i64, _i64, ctypes.POINTER(_sz))),
     "intent_hip_linear_mxfp4": (_int, (_int, *[_p] * 4, *[_i64] * 7, _p, _sz, _p)),
+    "intent_hip_residual_norm": (_int, (_int, *[_p] * 7, *[_i64] * 4, ctypes.POINTER(_i64), _f32, _f32, _f32, _p)),
+    "intent_hip_residual_norm_i8": (_int, (_int, *[_p] * 8, *[_i64] * 4, ctypes.POINTER(_i64), _f32, _f32, _f32, _p)),
+    "intent_hip_residual_norm_backward_workspace_bytes": (_int, (_i64, _i64, _i64, ctypes.POINTER(_sz))),
+    "intent_hip_residual_norm_backward": (_int, (_int, *[_p] * 12, *[_i64] * 4, ctypes.POINTER(_i64), _f32, _f32, _f32, _p, _sz,
+                                                 _p)),
+    "intent_hip_quantize_rows": (_int, (_int, *[_p] * 3, *[_i64] * 4, _p)),
+    "intent_hip_swiglu_quantize_rows": (_int, (_int, *[_p] * 4, *[_i64] * 5, _p)),
+    "intent_hip_linear_i8_workspace_bytes": (_int, (_i64, _i64, _i64, ctypes.POINTER(_sz))),
+    "intent_hip_linear_i8": (_int, (_int, *[_p] * 6, *[_i64] * 6, _p, _sz, _p)),
+    "intent_hip_paged_gqa_decode_prefix_workspace_bytes": (_int, (*[_i64] * 8, ctypes.POINTER(_sz))),
+    "intent_hip_paged_gqa_decode_prefix": (_int, (_int, *[_p] * 9, *[_i64] * 9, ctypes.POINTER(_i64), _f32, _p, _sz, _p)),
     "intent_hip_mfma_probe": (_int, (_int, _int, _i64, _i64, _p, _p)),
 }
 

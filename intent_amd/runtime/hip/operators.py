@@ -42,6 +42,13 @@ Recognised definitions (reference file:line of the semantics each kernel follows
   paged_cache_read_{f16,bf16}       streaming/mx_cache.py          intent_hip_paged_cache_read
   paged_gqa_decode_mx_{f16,bf16}    streaming/mx_cache.py          intent_hip_paged_gqa_decode_mx
   linear_mxfp4_{f16,bf16}           contraction/linear_mxfp4.py    intent_hip_linear_mxfp4
+  residual_norm_{f16,bf16}          normalization/residual_norm.py intent_hip_residual_norm
+  residual_norm_i8_{f16,bf16}       normalization/residual_norm.py intent_hip_residual_norm_i8
+  residual_norm_backward_{f16,bf16} backward/residual_norm.py      intent_hip_residual_norm_backward
+  quantize_rows_{f16,bf16}          normalization/quantize_rows.py intent_hip_quantize_rows
+  swiglu_quantize_rows_{f16,bf16}   normalization/quantize_rows.py intent_hip_swiglu_quantize_rows
+  linear_i8_{f16,bf16}              contraction/linear_i8.py       intent_hip_linear_i8
+  paged_gqa_decode_prefix_{f16,bf16} streaming/prefix_decode.py    intent_hip_paged_gqa_decode_prefix
 
 Layout handling: kernels read rows with unit inner stride. An input whose inner
 stride is not 1 is copied into a contiguous device buffer at every launch (on
@@ -61,7 +68,8 @@ from ...diagnostics import CompilationStageError
 from ..torch_views import raw_stream_getter
 from .library import (BF16, F16, F32, STATIC_SCRATCH_BYTES, OP_ATTENTION_BWD_DELTA, OP_ATTENTION_BWD_DKDV, OP_ATTENTION_BWD_DQ,
                       OP_ATTENTION_FWD, OP_ATTENTION_FWD_F16, OP_ATTENTION_BIAS, OP_ATTENTION_VARLEN, OP_MLA_PREFILL, OP_CSR_SPMV_F32, OP_GEMM, OP_GEMM_F32, OP_GEMM_I8, OP_QUANTIZED_GEMM,
-                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ, OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
+                      OP_CSR_SPMM_F32, OP_CONTINUOUS_DECODE, OP_GROUPED_DECODE_PARTIALS, OP_PAGED_DECODE_PARTIALS, OP_PAGED_CACHE_APPEND, OP_PAGED_CACHE_READ, OP_PAGED_GQA_DECODE_MX, OP_LINEAR_MXFP4, OP_LINEAR_I8, OP_PAGED_GQA_DECODE_PREFIX, OP_QUANTIZE_ROWS, OP_SWIGLU_QUANTIZE_ROWS,
+                      OP_RESIDUAL_NORM, OP_RESIDUAL_NORM_BACKWARD, OP_RESIDUAL_NORM_I8, OP_QK_NORM_ROPE, OP_QK_NORM_ROPE_BACKWARD, OP_VARLEN_DECODE, OP_SOFTMAX_BWD, OP_SOFTMAX_FWD, OP_SPLITK_REDUCE)
 
 
 @dataclass
@@ -87,9 +95,14 @@ class OperatorSpec:
     signature: tuple              # per runtime parameter: ("view", access, dtype, rank) | ("scalar", dtype)
     constexprs: tuple[str, ...]
     plan: Callable
-    inplace_safe: bool = False    # an Out may be exactly one of the inputs (same address and strides)
+    # An Out may be exactly one of the inputs (same address and strides): True, or the pairs of positions of which that holds.
+    inplace_safe: bool | frozenset = False
     derived: tuple = ()           # (symbol, source symbol, offset): extent(symbol) = extent(source) + offset
     repeats: bool = False         # its launches can be made again for other arguments of their layout (Launch.again)
+
+    def may_be_one(self, left: int, right: int) -> bool:
+        """Whether the parameters at two positions, of which one is written, may be the same view."""
+        return self.inplace_safe is True or bool(self.inplace_safe) and (left, right) in self.inplace_safe
 
     @property
     def entry_point(self) -> str:
@@ -1230,6 +1243,212 @@ def _linear_mxfp4(dtype_code):
     return plan
 
 
+# ------------------------------------------------------------------------------ norm of the residual stream
+def _residual_norm_checked(gate, post_weight, weight, tokens):
+    """(number of gates, of the block's norm's weights), each 0 where there is none."""
+    gates, post, d = gate.shape[0], post_weight.shape[0], weight.shape[0]
+    if gates not in (0, tokens):
+        raise ValueError(f"gate holds a number for each of {tokens} tokens, or none at all; got {gates}")
+    if post not in (0, d):
+        raise ValueError(f"post_weight holds a number for each of {d} columns, or none at all; got {post}")
+    return gates, post
+
+
+def _rows_mixed(wide, narrow=()) -> int:
+    """`_mixed` of rows of 16 bits and of weights, and of rows of 8 bits at twice their size: pieces of 16 and of 8 bytes."""
+    return _mixed(*wide) | 2 * _mixed(*narrow)
+
+
+def _residual_norm(dtype_code, narrow: bool):
+    """residual_norm, residual_norm_i8: rows are read through their own strides, staged only where their inner stride is not 1."""
+    name = "residual_norm_i8" if narrow else "residual_norm"
+
+    def plan(lib, bound, constexprs, device):
+        import ctypes
+
+        block, residual, gate, post_weight, weight, total, output, *more = bound.arguments
+        scales, numbers = more[:-3], more[-3:]
+        (tokens, d), (gates, post) = block.shape, _residual_norm_checked(gate, post_weight, weight, block.shape[0])
+        keep, before, after = [], [], []
+        block, residual, post_weight, weight = (_readable(t, keep, before) for t in (block, residual, post_weight, weight))
+        total, output, *scales = (_writable(t, keep, after) for t in (total, output, *scales))
+        strides = (ctypes.c_int64 * 5)(*(t.stride(0) for t in (block, residual, gate, total, output)))
+        fn, op = lib.fn[name], OP_RESIDUAL_NORM_I8 if narrow else OP_RESIDUAL_NORM
+        configuration = (("tokens", tokens), ("d", d), ("gates", gates), ("post", post))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values[:-3]], tokens, d, gates, post, strides, *map(float, values[-3:]))
+            rows = (*values[:2], *values[3:6])
+            return Launch("intent_hip_" + name, lambda stream: fn(*args, stream), values, configuration=configuration,
+                          resources=lambda: lib.call_resources(op, dtype_code, d, post, _rows_mixed(rows, values[6:7]) if narrow
+                                                               else _rows_mixed((*rows, values[6]))))
+        return _staged(again, (block, residual, gate, post_weight, weight, total, output, *scales, *numbers), bound, before, after)
+    return plan
+
+
+def _residual_norm_backward(dtype_code):
+    """residual_norm_backward: each slot of tokens keeps its share of the weights' gradients, summed in order through a workspace."""
+    def plan(lib, bound, constexprs, device):
+        import ctypes
+
+        block, total, gate, post_weight, weight, *rest = bound.arguments
+        grads, (grad_block, grad_residual, grad_gate, *grad_weights), numbers = rest[:2], rest[2:7], rest[7:]
+        (tokens, d), (gates, post) = block.shape, _residual_norm_checked(gate, post_weight, weight, block.shape[0])
+        _no_static("residual_norm_backward", "sums the weights' gradients through")
+        keep, before, after = [], [], []
+        block, total, post_weight, weight, *grads = (_readable(t, keep, before) for t in (block, total, post_weight, weight, *grads))
+        grad_block, grad_residual, *grad_weights = (_writable(t, keep, after) for t in (grad_block, grad_residual, *grad_weights))
+        strides = (ctypes.c_int64 * 8)(*(t.stride(0) for t in (block, total, gate, *grads, grad_block, grad_residual, grad_gate)))
+        size = ctypes.c_size_t(0)
+        lib.check(lib.fn["residual_norm_backward_workspace_bytes"](tokens, d, post, ctypes.byref(size)), "provider_preparation")
+        fn, size = lib.fn["residual_norm_backward"], size.value
+        configuration = (("tokens", tokens), ("d", d), ("gates", gates), ("post", post), ("workspace_bytes", size))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values[:12]], tokens, d, gates, post, strides, *map(float, values[12:]))
+            keep = [values]
+            return Launch("intent_hip_residual_norm_backward", _optional_workspace_run(fn, args, size, device, keep), tuple(keep),
+                          configuration=configuration,
+                          resources=lambda: lib.call_resources(OP_RESIDUAL_NORM_BACKWARD, dtype_code, d, post,
+                                                               _rows_mixed((*values[:2], *values[3:9]))))
+        return _staged(again, (block, total, gate, post_weight, weight, *grads, grad_block, grad_residual, grad_gate, *grad_weights,
+                               *numbers), bound, before, after)
+    return plan
+
+
+def _residual_norm_signature(element, kind):
+    rows, weight, number = _view(IN, element, 2), _view(IN, "f32", 1), ("scalar", "f32")
+    out, out_weight = _view(OUT, element, 2), _view(OUT, "f32", 1)
+    if kind == "backward":
+        return (rows, rows, *[weight] * 3, rows, rows, out, out, *[out_weight] * 3, *[number] * 3)
+    outputs = (out, _view(OUT, "i8", 2), out_weight) if kind == "i8" else (out, out)
+    return (rows, rows, *[weight] * 3, *outputs, *[number] * 3)
+
+
+# Rows that may be written where rows were read, each element by the thread that read it: sum and output over block and residual
+# (8-bit rows are others), gradients over any rows.
+_NORM_IN_PLACE = frozenset(((0, 5), (1, 5), (0, 6), (1, 6)))
+_NORM_I8_IN_PLACE = frozenset(((0, 5), (1, 5)))
+_NORM_BACKWARD_IN_PLACE = frozenset((i, j) for i in (0, 1, 5, 6) for j in (7, 8))
+
+
+# ------------------------------------------------------------------------------ products of 8-bit integers
+def _quantize_rows(dtype_code, gated: bool):
+    """quantize_rows, swiglu_quantize_rows: rows (halves of one projection's, say) are read through their own strides."""
+    name, op = ("swiglu_quantize_rows", OP_SWIGLU_QUANTIZE_ROWS) if gated else ("quantize_rows", OP_QUANTIZE_ROWS)
+
+    def plan(lib, bound, constexprs, device):
+        *rows, output, scales = bound.arguments
+        keep, before, after = [], [], []
+        rows = [_readable(t, keep, before) for t in rows]
+        output, scales = (_writable(t, keep, after) for t in (output, scales))
+        count, d = output.shape
+        strides = tuple(t.stride(0) for t in (*rows, output))
+        fn = lib.fn[name]
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values], count, d, *strides)
+            return Launch("intent_hip_" + name, lambda stream: fn(*args, stream), values, configuration=(("rows", count), ("d", d)),
+                          resources=lambda: lib.call_resources(op, dtype_code, d, _rows_mixed(values[:-2], values[-2:-1])))
+        return _staged(again, (*rows, output, scales), bound, before, after)
+    return plan
+
+
+def _quantize_rows_signature(element, gated):
+    return (*[_view(IN, element, 2)] * (2 if gated else 1), _view(OUT, "i8", 2), _view(OUT, "f32", 1))
+
+
+def _linear_i8(dtype_code):
+    """linear_i8: x is staged where its layout is not the kernel's; a weight never is."""
+    def plan(lib, bound, constexprs, device):
+        import ctypes
+
+        x, weight, x_scales, weight_scales, bias, out = bound.arguments
+        (m, k), n, biases = x.shape, weight.shape[0], bias.shape[0]
+        if k % 16:
+            raise ValueError(f"products of 8-bit integers take K in multiples of 16, got {k}")
+        if biases not in (0, n):
+            raise ValueError(f"bias holds a number for each of {n} columns, or none at all; got {biases}")
+        if not _aligned(weight, 16):
+            raise ValueError(f"weights need unit inner stride, rows in multiples of 16 bytes and a 16-byte aligned start; got strides "
+                             f"{tuple(weight.stride())}")
+        keep, before, after = [], [], []
+        x, out = _readable(x, keep, before, 16), _writable(out, keep, after)
+        x_scales, weight_scales, bias = (_readable(t, keep, before) for t in (x_scales, weight_scales, bias))
+        extents = (m, n, k, *(_outer_strides(t)[0] for t in (x, weight, out)))
+        size = ctypes.c_size_t(0)
+        lib.check(lib.fn["linear_i8_workspace_bytes"](m, n, k, ctypes.byref(size)), "provider_preparation")
+        fn, size = lib.fn["linear_i8"], size.value
+        if size:
+            _no_static("linear_i8", "divides K of few tiles over workgroups whose sums meet in")
+        configuration = (("m", m), ("n", n), ("k", k), ("bias", biases > 0), ("workspace_bytes", size))
+
+        def again(values):
+            addresses = [t.data_ptr() for t in values]
+            if not biases:
+                addresses[4] = None
+            args = (dtype_code, *addresses, *extents)
+            keep = [values]
+            return Launch("intent_hip_linear_i8", _optional_workspace_run(fn, args, size, device, keep), tuple(keep),
+                          configuration=configuration, resources=lambda: lib.call_resources(OP_LINEAR_I8, dtype_code, m, n, k))
+        return _staged(again, (x, weight, x_scales, weight_scales, bias, out), bound, before, after)
+    return plan
+
+
+def _linear_i8_signature(element):
+    return (_view(IN, "i8", 2), _view(IN, "i8", 2), *[_view(IN, "f32", 1)] * 3, _view(OUT, element, 2))
+
+
+# ------------------------------------------------------------------------------ decode behind a shared prefix
+def _paged_decode_prefix(dtype_code):
+    """paged_gqa_decode_prefix: parts of the prefix and jobs of the sequences' pages, whose states a second kernel joins through a
+    workspace. The caches are read in place, never staged."""
+    def plan(lib, bound, constexprs, device):
+        import ctypes
+
+        q, *caches, prefix_indices, prefix_length, page_offsets, page_indices, lengths, output, scale = bound.arguments
+        group = _positive_constexpr(constexprs, "HEAD_GROUP")
+        batch, q_heads, d = q.shape
+        pages, ps, kv_heads, _ = caches[0].shape
+        if kv_heads * group != q_heads:
+            raise ValueError(f"query heads ({q_heads}) must equal key/value heads ({kv_heads}) * HEAD_GROUP ({group})")
+        if prefix_length.shape[0] != 1:
+            raise ValueError(f"prefix_length holds one number, got {prefix_length.shape[0]}")
+        if page_offsets.shape[0] != batch + 1:
+            raise ValueError(f"page_offsets must hold batch + 1 = {batch + 1} entries, got {page_offsets.shape[0]}")
+        for name, cache in zip(("key_cache", "value_cache"), caches):
+            if not _aligned(cache, 8):
+                raise ValueError(f"{name} needs unit inner stride, other strides in multiples of 8 and a 16-byte aligned start, got "
+                                 f"strides {tuple(cache.stride())}")
+        _no_static("paged_gqa_decode_prefix", "joins the states of its jobs through")
+        keep, before, after = [], [], []
+        q, output = _readable(q, keep, before, 8), _writable(output, keep, after)
+        tables = [_readable(t, keep, before) for t in (prefix_indices, prefix_length, page_offsets, page_indices, lengths)]
+        strides = (ctypes.c_int64 * 14)(*(st for t in (q, *caches, output) for st in (*_outer_strides(t), 1)))
+        extents = (batch, q_heads, kv_heads, group, d)
+        positions, size = (prefix_indices.shape[0], page_indices.shape[0]), ctypes.c_size_t(0)
+        lib.check(lib.fn["paged_gqa_decode_prefix_workspace_bytes"](*extents, ps, *positions, ctypes.byref(size)),
+                  "provider_preparation")
+        fn, size = lib.fn["paged_gqa_decode_prefix"], size.value
+        configuration = (("batch", batch), ("q_heads", q_heads), ("kv_heads", kv_heads), ("d", d), ("pages", pages), ("ps", ps),
+                         ("prefix_positions", positions[0]), ("positions", positions[1]), ("workspace_bytes", size))
+
+        def again(values):
+            args = (dtype_code, *[t.data_ptr() for t in values[:9]], *extents, pages, ps, *positions, strides, float(values[9]))
+            keep = [values]
+            return Launch("intent_hip_paged_gqa_decode_prefix", _optional_workspace_run(fn, args, size, device, keep), tuple(keep),
+                          configuration=configuration,
+                          resources=lambda: lib.call_resources(OP_PAGED_GQA_DECODE_PREFIX, dtype_code, batch, kv_heads, group, d, ps,
+                                                               *positions))
+        return _staged(again, (q, *caches, *tables, output, scale), bound, before, after)
+    return plan
+
+
+def _decode_prefix_signature(element):
+    rows, cache, table = _view(IN, element, 3), _view(IN, element, 4), _view(IN, "i32", 1)
+    return (rows, cache, cache, *[table] * 5, _view(OUT, element, 3), ("scalar", "f32"))
+
+
 _repeated = functools.partial(OperatorSpec, repeats=True)
 _SPECS = (
     OperatorSpec("stable_softmax", (_view(IN, "f32", 2), _view(OUT, "f32", 2)), (), _softmax_fwd(F32), True),
@@ -1321,6 +1540,26 @@ _SPECS = (
               _linear_mxfp4(F16)),
     _repeated("linear_mxfp4_bf16", (_view(IN, "bf16", 2), _view(IN, "u8", 2), _view(IN, "u8", 2), _view(OUT, "bf16", 2)), (),
               _linear_mxfp4(BF16)),
+    _repeated("residual_norm_f16", _residual_norm_signature("f16", ""), (), _residual_norm(F16, False),
+              inplace_safe=_NORM_IN_PLACE),
+    _repeated("residual_norm_bf16", _residual_norm_signature("bf16", ""), (), _residual_norm(BF16, False),
+              inplace_safe=_NORM_IN_PLACE),
+    _repeated("residual_norm_i8_f16", _residual_norm_signature("f16", "i8"), (), _residual_norm(F16, True),
+              inplace_safe=_NORM_I8_IN_PLACE),
+    _repeated("residual_norm_i8_bf16", _residual_norm_signature("bf16", "i8"), (), _residual_norm(BF16, True),
+              inplace_safe=_NORM_I8_IN_PLACE),
+    _repeated("residual_norm_backward_f16", _residual_norm_signature("f16", "backward"), (), _residual_norm_backward(F16),
+              inplace_safe=_NORM_BACKWARD_IN_PLACE),
+    _repeated("residual_norm_backward_bf16", _residual_norm_signature("bf16", "backward"), (), _residual_norm_backward(BF16),
+              inplace_safe=_NORM_BACKWARD_IN_PLACE),
+    _repeated("quantize_rows_f16", _quantize_rows_signature("f16", False), (), _quantize_rows(F16, False)),
+    _repeated("quantize_rows_bf16", _quantize_rows_signature("bf16", False), (), _quantize_rows(BF16, False)),
+    _repeated("swiglu_quantize_rows_f16", _quantize_rows_signature("f16", True), (), _quantize_rows(F16, True)),
+    _repeated("swiglu_quantize_rows_bf16", _quantize_rows_signature("bf16", True), (), _quantize_rows(BF16, True)),
+    _repeated("linear_i8_f16", _linear_i8_signature("f16"), (), _linear_i8(F16)),
+    _repeated("linear_i8_bf16", _linear_i8_signature("bf16"), (), _linear_i8(BF16)),
+    _repeated("paged_gqa_decode_prefix_f16", _decode_prefix_signature("f16"), ("HEAD_GROUP",), _paged_decode_prefix(F16)),
+    _repeated("paged_gqa_decode_prefix_bf16", _decode_prefix_signature("bf16"), ("HEAD_GROUP",), _paged_decode_prefix(BF16)),
 )
 
 SPECS = {spec.name: spec for spec in _SPECS}
@@ -1351,6 +1590,9 @@ ENTRY_POINTS = {
     "paged_cache_read_f16": "intent_hip_paged_cache_read", "paged_cache_read_bf16": "intent_hip_paged_cache_read",
     "paged_gqa_decode_mx_f16": "intent_hip_paged_gqa_decode_mx", "paged_gqa_decode_mx_bf16": "intent_hip_paged_gqa_decode_mx",
     "linear_mxfp4_f16": "intent_hip_linear_mxfp4", "linear_mxfp4_bf16": "intent_hip_linear_mxfp4",
+    **{f"{name}_{element}": "intent_hip_" + name for element in ("f16", "bf16")
+       for name in ("residual_norm", "residual_norm_i8", "residual_norm_backward", "quantize_rows", "swiglu_quantize_rows", "linear_i8",
+                    "paged_gqa_decode_prefix")},
 }
 assert set(ENTRY_POINTS) == set(SPECS)
 

@@ -190,7 +190,7 @@ class HipProgram:
             if not (lf.begin < lf.end and rf.begin < rf.end and lf.begin < rf.end and rf.begin < lf.end):
                 continue
             exact = (lf.pointer == rf.pointer and lf.shape == rf.shape and lf.strides == rf.strides)
-            if (exact and self.spec.inplace_safe and not both) or share_no_byte(lf, rf):
+            if (exact and self.spec.may_be_one(i, j) and not both) or share_no_byte(lf, rf):
                 continue
             left, right = self.interface.parameters[i], self.interface.parameters[j]
             raise ValueError(f"{left.name} and {right.name} overlap; the hip kernel for "
