@@ -3,9 +3,9 @@
 //
 // For query head h of sequence s, over the prefix's tokens and the sequence's own:
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = exp2(scale * log2(e) * (q . k_j) - peak)        0 where there is no token
-// Products are summed in f32. Weights enter the second product in the queries' type: f16 numbers of 11 bits, held at 2^11 times their
-// share of the largest so that those down to 2^-25 of it keep all bits (and none matters below 2^-35), or two bf16 numbers of 8 bits
-// each. The sum that divides is of the weights as they were rounded, so a rounding moves a weight and no more.
+// Products are summed in f32. Weights enter the second product as two numbers of the queries' type each: two of f16 hold 21 bits, at 2^11
+// times their share of the largest, which leaves out no more than 2^-36 of that; two of bf16 hold 16. The sum that divides is of the
+// weights as they were rounded, so a rounding moves a weight and no more.
 //
 // Design. One launch does two kinds of jobs, whose states (peak, sum of weights, weighted sum of values) a second kernel joins:
 //   * the prefix: the query heads of all sequences that share a key head are the rows of one product, so the prefix is read once for 64
@@ -36,6 +36,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -73,26 +74,33 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-template <typename E>
-constexpr int kParts = std::is_same_v<E, f16_t> ? 1 : 2;          // numbers of a weight
+constexpr int kParts = 2;              // numbers of a weight
 // Weights are held at this power of two (times 2^kSlack they stay below the largest f16).
 template <typename E>
 constexpr float kRaise = std::is_same_v<E, f16_t> ? 11.0f : 0.0f;
 
-// Two weights as kParts numbers each, and what these add up to.
+// Two weights as kParts numbers each, and what these add up to. No part of a weight that counts is 0, so that an infinite value gives an
+// infinity and not 0 times it: of f16 the first number is cut off below the weight, which leaves a second of 2^-10 of it at least (for
+// weights from 2^-25 of the largest on); of bf16 a number of 0 becomes 2^-126.
 template <typename E>
-__device__ __forceinline__ void rounded(float &a, float &b, uint32_t (&part)[kParts<E>]) {
+__device__ __forceinline__ void rounded(float &a, float &b, uint32_t (&part)[kParts]) {
   if constexpr (std::is_same_v<E, f16_t>) {
-    const f16x2_t h = __builtin_convertvector(f32x2_t{a, b}, f16x2_t);
-    part[0] = __builtin_bit_cast(uint32_t, h);
-    a = static_cast<float>(h[0]), b = static_cast<float>(h[1]);
+    constexpr float kBelow = 1.0f - 0x1p-10f;
+    const f16x2_t high = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_cvt_pkrtz(a * kBelow, b * kBelow));
+    const float high_a = static_cast<float>(high[0]), high_b = static_cast<float>(high[1]);
+    const f16x2_t low = __builtin_convertvector(f32x2_t{a - high_a, b - high_b}, f16x2_t);
+    part[0] = __builtin_bit_cast(uint32_t, high), part[1] = __builtin_bit_cast(uint32_t, low);
+    a = high_a + static_cast<float>(low[0]), b = high_b + static_cast<float>(low[1]);
   } else {
     // The first 8 bits cut off, the rest rounded to 8.
+    constexpr uint32_t kTiny = 0x00800080u;
+    const auto raised = [=](uint32_t pair) {
+      return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, pair), __builtin_bit_cast(u16x2_t, kTiny)));
+    };
     const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
-    part[0] = __builtin_amdgcn_perm(v, u, 0x07060302);
     const float high_a = __uint_as_float(u & 0xFFFF0000u), high_b = __uint_as_float(v & 0xFFFF0000u);
     const bf16x2_t low = __builtin_convertvector(f32x2_t{a - high_a, b - high_b}, bf16x2_t);
-    part[1] = __builtin_bit_cast(uint32_t, low);
+    part[0] = raised(__builtin_amdgcn_perm(v, u, 0x07060302)), part[1] = raised(__builtin_bit_cast(uint32_t, low));
     a = high_a + __uint_as_float(part[1] << 16), b = high_b + __uint_as_float(part[1] & 0xFFFF0000u);
   }
 }
@@ -123,7 +131,7 @@ __device__ __forceinline__ float sum_of_row(float v) {
 
 // The weights of 32 keys for 16 query rows, from their scores: key 16 t + 4 g + i of the step in s[t][i]. `live` keys count.
 template <typename E, int D>
-__device__ __forceinline__ void weigh(State<D> &state, f32x4_t (&s)[2], float scale, int live, int g, uint4 (&weights)[kParts<E>]) {
+__device__ __forceinline__ void weigh(State<D> &state, f32x4_t (&s)[2], float scale, int live, int g, uint4 (&weights)[kParts]) {
   float most = -INFINITY;
   float z[2][4];
 #pragma unroll
@@ -144,7 +152,7 @@ __device__ __forceinline__ void weigh(State<D> &state, f32x4_t (&s)[2], float sc
   }
   // A row all of whose scores are -inf so far has no peak; its weights are 0.
   const float base = state.peak == -INFINITY ? 0.0f : kRaise<E> - state.peak;
-  uint32_t words[4][kParts<E>];
+  uint32_t words[4][kParts];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -154,7 +162,7 @@ __device__ __forceinline__ void weigh(State<D> &state, f32x4_t (&s)[2], float sc
       state.total += a + b;
     }
 #pragma unroll
-  for (int n = 0; n < kParts<E>; ++n) weights[n] = make_uint4(words[0][n], words[1][n], words[2][n], words[3][n]);
+  for (int n = 0; n < kParts; ++n) weights[n] = make_uint4(words[0][n], words[1][n], words[2][n], words[3][n]);
 }
 
 // Column j of a lane's eight keys, from the D / 16 columns of each.
@@ -273,7 +281,7 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, uint4 *se
             for (int n = 0; n < NQ; ++n) s[n][t] = mfma<E>(key, q[n][c], s[n][t]);
           }
         }
-        uint4 weights[NQ][kParts<E>];
+        uint4 weights[NQ][kParts];
         const int live = last - first - (t0 + u) * kStep;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) weigh<E, D>(state[n], s[n], scale, live, g, weights[n]);
@@ -295,7 +303,7 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, uint4 *se
 #pragma unroll
           for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int k = 0; k < kParts<E>; ++k) state[n].sums[j] = mfma<E>(v, weights[n][k], state[n].sums[j]);
+            for (int k = 0; k < kParts; ++k) state[n].sums[j] = mfma<E>(v, weights[n][k], state[n].sums[j]);
         }
       }
     }
@@ -423,13 +431,13 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
     for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) s[half] = mfma<E>(now.keys[half][c], q[c], s[half]);
-    uint4 weights[kParts<E>];
+    uint4 weights[kParts];
     weigh<E, D>(state, s, scale, last - first - t * kStep, g, weights);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const uint4 v = column<C>(now.values, j);
 #pragma unroll
-      for (int k = 0; k < kParts<E>; ++k) state.sums[j] = mfma<E>(v, weights[k], state.sums[j]);
+      for (int k = 0; k < kParts; ++k) state.sums[j] = mfma<E>(v, weights[k], state.sums[j]);
     }
   }
   // The waves' states, through the LDS: peaks and sums of weights, then the weighted values at the common peak, half of each lane's
