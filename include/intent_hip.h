@@ -134,7 +134,8 @@ int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int64_t cols,
  *   PAGED_GQA_DECODE_MX    batch, kv_heads, head_group, d, ps, positions and, if not left out, the largest stride of a token
  *                          among the cache's four arrays (of the two kernels of a joined call the first)
  *   LINEAR_MXFP4, LINEAR_I8  m, n, k (of the kernels of a call the first, not the fold)
- *   PAGED_GQA_DECODE_PREFIX  batch, kv_heads, head_group, d, ps, prefix_positions, positions (the first, not the join)
+ *   PAGED_GQA_DECODE_PREFIX  batch, kv_heads, head_group, d, ps, prefix_positions, positions, the largest of the two caches' strides
+ *                          of a page, and of a token times ps (of the two kernels the first, not the join)
  *   RESIDUAL_NORM, RESIDUAL_NORM_I8, RESIDUAL_NORM_BACKWARD  d, post, every address and stride in bytes of the rows and weights,
  *                          or-ed, those of the 8-bit rows doubled (of the kernels of a call the first, not the fold)
  *   QUANTIZE_ROWS, SWIGLU_QUANTIZE_ROWS  d, the same

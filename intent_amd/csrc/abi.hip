@@ -167,7 +167,7 @@ extern "C" int intent_hip_kernel_resources(int op, int dtype, int64_t rows, int6
     case INTENT_HIP_OP_QUANTIZE_ROWS: return quantize_rows_resources(dtype, 0, cols, 0, out);
     case INTENT_HIP_OP_SWIGLU_QUANTIZE_ROWS: return quantize_rows_resources(dtype, 1, cols, 0, out);
     case INTENT_HIP_OP_LINEAR_I8: return linear_i8_resources(dtype, rows, cols, 4096, out);
-    case INTENT_HIP_OP_PAGED_GQA_DECODE_PREFIX: return prefix_decode_resources(dtype, 16, 1, rows, cols, 16, 1024, 1024, out);
+    case INTENT_HIP_OP_PAGED_GQA_DECODE_PREFIX: return prefix_decode_resources(dtype, 16, 1, rows, cols, 16, 1024, 1024, 0, out);
     case INTENT_HIP_OP_GEMM_I8: return gemm_i8_resources(rows, cols, out);
     case INTENT_HIP_OP_QUANTIZED_GEMM:
       return quantized_gemm_resources(nullptr, nullptr, nullptr, nullptr, rows, (cols + 7) / 8 * 8, 64, 64, 64, 64, 64, out);
@@ -222,8 +222,8 @@ extern "C" int intent_hip_call_resources(int op, int dtype, const int64_t *facts
       if (const int rc = takes(3)) return rc;
       return linear_i8_resources(dtype, f[0], f[1], f[2], out);
     case INTENT_HIP_OP_PAGED_GQA_DECODE_PREFIX:
-      if (const int rc = takes(7)) return rc;
-      return prefix_decode_resources(dtype, f[0], f[1], f[2], f[3], f[4], f[5], f[6], out);
+      if (const int rc = takes(8)) return rc;
+      return prefix_decode_resources(dtype, f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7], out);
     case INTENT_HIP_OP_RESIDUAL_NORM: case INTENT_HIP_OP_RESIDUAL_NORM_I8: case INTENT_HIP_OP_RESIDUAL_NORM_BACKWARD:
       if (const int rc = takes(3)) return rc;
       return residual_norm_resources(dtype, op - INTENT_HIP_OP_RESIDUAL_NORM, f[0], f[1], static_cast<uint64_t>(f[2]), out);

@@ -61,7 +61,7 @@ int residual_norm_resources(int dtype, int kind, int64_t d, int64_t post, uint64
 int quantize_rows_resources(int dtype, int gated, int64_t d, uint64_t mix, IntentHipKernelResources *out);
 int linear_i8_resources(int dtype, int64_t m, int64_t n, int64_t k, IntentHipKernelResources *out);
 int prefix_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t prefix_positions,
-                            int64_t positions, IntentHipKernelResources *out);
+                            int64_t positions, int64_t reach, IntentHipKernelResources *out);
 int mx_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t positions,
                         int64_t reach, IntentHipKernelResources *out);
 

@@ -13,8 +13,9 @@
 //     whose keys and values pass through the LDS 32 tokens at a time;
 //   * a sequence's own tokens: a job is a run of its pages for one key head; the 4 waves take 32 tokens in turn, straight to registers.
 // Scores are formed with 16 keys as rows and 16 query rows as columns (v_mfma_f32_16x16x32), which leaves the weights of keys 4 g .. 4 g
-// + 3 in lane (r, g), where the second product wants them: columns of the values as rows, 32 keys (4 of each 16 a lane) summed over. A
-// lane reads D / 16 columns of its eight keys and pairs them with v_perm. The peak is raised only when a score passes it by 2^4.
+// + 3 in lane (r, g), where the second product wants them: columns of the values as rows, 32 keys (4 of each 16 a lane) summed over. The
+// LDS gives those columns turned (ds_read_b64_tr_b16); from memory a lane reads D / 16 columns of its eight keys and pairs them with
+// v_perm. The peak is raised only when a score passes it by 2^4.
 #include <stdio.h>
 
 #include <algorithm>
@@ -30,12 +31,15 @@ constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kStep = 32;              // tokens of a step: two tiles of 16
 constexpr float kSlack = 4.0f;
 constexpr float kNoToken = -1.0f;      // the sum of a state without a token (weights are not negative)
-constexpr int kSets = 4;               // LDS stages of a prefix job
+constexpr int kSets = 3;               // LDS stages of a prefix job
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
@@ -47,7 +51,9 @@ struct Decode {
   const int32_t *prefix, *prefix_length, *offsets, *indices, *lengths;
   int64_t qs[2], ks[3], vs[3], outs[2];          // strides: sequence, head; page, token, head
   int64_t pages;
-  int prefix_positions, positions, ps, shift;    // shift: log2 of ps, -1 where it is no power of two
+  int prefix_positions, positions, ps;
+  uint32_t magic, shift;                         // a token's place over ps: (high half of magic times it, plus it) >> shift
+  uint32_t of_page[2], of_token[2];              // bytes, of keys and of values, where they and a page stay below 2^32 (kTile)
   int batch, kv_heads, group;
   int row_tiles, parts, prefix_blocks;           // of the prefix: tiles of query rows, parts of its tokens
   int head_tiles, job_pages, jobs;               // of the sequences
@@ -79,88 +85,87 @@ constexpr int kParts = 2;              // numbers of a weight
 template <typename E>
 constexpr float kRaise = std::is_same_v<E, f16_t> ? 11.0f : 0.0f;
 
-// Two weights as kParts numbers each, and what these add up to. No part of a weight that counts is 0, so that an infinite value gives an
-// infinity and not 0 times it: of f16 the first number is cut off below the weight, which leaves a second of 2^-10 of it at least (for
-// weights from 2^-25 of the largest on); of bf16 a number of 0 becomes 2^-126.
+// Two weights as kParts numbers each. No part of a weight that counts is 0, so that an infinite value gives an infinity and not 0 times
+// it: of f16 the first number is cut off below the weight, which leaves a second of 2^-10 of it at least (for weights from 2^-25 of the
+// largest on); of bf16 a second number of 0 becomes 2^-126.
 template <typename E>
-__device__ __forceinline__ void rounded(float &a, float &b, uint32_t (&part)[kParts]) {
+__device__ __forceinline__ void rounded(float a, float b, uint32_t (&part)[kParts]) {
   if constexpr (std::is_same_v<E, f16_t>) {
     constexpr float kBelow = 1.0f - 0x1p-10f;
     const f16x2_t high = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_cvt_pkrtz(a * kBelow, b * kBelow));
-    const float high_a = static_cast<float>(high[0]), high_b = static_cast<float>(high[1]);
-    const f16x2_t low = __builtin_convertvector(f32x2_t{a - high_a, b - high_b}, f16x2_t);
+    const f16x2_t low = __builtin_convertvector(f32x2_t{a - static_cast<float>(high[0]), b - static_cast<float>(high[1])}, f16x2_t);
     part[0] = __builtin_bit_cast(uint32_t, high), part[1] = __builtin_bit_cast(uint32_t, low);
-    a = high_a + static_cast<float>(low[0]), b = high_b + static_cast<float>(low[1]);
   } else {
     // The first 8 bits cut off, the rest rounded to 8.
-    constexpr uint32_t kTiny = 0x00800080u;
-    const auto raised = [=](uint32_t pair) {
-      return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, pair), __builtin_bit_cast(u16x2_t, kTiny)));
-    };
     const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
-    const float high_a = __uint_as_float(u & 0xFFFF0000u), high_b = __uint_as_float(v & 0xFFFF0000u);
-    const bf16x2_t low = __builtin_convertvector(f32x2_t{a - high_a, b - high_b}, bf16x2_t);
-    part[0] = raised(__builtin_amdgcn_perm(v, u, 0x07060302)), part[1] = raised(__builtin_bit_cast(uint32_t, low));
-    a = high_a + __uint_as_float(part[1] << 16), b = high_b + __uint_as_float(part[1] & 0xFFFF0000u);
+    const float rest_a = a - __uint_as_float(u & 0xFFFF0000u), rest_b = b - __uint_as_float(v & 0xFFFF0000u);
+    const bf16x2_t low = __builtin_convertvector(f32x2_t{rest_a, rest_b}, bf16x2_t);
+    part[0] = __builtin_amdgcn_perm(v, u, 0x07060302);
+    part[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, low), u16x2_t{0x0080, 0x0080}));
   }
 }
 
-// The state of 16 query rows: lane (r, g) has the peak of row r, its own share of the sum of weights, and columns 4 C g .. of the
-// weighted values, C = D / 16: product j gives column C (4 g + i) + j in sums[j][i].
+// The state of 16 query rows, weights being exp2(score + base): lane (r, g) has row r's base (+inf before any score has counted), the sum
+// of its weights (in each of the four), and in sums[j][i] the weighted values of row 4 g + i of product j, C = D / 16 products: column 16
+// j + 4 g + i of the prefix's, whose values come through the LDS, column C (4 g + i) + j of a sequence's own. The sum is a product with ones, so it is of the weights as the values met them.
 template <int D>
 struct State {
   static constexpr int C = D / 16;
-  float peak, total;
-  f32x4_t sums[C];
+  float base;
+  f32x4_t total, sums[C];
   __device__ __forceinline__ void clear() {
-    peak = -INFINITY, total = 0.0f;
+    base = INFINITY, total = f32x4_t{0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < C; ++j) sums[j] = f32x4_t{0, 0, 0, 0};
   }
 };
 
-// Largest and sum over the four lanes of a query row.
+// Eight ones.
+template <typename E>
+__device__ __forceinline__ uint4 ones() {
+  constexpr uint32_t two = std::is_same_v<E, f16_t> ? 0x3C003C00u : 0x3F803F80u;
+  return make_uint4(two, two, two, two);
+}
+
+// Largest over the four lanes of a query row.
 __device__ __forceinline__ float largest_of_row(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
   return fmaxf(v, __shfl_xor(v, 32));
 }
-__device__ __forceinline__ float sum_of_row(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float v;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(v) : "v"(a), "v"(b), "v"(c));       // (fmaxf first makes each of its operands quiet)
+  return v;
 }
 
 // The weights of 32 keys for 16 query rows, from their scores: key 16 t + 4 g + i of the step in s[t][i]. `live` keys count.
 template <typename E, int D>
-__device__ __forceinline__ void weigh(State<D> &state, f32x4_t (&s)[2], float scale, int live, int g, uint4 (&weights)[kParts]) {
-  float most = -INFINITY;
-  float z[2][4];
+__device__ __forceinline__ void weigh(State<D> &state, const f32x4_t (&s)[2], float scale, int live, int g, uint4 (&weights)[kParts]) {
+  float z[8];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int i = 0; i < 8; ++i) z[i] = fmaf(s[i / 4][i % 4], scale, state.base);
+  const float half = largest(z[0], z[1], z[2]), rest = largest(z[3], z[4], z[5]), most = largest(half, rest, largest(z[6], z[7], z[7]));
+  // Also where no score of a lane is a number (a row without a base whose scores are -inf), and where not all keys count.
+  if (live < kStep || __builtin_amdgcn_ballot_w64(!(most <= kRaise<E> + kSlack))) {
+    float largest = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      z[t][i] = s[t][i] * scale;
-      if (live < kStep && t * 16 + g * 4 + i >= live) z[t][i] = -INFINITY;
-      most = fmaxf(most, z[t][i]);
+    for (int i = 0; i < 8; ++i) {
+      z[i] = i / 4 * 16 + g * 4 + i % 4 >= live ? -INFINITY : s[i / 4][i % 4] * scale;
+      largest = fmaxf(largest, z[i]);
     }
-  if (__builtin_amdgcn_ballot_w64(most > state.peak + kSlack)) {
-    const float peak = fmaxf(state.peak, largest_of_row(most));
-    const float down = peak == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(state.peak - peak);
-    state.peak = peak;
+    const float base = fminf(state.base, kRaise<E> - largest_of_row(largest));      // +inf while every score is -inf
+    const float down = base == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - state.base);
+    state.base = base;
     state.total *= down;
 #pragma unroll
     for (int j = 0; j < State<D>::C; ++j) state.sums[j] *= down;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] += base == INFINITY ? 0.0f : base;
   }
-  // A row all of whose scores are -inf so far has no peak; its weights are 0.
-  const float base = state.peak == -INFINITY ? 0.0f : kRaise<E> - state.peak;
   uint32_t words[4][kParts];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      float a = __builtin_amdgcn_exp2f(z[t][i] + base), b = __builtin_amdgcn_exp2f(z[t][i + 1] + base);
-      rounded<E>(a, b, words[t * 2 + i / 2]);
-      state.total += a + b;
-    }
+  for (int i = 0; i < 8; i += 2) rounded<E>(__builtin_amdgcn_exp2f(z[i]), __builtin_amdgcn_exp2f(z[i + 1]), words[i / 2]);
 #pragma unroll
   for (int n = 0; n < kParts; ++n) weights[n] = make_uint4(words[0][n], words[1][n], words[2][n], words[3][n]);
 }
@@ -175,7 +180,10 @@ __device__ __forceinline__ uint4 column(const uint32_t (&rows)[8][C / 2], int j)
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ int page_of(const Decode &p, int token) { return p.shift >= 0 ? token >> p.shift : token / p.ps; }
+// token / ps of tokens below 2^31.
+__device__ __forceinline__ int page_of(const Decode &p, int token) {
+  return static_cast<int>((__umulhi(p.magic, static_cast<uint32_t>(token)) + static_cast<uint32_t>(token)) >> p.shift);
+}
 
 // The physical page of entry `at` of a table: entries outside the table and pages outside the cache read the nearest.
 __device__ __forceinline__ int physical(const Decode &p, const int32_t *table, int entries, int at) {
@@ -183,20 +191,31 @@ __device__ __forceinline__ int physical(const Decode &p, const int32_t *table, i
   return static_cast<int>(min<int64_t>(max(page, 0), p.pages - 1));
 }
 
-// Writes the state of a query row (its four lanes together) to row `at` of the states.
-template <int D>
-__device__ __forceinline__ void keep(const Decode &p, const State<D> &state, int64_t at, int g, bool any) {
-  constexpr int C = D / 16;
-  const float total = sum_of_row(state.total);
-  if (g == 0) p.peak[at] = state.peak, p.total[at] = any ? total : kNoToken;
-  if (!any) return;
-  float *to = p.sums + at * D + 4 * C * g;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < C; j += 4)
-      *reinterpret_cast<float4 *>(to + C * i + j) = make_float4(state.sums[j][i], state.sums[j + 1][i], state.sums[j + 2][i], state.sums[j + 3][i]);
+// The page of an entry that is the wave's (clamped to `entries`, if any), as the table has it, through the scalar cache: a vector load here would be waited for together
+// with every load of keys and values before it.
+typedef const __attribute__((address_space(4))) int32_t *table_t;
+__device__ __forceinline__ int page_of_wave(const int32_t *table, int entries, int at) {
+  return ((table_t)(table))[entries > 0 ? min(max(at, 0), entries - 1) : at];
 }
+
+// T tokens of one page, the wave's: the page as the table has it, the first one's place in it, and the last that counts.
+template <int T>
+struct WaveTile {
+  int page, in, most;
+  // `entries`: of the table; 0 where the entry is known to be one of its.
+  __device__ __forceinline__ void find(const Decode &p, const int32_t *table, int entries, int begin, int token, int last) {
+    const int base = min(token, last - 1) & ~(T - 1), entry = page_of(p, base);
+    page = page_of_wave(table, entries, begin + entry);
+    in = base - entry * p.ps, most = last - 1 - base;
+    if (token >= last) in += most, most = 0;           // a tile behind the last token reads that one alone
+  }
+  // Its first row, of keys (0) or of values (1).
+  __device__ __forceinline__ const uint16_t *rows(const Decode &p, const uint16_t *cache, int which) const {
+    const uint32_t at = static_cast<uint32_t>(min(max(page, 0), static_cast<int>(p.pages) - 1));
+    return reinterpret_cast<const uint16_t *>(reinterpret_cast<const char *>(cache) + static_cast<uint64_t>(at) * p.of_page[which] +
+                                              static_cast<uint32_t>(in) * p.of_token[which]);
+  }
+};
 
 // ---------------------------------------------------------------- the prefix
 // Unit (16 bytes) u of row `row` of a stage lies at u ^ place(row): the 16 rows of a read of keys are then in different banks.
@@ -205,9 +224,21 @@ __device__ __forceinline__ int place(int row) {
   return D == 128 ? row & 15 : (row >> 1) & 7;
 }
 
-// kTiles: pages hold whole tiles of 16 tokens, so a tile's page is the wave's to look up.
-template <typename E, int D, int NQ, bool kTiles>
-__device__ __forceinline__ void prefix_job(const Decode &p, int block, uint4 *set_0, uint4 *set_1, uint4 *set_2, uint4 *set_3) {
+// Writes the state of a query row of the prefix (its four lanes together) to row `at` of the states.
+template <int D>
+__device__ __forceinline__ void keep(const Decode &p, const State<D> &state, int64_t at, int g, bool any) {
+  constexpr int C = D / 16;
+  if (g == 0) p.peak[at] = -state.base, p.total[at] = any ? state.total[0] : kNoToken;
+  if (!any) return;
+  float *to = p.sums + at * D + 4 * g;
+#pragma unroll
+  for (int j = 0; j < C; ++j) *reinterpret_cast<f32x4_t *>(to + 16 * j) = state.sums[j];
+}
+
+// kTile: pages hold whole tiles of so many tokens (16 or 32), so a tile's page is the wave's to look up; 0: any pages.
+template <typename E, int D, int NQ, int kTile>
+__device__ __forceinline__ void prefix_job(const Decode &p, int block, const uint16_t *__restrict__ key_cache, const uint16_t *__restrict__ value_cache,
+                                           uint4 *lds) {
   constexpr int kRowUnits = D / 8, kUnits = kStep * kRowUnits, kLoads = kUnits / kThreads, kChunks = D / 32, C = D / 16;
   constexpr int kIssued = 2 * kLoads;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -234,78 +265,110 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, uint4 *se
       for (int c = 0; c < kChunks; ++c) q[n][c] = *reinterpret_cast<const uint4 *>(from + (c * 4 + g) * 8);
     }
     const float scale = p.scale * kLog2e;
-    const auto set_of = [&](int u) -> uint4 * { return u == 0 ? set_0 : u == 1 ? set_1 : u == 2 ? set_2 : set_3; };
-    const auto issue = [&](int t, int set) {           // step t (the last again behind it)
-      uint4 *stage = set_of(set);
+    const uint16_t *const keys_of = key_cache + kh * p.ks[2], *const values_of = value_cache + kh * p.vs[2];      // this head's
+    constexpr int T = kTile > 0 ? kTile : 16;
+    WaveTile<T> next[kLoads];                          // of the next step to be issued
+    const auto find = [&](int t) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int slot = (i * kWaves + wave) * kWave + lane, row = slot / kRowUnits;
-        const int at = first + min(t, count - 1) * kStep;
-        const int token = min(at + row, last - 1);
-        int page, in;
-        if constexpr (kTiles) {                        // rows of one tile of 16: this wave's
-          const int base = min(at + __builtin_amdgcn_readfirstlane(row) / 16 * 16, last - 1) & ~15, entry = page_of(p, base);
-          page = physical(p, p.prefix, p.prefix_positions, entry);
-          in = token - entry * p.ps;
-        } else {
-          const int entry = page_of(p, token);
-          page = physical(p, p.prefix, p.prefix_positions, entry);
-          in = token - entry * p.ps;
+        if (T == kStep && i > 0) {
+          next[i] = next[0];
+          continue;
         }
-        const int unit = slot % kRowUnits ^ place<D>(row);
-        const uint16_t *k = p.k + page * p.ks[0] + in * p.ks[1] + kh * p.ks[2] + unit * 8;
-        const uint16_t *v = p.v + page * p.vs[0] + in * p.vs[1] + kh * p.vs[2] + unit * 8;
+        const int row = __builtin_amdgcn_readfirstlane((i * kWaves + wave) * kWave / kRowUnits);
+        next[i].find(p, p.prefix, 0, 0, first + min(t, count - 1) * kStep + row / T * T, last);
+      }
+    };
+    // Where this lane's unit of each load lies from its tile's first row on.
+    int row_of[kLoads], unit_of[kLoads];
+    uint32_t near_key[kLoads], near_value[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int slot = (i * kWaves + wave) * kWave + lane, row = slot / kRowUnits;
+      row_of[i] = row, unit_of[i] = (slot % kRowUnits ^ place<D>(row)) * 8;
+      near_key[i] = (row % T) * p.of_token[0] + unit_of[i] * 2, near_value[i] = (row % T) * p.of_token[1] + unit_of[i] * 2;
+    }
+    const auto issue = [&](int t, int set) {           // step t (the last again behind it)
+      uint4 *stage = lds + set * 2 * kUnits;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint16_t *k, *v;
+        if constexpr (kTile > 0) {
+          uint32_t to_key = near_key[i], to_value = near_value[i];
+          if (next[i].most < T - 1) {
+            const uint32_t row = min(row_of[i] % T, next[i].most);
+            to_key = row * p.of_token[0] + unit_of[i] * 2, to_value = row * p.of_token[1] + unit_of[i] * 2;
+          }
+          k = next[i].rows(p, keys_of, 0) + to_key / 2, v = next[i].rows(p, values_of, 1) + to_value / 2;
+        } else {
+          const int token = min(first + min(t, count - 1) * kStep + row_of[i], last - 1), entry = page_of(p, token);
+          const int page = physical(p, p.prefix, p.prefix_positions, entry), in = token - entry * p.ps;
+          k = keys_of + page * p.ks[0] + in * p.ks[1] + unit_of[i], v = values_of + page * p.vs[0] + in * p.vs[1] + unit_of[i];
+        }
         __builtin_amdgcn_global_load_lds(k, (lds_void_t *)(stage + (i * kWaves + wave) * kWave), 16, 0, 0);
         __builtin_amdgcn_global_load_lds(v, (lds_void_t *)(stage + kUnits + (i * kWaves + wave) * kWave), 16, 0, 0);
       }
+      if constexpr (kTile > 0) find(t + 1);
     };
+    if constexpr (kTile > 0) find(0);
 #pragma unroll
-    for (int u = 0; u < kSets - 1; ++u) issue(u, u);
-    for (int t0 = 0; t0 < count; t0 += kSets) {
+    for (int t = 0; t < kSets - 1; ++t) issue(t, t);
+    for (int step = 0, set = 0; step < count; ++step, set = set == kSets - 1 ? 0 : set + 1) {
+      INTENT_WAIT_VMCNT((kSets - 2) * kIssued);        // this wave's loads of the step have come
+      stage_barrier();                                 // everybody's have, and nobody reads the set that is filled next
+      issue(step + kSets - 1, set == 0 ? kSets - 1 : set - 1);
+      const uint4 *keys = lds + set * 2 * kUnits, *values = keys + kUnits;
+      uint4 key[2][kChunks];
 #pragma unroll
-      for (int u = 0; u < kSets; ++u) {
-        if (t0 + u >= count) break;
-        INTENT_WAIT_VMCNT((kSets - 2) * kIssued);      // this wave's loads of the step have come
-        stage_barrier();                               // everybody's have, and nobody reads the set that is filled next
-        issue(t0 + u + kSets - 1, (u + kSets - 1) % kSets);
-        const uint4 *keys = set_of(u), *values = keys + kUnits;
-        f32x4_t s[NQ][2];
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) key[t][c] = keys[(t * 16 + r) * kRowUnits + ((c * 4 + g) ^ place<D>(t * 16 + r))];
+      __builtin_amdgcn_sched_barrier(0);               // all of them asked for before the first product
+      f32x4_t s[NQ][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n][t] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[n][t] = mfma<E>(key[t][c], q[n][c], s[n][t]);
+      }
+      // Columns 16 j + r of keys 4 g .. 4 g + 3 of each tile: lane m of a group of 16 points at four columns of key m / 4, and lane i
+      // gets column i of all four. They are asked for two products ahead.
+      uint4 column[3];
+      const auto ask = [&](int j) {
+        u32x2_t half[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) s[n][t] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            const uint4 key = keys[(t * 16 + r) * kRowUnits + ((c * 4 + g) ^ place<D>(t * 16 + r))];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) s[n][t] = mfma<E>(key, q[n][c], s[n][t]);
-          }
+          const int row = t * 16 + g * 4 + (r >> 2), unit = (j * 2 + ((r >> 1) & 1)) ^ place<D>(row);
+          const uint16_t *at = reinterpret_cast<const uint16_t *>(values + row * kRowUnits + unit) + (r & 1) * 4;
+          half[t] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t *)(at)));
         }
-        uint4 weights[NQ][kParts];
-        const int live = last - first - (t0 + u) * kStep;
+        column[j % 3] = make_uint4(half[0][0], half[0][1], half[1][0], half[1][1]);
+      };
+      ask(0), ask(1);
+      uint4 weights[NQ][kParts];
+      const int live = last - first - step * kStep;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) weigh<E, D>(state[n], s[n], scale, live, g, weights[n]);
-        uint32_t own[8][C / 2];
+      for (int n = 0; n < NQ; ++n) weigh<E, D>(state[n], s[n], scale, live, g, weights[n]);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = i / 4 * 16 + g * 4 + i % 4;
-          if constexpr (D == 128) {
-            const uint4 v = values[row * kRowUnits + (r ^ place<D>(row))];
-            own[i][0] = v.x, own[i][1] = v.y, own[i][2] = v.z, own[i][3] = v.w;
-          } else {
-            const uint2 v = reinterpret_cast<const uint2 *>(values + row * kRowUnits + ((r >> 1) ^ place<D>(row)))[r & 1];
-            own[i][0] = v.x, own[i][1] = v.y;
-          }
-        }
+      for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-          const uint4 v = column<C>(own, j);
+        for (int k = 0; k < kParts; ++k) state[n].total = mfma<E>(ones<E>(), weights[n][k], state[n].total);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n)
+      for (int j = 0; j < C; ++j) {
+        if (j + 2 < C) ask(j + 2);
 #pragma unroll
-            for (int k = 0; k < kParts; ++k) state[n].sums[j] = mfma<E>(v, weights[n][k], state[n].sums[j]);
-        }
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) state[n].sums[j] = mfma<E>(column[j % 3], weights[n][k], state[n].sums[j]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);           // reads of the LDS, then products
+        __builtin_amdgcn_sched_group_barrier(0x008, NQ * kParts, 0);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
     INTENT_WAIT_VMCNT(0);                              // nothing is on its way into the LDS of an ended workgroup
   }
@@ -350,7 +413,7 @@ __device__ __forceinline__ Sequence job_sequence(const Decode &p, int job) {
   return Sequence{first + at, from, held_tokens(p, from, __builtin_amdgcn_readlane(next, at), __builtin_amdgcn_readlane(length, at))};
 }
 
-template <typename E, int D, bool kTiles>
+template <typename E, int D, int kTile>
 __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums, float *peaks) {
   constexpr int kChunks = D / 32, C = D / 16;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -377,78 +440,92 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
     for (int c = 0; c < kChunks; ++c) q[c] = *reinterpret_cast<const uint4 *>(row + (c * 4 + g) * 8);
   }
   const float scale = p.scale * kLog2e;
-  struct Tokens {
-    uint4 keys[2][kChunks];
-    uint32_t values[8][C / 2];
+  // The tiles of a step, where a tile's page is the wave's: of the step at hand, of the next, whose keys are on their way, and of the one
+  // after it, whose page is.
+  constexpr int T = kTile > 0 ? kTile : 16, kHalves = kStep / T;
+  struct Step {
+    WaveTile<T> tile[kHalves];
   };
-  // Offsets of a token's row in the caches.
-  const auto load = [&](int t, Tokens &to) {           // step t of the wave
-    const int base = first + t * kStep;
+  const auto find = [&](int t) {
+    Step found{};
+    if constexpr (kTile > 0) {
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i)
+        found.tile[i].find(p, p.indices, p.positions, sequence.first, first + t * kStep + i * T, last);
+    }
+    return found;
+  };
+  const uint16_t *const keys_of = p.k + kh * p.ks[2], *const values_of = p.v + kh * p.vs[2];
+  // Row `row` of 32 of step t, its element `at`, of keys (0) or of values (1).
+  const auto row_of = [&](const Step &step, int t, int row, int at, int which) {
+    const uint16_t *const cache = which ? values_of : keys_of;
+    if constexpr (kTile > 0) {
+      const WaveTile<T> &tile = step.tile[row / 16 * 16 / T];
+      return tile.rows(p, cache, which) + (static_cast<uint32_t>(min(row % T, tile.most)) * p.of_token[which] + at * 2) / 2;
+    } else {
+      const int64_t(&strides)[3] = which ? p.vs : p.ks;
+      const int token = min(first + t * kStep + row, last - 1), entry = page_of(p, token);
+      return cache + physical(p, p.indices, p.positions, sequence.first + entry) * strides[0] + (token - entry * p.ps) * strides[1] + at;
+    }
+  };
+  const auto load_keys = [&](const Step &step, int t, uint4 (&to)[2][kChunks]) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      int whole_page = 0, whole_entry = 0;
-      if constexpr (kTiles) {
-        whole_entry = page_of(p, min(base + half * 16, last - 1) & ~15);
-        whole_page = physical(p, p.indices, p.positions, sequence.first + whole_entry);
-      }
-      const auto find = [&](int token, int &page, int &in) {
-        token = min(token, last - 1);
-        if constexpr (kTiles) {
-          page = whole_page, in = token - whole_entry * p.ps;
-        } else {
-          const int entry = page_of(p, token);
-          page = physical(p, p.indices, p.positions, sequence.first + entry), in = token - entry * p.ps;
-        }
-      };
-      int page, in;
-      find(base + half * 16 + r, page, in);
-      const uint16_t *key = p.k + page * p.ks[0] + in * p.ks[1] + kh * p.ks[2];
+      const uint16_t *const key = row_of(step, t, half * 16 + r, g * 8, 0);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) to.keys[half][c] = *reinterpret_cast<const uint4 *>(key + (c * 4 + g) * 8);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        find(base + half * 16 + g * 4 + i, page, in);
-        const uint16_t *value = p.v + page * p.vs[0] + in * p.vs[1] + kh * p.vs[2] + r * C;
-        uint32_t(&row)[C / 2] = to.values[half * 4 + i];
-        if constexpr (D == 128) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(value);
-          row[0] = v.x, row[1] = v.y, row[2] = v.z, row[3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2 *>(value);
-          row[0] = v.x, row[1] = v.y;
-        }
-      }
+      for (int c = 0; c < kChunks; ++c) to[half][c] = *reinterpret_cast<const uint4 *>(key + c * 32);
     }
   };
   const int count = (last - first + kStep - 1) / kStep;
-  Tokens next;
-  if (wave < count) load(wave, next);
+  uint4 next_keys[2][kChunks];
+  Step next = find(wave), after = find(wave + kWaves);
+  if (wave < count) load_keys(next, wave, next_keys);
   for (int t = wave; t < count; t += kWaves) {
-    const Tokens now = next;
-    if (t + kWaves < count) load(t + kWaves, next);
+    const Step now = next;
+    uint4 keys[2][kChunks];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) keys[half][c] = next_keys[half][c];
+    uint32_t values[8][C / 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t *const value = row_of(now, t, i / 4 * 16 + g * 4 + i % 4, r * C, 1);
+      if constexpr (D == 128) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(value);
+        values[i][0] = v.x, values[i][1] = v.y, values[i][2] = v.z, values[i][3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(value);
+        values[i][0] = v.x, values[i][1] = v.y;
+      }
+    }
+    next = after;
+    if (t + kWaves < count) load_keys(next, t + kWaves, next_keys);
+    after = find(t + 2 * kWaves);
     f32x4_t s[2] = {f32x4_t{0, 0, 0, 0}, f32x4_t{0, 0, 0, 0}};
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) s[half] = mfma<E>(now.keys[half][c], q[c], s[half]);
+      for (int c = 0; c < kChunks; ++c) s[half] = mfma<E>(keys[half][c], q[c], s[half]);
     uint4 weights[kParts];
     weigh<E, D>(state, s, scale, last - first - t * kStep, g, weights);
 #pragma unroll
+    for (int k = 0; k < kParts; ++k) state.total = mfma<E>(ones<E>(), weights[k], state.total);
+#pragma unroll
     for (int j = 0; j < C; ++j) {
-      const uint4 v = column<C>(now.values, j);
+      const uint4 v = column<C>(values, j);
 #pragma unroll
       for (int k = 0; k < kParts; ++k) state.sums[j] = mfma<E>(v, weights[k], state.sums[j]);
     }
   }
   // The waves' states, through the LDS: peaks and sums of weights, then the weighted values at the common peak, half of each lane's
   // columns at a time.
-  const float total = sum_of_row(state.total);
-  if (g == 0) peaks[wave * 16 + r] = state.peak;
+  if (g == 0) peaks[wave * 16 + r] = -state.base;
   __syncthreads();
   float peak = -INFINITY;
   for (int i = 0; i < min(kWaves, count); ++i) peak = fmaxf(peak, peaks[i * 16 + r]);
-  const float share = wave >= count ? 0.0f : peak == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(state.peak - peak);
-  if (g == 0) peaks[(kWaves + wave) * 16 + r] = wave < count ? total * share : 0.0f;
+  const float share = wave >= count ? 0.0f : peak == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-state.base - peak);
+  if (g == 0) peaks[(kWaves + wave) * 16 + r] = wave < count ? state.total[0] * share : 0.0f;
   // Wave w joins rows 4 w .. 4 w + 3, a lane the D / 16 columns of one from r D / 16 on.
   const int row = wave * 4 + g, of_group = tile * 16 + row;
   float joined[C];
@@ -483,24 +560,29 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
     *reinterpret_cast<float4 *>(p.sums + to * D + r * C + j) = make_float4(joined[j], joined[j + 1], joined[j + 2], joined[j + 3]);
 }
 
-template <typename E, int D, int NQ, bool kTiles>
+template <typename E, int D, int NQ, int kTile>
 __global__ __launch_bounds__(kThreads, 2) void prefix_decode_jobs(Decode p) {
-  constexpr int kStage = 2 * kStep * D / 8;           // keys and values of a step; each has an array of its own, so that the compiler
-  __shared__ uint4 set_0[kStage], set_1[kStage], set_2[kStage], set_3[kStage];      // knows which loads a read has to wait for
-  static_assert(kSets == 4 && kStage * sizeof(uint4) >= kWaves * 16 * (D / 2) * sizeof(float), "the waves' states fit a set");
-  const int block = grid_block();
-  if (block < p.prefix_blocks)
-    prefix_job<E, D, NQ, kTiles>(p, block, set_0, set_1, set_2, set_3);
-  else if (block - p.prefix_blocks < p.jobs * p.kv_heads * p.head_tiles)
-    own_job<E, D, kTiles>(p, block - p.prefix_blocks, reinterpret_cast<float *>(set_0), reinterpret_cast<float *>(set_1));
+  constexpr int kStage = 2 * kStep * D / 8;            // keys and values of a step
+  static_assert(kSets * kStage * sizeof(uint4) >= kWaves * 16 * (D / 2) * sizeof(float) + kStage * sizeof(uint4), "the waves' states fit behind the first set");
+  __shared__ uint4 lds[kSets * kStage];
+  const int block = grid_block(), own_blocks = p.jobs * p.kv_heads * p.head_tiles;
+  const bool own = block >= p.prefix_blocks;
+  const int at = own ? block - p.prefix_blocks : block;
+  if (!own)
+    prefix_job<E, D, NQ, kTile>(p, at, p.k, p.v, lds);
+  else if (at < own_blocks)
+    own_job<E, D, kTile>(p, at, reinterpret_cast<float *>(lds + kStage), reinterpret_cast<float *>(lds));
 }
 
-// The states of a query head's parts of the prefix and of its sequence's jobs, joined: a wave per head.
+// The states of a query head's parts of the prefix and of its sequence's jobs, joined: a workgroup per head, whose waves take a quarter
+// of the states each, 64 peaks and sums at a time, a lane each.
 template <typename E, int D>
 __global__ __launch_bounds__(kThreads) void prefix_decode_join(Decode p) {
   constexpr int kOwn = D / kWave;
-  const int lane = threadIdx.x & 63, q_heads = p.kv_heads * p.group;
-  const int64_t row = static_cast<int64_t>(grid_block()) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float joined[kWaves][D + 2];
+  __shared__ bool live_of[kWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q_heads = p.kv_heads * p.group;
+  const int64_t row = grid_block();
   if (row >= static_cast<int64_t>(p.batch) * q_heads) return;
   const int b = static_cast<int>(row / q_heads), h = static_cast<int>(row % q_heads);
   const int begin = p.offsets[b], next = p.offsets[b + 1];
@@ -513,26 +595,67 @@ __global__ __launch_bounds__(kThreads) void prefix_decode_join(Decode p) {
     return i < p.parts ? i * of_prefix + row : p.parts * of_prefix + (own + i - p.parts) * q_heads + h;
   };
   const int count = p.parts + jobs;
-  float peak = -INFINITY;
-  for (int i = lane; i < count; i += kWave)
-    if (p.total[state(i)] >= 0.0f || p.total[state(i)] != p.total[state(i)]) peak = fmaxf(peak, p.peak[state(i)]);
-  peak = wave_max(peak);
-  float total = 0.0f, sums[kOwn] = {};
+  float peak = -INFINITY, total = 0.0f, sums[kOwn] = {};
   bool any = false;
-#pragma unroll 4
-  for (int i = 0; i < count; ++i) {
-    const int64_t at = state(i);
-    const float held = p.total[at];
-    if (held == kNoToken) continue;
-    any = true;
-    const float share = peak == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(p.peak[at] - peak);
-    total += held * share;
+  constexpr int kAhead = 8;                            // states on their way
+  float held[kAhead][kOwn];
+  const int of_wave = (count + kWaves - 1) / kWaves, last = min(count, (wave + 1) * of_wave);
+  // The values of states first .. of this wave (of the last again behind it); not all of them were written.
+  const auto ask = [&](int first) {
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) sums[j] += p.sums[at * D + lane * kOwn + j] * share;
+    for (int i = 0; i < kAhead; ++i) {
+      const float *from = p.sums + state(min(first + i, last - 1)) * D + lane * kOwn;
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) held[i][j] = from[j];
+    }
+  };
+  for (int first = wave * of_wave; first < last; first += kWave) {
+    const int at = min(first + lane, last - 1);
+    const float of_state = p.total[state(at)], peak_of = p.peak[state(at)];
+    ask(first);
+    const bool live = first + lane < last && of_state != kNoToken;
+    const float most = fmaxf(peak, wave_max(live ? peak_of : -INFINITY));
+    const float down = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(peak - most);
+    const float share = !live ? 0.0f : most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(peak_of - most);
+    any = any || __builtin_amdgcn_ballot_w64(live);
+    total = total * down + wave_sum(live ? of_state * share : 0.0f);
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) sums[j] *= down;
+    peak = most;
+    const int here = min(last - first, kWave);
+    for (int i0 = 0; i0 < here; i0 += kAhead) {
+      if (i0 > 0) ask(first + i0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const bool counts = i0 + i < here && __builtin_amdgcn_readlane(live, (i0 + i) & 63);
+        const float weight = lane_value(share, (i0 + i) & 63);
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) sums[j] += counts ? held[i][j] * weight : 0.0f;
+      }
+    }
   }
-  uint16_t *out = p.out + b * p.outs[0] + h * p.outs[1] + lane * kOwn;
+  // The waves' own, at the common peak.
 #pragma unroll
-  for (int j = 0; j < kOwn; ++j) out[j] = from_f32<E>(any ? sums[j] / total : 0.0f).bits;
+  for (int j = 0; j < kOwn; ++j) joined[wave][lane * kOwn + j] = sums[j];
+  if (lane == 0) joined[wave][D] = peak, joined[wave][D + 1] = total, live_of[wave] = any;
+  __syncthreads();
+  if (wave > 0) return;
+  float of_all = -INFINITY, weight = 0.0f, out[kOwn] = {};
+  any = false;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    if (live_of[w]) any = true, of_all = fmaxf(of_all, joined[w][D]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (!live_of[w]) continue;
+    const float share = of_all == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(joined[w][D] - of_all);
+    weight += joined[w][D + 1] * share;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) out[j] += joined[w][lane * kOwn + j] * share;
+  }
+  uint16_t *to = p.out + b * p.outs[0] + h * p.outs[1] + lane * kOwn;
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) to[j] = from_f32<E>(any ? out[j] / weight : 0.0f).bits;
 }
 
 // How a call is cut.
@@ -557,13 +680,18 @@ Cut cut(int64_t batch, int64_t kv_heads, int64_t group, int64_t ps, int64_t pref
   return c;
 }
 
+// The tiles of tokens that pages come in; `reach`: the largest stride of a page, or elements from a page's first token to behind its last,
+// which are counted in 32 bits of bytes then.
+int tile_of(int64_t ps, int64_t reach) { return reach >= int64_t{1} << 31 || ps == 0 || ps % 16 ? 0 : ps % 32 ? 16 : 32; }
+
 size_t states_of(const Cut &c, int64_t batch, int64_t q_heads) { return (static_cast<size_t>(c.parts) * batch + c.jobs) * q_heads; }
 
 template <typename E, typename F>
-int with_kernel(int64_t d, int nq, bool tiles, F f) {
+int with_kernel(int64_t d, int nq, int tile, F f) {
   const auto of = [&](auto width, auto rows) {
-    return tiles ? f(prefix_decode_jobs<E, width.value, rows.value, true>, prefix_decode_join<E, width.value>)
-                 : f(prefix_decode_jobs<E, width.value, rows.value, false>, prefix_decode_join<E, width.value>);
+    return tile == 32   ? f(prefix_decode_jobs<E, width.value, rows.value, 32>, prefix_decode_join<E, width.value>)
+           : tile == 16 ? f(prefix_decode_jobs<E, width.value, rows.value, 16>, prefix_decode_join<E, width.value>)
+                        : f(prefix_decode_jobs<E, width.value, rows.value, 0>, prefix_decode_join<E, width.value>);
   };
   const std::integral_constant<int, 64> narrow;
   const std::integral_constant<int, 128> wide;
@@ -592,17 +720,16 @@ int check(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t group, int64
 }  // namespace
 
 int prefix_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t prefix_positions,
-                            int64_t positions, IntentHipKernelResources *out) {
+                            int64_t positions, int64_t reach, IntentHipKernelResources *out) {
   if (int rc = check(batch, kv_heads * group, kv_heads, group, d, 1, ps, prefix_positions, positions)) return rc;
   const Cut c = cut(batch, kv_heads, group, ps, prefix_positions, positions);
-  const bool tiles = ps % 16 == 0;
+  const int tile = tile_of(ps, reach);
   char name[64];
-  snprintf(name, sizeof(name), "prefix_decode_jobs<%s,%lld,%d,%s>", dtype == INTENT_HIP_F16 ? "f16" : "bf16", static_cast<long long>(d), c.nq,
-           tiles ? "true" : "false");
+  snprintf(name, sizeof(name), "prefix_decode_jobs<%s,%lld,%d,%d>", dtype == INTENT_HIP_F16 ? "f16" : "bf16", static_cast<long long>(d), c.nq, tile);
   const auto describe = [&](void (*kernel)(Decode), void (*)(Decode)) {
     return describe_kernel(reinterpret_cast<const void *>(kernel), name, kThreads, out);
   };
-  return dtype == INTENT_HIP_F16 ? with_kernel<f16_t>(d, c.nq, tiles, describe) : with_kernel<bf16_t>(d, c.nq, tiles, describe);
+  return dtype == INTENT_HIP_F16 ? with_kernel<f16_t>(d, c.nq, tile, describe) : with_kernel<bf16_t>(d, c.nq, tile, describe);
 }
 
 }  // namespace intent_hip
@@ -661,9 +788,11 @@ extern "C" int intent_hip_paged_gqa_decode_prefix(int dtype, const void *q, cons
   p.prefix = prefix_indices, p.prefix_length = prefix_length, p.offsets = page_offsets, p.indices = page_indices, p.lengths = lengths;
   p.qs[0] = strides[0], p.qs[1] = strides[1], p.outs[0] = strides[11], p.outs[1] = strides[12];
   for (int i = 0; i < 3; ++i) p.ks[i] = strides[3 + i], p.vs[i] = strides[7 + i];
-  p.pages = ps > 0 ? pages : 0, p.ps = static_cast<int>(ps), p.shift = -1;
-  for (int i = 0; i < 21; ++i)
-    if (ps == int64_t{1} << i) p.shift = i;
+  p.pages = ps > 0 ? pages : 0, p.ps = static_cast<int>(ps);
+  if (ps > 0) {
+    while (int64_t{1} << p.shift < ps) ++p.shift;
+    p.magic = static_cast<uint32_t>(((((uint64_t{1} << p.shift) - ps) << 32) / ps) + 1);
+  }
   p.prefix_positions = static_cast<int>(prefix_positions), p.positions = static_cast<int>(positions);
   p.batch = static_cast<int>(batch), p.kv_heads = static_cast<int>(kv_heads), p.group = static_cast<int>(head_group);
   p.row_tiles = c.row_tiles, p.parts = c.parts, p.prefix_blocks = static_cast<int>(c.row_tiles * kv_heads * c.parts);
@@ -672,12 +801,19 @@ extern "C" int intent_hip_paged_gqa_decode_prefix(int dtype, const void *q, cons
   const int64_t blocks = p.prefix_blocks + static_cast<int64_t>(c.jobs) * kv_heads * c.head_tiles;
   const auto run = [&](void (*jobs)(Decode), void (*join)(Decode)) {
     jobs<<<tile_grid(blocks, 1), kThreads, 0, as_stream(stream)>>>(p);
-    join<<<tile_grid((batch * q_heads + kWaves - 1) / kWaves, 1), kThreads, 0, as_stream(stream)>>>(p);
+    join<<<tile_grid(batch * q_heads, 1), kThreads, 0, as_stream(stream)>>>(p);
     return 0;
   };
+  int64_t reach = 0;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t *const of = i == 0 ? p.ks : p.vs;
+    reach = std::max({reach, of[0], of[1] >= int64_t{1} << 31 ? of[1] : of[1] * ps});
+    p.of_page[i] = static_cast<uint32_t>(of[0] * 2), p.of_token[i] = static_cast<uint32_t>(of[1] * 2);
+  }
+  const int tile = tile_of(ps, reach);
   if (dtype == INTENT_HIP_F16)
-    with_kernel<f16_t>(d, c.nq, ps % 16 == 0, run);
+    with_kernel<f16_t>(d, c.nq, tile, run);
   else
-    with_kernel<bf16_t>(d, c.nq, ps % 16 == 0, run);
+    with_kernel<bf16_t>(d, c.nq, tile, run);
   return hipPeekAtLastError() != hipSuccess ? launch_status("paged_gqa_decode_prefix") : INTENT_HIP_OK;
 }

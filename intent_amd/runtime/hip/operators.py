@@ -1425,7 +1425,7 @@ def _paged_decode_prefix(dtype_code):
         q, output = _readable(q, keep, before, 8), _writable(output, keep, after)
         tables = [_readable(t, keep, before) for t in (prefix_indices, prefix_length, page_offsets, page_indices, lengths)]
         strides = (ctypes.c_int64 * 14)(*(st for t in (q, *caches, output) for st in (*_outer_strides(t), 1)))
-        extents = (batch, q_heads, kv_heads, group, d)
+        extents, reach = (batch, q_heads, kv_heads, group, d), max(strides[3], strides[7], strides[4] * ps, strides[8] * ps)
         positions, size = (prefix_indices.shape[0], page_indices.shape[0]), ctypes.c_size_t(0)
         lib.check(lib.fn["paged_gqa_decode_prefix_workspace_bytes"](*extents, ps, *positions, ctypes.byref(size)),
                   "provider_preparation")
@@ -1439,7 +1439,7 @@ def _paged_decode_prefix(dtype_code):
             return Launch("intent_hip_paged_gqa_decode_prefix", _optional_workspace_run(fn, args, size, device, keep), tuple(keep),
                           configuration=configuration,
                           resources=lambda: lib.call_resources(OP_PAGED_GQA_DECODE_PREFIX, dtype_code, batch, kv_heads, group, d, ps,
-                                                               *positions))
+                                                               *positions, reach))
         return _staged(again, (q, *caches, *tables, output, scale), bound, before, after)
     return plan
 
