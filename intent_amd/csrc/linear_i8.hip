@@ -281,100 +281,164 @@ __global__ __launch_bounds__(256) void linear_fold(Linear p) {
 }
 
 // ---------------------------------------------------------------- large tiles, both operands through the LDS
-// 256 rows of x by 256 weight rows, 8 waves in 2 x 4 of 128 x 64 = 4 x 2 products of 32 x 32 x 32. A stage is 64 bytes of K of both, 32
-// KB; five of them arrive by loads into the LDS, and the two waves of a SIMD alternate, one barrier apart, between their matrix
-// products and their reads and loads.
-constexpr int kBM = 256, kBN = 256, kBK = 64, kBigThreads = 512, kBigStages = 5;
+// 256 rows of x by 256 weight rows, 4 waves of 128 x 128 = 4 x 4 products of 32 x 32 x 32, so that a byte read from the LDS meets 128
+// others. A stage is 64 bytes of K of both, 32 KB; five of them arrive by loads into the LDS. A wave has its SIMD to itself and hides its
+// reads behind its own products: while 16 products of half a stage run, the operands of the next half are read.
+constexpr int kBM = 256, kBN = 256, kBK = 64, kBigWaves = 4, kBigThreads = kBigWaves * kWave, kBigStages = 5;
 constexpr int kHalf = kBM * kBK / kUnit, kStageUnits = 2 * kHalf;
+constexpr int kGroupM = 8;             // tiles of x that share a walk along the weight rows
+
+// Tiles in groups of kGroupM rows of tiles, walked column by column: those that run at one time share rows and columns.
+__device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int &tm, int &tn) {
+  const int per_group = kGroupM * n_tiles, group = t / per_group, first = group * kGroupM;
+  const int rows = min(m_tiles - first, kGroupM), in = t - group * per_group;
+  tm = first + in % rows, tn = in / rows;
+}
 
 template <typename E>
 __global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
   __shared__ uint4 lds[kBigStages * kStageUnits];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 2, wn = wave & 3;
+  const int wm = wave >> 1, wn = wave & 1;
   const int tile = xcd_tile(grid_block(), p.m_tiles * p.n_tiles);
   if (tile < 0) return;
-  const int m0 = tile % p.m_tiles * kBM, n0 = tile / p.m_tiles * kBN;
-  // Each wave moves 2 KB of x and 2 KB of the weight a stage. Unit c of row r lies at place c ^ (r / 4) % 4 of its four.
-  const int8_t *x_src[2], *w_src[2];
-  int unit[2];
+  int tm, tn;
+  tile_at(tile, p.m_tiles, p.n_tiles, tm, tn);
+  const int m0 = tm * kBM, n0 = tn * kBN;
+  // Each wave moves 4 KB of x and 4 KB of the weight a stage. Unit c of row r lies at place c ^ (r / 4) % 4 of its four.
+  constexpr int kLoads = kHalf / kBigThreads;
+  const int8_t *x_src[kLoads], *w_src[kLoads];
+  int unit[kLoads];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int slot = (wave * 2 + i) * kWave + lane, row = slot >> 2;
+  for (int i = 0; i < kLoads; ++i) {
+    const int slot = (wave * kLoads + i) * kWave + lane, row = slot >> 2;
     unit[i] = (slot & 3) ^ ((row >> 2) & 3);
     x_src[i] = p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx + unit[i] * kUnit;
     w_src[i] = p.w + static_cast<int64_t>(min(n0 + row, p.n - 1)) * p.ldw + unit[i] * kUnit;
   }
-  const int stages = (p.units + 3) / 4;
-  const auto issue = [&](int t) {
+  const int stages = p.units / 4, rest = p.units % 4;  // whole ones; units behind them
+  const auto issue = [&](int t, int i) {               // load i of stage t (the last again behind it, so that as many are always on their way)
     uint4 *stage = lds + (t % kBigStages) * kStageUnits;
-    const int64_t k0 = static_cast<int64_t>(t) * kBK;
-    const bool whole = t * 4 + 4 <= p.units;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool held = whole || t * 4 + unit[i] < p.units;
-      const int8_t *zero = reinterpret_cast<const int8_t *>(&kZeroUnit);
-      __builtin_amdgcn_global_load_lds(held ? x_src[i] + k0 : zero, (lds_void_t *)(stage + (wave * 2 + i) * kWave), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(held ? w_src[i] + k0 : zero, (lds_void_t *)(stage + kHalf + (wave * 2 + i) * kWave), 16, 0, 0);
-    }
+    const int64_t k0 = static_cast<int64_t>(min(t, stages - 1)) * kBK;
+    const int j = i / 2;
+    __builtin_amdgcn_global_load_lds(i % 2 ? w_src[j] + k0 : x_src[j] + k0, (lds_void_t *)(stage + i % 2 * kHalf + (wave * kLoads + j) * kWave), 16, 0, 0);
   };
-  i32x16_t acc[4][2];
+  i32x16_t acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
   const int row = lane & 31, half = lane >> 5, turn = (row >> 2) & 3;
-  const bool lag = wave >= 4;
-#pragma unroll
-  for (int t = 0; t < kBigStages - 1; ++t)
-    if (t < stages) issue(t);
-  const auto wait_stage = [&](int t) {                 // this wave's loads of stage t have come; later ones may be on their way
-    const int later = min(stages - 1 - t, kBigStages - 2);
-    if (later >= 3) INTENT_WAIT_VMCNT(12);
-    else if (later == 2) INTENT_WAIT_VMCNT(8);
-    else if (later == 1) INTENT_WAIT_VMCNT(4);
-    else INTENT_WAIT_VMCNT(0);
-  };
-  wait_stage(0);
-  stage_barrier();
-  if (lag) stage_barrier();
-  i32x4_t xf[2][4], wf[2][2];
-  for (int t = 0; t < stages; ++t) {
+  i32x4_t xf[2][4], wf[2][4];
+  const auto read = [&](int t, int k, int i) {         // of half k of stage t: operand i of the weight, then of x
     const uint4 *sx = lds + (t % kBigStages) * kStageUnits, *sw = sx + kHalf;
+    const int at = (i % 4 * 32 + row) * 4 + ((k * 2 + half) ^ turn);
+    if (i < 4)
+      wf[k][i] = __builtin_bit_cast(i32x4_t, sw[wn * 128 * 4 + at]);
+    else
+      xf[k][i - 4] = __builtin_bit_cast(i32x4_t, sx[wm * 128 * 4 + at]);
+  };
+  const auto multiply = [&](int k, int at) {           // product `at` of 16 of half k
+    const int i = at / 4, j = at % 4;
+    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k][j], xf[k][i], acc[i][j], 0, 0, 0);
+  };
+  if (stages > 0) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int t = 0; t < kBigStages - 1; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xf[k][i] = __builtin_bit_cast(i32x4_t, sx[(wm * 128 + i * 32 + row) * 4 + ((k * 2 + half) ^ turn)]);
+      for (int i = 0; i < 2 * kLoads; ++i) issue(t, i);
+    INTENT_WAIT_VMCNT((kBigStages - 2) * 2 * kLoads);
+    stage_barrier();
 #pragma unroll
-      for (int j = 0; j < 2; ++j) wf[k][j] = __builtin_bit_cast(i32x4_t, sw[(wn * 64 + j * 32 + row) * 4 + ((k * 2 + half) ^ turn)]);
+    for (int i = 0; i < 8; ++i) read(0, 0, i);
+    for (int t = 0; t < stages; ++t) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {                    // a read and two products at a time, in this order
+        read(t, 1, i);
+        multiply(0, 2 * i);
+        multiply(0, 2 * i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      INTENT_WAIT_VMCNT((kBigStages - 3) * 2 * kLoads);                // this wave's loads of the next stage have come
+      stage_barrier();                                 // everybody's have, and everybody has read the stage that is filled next
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {                    // and a load
+        read(t + 1, 0, i);                             // behind the last stage: the last again, never used
+        issue(t + kBigStages - 1, i);
+        multiply(1, 2 * i);
+        multiply(1, 2 * i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    if (t + kBigStages - 1 < stages) issue(t + kBigStages - 1);
-    if (lag) wait_stage(t + 1);
-    INTENT_WAIT_LGKMCNT0();
-    stage_barrier();
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k][j], xf[k][i], acc[i][j], 0, 0, 0);
-    if (!lag) wait_stage(t + 1);
-    stage_barrier();
+    INTENT_WAIT_VMCNT(0);                              // nothing is on its way into the LDS of an ended workgroup
   }
-  if (!lag) stage_barrier();
-  // acc[i][j][4 q + e] is row 32 i + (lane % 32) of x with weight row 32 j + 8 q + 4 half + e.
+  if (rest > 0) {                                      // the end of K, zeros behind it
+    stage_barrier();
+    const int64_t k0 = static_cast<int64_t>(stages) * kBK;
+    const int8_t *const zero = reinterpret_cast<const int8_t *>(&kZeroUnit);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kLoads; ++i) {
+      __builtin_amdgcn_global_load_lds(unit[i] < rest ? x_src[i] + k0 : zero, (lds_void_t *)(lds + (wave * kLoads + i) * kWave), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(unit[i] < rest ? w_src[i] + k0 : zero, (lds_void_t *)(lds + kHalf + (wave * kLoads + i) * kWave), 16, 0, 0);
+    }
+    INTENT_WAIT_VMCNT(0);
+    stage_barrier();
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < 16; ++i) read(0, i / 8, i % 8);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) multiply(i / 16, i % 16);
+  }
+  // acc[i][j][4 q + e] is row 32 i + (lane % 32) of x with weight row 32 j + 8 q + 4 half + e. The results of 32 rows go through the
+  // wave's own part of the LDS, from where whole rows of 128 are written (straight from registers, 8 bytes a lane and row with a load of
+  // their scales: 39 us a tile, as long as K = 2700 takes).
+  __syncthreads();
+  constexpr int kRowUnits = 17;                        // 128 results and 16 bytes, so that rows lie in different banks
+  float *const scales = reinterpret_cast<float *>(lds + kBigWaves * 32 * kRowUnits);      // of the tile's weight rows, then their biases
+  for (int i = tid; i < kBN; i += kBigThreads) {
+    const int n = min(n0 + i, p.n - 1);
+    scales[i] = p.ws[n], scales[kBN + i] = p.bias != nullptr ? p.bias[n] : 0.0f;
+  }
+  float xs[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) xs[i] = p.xs[min(m0 + wm * 128 + i * 32 + row, p.m - 1)];
+  __syncthreads();
+  uint4 *const own = lds + wave * 32 * kRowUnits;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int sum[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        store<E>(p, m0 + wm * 128 + i * 32 + row, n0 + wn * 64 + j * 32 + 8 * q + 4 * half, sum);
+        const int at = wn * 128 + j * 32 + 8 * q + 4 * half;
+        const float4 ws = *reinterpret_cast<const float4 *>(scales + at), bias = *reinterpret_cast<const float4 *>(scales + kBN + at);
+        const auto result = [&](int e, float w, float b) {
+          const float y = static_cast<float>(acc[i][j][4 * q + e]) * xs[i] * w;
+          return static_cast<uint32_t>(from_f32<E>(p.bias != nullptr ? y + b : y).bits);
+        };
+        reinterpret_cast<uint2 *>(own + row * kRowUnits)[j * 8 + 2 * q + half] =
+            make_uint2(result(0, ws.x, bias.x) | result(1, ws.y, bias.y) << 16, result(2, ws.z, bias.z) | result(3, ws.w, bias.w) << 16);
       }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int of = k * 4 + (lane >> 4), m = m0 + wm * 128 + i * 32 + of, n = n0 + wn * 128 + (lane & 15) * 8;
+      const uint4 v = own[of * kRowUnits + (lane & 15)];
+      if (m >= p.m || n >= p.n) continue;
+      uint16_t *const y = p.y + m * p.ldy + n;
+      if (p.wide == 8) {
+        *reinterpret_cast<uint4 *>(y) = v;
+      } else {
+        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < p.n) y[e] = static_cast<uint16_t>(words[e / 2] >> (16 * (e & 1)));
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
 }
 
 // ---------------------------------------------------------------- which kernel
