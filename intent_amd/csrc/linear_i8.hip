@@ -30,6 +30,7 @@ struct Linear {
   int64_t ldx, ldw, ldy;
   int m, n, units;                     // units: K / 16
   int m_tiles, n_tiles, parts, stages; // tiles; stages of a part (or of a wave)
+  int full;                            // linear_big: tiles of I = 4
   int wide;                            // y takes stores of so many elements (1, 4 or 8)
 };
 
@@ -281,12 +282,17 @@ __global__ __launch_bounds__(256) void linear_fold(Linear p) {
 }
 
 // ---------------------------------------------------------------- large tiles, both operands through the LDS
-// 256 rows of x by 256 weight rows, 4 waves of 128 x 128 = 4 x 4 products of 32 x 32 x 32, so that a byte read from the LDS meets 128
-// others. A stage is 64 bytes of K of both, 32 KB; five of them arrive by loads into the LDS. A wave has its SIMD to itself and hides its
-// reads behind its own products: while 16 products of half a stage run, the operands of the next half are read.
-constexpr int kBM = 256, kBN = 256, kBK = 64, kBigWaves = 4, kBigThreads = kBigWaves * kWave, kBigStages = 5;
-constexpr int kHalf = kBM * kBK / kUnit, kStageUnits = 2 * kHalf;
+// 64 I rows of x by 256 weight rows, 4 waves of 32 I x 128 = I x 4 products of 32 x 32 x 32 (I = 4: a byte read from the LDS meets 128
+// others). A stage is 64 bytes of K of both; stages arrive by loads into the LDS, as many as it holds. A wave has its SIMD to itself and
+// hides its reads behind its own products: while the 4 I products of half a stage run, the operands of the next half are read.
+// Whole rounds of tiles over the CUs have I = 4; where at most half a round is left, or less than that is all there is, that is done by
+// twice as many tiles of I = 2 (4096 x 14336 x 4096, three rounds and a half: 273 us without).
+constexpr int kBN = 256, kBK = 64, kBigWaves = 4, kBigThreads = kBigWaves * kWave;
 constexpr int kGroupM = 8;             // tiles of x that share a walk along the weight rows
+constexpr int big_rows(int i) { return 64 * i; }
+constexpr int big_stages(int i) { return i == 4 ? 5 : 6; }
+constexpr int kBigUnits = big_stages(4) * (big_rows(4) + kBN) * kBK / kUnit;      // 160 KB
+static_assert(big_stages(2) * (big_rows(2) + kBN) * kBK / kUnit <= kBigUnits, "all kinds of tiles share one array");
 
 // Tiles in groups of kGroupM rows of tiles, walked column by column: those that run at one time share rows and columns.
 __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int &tm, int &tn) {
@@ -295,81 +301,75 @@ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int &tm
   tm = first + in % rows, tn = in / rows;
 }
 
-template <typename E>
-__global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
-  __shared__ uint4 lds[kBigStages * kStageUnits];
+// The tile from row m0 of x and weight row n0 on.
+template <typename E, int I>
+__device__ __forceinline__ void big_tile(const Linear &p, int m0, int n0, uint4 *lds) {
+  constexpr int kStages = big_stages(I), kXUnits = big_rows(I) * kBK / kUnit, kWUnits = kBN * kBK / kUnit, kStageUnits = kXUnits + kWUnits;
+  constexpr int kXLoads = kXUnits / kBigThreads, kWLoads = kWUnits / kBigThreads, kLoads = kXLoads + kWLoads, kReads = I + 4, kProducts = 4 * I;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  const int tile = xcd_tile(grid_block(), p.m_tiles * p.n_tiles);
-  if (tile < 0) return;
-  int tm, tn;
-  tile_at(tile, p.m_tiles, p.n_tiles, tm, tn);
-  const int m0 = tm * kBM, n0 = tn * kBN;
-  // Each wave moves 4 KB of x and 4 KB of the weight a stage. Unit c of row r lies at place c ^ (r / 4) % 4 of its four.
-  constexpr int kLoads = kHalf / kBigThreads;
-  const int8_t *x_src[kLoads], *w_src[kLoads];
+  // Unit c of row r lies at place c ^ (r / 4) % 4 of its four.
+  const int8_t *src[kLoads];                           // of x, then of the weight
   int unit[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int slot = (wave * kLoads + i) * kWave + lane, row = slot >> 2;
+    const int slot = (wave * (i < kXLoads ? kXLoads : kWLoads) + (i < kXLoads ? i : i - kXLoads)) * kWave + lane, row = slot >> 2;
     unit[i] = (slot & 3) ^ ((row >> 2) & 3);
-    x_src[i] = p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx + unit[i] * kUnit;
-    w_src[i] = p.w + static_cast<int64_t>(min(n0 + row, p.n - 1)) * p.ldw + unit[i] * kUnit;
+    src[i] = (i < kXLoads ? p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx : p.w + static_cast<int64_t>(min(n0 + row, p.n - 1)) * p.ldw) + unit[i] * kUnit;
   }
+  const auto place = [&](int i) { return i < kXLoads ? (wave * kXLoads + i) * kWave : kXUnits + (wave * kWLoads + i - kXLoads) * kWave; };
   const int stages = p.units / 4, rest = p.units % 4;  // whole ones; units behind them
   const auto issue = [&](int t, int i) {               // load i of stage t (the last again behind it, so that as many are always on their way)
-    uint4 *stage = lds + (t % kBigStages) * kStageUnits;
     const int64_t k0 = static_cast<int64_t>(min(t, stages - 1)) * kBK;
-    const int j = i / 2;
-    __builtin_amdgcn_global_load_lds(i % 2 ? w_src[j] + k0 : x_src[j] + k0, (lds_void_t *)(stage + i % 2 * kHalf + (wave * kLoads + j) * kWave), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds(src[i] + k0, (lds_void_t *)(lds + (t % kStages) * kStageUnits + place(i)), 16, 0, 0);
   };
-  i32x16_t acc[4][4];
+  i32x16_t acc[I][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < I; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
   const int row = lane & 31, half = lane >> 5, turn = (row >> 2) & 3;
-  i32x4_t xf[2][4], wf[2][4];
+  i32x4_t xf[2][I], wf[2][4];
   const auto read = [&](int t, int k, int i) {         // of half k of stage t: operand i of the weight, then of x
-    const uint4 *sx = lds + (t % kBigStages) * kStageUnits, *sw = sx + kHalf;
-    const int at = (i % 4 * 32 + row) * 4 + ((k * 2 + half) ^ turn);
+    const uint4 *sx = lds + (t % kStages) * kStageUnits, *sw = sx + kXUnits;
+    const int at = ((i < 4 ? i : i - 4) * 32 + row) * 4 + ((k * 2 + half) ^ turn);
     if (i < 4)
       wf[k][i] = __builtin_bit_cast(i32x4_t, sw[wn * 128 * 4 + at]);
     else
-      xf[k][i - 4] = __builtin_bit_cast(i32x4_t, sx[wm * 128 * 4 + at]);
+      xf[k][i - 4] = __builtin_bit_cast(i32x4_t, sx[wm * 32 * I * 4 + at]);
   };
-  const auto multiply = [&](int k, int at) {           // product `at` of 16 of half k
-    const int i = at / 4, j = at % 4;
-    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k][j], xf[k][i], acc[i][j], 0, 0, 0);
+  const auto multiply = [&](int k, int at) {           // product `at` of half k
+    acc[at / 4][at % 4] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k][at % 4], xf[k][at / 4], acc[at / 4][at % 4], 0, 0, 0);
   };
+  constexpr int kEach = kProducts / 8;                 // products behind each of eight reads (and loads)
   if (stages > 0) {
 #pragma unroll
-    for (int t = 0; t < kBigStages - 1; ++t)
+    for (int t = 0; t < kStages - 1; ++t)
 #pragma unroll
-      for (int i = 0; i < 2 * kLoads; ++i) issue(t, i);
-    INTENT_WAIT_VMCNT((kBigStages - 2) * 2 * kLoads);
+      for (int i = 0; i < kLoads; ++i) issue(t, i);
+    INTENT_WAIT_VMCNT((kStages - 2) * kLoads);
     stage_barrier();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) read(0, 0, i);
+    for (int i = 0; i < kReads; ++i) read(0, 0, i);
     for (int t = 0; t < stages; ++t) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {                    // a read and two products at a time, in this order
-        read(t, 1, i);
-        multiply(0, 2 * i);
-        multiply(0, 2 * i + 1);
+      for (int i = 0; i < 8; ++i) {                    // a read and some products at a time, in this order
+        if (i < kReads) read(t, 1, i);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) multiply(0, kEach * i + j);
         __builtin_amdgcn_sched_barrier(0);
       }
-      INTENT_WAIT_VMCNT((kBigStages - 3) * 2 * kLoads);                // this wave's loads of the next stage have come
+      INTENT_WAIT_VMCNT((kStages - 3) * kLoads);       // this wave's loads of the next stage have come
       stage_barrier();                                 // everybody's have, and everybody has read the stage that is filled next
 #pragma unroll
       for (int i = 0; i < 8; ++i) {                    // and a load
-        read(t + 1, 0, i);                             // behind the last stage: the last again, never used
-        issue(t + kBigStages - 1, i);
-        multiply(1, 2 * i);
-        multiply(1, 2 * i + 1);
+        if (i < kReads) read(t + 1, 0, i);             // behind the last stage: the last again, never used
+        if (i < kLoads) issue(t + kStages - 1, i);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) multiply(1, kEach * i + j);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -377,19 +377,17 @@ __global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
   }
   if (rest > 0) {                                      // the end of K, zeros behind it
     stage_barrier();
-    const int64_t k0 = static_cast<int64_t>(stages) * kBK;
-    const int8_t *const zero = reinterpret_cast<const int8_t *>(&kZeroUnit);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      __builtin_amdgcn_global_load_lds(unit[i] < rest ? x_src[i] + k0 : zero, (lds_void_t *)(lds + (wave * kLoads + i) * kWave), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(unit[i] < rest ? w_src[i] + k0 : zero, (lds_void_t *)(lds + kHalf + (wave * kLoads + i) * kWave), 16, 0, 0);
+      const int8_t *const from = unit[i] < rest ? src[i] + static_cast<int64_t>(stages) * kBK : reinterpret_cast<const int8_t *>(&kZeroUnit);
+      __builtin_amdgcn_global_load_lds(from, (lds_void_t *)(lds + place(i)), 16, 0, 0);
     }
     INTENT_WAIT_VMCNT(0);
     stage_barrier();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) read(0, i / 8, i % 8);
+    for (int i = 0; i < 2 * kReads; ++i) read(0, i / kReads, i % kReads);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) multiply(i / 16, i % 16);
+    for (int i = 0; i < 2 * kProducts; ++i) multiply(i / kProducts, i % kProducts);
   }
   // acc[i][j][4 q + e] is row 32 i + (lane % 32) of x with weight row 32 j + 8 q + 4 half + e. The results of 32 rows go through the
   // wave's own part of the LDS, from where whole rows of 128 are written (straight from registers, 8 bytes a lane and row with a load of
@@ -401,13 +399,13 @@ __global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
     const int n = min(n0 + i, p.n - 1);
     scales[i] = p.ws[n], scales[kBN + i] = p.bias != nullptr ? p.bias[n] : 0.0f;
   }
-  float xs[4];
+  float xs[I];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) xs[i] = p.xs[min(m0 + wm * 128 + i * 32 + row, p.m - 1)];
+  for (int i = 0; i < I; ++i) xs[i] = p.xs[min(m0 + (wm * I + i) * 32 + row, p.m - 1)];
   __syncthreads();
   uint4 *const own = lds + wave * 32 * kRowUnits;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < I; ++i) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -424,7 +422,7 @@ __global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int of = k * 4 + (lane >> 4), m = m0 + wm * 128 + i * 32 + of, n = n0 + wn * 128 + (lane & 15) * 8;
+      const int of = k * 4 + (lane >> 4), m = m0 + (wm * I + i) * 32 + of, n = n0 + wn * 128 + (lane & 15) * 8;
       const uint4 v = own[of * kRowUnits + (lane & 15)];
       if (m >= p.m || n >= p.n) continue;
       uint16_t *const y = p.y + m * p.ldy + n;
@@ -438,6 +436,26 @@ __global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+// full: tiles of I = 4, the first of the order of tiles; the others are halved.
+template <typename E>
+__global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
+  __shared__ uint4 lds[kBigUnits];
+  const int block = grid_block(), tiles = p.m_tiles * p.n_tiles, full_blocks = (p.full + 7) / 8 * 8;
+  int tm, tn;
+  if (block < full_blocks) {
+    const int tile = xcd_tile(block, p.full);
+    if (tile < 0) return;
+    tile_at(tile, p.m_tiles, p.n_tiles, tm, tn);
+    big_tile<E, 4>(p, tm * big_rows(4), tn * kBN, lds);
+  } else {
+    const int tile = xcd_tile(block - full_blocks, 2 * (tiles - p.full));
+    if (tile < 0) return;
+    tile_at(p.full + tile / 2, p.m_tiles, p.n_tiles, tm, tn);
+    const int m0 = tm * big_rows(4) + tile % 2 * big_rows(2);
+    if (m0 < p.m) big_tile<E, 2>(p, m0, tn * kBN, lds);
   }
 }
 
@@ -490,8 +508,10 @@ void launch(Linear p, const Cut &c, hipStream_t s) {
       p.stages = ((p.units + 7) / 8 + waves - 1) / waves;
       grid = tile_grid((p.n + 16 * c.nt - 1) / (16 * c.nt), 1);
     } else if (c.mt == 16) {
-      p.m_tiles = (p.m + kBM - 1) / kBM, p.n_tiles = (p.n + kBN - 1) / kBN;
-      grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles, 1);
+      p.m_tiles = (p.m + big_rows(4) - 1) / big_rows(4), p.n_tiles = (p.n + kBN - 1) / kBN;
+      const int tiles = p.m_tiles * p.n_tiles, cus = device_cus(), left = tiles % cus;
+      p.full = 2 * left <= cus ? tiles - left : tiles;
+      grid = tile_grid((p.full + 7) / 8 * 8 + 2 * static_cast<int64_t>(tiles - p.full), 1);
     } else {
       const int of_stage = stage_bytes(c.mt) / kUnit;
       p.stages = ((p.units + of_stage - 1) / of_stage + c.parts - 1) / c.parts;
