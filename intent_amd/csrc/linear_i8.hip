@@ -26,9 +26,9 @@ struct Linear {
   const int8_t *x, *w;
   const float *xs, *ws, *bias;         // bias: null for none
   uint16_t *y;
-  int32_t *sums;                       // [parts][m][n] where K is divided
+  int32_t *sums;                       // [parts][m][pitch] where K is divided, pitch: n in whole fours
   int64_t ldx, ldw, ldy;
-  int m, n, units;                     // units: K / 16
+  int m, n, pitch, units;              // units: K / 16
   int m_tiles, n_tiles, parts, stages; // tiles; stages of a part (or of a wave)
   int full;                            // linear_big: tiles of I = 4
   int wide;                            // y takes stores of so many elements (1, 4 or 8)
@@ -181,7 +181,8 @@ __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
   const int m0 = tile % p.m_tiles * kRows, n0 = (tile / p.m_tiles * W + wave) * 16 * NT;
   const int first = min(part * p.stages * kRowUnits, p.units), last = min(p.units, first + p.stages * kRowUnits);     // units of this part
   const int stages = (last - first + kRowUnits - 1) / kRowUnits;
-  const auto place = [](int row) { return kRowUnits == 16 ? row & 15 : (row >> 1) & 7; };
+  static_assert(kRowUnits == 8, "the 16 rows of a read lie in different banks");
+  const auto place = [](int row) { return (row >> 1) & 7; };
   const int8_t *from[kLoads];
   int unit[kLoads];
 #pragma unroll
@@ -251,33 +252,24 @@ __global__ __launch_bounds__(W *kWave, 2) void linear_tiles(Linear p) {
     if (p.parts == 1) {
       store<E>(p, m, n, row);
     } else if (m < p.m) {
-      int32_t *to = p.sums + (static_cast<int64_t>(part) * p.m + m) * p.n + n;
-      if (p.wide >= 4) {
+      int32_t *to = p.sums + (static_cast<int64_t>(part) * p.m + m) * p.pitch + n;
 #pragma unroll
-        for (int k = 0; k < 4 * NT; k += 4)
-          if (n + k < p.n) *reinterpret_cast<i32x4_t *>(to + k) = i32x4_t{row[k], row[k + 1], row[k + 2], row[k + 3]};
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4 * NT; ++k)
-          if (n + k < p.n) to[k] = row[k];
-      }
+      for (int k = 0; k < 4 * NT; k += 4)
+        if (n + k < p.pitch) *reinterpret_cast<i32x4_t *>(to + k) = i32x4_t{row[k], row[k + 1], row[k + 2], row[k + 3]};
     }
   }
 }
 
-// y from the parts' sums: kCount columns a thread.
-template <typename E, int kCount>
+// y from the parts' sums, four columns a thread.
+template <typename E>
 __global__ __launch_bounds__(256) void linear_fold(Linear p) {
-  const int64_t all = static_cast<int64_t>(p.m) * p.n, at = (static_cast<int64_t>(grid_block()) * 256 + threadIdx.x) * kCount;
+  const int64_t all = static_cast<int64_t>(p.m) * p.pitch, at = (static_cast<int64_t>(grid_block()) * 256 + threadIdx.x) * 4;
   if (at >= all) return;
-  typedef int held_t __attribute__((ext_vector_type(kCount)));
-  held_t total = 0;
+  i32x4_t total = {0, 0, 0, 0};
 #pragma unroll 8
-  for (int i = 0; i < p.parts; ++i) total += *reinterpret_cast<const held_t *>(p.sums + i * all + at);
-  const int m = static_cast<int>(at / p.n), n = static_cast<int>(at - static_cast<int64_t>(m) * p.n);
-  int sum[kCount];
-#pragma unroll
-  for (int i = 0; i < kCount; ++i) sum[i] = total[i];
+  for (int i = 0; i < p.parts; ++i) total += *reinterpret_cast<const i32x4_t *>(p.sums + i * all + at);
+  const int m = static_cast<int>(at / p.pitch), n = static_cast<int>(at - static_cast<int64_t>(m) * p.pitch);
+  const int sum[4] = {total[0], total[1], total[2], total[3]};
   store<E>(p, m, n, sum);
 }
 
@@ -301,14 +293,15 @@ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int &tm
   tm = first + in % rows, tn = in / rows;
 }
 
-// The tile from row m0 of x and weight row n0 on.
-template <typename E, int I>
-__device__ __forceinline__ void big_tile(const Linear &p, int m0, int n0, uint4 *lds) {
+// The tile from row m0 of x and weight row n0 on, over the part of K that is `part` if kDivided.
+template <typename E, int I, bool kDivided>
+__device__ __forceinline__ void big_tile(const Linear &p, int m0, int n0, int part, uint4 *lds) {
   constexpr int kStages = big_stages(I), kXUnits = big_rows(I) * kBK / kUnit, kWUnits = kBN * kBK / kUnit, kStageUnits = kXUnits + kWUnits;
   constexpr int kXLoads = kXUnits / kBigThreads, kWLoads = kWUnits / kBigThreads, kLoads = kXLoads + kWLoads, kReads = I + 4, kProducts = 4 * I;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
+  const int first = kDivided ? part * p.stages * 4 : 0, units = kDivided ? max(0, min(p.units - first, p.stages * 4)) : p.units;
   // Unit c of row r lies at place c ^ (r / 4) % 4 of its four.
   const int8_t *src[kLoads];                           // of x, then of the weight
   int unit[kLoads];
@@ -316,10 +309,10 @@ __device__ __forceinline__ void big_tile(const Linear &p, int m0, int n0, uint4 
   for (int i = 0; i < kLoads; ++i) {
     const int slot = (wave * (i < kXLoads ? kXLoads : kWLoads) + (i < kXLoads ? i : i - kXLoads)) * kWave + lane, row = slot >> 2;
     unit[i] = (slot & 3) ^ ((row >> 2) & 3);
-    src[i] = (i < kXLoads ? p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx : p.w + static_cast<int64_t>(min(n0 + row, p.n - 1)) * p.ldw) + unit[i] * kUnit;
+    src[i] = (i < kXLoads ? p.x + static_cast<int64_t>(min(m0 + row, p.m - 1)) * p.ldx : p.w + static_cast<int64_t>(min(n0 + row, p.n - 1)) * p.ldw) + (unit[i] + first) * kUnit;
   }
   const auto place = [&](int i) { return i < kXLoads ? (wave * kXLoads + i) * kWave : kXUnits + (wave * kWLoads + i - kXLoads) * kWave; };
-  const int stages = p.units / 4, rest = p.units % 4;  // whole ones; units behind them
+  const int stages = units / 4, rest = units % 4;      // whole ones; units behind them
   const auto issue = [&](int t, int i) {               // load i of stage t (the last again behind it, so that as many are always on their way)
     const int64_t k0 = static_cast<int64_t>(min(t, stages - 1)) * kBK;
     __builtin_amdgcn_global_load_lds(src[i] + k0, (lds_void_t *)(lds + (t % kStages) * kStageUnits + place(i)), 16, 0, 0);
@@ -389,7 +382,24 @@ __device__ __forceinline__ void big_tile(const Linear &p, int m0, int n0, uint4 
 #pragma unroll
     for (int i = 0; i < 2 * kProducts; ++i) multiply(i / kProducts, i % kProducts);
   }
-  // acc[i][j][4 q + e] is row 32 i + (lane % 32) of x with weight row 32 j + 8 q + 4 half + e. The results of 32 rows go through the
+  // acc[i][j][4 q + e] is row 32 i + (lane % 32) of x with weight row 32 j + 8 q + 4 half + e.
+  if constexpr (kDivided) {
+    int m = m0 + wm * I * 32 + row;
+    const int n = n0 + wn * 128 + 4 * half;
+    int32_t *to = p.sums + (static_cast<int64_t>(part) * p.m + m) * p.pitch + n;
+#pragma unroll
+    for (int i = 0; i < I; ++i, m += 32, to += static_cast<int64_t>(32) * p.pitch) {
+      if (m >= p.m) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + j * 32 + 8 * q < p.pitch)
+            *reinterpret_cast<i32x4_t *>(to + j * 32 + 8 * q) = i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    }
+    return;
+  }
+  // The results of 32 rows go through the
   // wave's own part of the LDS, from where whole rows of 128 are written (straight from registers, 8 bytes a lane and row with a load of
   // their scales: 39 us a tile, as long as K = 2700 takes).
   __syncthreads();
@@ -443,46 +453,77 @@ __device__ __forceinline__ void big_tile(const Linear &p, int m0, int n0, uint4 
 template <typename E>
 __global__ __launch_bounds__(kBigThreads, 1) void linear_big(Linear p) {
   __shared__ uint4 lds[kBigUnits];
-  const int block = grid_block(), tiles = p.m_tiles * p.n_tiles, full_blocks = (p.full + 7) / 8 * 8;
+  const int tiles = p.m_tiles * p.n_tiles, full_blocks = (p.full + 7) / 8 * 8;
   int tm, tn;
-  if (block < full_blocks) {
+  if (const int block = grid_block(); block < full_blocks) {
     const int tile = xcd_tile(block, p.full);
     if (tile < 0) return;
     tile_at(tile, p.m_tiles, p.n_tiles, tm, tn);
-    big_tile<E, 4>(p, tm * big_rows(4), tn * kBN, lds);
+    big_tile<E, 4, false>(p, tm * big_rows(4), tn * kBN, 0, lds);
   } else {
     const int tile = xcd_tile(block - full_blocks, 2 * (tiles - p.full));
     if (tile < 0) return;
     tile_at(p.full + tile / 2, p.m_tiles, p.n_tiles, tm, tn);
     const int m0 = tm * big_rows(4) + tile % 2 * big_rows(2);
-    if (m0 < p.m) big_tile<E, 2>(p, m0, tn * kBN, lds);
+    if (m0 < p.m) big_tile<E, 2, false>(p, m0, tn * kBN, 0, lds);
   }
 }
 
+// Tiles of one kind over parts of K, one part after the other. A kernel of its own: with both ends in one registers spilled, and 4096 x
+// 4096 x 4096 took 80 us for 77.
+template <typename E, int I>
+__global__ __launch_bounds__(kBigThreads, 1) void linear_big_part(Linear p) {
+  __shared__ uint4 lds[kBigUnits];
+  const int job = xcd_tile(grid_block(), p.m_tiles * p.n_tiles * p.parts);
+  if (job < 0) return;
+  int tm, tn;
+  tile_at(job % (p.m_tiles * p.n_tiles), p.m_tiles, p.n_tiles, tm, tn);
+  big_tile<E, I, true>(p, tm * big_rows(I), tn * kBN, job / (p.m_tiles * p.n_tiles), lds);
+}
+
 // ---------------------------------------------------------------- which kernel
-// How a product is cut. mt = 0: linear_few; 1: of one row; 16: linear_big.
+// How a product is cut. mt = 0: linear_few; 1: of one row; 16: linear_big, of nt = 2 tiles of I = 2 alone, of 4 tiles of I = 4, but for what
+// at most half fills the last round of an undivided K.
 struct Cut {
   int mt, nt, parts;
 };
-constexpr int tile_waves(int mt) { return mt == 2 ? 8 : 4; }
-constexpr int stage_bytes(int mt) { return mt == 2 ? 256 : 128; }
+int big_full(int tiles, const Cut &c) {
+  const int left = tiles % device_cus();
+  return c.nt == 2 ? 0 : 2 * left <= device_cus() ? tiles - left : tiles;
+}
+constexpr int kTileWaves = 4, kTileStage = 128;
 
+// linear_few for up to 16 rows, NT by the weight rows there are for the workgroups. Otherwise by an estimate from what the tiles measured:
+// us a round of workgroups takes besides its stages, a stage (of 128 bytes of K) of a workgroup that has a CU for itself and of each of
+// several on a CU, and what writing, reading and adding the parts' sums takes. Large tiles have a CU each, whole ones and halves in rounds
+// of their own. Over M of 17 to 1024 and three N x K the choice was within a tenth of the best of all tiles and parts.
 Cut cut(int64_t m, int64_t n, int64_t k) {
-  const int cus = device_cus();
-  if (m == 1) return {1, n >= 24 * cus ? 2 : 1, 1};
-  if (m <= 16) return {0, n >= 24 * cus ? 2 : 1, 1};
-  constexpr struct { int mt, nt; float alone, shared; } kKinds[] = {{2, 1, 0.53f, 0.5f}, {4, 2, 0.55f, 0.45f}, {8, 2, 0.8f, 0.65f}, {16, 16, 0.62f, 0.62f}};
+  const int64_t cus = device_cus();
+  if (m <= 16) return {m == 1 ? 1 : 0, n >= 24 * cus ? 2 : 1, 1};
+  constexpr struct { int mt, nt; float round, alone, shared; } kKinds[] = {{4, 2, 5.0f, 0.62f, 0.61f}, {8, 2, 5.0f, 1.0f, 0.85f}};
+  constexpr float kFullRound = 9.0f, kFullStage = 1.84f, kHalfRound = 5.0f, kHalfStage = 1.14f, kStart = 5.0f;
+  const int64_t stages = (k + kTileStage - 1) / kTileStage, big = (m + big_rows(4) - 1) / big_rows(4) * ((n + kBN - 1) / kBN);
+  const int64_t halves = (m + big_rows(2) - 1) / big_rows(2) * ((n + kBN - 1) / kBN);
   Cut best{};
   float least = 0.0f;
-  for (const auto &kind : kKinds) {
-    const int64_t per_tile = kind.mt == 16 ? kBN : 16 * tile_waves(kind.mt) * kind.nt;
-    const int64_t tiles = ((m + 16 * kind.mt - 1) / (16 * kind.mt)) * ((n + per_tile - 1) / per_tile);
-    const int64_t bytes = kind.mt == 16 ? kBK : stage_bytes(kind.mt), stages = (k + bytes - 1) / bytes;
-    for (int parts = 1; parts <= (kind.mt == 16 ? 1 : 16) && (parts == 1 || parts * 4 <= stages); ++parts) {
+  const auto consider = [&](Cut c, float us) {
+    if (c.parts > 1) us += 3.0f + static_cast<float>(c.parts) * static_cast<float>(m) * static_cast<float>(n) * 2.1e-6f;
+    if (best.parts == 0 || us < least) best = c, least = us;
+  };
+  for (int parts = 1; parts <= 16 && (parts == 1 || parts * 4 <= stages); ++parts) {
+    const float of_part = static_cast<float>((stages + parts - 1) / parts);
+    for (const auto &kind : kKinds) {
+      const int64_t tiles = (m + 16 * kind.mt - 1) / (16 * kind.mt) * ((n + 16 * kTileWaves * kind.nt - 1) / (16 * kTileWaves * kind.nt));
       const float on_one = static_cast<float>((tiles * parts + cus - 1) / cus), shared = kind.shared * on_one;
-      float us = static_cast<float>((stages + parts - 1) / parts) * (kind.alone > shared ? kind.alone : shared);
-      if (parts > 1) us += 3.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(n) * 2.3e-6f;
-      if (best.parts == 0 || us < least) best = {kind.mt, kind.nt, parts}, least = us;
+      consider({kind.mt, kind.nt, parts}, kind.round + of_part * (kind.alone > shared ? kind.alone : shared));
+    }
+    const float half = kHalfRound + of_part * kHalfStage, whole = kFullRound + of_part * kFullStage;
+    consider({16, 2, parts}, kStart + static_cast<float>((halves * parts + cus - 1) / cus) * half);
+    if (parts > 1) {
+      consider({16, 4, parts}, kStart + static_cast<float>((big * parts + cus - 1) / cus) * whole);
+    } else {
+      const bool split = 2 * (big % cus) <= cus;
+      consider({16, 4, 1}, kStart + static_cast<float>(split ? big / cus : (big + cus - 1) / cus) * whole + (split && big % cus ? half : 0.0f));
     }
   }
   return best;
@@ -493,10 +534,10 @@ template <typename E, typename F>
 int with_kernel(const Cut &c, F f) {
   if (c.mt == 0) return c.nt == 1 ? f(linear_few<E, 1, false>, "linear_few", kFewWaves) : f(linear_few<E, 2, false>, "linear_few", kFewWaves);
   if (c.mt == 1) return c.nt == 1 ? f(linear_few<E, 1, true>, "linear_few", kFewWaves) : f(linear_few<E, 2, true>, "linear_few", kFewWaves);
-  if (c.mt == 16) return f(linear_big<E>, "linear_big", kBigThreads / kWave);
-  return c.mt == 2   ? f(linear_tiles<E, 2, 1, 4, tile_waves(2), stage_bytes(2)>, "linear_tiles", tile_waves(2))
-         : c.mt == 4 ? f(linear_tiles<E, 4, 2, 4, tile_waves(4), stage_bytes(4)>, "linear_tiles", tile_waves(4))
-                     : f(linear_tiles<E, 8, 2, 4, tile_waves(8), stage_bytes(8)>, "linear_tiles", tile_waves(8));
+  if (c.mt == 16 && c.parts == 1) return f(linear_big<E>, "linear_big", kBigThreads / kWave);
+  if (c.mt == 16) return f(c.nt == 2 ? linear_big_part<E, 2> : linear_big_part<E, 4>, "linear_big_part", kBigThreads / kWave);
+  return c.mt == 4 ? f(linear_tiles<E, 4, 2, 4, kTileWaves, kTileStage>, "linear_tiles", kTileWaves)
+                   : f(linear_tiles<E, 8, 2, 4, kTileWaves, kTileStage>, "linear_tiles", kTileWaves);
 }
 
 template <typename E>
@@ -508,12 +549,18 @@ void launch(Linear p, const Cut &c, hipStream_t s) {
       p.stages = ((p.units + 7) / 8 + waves - 1) / waves;
       grid = tile_grid((p.n + 16 * c.nt - 1) / (16 * c.nt), 1);
     } else if (c.mt == 16) {
-      p.m_tiles = (p.m + big_rows(4) - 1) / big_rows(4), p.n_tiles = (p.n + kBN - 1) / kBN;
-      const int tiles = p.m_tiles * p.n_tiles, cus = device_cus(), left = tiles % cus;
-      p.full = 2 * left <= cus ? tiles - left : tiles;
-      grid = tile_grid((p.full + 7) / 8 * 8 + 2 * static_cast<int64_t>(tiles - p.full), 1);
+      p.stages = ((p.units + 3) / 4 + c.parts - 1) / c.parts;
+      const int rows = c.parts == 1 ? big_rows(4) : big_rows(c.nt);
+      p.m_tiles = (p.m + rows - 1) / rows, p.n_tiles = (p.n + kBN - 1) / kBN;
+      const int tiles = p.m_tiles * p.n_tiles;
+      if (c.parts == 1) {
+        p.full = big_full(tiles, c);
+        grid = tile_grid((p.full + 7) / 8 * 8 + (2 * static_cast<int64_t>(tiles - p.full) + 7) / 8 * 8, 1);
+      } else {
+        grid = tile_grid(static_cast<int64_t>(tiles) * c.parts, 1);
+      }
     } else {
-      const int of_stage = stage_bytes(c.mt) / kUnit;
+      constexpr int of_stage = kTileStage / kUnit;
       p.stages = ((p.units + of_stage - 1) / of_stage + c.parts - 1) / c.parts;
       p.m_tiles = (p.m + 16 * c.mt - 1) / (16 * c.mt), p.n_tiles = (p.n + 16 * waves * c.nt - 1) / (16 * waves * c.nt);
       grid = tile_grid(static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.parts, 1);
@@ -522,11 +569,11 @@ void launch(Linear p, const Cut &c, hipStream_t s) {
     return 0;
   });
   if (c.parts == 1) return;
-  const int64_t all = static_cast<int64_t>(p.m) * p.n;
-  if (p.wide >= 4)
-    linear_fold<E, 4><<<tile_grid((all / 4 + 255) / 256, 1), 256, 0, s>>>(p);
-  else
-    linear_fold<E, 1><<<tile_grid((all + 255) / 256, 1), 256, 0, s>>>(p);
+  linear_fold<E><<<tile_grid((static_cast<int64_t>(p.m) * p.pitch / 4 + 255) / 256, 1), 256, 0, s>>>(p);
+}
+
+size_t sums_bytes(const Cut &c, int64_t m, int64_t n) {
+  return c.parts > 1 ? static_cast<size_t>(c.parts) * m * ((n + 3) / 4 * 4) * sizeof(int32_t) : 0;
 }
 
 int check(int64_t m, int64_t n, int64_t k) {
@@ -559,8 +606,7 @@ extern "C" int intent_hip_linear_i8_workspace_bytes(int64_t m, int64_t n, int64_
   *bytes = 0;
   if (int rc = check(m, n, k)) return rc;
   if (m == 0 || n == 0) return INTENT_HIP_OK;
-  const Cut c = cut(m, n, k);
-  if (c.parts > 1) *bytes = static_cast<size_t>(c.parts) * m * n * sizeof(int32_t);
+  *bytes = sums_bytes(cut(m, n, k), m, n);
   return INTENT_HIP_OK;
 }
 
@@ -582,11 +628,11 @@ extern "C" int intent_hip_linear_i8(int dtype, const int8_t *x, const int8_t *we
   Linear p{};
   p.x = x, p.w = weight, p.xs = x_scales, p.ws = weight_scales, p.bias = bias, p.y = static_cast<uint16_t *>(y);
   p.ldx = ldx, p.ldw = ldw, p.ldy = ldy;
-  p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.units = static_cast<int>(k / kUnit);
+  p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.pitch = (p.n + 3) / 4 * 4, p.units = static_cast<int>(k / kUnit);
   p.wide = n % 8 == 0 && ldy % 8 == 0 && aligned(y, 16) ? 8 : n % 4 == 0 && ldy % 4 == 0 && aligned(y, 8) ? 4 : 1;
   const Cut c = cut(m, n, k);
   if (c.parts > 1) {
-    const size_t bytes = static_cast<size_t>(c.parts) * m * n * sizeof(int32_t);
+    const size_t bytes = sums_bytes(c, m, n);
     if (workspace == nullptr || workspace_bytes < bytes || !aligned(workspace, 16))
       return fail(INTENT_HIP_ERR_WORKSPACE, "linear_i8 needs %zu workspace bytes, 16-byte aligned", bytes);
     p.sums = static_cast<int32_t *>(workspace);
