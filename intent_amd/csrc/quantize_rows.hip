@@ -43,10 +43,10 @@ __global__ __launch_bounds__(W *kWave) void quantize_rows(Quantize p) {
   uint32_t most[1] = {0};
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    widen_piece<E>(x[j], a[j]);
+    widen_piece<E>(settled(x[j], at, j), a[j]);
     if constexpr (kGated) {
       float u[kPiece];
-      widen_piece<E>(up[j], u);
+      widen_piece<E>(settled(up[j], at, j), u);
 #pragma unroll
       for (int i = 0; i < kPiece; ++i) a[j][i] = a[j][i] * __builtin_amdgcn_rcpf(1.0f + __expf(-a[j][i])) * u[i];
     }

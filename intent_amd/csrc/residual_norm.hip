@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kWaveRows = 4;           // rows of a workgroup where a wave holds a row
 constexpr int kFoldParts = 64;
+constexpr int kBackwardWaves = 8;      // of a workgroup of the backward, but for rows that take more
 
 struct Norm {
   const uint16_t *block, *residual;    // backward: residual is the stored sum
@@ -62,6 +63,8 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_rows(Norm p) {
   float w[P][kPiece], h[P][kPiece];
 #pragma unroll
   for (int j = 0; j < P; ++j) load_weights(p.weight, at, j, w[j]);
+#pragma unroll
+  for (int j = 0; j < P; ++j) block[j] = settled(block[j], at, j), residual[j] = settled(residual[j], at, j);
   float r = 1.0f;
   if constexpr (kPost) {
     float sum[1] = {0.0f};
@@ -118,19 +121,24 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_rows(Norm p) {
   }
 }
 
-// Rows walk over the slots (a workgroup, or a wave where a wave holds a row); a slot keeps its share of the weights' gradients in
-// registers until its end. The rows of the next token are on their way while this one's sums are formed, where registers allow.
+// A workgroup takes `rows` tokens at a time, and keeps its share of the weights' gradients in registers until its end. The rows of the
+// next tokens are on their way while these ones' sums are formed, where registers allow.
 template <typename E, int P, int W, bool kPieces, bool kPost>
 __global__ __launch_bounds__(W *kWave) void residual_norm_backward_rows(Norm p) {
   __shared__ RowSlots<3> first[2];
   __shared__ RowSlots<1> second[2];
-  const int64_t slot = p.waves == 1 ? static_cast<int64_t>(blockIdx.x) * kWaveRows + (threadIdx.x >> 6) : blockIdx.x;
-  if (slot >= p.slots) return;
-  const RowPlace<kPieces> at{p.d, p.waves * kWave, static_cast<int>(p.waves == 1 ? threadIdx.x & 63 : threadIdx.x)};
+  constexpr int kWeights = kPost ? 2 : 1;
+  constexpr bool kShared = W == kBackwardWaves;      // by several rows
+  __shared__ float4 shares[kShared ? kWeights * P * W * kWave * kPiece / 4 : 1];     // [row][weight, post][d]
+  const int row = kShared ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / p.waves : 0, row_wave = row * p.waves;
+  const int rows = kShared ? static_cast<int>(blockDim.x) / (p.waves * kWave) : 1, thread = static_cast<int>(threadIdx.x) - row_wave * kWave;
   struct Rows {
     uint4 x, h, gh, gy;
   };
+  // Behind the last token: rows without elements.
+  const auto place = [&](int64_t token) { return RowPlace<kPieces>{!kShared || token < p.tokens ? p.d : 0, p.waves * kWave, thread}; };
   const auto load = [&](int64_t token, Rows (&to)[P]) {
+    const auto at = place(token);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       to[j].h = load_piece(p.residual + token * p.rs, at, j);
@@ -140,20 +148,27 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_backward_rows(Norm p) 
     }
   };
   float dw[P][kPiece] = {}, dwp[P][kPiece] = {};
-  constexpr bool kAhead = kPieces && W <= 8;
+  constexpr bool kAhead = P == 1;
   Rows next[P];
-  if constexpr (kAhead) load(slot, next);
+  int64_t at_once = static_cast<int64_t>(blockIdx.x) * rows;
+  if constexpr (kAhead) load(at_once + row, next);
   int turn = 0;
-  for (int64_t token = slot; token < p.tokens; token += p.slots, turn ^= 1) {
+  for (; at_once < p.tokens; at_once += static_cast<int64_t>(p.slots) * rows, turn ^= 1) {
+    const int64_t token = at_once + row;
+    const auto at = place(token);
+    const bool live = !kShared || token < p.tokens;
     Rows now[P];
     if constexpr (kAhead) {
 #pragma unroll
       for (int j = 0; j < P; ++j) now[j] = next[j];
-      if (token + p.slots < p.tokens) load(token + p.slots, next);
+      if (at_once + static_cast<int64_t>(p.slots) * rows < p.tokens) load(token + static_cast<int64_t>(p.slots) * rows, next);
     } else {
       load(token, now);
     }
-    const float factor = gate_of(p, token);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      for (uint4 *v : {&now[j].x, &now[j].h, &now[j].gh, &now[j].gy}) *v = settled(*v, at, j);
+    const float factor = live ? gate_of(p, token) : 0.0f;
     float sums[3] = {0.0f, 0.0f, 0.0f};              // of h^2, gy w h, x^2
 #pragma unroll
     for (int j = 0; j < P; ++j) {
@@ -169,9 +184,9 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_backward_rows(Norm p) 
         if constexpr (kPost) sums[2] += x[i] * x[i];
       }
     }
-    row_reduce(sums, p.waves, first[turn]);
-    const float rh = rsqrtf(sums[0] * p.inverse_d + p.eps), along = sums[1] * rh * p.inverse_d;
-    const float rx = kPost ? rsqrtf(sums[2] * p.inverse_d + p.eps) : 1.0f;
+    row_reduce(sums, p.waves, first[turn], row_wave);
+    const float rh = live ? rsqrtf(sums[0] * p.inverse_d + p.eps) : 0.0f, along = sums[1] * rh * p.inverse_d;
+    const float rx = !live ? 0.0f : kPost ? rsqrtf(sums[2] * p.inverse_d + p.eps) : 1.0f;
     float dh[P][kPiece], inner[1] = {0.0f};          // sum of dh u
 #pragma unroll
     for (int j = 0; j < P; ++j) {
@@ -194,8 +209,8 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_backward_rows(Norm p) 
       store_piece(p.sum + token * p.ss, at, j, narrow_piece<E>(grad));
     }
     if (kPost || p.grad_gate != nullptr) {
-      row_reduce(inner, p.waves, second[turn]);
-      if (p.grad_gate != nullptr && at.thread == 0) p.grad_gate[token * p.ggs] = p.block_scale * inner[0];
+      row_reduce(inner, p.waves, second[turn], row_wave);
+      if (p.grad_gate != nullptr && live && thread == 0) p.grad_gate[token * p.ggs] = p.block_scale * inner[0];
     }
     const float back = factor * inner[0] * p.inverse_d;
 #pragma unroll
@@ -219,22 +234,20 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_backward_rows(Norm p) 
       store_piece(p.out + token * p.os, at, j, narrow_piece<E>(grad));
     }
   }
-  float *to = p.partial + slot * (kPost ? 2 : 1) * p.d;
+  const auto at = RowPlace<kPieces>{p.d, p.waves * kWave, thread};
+  float *const to = p.partial + static_cast<int64_t>(blockIdx.x) * kWeights * p.d;
+  float *const mine = rows == 1 ? to : reinterpret_cast<float *>(shares) + row * kWeights * p.d;
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    const auto keep = [&](float *row, const float (&v)[kPiece]) {
-      if constexpr (kPieces) {
-        if (!at.holds(j, 0)) return;
-        *reinterpret_cast<float4 *>(row + at.column(j, 0)) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4 *>(row + at.column(j, 0) + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPiece; ++i)
-          if (at.holds(j, i)) row[at.column(j, i)] = v[i];
-      }
-    };
-    keep(to, dw[j]);
-    if constexpr (kPost) keep(to + p.d, dwp[j]);
+    store_weights(mine, at, j, dw[j]);
+    if constexpr (kPost) store_weights(mine + p.d, at, j, dwp[j]);
+  }
+  if (rows == 1) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kWeights * p.d; i += blockDim.x) {
+    float total = 0.0f;
+    for (int r = 0; r < rows; ++r) total += reinterpret_cast<const float *>(shares)[r * kWeights * p.d + i];
+    to[i] = total;
   }
 }
 
@@ -263,12 +276,15 @@ struct Layout {
   int pieces, most;
 };
 Layout forward_layout(int64_t d) { return row_waves(d, 1) <= 4 ? Layout{1, 4} : Layout{2, 16}; }
-Layout backward_layout(int64_t d) { return row_waves(d, 1) <= 8 ? Layout{1, 8} : row_waves(d, 2) <= 8 ? Layout{2, 8} : Layout{2, 16}; }
+Layout backward_layout(int64_t d) { return row_waves(d, 1) <= 8 ? Layout{1, 8} : row_waves(d, 1) <= 16 ? Layout{1, 16} : Layout{2, 16}; }
 int layout_waves(int64_t d, Layout layout) { return std::max(1, row_waves(d, layout.pieces)); }
 
-// Slots of the backward: what keeps the chip busy, each with as many rows as that leaves.
+// Of the backward: tokens that a workgroup takes at a time, and workgroups, as many as there is room for: registers leave a SIMD four
+// waves, and a workgroup of five waves takes the room of eight (16384 x 2056 with three of them for a CU: 157 us, with two 123).
+int backward_rows(int64_t d) { return std::max(1, kBackwardWaves / layout_waves(d, backward_layout(d))); }
 int backward_slots(int64_t tokens, int64_t d) {
-  return static_cast<int>(std::min<int64_t>(tokens, int64_t{16} / layout_waves(d, backward_layout(d)) * device_cus()));
+  const int64_t rows = backward_rows(d);
+  return static_cast<int>(std::min<int64_t>((tokens + rows - 1) / rows, (backward_layout(d).most == kBackwardWaves ? 2 : 1) * int64_t{device_cus()}));
 }
 
 int check(const char *name, int dtype, int64_t tokens, int64_t d, int64_t gates, int64_t post) {
@@ -330,11 +346,12 @@ int with_backward(int dtype, int64_t d, bool in_pieces, bool post, F f) {
       const std::integral_constant<int, 2> two;
       const std::integral_constant<int, 8> eight;
       const std::integral_constant<int, 16> sixteen;
-      return layout.pieces == 1 ? of(one, eight) : layout.most == 8 ? of(two, eight) : of(two, sixteen);
+      return layout.most == 8 ? of(one, eight) : layout.pieces == 1 ? of(one, sixteen) : of(two, sixteen);
     });
   });
 }
 
+int backward_threads(int64_t d) { return layout_waves(d, backward_layout(d)) * backward_rows(d) * kWave; }
 unsigned row_threads(int waves) { return static_cast<unsigned>((waves == 1 ? kWaveRows : waves) * kWave); }
 
 }  // namespace
@@ -347,7 +364,7 @@ int residual_norm_resources(int dtype, int kind, int64_t d, int64_t post, uint64
   snprintf(name, sizeof(name), "residual_norm_%srows<%s,%d,%s,%s%s>", kind == 2 ? "backward_" : "", dtype == INTENT_HIP_F16 ? "f16" : "bf16", layout.pieces,
            whole ? "true" : "false", post ? "true" : "false", kind == 2 ? "" : kind == 1 ? ",true" : ",false");
   const auto describe = [&](void (*kernel)(Norm)) {
-    return describe_kernel(reinterpret_cast<const void *>(kernel), name, static_cast<int>(row_threads(layout_waves(d, layout))), out);
+    return describe_kernel(reinterpret_cast<const void *>(kernel), name, kind == 2 ? backward_threads(d) : static_cast<int>(row_threads(layout_waves(d, layout))), out);
   };
   return kind == 2 ? with_backward(dtype, d, whole, post != 0, describe) : with_forward(dtype, d, whole, post != 0, kind == 1, describe);
 }
@@ -424,7 +441,7 @@ extern "C" int intent_hip_residual_norm_backward(int dtype, const void *block, c
   if (d == 0 && gates == 0) return INTENT_HIP_OK;
   if ((d > 0 && grad_weight == nullptr) || (post > 0 && grad_post_weight == nullptr) || (gates > 0 && (gate == nullptr || grad_gate == nullptr)))
     return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null pointer");
-  const int slots = d > 0 ? backward_slots(tokens, d) : static_cast<int>(std::min<int64_t>(tokens, device_cus()));
+  const int slots = backward_slots(tokens, d);
   const int weights = post > 0 ? 2 : 1;
   const size_t bytes = static_cast<size_t>(slots) * weights * d * sizeof(float);
   if (slots > 0) {
@@ -447,9 +464,8 @@ extern "C" int intent_hip_residual_norm_backward(int dtype, const void *block, c
     p.waves = layout_waves(d, backward_layout(d)), p.slots = slots;
     const uint64_t wide = mixed_rows({block, sum, grad_sum, grad_output, grad_block, grad_residual, weight, post > 0 ? post_weight : nullptr},
                                      {p.bs, p.rs, p.gss, p.gos, p.os, p.ss}, tokens);
-    const int rows = p.waves == 1 ? kWaveRows : 1;
     with_backward(dtype, d, in_pieces(d, wide, 0), post > 0, [&](void (*kernel)(Norm)) {
-      kernel<<<static_cast<unsigned>((slots + rows - 1) / rows), row_threads(p.waves), 0, as_stream(stream)>>>(p);
+      kernel<<<static_cast<unsigned>(slots), static_cast<unsigned>(backward_threads(d)), 0, as_stream(stream)>>>(p);
       return 0;
     });
     if (hipPeekAtLastError() != hipSuccess) return launch_status("residual_norm_backward");

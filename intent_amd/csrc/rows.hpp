@@ -10,68 +10,115 @@ namespace intent_hip {
 constexpr int kPiece = 8;              // elements of a thread's piece
 constexpr int kMaxRowWaves = 16;
 
-// Where the elements of a row lie in its threads: piece j of thread i is 16 bytes at 8 (i + threads j), or, for rows that do not
-// come in aligned pieces, eight elements that lie `threads` apart, so that a wave still reads neighbours.
+// Pieces as they may lie in rows of any alignment: an access of 16 bytes may begin at any byte here.
+typedef uint32_t loose_x4_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t loose_x2_t __attribute__((ext_vector_type(2), aligned(1)));
+typedef float loose_f4_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// Where the elements of a row lie in its threads: piece j of thread i is eight elements from 8 (i + threads j) on. kPieces: pieces
+// begin at 16 bytes (8, of 8-bit integers) and each is whole or behind the row; otherwise the row's last piece goes by elements.
 template <bool kPieces>
 struct RowPlace {
   int d, threads, thread;
-  __device__ __forceinline__ int column(int j, int i) const {
-    return kPieces ? kPiece * (thread + threads * j) + i : thread + threads * (kPiece * j + i);
-  }
-  // Whether element i of piece j is of the row (of a 16-byte piece all are or none).
-  __device__ __forceinline__ bool holds(int j, int i) const { return column(j, kPieces ? 0 : i) < d; }
+  __device__ __forceinline__ int column(int j) const { return kPiece * (thread + threads * j); }
+  __device__ __forceinline__ bool holds(int j, int i) const { return column(j) + (kPieces ? 0 : i) < d; }
+  __device__ __forceinline__ bool whole(int j) const { return column(j) + (kPieces ? 0 : kPiece - 1) < d; }
 };
 
-// Eight elements as they lie in memory; 0 behind the row.
+// A piece on its way: of a row's last one that is not whole, the last eight elements of the row, so that every thread loads once and
+// none waits; `settled` is the piece itself, 0 behind the row.
 template <bool kPieces>
 __device__ __forceinline__ uint4 load_piece(const uint16_t *row, const RowPlace<kPieces> &at, int j) {
   if constexpr (kPieces) {
-    return at.holds(j, 0) ? *reinterpret_cast<const uint4 *>(row + at.column(j, 0)) : make_uint4(0, 0, 0, 0);
+    return at.whole(j) ? *reinterpret_cast<const uint4 *>(row + at.column(j)) : make_uint4(0, 0, 0, 0);
   } else {
-    uint32_t v[kPiece];
+    loose_x4_t v = {0, 0, 0, 0};
+    if (at.d >= kPiece) {
+      if (at.holds(j, 0)) v = *reinterpret_cast<const loose_x4_t *>(row + min(at.column(j), at.d - kPiece));
+    } else if (at.column(j) == 0) {
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) v[i] = at.holds(j, i) ? row[at.column(j, i)] : 0;
-    return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+      for (int i = 0; i < kPiece - 1; ++i)
+        if (i < at.d) v[i / 2] |= static_cast<uint32_t>(row[i]) << (16 * (i & 1));
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
 
 template <bool kPieces>
+__device__ __forceinline__ uint4 settled(uint4 v, const RowPlace<kPieces> &at, int j) {
+  if constexpr (!kPieces) {
+    const int by = at.column(j) - (at.d - kPiece);
+    if (at.d >= kPiece && by > 0 && by < kPiece) {
+      if (by & 1)
+        v = make_uint4(__builtin_amdgcn_alignbit(v.y, v.x, 16), __builtin_amdgcn_alignbit(v.z, v.y, 16), __builtin_amdgcn_alignbit(v.w, v.z, 16), v.w >> 16);
+      if (by & 2) v = make_uint4(v.y, v.z, v.w, 0);
+      if (by & 4) v = make_uint4(v.z, v.w, 0, 0);
+    }
+  }
+  return v;
+}
+
+template <bool kPieces>
 __device__ __forceinline__ void store_piece(uint16_t *row, const RowPlace<kPieces> &at, int j, uint4 v) {
+  row += at.column(j);
   if constexpr (kPieces) {
-    if (at.holds(j, 0)) *reinterpret_cast<uint4 *>(row + at.column(j, 0)) = v;
+    if (at.whole(j)) *reinterpret_cast<uint4 *>(row) = v;
   } else {
-    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+    const loose_x4_t words = {v.x, v.y, v.z, v.w};
+    if (at.whole(j)) {
+      *reinterpret_cast<loose_x4_t *>(row) = words;
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-      if (at.holds(j, i)) row[at.column(j, i)] = static_cast<uint16_t>(words[i / 2] >> (16 * (i & 1)));
+      for (int i = 0; i < kPiece - 1; ++i)
+        if (at.holds(j, i)) row[i] = static_cast<uint16_t>(words[i / 2] >> (16 * (i & 1)));
+    }
   }
 }
 
 template <bool kPieces>
 __device__ __forceinline__ void store_piece(int8_t *row, const RowPlace<kPieces> &at, int j, uint2 v) {
+  row += at.column(j);
   if constexpr (kPieces) {
-    if (at.holds(j, 0)) *reinterpret_cast<uint2 *>(row + at.column(j, 0)) = v;
+    if (at.whole(j)) *reinterpret_cast<uint2 *>(row) = v;
   } else {
-    const uint32_t words[2] = {v.x, v.y};
+    const loose_x2_t words = {v.x, v.y};
+    if (at.whole(j)) {
+      *reinterpret_cast<loose_x2_t *>(row) = words;
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-      if (at.holds(j, i)) row[at.column(j, i)] = static_cast<int8_t>(words[i / 4] >> (8 * (i & 3)));
+      for (int i = 0; i < kPiece - 1; ++i)
+        if (at.holds(j, i)) row[i] = static_cast<int8_t>(words[i / 4] >> (8 * (i & 3)));
+    }
   }
 }
 
-// The f32 weights of a piece; 0 behind the row.
+// The f32 weights of a piece; 0 behind the row. (Taken as the rows' pieces are, 16384 x 2049 took 71 us forward for 66.)
 template <bool kPieces>
 __device__ __forceinline__ void load_weights(const float *w, const RowPlace<kPieces> &at, int j, float (&out)[kPiece]) {
-  if constexpr (kPieces) {
-    float4 u = make_float4(0, 0, 0, 0), v = u;
-    if (at.holds(j, 0)) {
-      u = *reinterpret_cast<const float4 *>(w + at.column(j, 0));
-      v = *reinterpret_cast<const float4 *>(w + at.column(j, 0) + 4);
-    }
-    out[0] = u.x, out[1] = u.y, out[2] = u.z, out[3] = u.w, out[4] = v.x, out[5] = v.y, out[6] = v.z, out[7] = v.w;
-  } else {
+  w += at.column(j);
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) out[i] = at.holds(j, i) ? w[at.column(j, i)] : 0.0f;
+  for (int i = 0; i < kPiece; ++i) out[i] = 0.0f;
+  if (at.whole(j)) {
+    const loose_f4_t u = *reinterpret_cast<const loose_f4_t *>(w), v = *reinterpret_cast<const loose_f4_t *>(w + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = u[i], out[4 + i] = v[i];
+  } else if constexpr (!kPieces) {
+#pragma unroll
+    for (int i = 0; i < kPiece - 1; ++i)
+      if (at.holds(j, i)) out[i] = w[i];
+  }
+}
+
+template <bool kPieces>
+__device__ __forceinline__ void store_weights(float *w, const RowPlace<kPieces> &at, int j, const float (&v)[kPiece]) {
+  w += at.column(j);
+  if (at.whole(j)) {
+    const loose_f4_t a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+    *reinterpret_cast<loose_f4_t *>(w) = a, *reinterpret_cast<loose_f4_t *>(w + 4) = b;
+  } else if constexpr (!kPieces) {
+#pragma unroll
+    for (int i = 0; i < kPiece - 1; ++i)
+      if (at.holds(j, i)) w[i] = v[i];
   }
 }
 
@@ -137,8 +184,9 @@ __device__ __forceinline__ void row_reduce(float (&sums)[N], uint32_t (&most)[M]
   }
 }
 
+// first: the row's first wave, where a workgroup holds several rows.
 template <int N>
-__device__ __forceinline__ void row_reduce(float (&sums)[N], int waves, RowSlots<N> &slots) {
+__device__ __forceinline__ void row_reduce(float (&sums)[N], int waves, RowSlots<N> &slots, int first = 0) {
 #pragma unroll
   for (int i = 0; i < N; ++i) sums[i] = wave_sum(sums[i]);
   if (waves == 1) return;
@@ -149,7 +197,7 @@ __device__ __forceinline__ void row_reduce(float (&sums)[N], int waves, RowSlots
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) sums[i] = 0.0f;
-  for (int w = 0; w < waves; ++w)
+  for (int w = first; w < first + waves; ++w)
 #pragma unroll
     for (int i = 0; i < N; ++i) sums[i] += __uint_as_float(slots.v[w][i]);
 }
