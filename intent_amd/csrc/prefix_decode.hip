@@ -676,7 +676,7 @@ Cut cut(int64_t batch, int64_t kv_heads, int64_t group, int64_t ps, int64_t pref
   const int64_t own = positions * ps, aim = 4 * cus / std::max<int64_t>(kv_heads * c.head_tiles, 1);
   const int64_t of_job = std::max<int64_t>(256, (own + std::max<int64_t>(aim, 1) - 1) / std::max<int64_t>(aim, 1));
   c.job_pages = ps > 0 ? static_cast<int>(std::max<int64_t>(1, (of_job + ps - 1) / ps)) : 1;
-  c.jobs = static_cast<int>(positions / c.job_pages + batch);
+  c.jobs = static_cast<int>((ps > 0 ? positions / c.job_pages : 0) + batch);
   return c;
 }
 
@@ -710,9 +710,9 @@ int check(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t group, int64
                 static_cast<long long>(q_heads), static_cast<long long>(kv_heads), static_cast<long long>(group));
   if (d != 64 && d != 128)
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "paged_gqa_decode_prefix takes heads of 64 or 128 dimensions, got %lld", static_cast<long long>(d));
-  // Tokens of a table and rows of queries are counted in 32 bits, and so are blocks.
+  // Tokens of a table (to behind the last part of them) and rows of queries are counted in 32 bits, and so are blocks.
   if (batch > (1 << 20) || q_heads > (1 << 16) || pages > INT32_MAX || ps > (1 << 20) || prefix_positions > (1 << 28) || positions > (1 << 28) ||
-      prefix_positions * ps > INT32_MAX - 64 || positions * ps > (int64_t{1} << 40) || batch * q_heads > (1 << 28))
+      prefix_positions * ps > INT32_MAX - (1 << 20) || positions * ps > (int64_t{1} << 40) || batch * q_heads > (1 << 28))
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
   return INTENT_HIP_OK;
 }

@@ -114,7 +114,7 @@ int launch(const char *name, bool gated, int dtype, const void *x, const void *u
     if (s < 0) return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "negative stride");
   if (d > kMaxQuantRow)
     return fail(INTENT_HIP_ERR_UNSUPPORTED, "%s takes rows of up to %d elements, got %lld", name, kMaxQuantRow, static_cast<long long>(d));
-  if (rows > INT32_MAX) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
+  if (rows > (1 << 30)) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
   if (rows == 0) return INTENT_HIP_OK;
   if (scales == nullptr || (d > 0 && (x == nullptr || output == nullptr || (gated && up == nullptr))))
     return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "null pointer");

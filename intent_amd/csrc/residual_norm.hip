@@ -297,7 +297,7 @@ int check(const char *name, int dtype, int64_t tokens, int64_t d, int64_t gates,
     return fail(INTENT_HIP_ERR_INVALID_ARGUMENT, "a norm of the block has %lld weights, rows of %lld", static_cast<long long>(post),
                 static_cast<long long>(d));
   if (d > kMaxRow) return fail(INTENT_HIP_ERR_UNSUPPORTED, "%s takes rows of up to %d elements, got %lld", name, kMaxRow, static_cast<long long>(d));
-  if (tokens > INT32_MAX) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");
+  if (tokens > (1 << 30)) return fail(INTENT_HIP_ERR_UNSUPPORTED, "extents too large");        // blocks count in 32 bits
   return INTENT_HIP_OK;
 }
 
