@@ -243,7 +243,8 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, const uin
   constexpr int kIssued = 2 * kLoads;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Blocks of one part and key head follow each other: their rows' tiles read the same run.
+  // Jobs of one part and key head follow each other, on one XCD: their rows' tiles read the same run, which its L2 then holds (64
+  // sequences, a prefix of 16384, 64 heads on 8: 410 MB read where the workgroups of a run lay on four XCDs).
   const int tile = block % p.row_tiles, kh = block / p.row_tiles % p.kv_heads, part = block / p.row_tiles / p.kv_heads;
   const int rows = p.batch * p.group, q_heads = p.kv_heads * p.group;
   const int64_t held = p.pages > 0 ? static_cast<int64_t>(p.prefix_positions) * p.ps : 0;
@@ -566,12 +567,13 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_decode_jobs(Decode p) {
   static_assert(kSets * kStage * sizeof(uint4) >= kWaves * 16 * (D / 2) * sizeof(float) + kStage * sizeof(uint4), "the waves' states fit behind the first set");
   __shared__ uint4 lds[kSets * kStage];
   const int block = grid_block(), own_blocks = p.jobs * p.kv_heads * p.head_tiles;
-  const bool own = block >= p.prefix_blocks;
-  const int at = own ? block - p.prefix_blocks : block;
-  if (!own)
-    prefix_job<E, D, NQ, kTile>(p, at, p.k, p.v, lds);
-  else if (at < own_blocks)
+  const int first_own = (p.prefix_blocks + 7) / 8 * 8, at = block - first_own;
+  if (at < 0) {
+    const int job = xcd_tile(block, p.prefix_blocks);
+    if (job >= 0) prefix_job<E, D, NQ, kTile>(p, job, p.k, p.v, lds);
+  } else if (at < own_blocks) {
     own_job<E, D, kTile>(p, at, reinterpret_cast<float *>(lds + kStage), reinterpret_cast<float *>(lds));
+  }
 }
 
 // The states of a query head's parts of the prefix and of its sequence's jobs, joined: a workgroup per head, whose waves take a quarter
@@ -798,7 +800,7 @@ extern "C" int intent_hip_paged_gqa_decode_prefix(int dtype, const void *q, cons
   p.row_tiles = c.row_tiles, p.parts = c.parts, p.prefix_blocks = static_cast<int>(c.row_tiles * kv_heads * c.parts);
   p.head_tiles = c.head_tiles, p.job_pages = c.job_pages, p.jobs = c.jobs, p.scale = scale;
   p.sums = static_cast<float *>(workspace), p.peak = p.sums + states * d, p.total = p.peak + states;
-  const int64_t blocks = p.prefix_blocks + static_cast<int64_t>(c.jobs) * kv_heads * c.head_tiles;
+  const int64_t blocks = (static_cast<int64_t>(p.prefix_blocks) + 7) / 8 * 8 + static_cast<int64_t>(c.jobs) * kv_heads * c.head_tiles;
   const auto run = [&](void (*jobs)(Decode), void (*join)(Decode)) {
     jobs<<<tile_grid(blocks, 1), kThreads, 0, as_stream(stream)>>>(p);
     join<<<tile_grid(batch * q_heads, 1), kThreads, 0, as_stream(stream)>>>(p);
