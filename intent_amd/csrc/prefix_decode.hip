@@ -139,30 +139,41 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
   return v;
 }
 
-// The weights of 32 keys for 16 query rows, from their scores: key 16 t + 4 g + i of the step in s[t][i]. `live` keys count.
-template <typename E, int D>
-__device__ __forceinline__ void weigh(State<D> &state, const f32x4_t (&s)[2], float scale, int live, int g, uint4 (&weights)[kParts]) {
-  float z[8];
+// The weights of 32 keys for 16 query rows, from their scores: key 16 t + 4 g + i of the step in s[n][t][i], for NQ tiles of rows. First
+// the powers z of two that they are, of the keys of which `live` count: the base is looked at once for all tiles.
+template <typename E, int D, int NQ>
+__device__ __forceinline__ void powers(State<D> (&state)[NQ], const f32x4_t (&s)[NQ][2], float scale, int live, int g, float (&z)[NQ][8]) {
+  bool low = true;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = fmaf(s[i / 4][i % 4], scale, state.base);
-  const float half = largest(z[0], z[1], z[2]), rest = largest(z[3], z[4], z[5]), most = largest(half, rest, largest(z[6], z[7], z[7]));
+  for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[n][i] = fmaf(s[n][i / 4][i % 4], scale, state[n].base);
+    const float half = largest(z[n][0], z[n][1], z[n][2]), rest = largest(z[n][3], z[n][4], z[n][5]);
+    low = low && largest(half, rest, largest(z[n][6], z[n][7], z[n][7])) <= kRaise<E> + kSlack;
+  }
   // Also where no score of a lane is a number (a row without a base whose scores are -inf), and where not all keys count.
-  if (live < kStep || __builtin_amdgcn_ballot_w64(!(most <= kRaise<E> + kSlack))) {
+  if (live >= kStep && !__builtin_amdgcn_ballot_w64(!low)) return;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
     float largest = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      z[i] = i / 4 * 16 + g * 4 + i % 4 >= live ? -INFINITY : s[i / 4][i % 4] * scale;
-      largest = fmaxf(largest, z[i]);
+      z[n][i] = i / 4 * 16 + g * 4 + i % 4 >= live ? -INFINITY : s[n][i / 4][i % 4] * scale;
+      largest = fmaxf(largest, z[n][i]);
     }
-    const float base = fminf(state.base, kRaise<E> - largest_of_row(largest));      // +inf while every score is -inf
-    const float down = base == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - state.base);
-    state.base = base;
-    state.total *= down;
+    const float base = fminf(state[n].base, kRaise<E> - largest_of_row(largest));      // +inf while every score is -inf
+    const float down = base == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - state[n].base);
+    state[n].base = base;
+    state[n].total *= down;
 #pragma unroll
-    for (int j = 0; j < State<D>::C; ++j) state.sums[j] *= down;
+    for (int j = 0; j < State<D>::C; ++j) state[n].sums[j] *= down;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] += base == INFINITY ? 0.0f : base;
+    for (int i = 0; i < 8; ++i) z[n][i] += base == INFINITY ? 0.0f : base;
   }
+}
+
+template <typename E>
+__device__ __forceinline__ void weigh(const float (&z)[8], uint4 (&weights)[kParts]) {
   uint32_t words[4][kParts];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) rounded<E>(__builtin_amdgcn_exp2f(z[i]), __builtin_amdgcn_exp2f(z[i + 1]), words[i / 2]);
@@ -336,8 +347,8 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, const uin
           for (int n = 0; n < NQ; ++n) s[n][t] = mfma<E>(key[t][c], q[n][c], s[n][t]);
       }
       // Columns 16 j + r of keys 4 g .. 4 g + 3 of each tile: lane m of a group of 16 points at four columns of key m / 4, and lane i
-      // gets column i of all four. They are asked for two products ahead.
-      uint4 column[3];
+      // gets column i of all four.
+      uint4 column[C];
       const auto ask = [&](int j) {
         u32x2_t half[2];
 #pragma unroll
@@ -346,30 +357,33 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, const uin
           const uint16_t *at = reinterpret_cast<const uint16_t *>(values + row * kRowUnits + unit) + (r & 1) * 4;
           half[t] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t *)(at)));
         }
-        column[j % 3] = make_uint4(half[0][0], half[0][1], half[1][0], half[1][1]);
+        column[j] = make_uint4(half[0][0], half[0][1], half[1][0], half[1][1]);
       };
-      ask(0), ask(1);
+#pragma unroll
+      for (int j = 0; j < C; ++j) ask(j);
       uint4 weights[NQ][kParts];
-      const int live = last - first - step * kStep;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) weigh<E, D>(state[n], s[n], scale, live, g, weights[n]);
+      float z[NQ][8];
+      powers<E, D, NQ>(state, s, scale, last - first - step * kStep, g, z);
+      weigh<E>(z[0], weights[0]);
       __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+      for (int n = 0; n < NQ; ++n) {                   // the next tile's weights beside this one's products
+        if (n + 1 < NQ) weigh<E>(z[n + 1], weights[n + 1]);
 #pragma unroll
         for (int k = 0; k < kParts; ++k) state[n].total = mfma<E>(ones<E>(), weights[n][k], state[n].total);
 #pragma unroll
-      for (int j = 0; j < C; ++j) {
-        if (j + 2 < C) ask(j + 2);
+        for (int j = 0; j < C; ++j)
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+          for (int k = 0; k < kParts; ++k) state[n].sums[j] = mfma<E>(column[j], weights[n][k], state[n].sums[j]);
+        if (n + 1 < NQ) {
 #pragma unroll
-          for (int k = 0; k < kParts; ++k) state[n].sums[j] = mfma<E>(column[j % 3], weights[n][k], state[n].sums[j]);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);           // reads of the LDS, then products
-        __builtin_amdgcn_sched_group_barrier(0x008, NQ * kParts, 0);
+          for (int j = 0; j < (C + 1) * kParts; ++j) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, 4, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_s_setprio(0);
     }
     INTENT_WAIT_VMCNT(0);                              // nothing is on its way into the LDS of an ended workgroup
   }
@@ -432,7 +446,8 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
     if (wave == 0 && g == 0) p.total[at] = kNoToken;
     return;
   }
-  State<D> state;
+  State<D> of_row[1];
+  State<D> &state = of_row[0];
   state.clear();
   uint4 q[kChunks];
   {
@@ -503,13 +518,15 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
     next = after;
     if (t + kWaves < count) load_keys(next, t + kWaves, next_keys);
     after = find(t + 2 * kWaves);
-    f32x4_t s[2] = {f32x4_t{0, 0, 0, 0}, f32x4_t{0, 0, 0, 0}};
+    f32x4_t s[1][2] = {{f32x4_t{0, 0, 0, 0}, f32x4_t{0, 0, 0, 0}}};
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) s[half] = mfma<E>(keys[half][c], q[c], s[half]);
+      for (int c = 0; c < kChunks; ++c) s[0][half] = mfma<E>(keys[half][c], q[c], s[0][half]);
+    float z[1][8];
+    powers<E, D, 1>(of_row, s, scale, last - first - t * kStep, g, z);
     uint4 weights[kParts];
-    weigh<E, D>(state, s, scale, last - first - t * kStep, g, weights);
+    weigh<E>(z[0], weights);
 #pragma unroll
     for (int k = 0; k < kParts; ++k) state.total = mfma<E>(ones<E>(), weights[k], state.total);
 #pragma unroll
