@@ -5,7 +5,14 @@
 // once to f32 by each factor and the bias, and once to its type.
 //
 // Design. x [M, K] and w [N, K] both lie along K, as the matrix instructions take them. Products are formed transposed, weight rows as
-// rows, so that a lane ends with consecutive columns of one row of y.
+// rows, so that a lane ends with consecutive columns of one row of y. Few rows are bound by the weights' bytes, many by the matrix pipe.
+//   * linear_few, up to 16 rows: K over the 16 waves of a workgroup, weights and x straight to registers. 1 x 14336 x 4096 14.0 us (4.2
+//     TB/s), 1 x 4096 x 14336 12.7 (4.6), 16 rows 17.9 and 18.0: what a launch's start and end leave of a burst of two to four steps a wave.
+//   * linear_tiles, 64 or 128 x 128 results: x through the LDS, weights to registers, K over several workgroups. 32 x 4096 x 14336 20 us, of
+//     which the fold is 4; 128 x 14336 x 4096 30.5, 256 40.
+//   * linear_big, 256 or 128 x 256 results of four waves: both operands through the LDS. 4096 x 14336 x 4096 247 us, 8192^3 510 (2160
+//     TOP/s), 1024 x 14336 x 4096 73, 512 51; 1021 x 4096 x 14336 97, K in two parts, 11 of them the fold. At 4096 x 4096 x 14336 (2180
+//     TOP/s) the clock falls to 1.9 GHz under this load, which is what bounds it then.
 #include <stdio.h>
 
 #include <type_traits>
@@ -399,8 +406,7 @@ __device__ __forceinline__ void big_tile(const Linear &p, int m0, int n0, int pa
     }
     return;
   }
-  // The results of 32 rows go through the
-  // wave's own part of the LDS, from where whole rows of 128 are written (straight from registers, 8 bytes a lane and row with a load of
+  // The results of 32 rows go through the wave's own part of the LDS, from where whole rows of 128 are written (straight from registers, 8 bytes a lane and row with a load of
   // their scales: 39 us a tile, as long as K = 2700 takes).
   __syncthreads();
   constexpr int kRowUnits = 17;                        // 128 results and 16 bytes, so that rows lie in different banks
@@ -493,8 +499,10 @@ int big_full(int tiles, const Cut &c) {
 }
 constexpr int kTileWaves = 4, kTileStage = 128;
 
-// linear_few for up to 16 rows, NT by the weight rows there are for the workgroups. Otherwise by an estimate from what the tiles measured:
-// us a round of workgroups takes besides its stages, a stage (of 128 bytes of K) of a workgroup that has a CU for itself and of each of
+// linear_few for up to 16 rows (tiles: 4 x 14336 x 4096 19.5 us for 16.0, 16 rows 20.0 for 18.2, 16 x 4096 x 4096 10.5 for 7.9), NT = 2 where
+// that leaves a workgroup for three CUs in four at least (1 x 14336 x 4096 14.5 us, NT = 1 16.3; 1 x 4096 x 14336 19.3 and 12.8; 1 x 8192 x
+// 4096 9.5 and 10.0). Otherwise by an estimate from what the tiles measured:
+// us that a round of workgroups takes besides its stages, a stage (of 128 bytes of K) of a workgroup that has a CU for itself and of each of
 // several on a CU, and what writing, reading and adding the parts' sums takes. Large tiles have a CU each, whole ones and halves in rounds
 // of their own. Over M of 17 to 1024 and three N x K the choice was within a tenth of the best of all tiles and parts.
 Cut cut(int64_t m, int64_t n, int64_t k) {

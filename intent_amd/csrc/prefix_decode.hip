@@ -16,6 +16,10 @@
 // + 3 in lane (r, g), where the second product wants them: columns of the values as rows, 32 keys (4 of each 16 a lane) summed over. The
 // LDS gives those columns turned (ds_read_b64_tr_b16); from memory a lane reads D / 16 columns of its eight keys and pairs them with
 // v_perm. The peak is raised only when a score passes it by 2^4.
+// Measured: 64 sequences behind 16384 tokens, up to 1000 of their own, 64 heads on 8, bf16, 106.5 us; the prefix alone 80 (matrix pipe 33%
+// busy, vector pipe 25%: two waves a SIMD, each of whose steps waits for its own LDS reads, products and weights in turn; three waves
+// spilled), the own tokens alone 52 (2.7 TB/s), the join 13 of each; own jobs between those of the prefix instead of behind them 130. 8
+// sequences behind 8191 tokens, up to 512, 32 heads on 8, f16, 21.8 us, of which the join is 5.
 #include <stdio.h>
 
 #include <algorithm>
@@ -107,7 +111,8 @@ __device__ __forceinline__ void rounded(float a, float b, uint32_t (&part)[kPart
 
 // The state of 16 query rows, weights being exp2(score + base): lane (r, g) has row r's base (+inf before any score has counted), the sum
 // of its weights (in each of the four), and in sums[j][i] the weighted values of row 4 g + i of product j, C = D / 16 products: column 16
-// j + 4 g + i of the prefix's, whose values come through the LDS, column C (4 g + i) + j of a sequence's own. The sum is a product with ones, so it is of the weights as the values met them.
+// j + 4 g + i of the prefix's, whose values come through the LDS, column C (4 g + i) + j of a sequence's own. The sum is a product with
+// ones, so it is of the weights as the values met them.
 template <int D>
 struct State {
   static constexpr int C = D / 16;
@@ -202,8 +207,8 @@ __device__ __forceinline__ int physical(const Decode &p, const int32_t *table, i
   return static_cast<int>(min<int64_t>(max(page, 0), p.pages - 1));
 }
 
-// The page of an entry that is the wave's (clamped to `entries`, if any), as the table has it, through the scalar cache: a vector load here would be waited for together
-// with every load of keys and values before it.
+// The page of an entry that is the wave's (clamped to `entries`, if any), as the table has it, through the scalar cache: a vector load here
+// would be waited for together with every load of keys and values before it.
 typedef const __attribute__((address_space(4))) int32_t *table_t;
 __device__ __forceinline__ int page_of_wave(const int32_t *table, int entries, int at) {
   return ((table_t)(table))[entries > 0 ? min(max(at, 0), entries - 1) : at];
@@ -682,18 +687,22 @@ struct Cut {
   int nq, row_tiles, parts, head_tiles, job_pages, jobs;
 };
 
-Cut cut(int64_t batch, int64_t kv_heads, int64_t group, int64_t ps, int64_t prefix_positions, int64_t positions) {
+// NQ = 2 reads the LDS half as often, NQ = 1 leaves room for more waves: us with NQ = 1 and 2 of 32 rows for a key head and 128 dimensions
+// (8 sequences, 8191 + 512 tokens, 8 key heads) 23.5 and 26.8, of 64 (16 sequences) 28.1 and 31.9, of 512 (64 sequences, 16384 + 1000) 118 and
+// 108; of 64 dimensions, 128 rows 24.3 and 28.1, 512 rows 65.4 and 62.6. Parts of the prefix for three workgroups a CU in place of two: 25.7
+// for 23.8 (one sequence, 16384 tokens), 107.0 for 106.5.
+Cut cut(int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t prefix_positions, int64_t positions) {
   Cut c{};
   const int64_t rows = batch * group, cus = device_cus();
-  c.nq = rows <= 64 ? 1 : 2;
+  c.nq = rows <= (d == 64 ? 128 : 64) ? 1 : 2;
   c.row_tiles = static_cast<int>((rows + kWaves * 16 * c.nq - 1) / (kWaves * 16 * c.nq));
   const int64_t tokens = prefix_positions * ps, tiles = std::max<int64_t>(c.row_tiles * kv_heads, 1);
   const int64_t most = (tokens + 127) / 128;           // a part walks four steps at least
   c.parts = static_cast<int>(tokens == 0 ? 0 : std::max<int64_t>(1, std::min<int64_t>(most, 2 * cus / tiles)));
   c.head_tiles = static_cast<int>((group + 15) / 16);
-  // Jobs of about 256 tokens, longer where there are many.
-  const int64_t own = positions * ps, aim = 4 * cus / std::max<int64_t>(kv_heads * c.head_tiles, 1);
-  const int64_t of_job = std::max<int64_t>(256, (own + std::max<int64_t>(aim, 1) - 1) / std::max<int64_t>(aim, 1));
+  // Jobs of 128 tokens, of more where that makes over two a CU: the 8 sequences 21.8 us (256: 23.5, 512: 26.3), the 64 106.5 (256: 108.5).
+  const int64_t own = positions * ps, aim = 2 * cus / std::max<int64_t>(kv_heads * c.head_tiles, 1);
+  const int64_t of_job = std::max<int64_t>(128, (own + std::max<int64_t>(aim, 1) - 1) / std::max<int64_t>(aim, 1));
   c.job_pages = ps > 0 ? static_cast<int>(std::max<int64_t>(1, (of_job + ps - 1) / ps)) : 1;
   c.jobs = static_cast<int>((ps > 0 ? positions / c.job_pages : 0) + batch);
   return c;
@@ -741,7 +750,7 @@ int check(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t group, int64
 int prefix_decode_resources(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t prefix_positions,
                             int64_t positions, int64_t reach, IntentHipKernelResources *out) {
   if (int rc = check(batch, kv_heads * group, kv_heads, group, d, 1, ps, prefix_positions, positions)) return rc;
-  const Cut c = cut(batch, kv_heads, group, ps, prefix_positions, positions);
+  const Cut c = cut(batch, kv_heads, group, d, ps, prefix_positions, positions);
   const int tile = tile_of(ps, reach);
   char name[64];
   snprintf(name, sizeof(name), "prefix_decode_jobs<%s,%lld,%d,%d>", dtype == INTENT_HIP_F16 ? "f16" : "bf16", static_cast<long long>(d), c.nq, tile);
@@ -762,7 +771,7 @@ extern "C" int intent_hip_paged_gqa_decode_prefix_workspace_bytes(int64_t batch,
   *bytes = 0;
   if (int rc = check(batch, q_heads, kv_heads, head_group, d, 0, ps, prefix_positions, positions)) return rc;
   if (batch == 0 || q_heads == 0) return INTENT_HIP_OK;
-  *bytes = states_of(cut(batch, kv_heads, head_group, ps, prefix_positions, positions), batch, q_heads) * (d + 2) * sizeof(float);
+  *bytes = states_of(cut(batch, kv_heads, head_group, d, ps, prefix_positions, positions), batch, q_heads) * (d + 2) * sizeof(float);
   return INTENT_HIP_OK;
 }
 
@@ -797,7 +806,7 @@ extern "C" int intent_hip_paged_gqa_decode_prefix(int dtype, const void *q, cons
     }
   }
   if (mixed % 16) return fail(INTENT_HIP_ERR_UNSUPPORTED, "rows of q and of the caches must be 16-byte aligned, their strides multiples of 8");
-  const Cut c = cut(batch, kv_heads, head_group, ps, prefix_positions, positions);
+  const Cut c = cut(batch, kv_heads, head_group, d, ps, prefix_positions, positions);
   const size_t states = states_of(c, batch, q_heads), bytes = states * (d + 2) * sizeof(float);
   if (workspace == nullptr || workspace_bytes < bytes || !aligned(workspace, 16))
     return fail(INTENT_HIP_ERR_WORKSPACE, "paged_gqa_decode_prefix needs %zu workspace bytes, 16-byte aligned", bytes);

@@ -13,7 +13,10 @@
 // where the mean of du wp x r_x is block_scale gate S / D.
 //
 // Bound by the rows' bytes, so each is read and written once: a row stays in the registers of its threads, one or two pieces of 16
-// bytes each, 16384 elements in all.
+// bytes each, 16384 elements in all. Measured, bf16 with both norms and a gate, forward, 8-bit and backward: 16384 x 4096 100.5, 90, 184 us
+// (5.3, 5.2, 4.4 TB/s), 16384 x 1024 27, 29, 53, 8192 x 8192 103, 92, 184, 4096 x 16384 103, 96, 305 (the backward's rows no longer fit the
+// registers of 16 waves, and 140 bytes a lane go by memory), 8192 x 8191 133, 122, 263, whose rows begin anywhere (two bytes at a time: 334,
+// 324, 1003).
 #include <stdio.h>
 
 #include <algorithm>
@@ -275,6 +278,8 @@ __global__ __launch_bounds__(16 * kFoldParts) void residual_norm_fold(const floa
 struct Layout {
   int pieces, most;
 };
+// Forward: 16384 x 2048 takes 50.9 us in one piece a thread, 53.0 in two, and 16384 x 4096 99.7 in two, 97.1 in one (8-bit rows 90.2 and 91.8).
+// Backward: one piece leaves registers for the rows of the next token (8192 x 8192 184 us; two pieces of 8 waves 191).
 Layout forward_layout(int64_t d) { return row_waves(d, 1) <= 4 ? Layout{1, 4} : Layout{2, 16}; }
 Layout backward_layout(int64_t d) { return row_waves(d, 1) <= 8 ? Layout{1, 8} : row_waves(d, 1) <= 16 ? Layout{1, 16} : Layout{2, 16}; }
 int layout_waves(int64_t d, Layout layout) { return std::max(1, row_waves(d, layout.pieces)); }
