@@ -145,6 +145,55 @@ def test_many_tokens(device, tokens, d):
         close(got[i], value, size, "bf16" if i < 2 else "f32")
 
 
+@pytest.mark.parametrize("tokens,d", [(5000, 512), (2501, 1000), (9001, 72), (1301, 2049), (700, 8191), (300, 8201)])
+def test_workgroups_take_several_turns(device, tokens, d):
+    """More tokens than all workgroups of the backward take at a time, and a last turn that not all of them fill. A weight's sum goes
+    through a chain of 3 turns, 8 rows, 8 workgroups and a tree of 6 at most, 25 roundings, which the share (64 of them) holds."""
+    announce("residual_norm several turns", tokens, d)
+    given = case(tokens, "bf16", tokens, d, True, True)
+    on = [t.to(device) for t in given]
+    total, _ = kernel("residual_norm_bf16").run(*on[:5], *NUMBERS)
+    run = kernel("residual_norm_backward_bf16")
+    got = run.run(on[0], total, *on[2:], *NUMBERS)
+    for a, b in zip(got, run.run(on[0], total, *on[2:], *NUMBERS)):
+        assert torch.equal(a, b)
+    for i, (value, size) in enumerate(plain_backward(given[0], total.cpu(), *given[2:])):
+        close(got[i], value, size, "bf16" if i < 2 else "f32")
+
+
+@pytest.mark.parametrize("tokens,d", [(1, 64), (5, 64), (3, 520), (9, 7)])
+def test_no_epsilon(device, tokens, d):
+    """Without an epsilon the rows behind the last token, which workgroups of several rows have, must not become NaN."""
+    announce("residual_norm no epsilon", tokens, d)
+    numbers = (*NUMBERS[:2], 0.0)
+    given = case(tokens, "f16", tokens, d, True, True)
+    on = [t.to(device) for t in given]
+    total, _ = kernel("residual_norm_f16").run(*on[:5], *numbers)
+    got = kernel("residual_norm_backward_f16").run(on[0], total, *on[2:], *numbers)
+    for i, (value, size) in enumerate(plain_backward(given[0], total.cpu(), *given[2:], numbers)):
+        close(got[i], value, size, "f16" if i < 2 else "f32")
+
+
+@pytest.mark.parametrize("d", [9, 255, 4095])
+def test_in_place_rows_of_any_alignment(device, d):
+    """Rows whose last piece is read together with elements of the piece before it, which another thread may have written by then."""
+    announce("residual_norm in place, any alignment", d)
+    for post in (False, True):
+        given = [t.to(device) for t in case(d, "bf16", 300, d, True, post)]
+        forward_run, back = kernel("residual_norm_bf16"), kernel("residual_norm_backward_bf16")
+        want = forward_run.run(*given[:5], *NUMBERS)
+        block, stream = given[0].clone(), given[1].clone()
+        forward_run(block, stream, *given[2:5], stream, block, *NUMBERS)
+        assert torch.equal(stream, want[0]) and torch.equal(block, want[1])
+        rows = (given[0], want[0], *given[2:])
+        want = back.run(*rows, *NUMBERS)
+        block, grad_sum = given[0].clone(), given[5].clone()
+        rest = [torch.empty_like(t) for t in want[2:]]
+        back(block, rows[1], *given[2:5], grad_sum, given[6], block, grad_sum, *rest, *NUMBERS)
+        for a, b in zip((block, grad_sum, *rest), want):
+            assert torch.equal(a, b)
+
+
 def test_gradients_against_differences(device):
     """Along random directions, the gradients give the change of sum(sum * grad_sum + output * grad_output) that the 64-bit forward has
     between x - s v and x + s v: a central difference, off by s^2 times a third derivative. The backward is given the sum as it is stored,
