@@ -16,9 +16,9 @@
 // + 3 in lane (r, g), where the second product wants them: columns of the values as rows, 32 keys (4 of each 16 a lane) summed over. The
 // LDS gives those columns turned (ds_read_b64_tr_b16); from memory a lane reads D / 16 columns of its eight keys and pairs them with
 // v_perm. The peak is raised only when a score passes it by 2^4.
-// Measured: 64 sequences behind 16384 tokens, up to 1000 of their own, 64 heads on 8, bf16, 106.5 us; the prefix alone 80 (matrix pipe 33%
+// Measured: 64 sequences behind 16384 tokens, up to 1000 of their own, 64 heads on 8, bf16, 105.5 us; the prefix alone 80 (matrix pipe 33%
 // busy, vector pipe 25%: two waves a SIMD, each of whose steps waits for its own LDS reads, products and weights in turn; three waves
-// spilled), the own tokens alone 52 (2.7 TB/s), the join 13 of each; own jobs between those of the prefix instead of behind them 130. 8
+// spilled), the own tokens alone 52 (2.7 TB/s), the join 12 of each; own jobs between those of the prefix instead of behind them 130. 8
 // sequences behind 8191 tokens, up to 512, 32 heads on 8, f16, 21.8 us, of which the join is 5.
 #include <stdio.h>
 
