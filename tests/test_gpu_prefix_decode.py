@@ -68,6 +68,16 @@ def test_flat_and_sharp_weights(device, dtype, size):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [0.0, 1.0, 20.0])
+@pytest.mark.parametrize("prefix,lengths,heads,kv_heads,d,ps", [
+    (300, [9] * 40, 16, 2, 64, 8), (200, [5, 0] * 15, 8, 1, 128, 20), (270, [33] * 20, 8, 1, 64, 32), (600, [50, 1] * 10, 32, 4, 128, 16)])
+def test_two_tiles_of_rows(device, dtype, size, prefix, lengths, heads, kv_heads, d, ps):
+    """So many query rows for a key head that a wave takes two tiles of them, whose peaks rise apart from each other."""
+    announce("decode behind a prefix, two tiles", dtype, size, prefix, len(lengths), d, ps)
+    check(device, dtype, case(6, dtype, prefix, lengths, heads, kv_heads, d, ps, size=size))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("bits", [10, 20, 30])
 def test_one_key_outweighs(device, dtype, bits):
     """The first key outweighs every other by 2^bits and has a value of 0, so the output is what the others add."""
