@@ -157,6 +157,17 @@ def test_every_tile(device, m, n, k):
     check(kernel("linear_i8_bf16").run(*(t.to(device) for t in given)), *given, "bf16")
 
 
+@pytest.mark.parametrize("dtype,m,n,k", [
+    ("f16", 1466, 775, 25120), ("bf16", 473, 5273, 4992), ("f16", 6285, 263, 11456), ("bf16", 142, 18518, 7168), ("f16", 954, 5812, 6160),
+    ("bf16", 1834, 329, 6976), ("f16", 82, 2834, 2256), ("bf16", 385, 12290, 4112), ("f16", 2866, 6617, 1104)])
+def test_parts_of_k_and_partial_tiles(device, dtype, m, n, k):
+    """K divided over each kind of tile, rows of sums that are not whole fours, last parts that are shorter than the others, rounds of
+    whole and halved tiles."""
+    announce("linear i8 parts", dtype, m, n, k)
+    given = case(m + n + k, m, n, k, m % 2 == 0)
+    check(kernel("linear_i8_" + dtype).run(*(t.to(device) for t in given)), *given, dtype)
+
+
 @pytest.mark.parametrize("m", [1, 9, 40, 300])
 def test_largest_sums(device, m):
     """Every element -128 at the largest K: sums just below 2^31."""
