@@ -76,6 +76,9 @@ __device__ __forceinline__ void stage_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// What keys behind the last token have as values: a weight of 0 times that token's own, were it infinite, would not be 0.
+__device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
+
 template <typename E>
 __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
   if constexpr (std::is_same_v<E, f16_t>)
@@ -307,20 +310,25 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, const uin
     }
     const auto issue = [&](int t, int set) {           // step t (the last again behind it)
       uint4 *stage = lds + set * 2 * kUnits;
+      const int begin = first + min(t, count - 1) * kStep;
+      const uint16_t *const zeros = reinterpret_cast<const uint16_t *>(&kZeroUnit);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const uint16_t *k, *v;
         if constexpr (kTile > 0) {
-          uint32_t to_key = near_key[i], to_value = near_value[i];
-          if (next[i].most < T - 1) {
+          k = next[i].rows(p, keys_of, 0), v = next[i].rows(p, values_of, 1);
+          if (next[i].most < T - 1) {                  // a tile that not all of counts: the last row again, as values zeros
             const uint32_t row = min(row_of[i] % T, next[i].most);
-            to_key = row * p.of_token[0] + unit_of[i] * 2, to_value = row * p.of_token[1] + unit_of[i] * 2;
+            k += (row * p.of_token[0] + unit_of[i] * 2) / 2;
+            v = begin + row_of[i] < last ? v + (row * p.of_token[1] + unit_of[i] * 2) / 2 : zeros;
+          } else {
+            k += near_key[i] / 2, v += near_value[i] / 2;
           }
-          k = next[i].rows(p, keys_of, 0) + to_key / 2, v = next[i].rows(p, values_of, 1) + to_value / 2;
         } else {
-          const int token = min(first + min(t, count - 1) * kStep + row_of[i], last - 1), entry = page_of(p, token);
+          const int token = min(begin + row_of[i], last - 1), entry = page_of(p, token);
           const int page = physical(p, p.prefix, p.prefix_positions, entry), in = token - entry * p.ps;
-          k = keys_of + page * p.ks[0] + in * p.ks[1] + unit_of[i], v = values_of + page * p.vs[0] + in * p.vs[1] + unit_of[i];
+          k = keys_of + page * p.ks[0] + in * p.ks[1] + unit_of[i];
+          v = begin + row_of[i] < last ? values_of + page * p.vs[0] + in * p.vs[1] + unit_of[i] : zeros;
         }
         __builtin_amdgcn_global_load_lds(k, (lds_void_t *)(stage + (i * kWaves + wave) * kWave), 16, 0, 0);
         __builtin_amdgcn_global_load_lds(v, (lds_void_t *)(stage + kUnits + (i * kWaves + wave) * kWave), 16, 0, 0);
@@ -529,9 +537,16 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) s[0][half] = mfma<E>(keys[half][c], q[c], s[0][half]);
     float z[1][8];
-    powers<E, D, 1>(of_row, s, scale, last - first - t * kStep, g, z);
+    const int live = last - first - t * kStep;
+    powers<E, D, 1>(of_row, s, scale, live, g, z);
     uint4 weights[kParts];
     weigh<E>(z[0], weights);
+    if (live < kStep) {                                // values of keys behind the last token: zeros
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < C / 2; ++c) values[i][c] = i / 4 * 16 + g * 4 + i % 4 < live ? values[i][c] : 0;
+    }
 #pragma unroll
     for (int k = 0; k < kParts; ++k) state.total = mfma<E>(ones<E>(), weights[k], state.total);
 #pragma unroll
