@@ -94,7 +94,7 @@ constexpr float kRaise = std::is_same_v<E, f16_t> ? 11.0f : 0.0f;
 
 // Two weights as kParts numbers each. No part of a weight that counts is 0, so that an infinite value gives an infinity and not 0 times
 // it: of f16 the first number is cut off below the weight, which leaves a second of 2^-10 of it at least (for weights from 2^-25 of the
-// largest on); of bf16 a second number of 0 becomes 2^-126.
+// largest on); of bf16 a second number of 0 becomes 2^-126, unless the first is 0 too: a weight of 0 stays 0.
 template <typename E>
 __device__ __forceinline__ void rounded(float a, float b, uint32_t (&part)[kParts]) {
   if constexpr (std::is_same_v<E, f16_t>) {
@@ -108,7 +108,8 @@ __device__ __forceinline__ void rounded(float a, float b, uint32_t (&part)[kPart
     const float rest_a = a - __uint_as_float(u & 0xFFFF0000u), rest_b = b - __uint_as_float(v & 0xFFFF0000u);
     const bf16x2_t low = __builtin_convertvector(f32x2_t{rest_a, rest_b}, bf16x2_t);
     part[0] = __builtin_amdgcn_perm(v, u, 0x07060302);
-    part[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, low), u16x2_t{0x0080, 0x0080}));
+    const u16x2_t least = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, part[0]), u16x2_t{0x0080, 0x0080});
+    part[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, low), least));
   }
 }
 

@@ -35,3 +35,26 @@ def test_infinite_last_value(device, dtype, prefix, lengths, heads, kv_heads, d,
             keep = torch.ones(got.shape, dtype=torch.bool, device=device)
             keep[sequences, :group, :3] = False
             assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_no_score_is_a_number_above_minus_infinity(device, dtype):
+    """A row all of whose scores are -inf has no attention: exp(-inf + inf) is not a number. Where only the prefix or only its own tokens are
+    so, the others count alone."""
+    announce("decode behind a prefix, all scores -inf", dtype)
+    given = list(case(8, dtype, 45, [40, 3, 0], 8, 2, 128, 16))
+    given[0][:, :4] = given[0][:, :4].abs() + 0.5
+    shared, own = given[3].long(), given[6].long()
+    everywhere, in_prefix, in_own = (given[1].clone() for _ in range(3))
+    everywhere[:, :, 0] = float("-inf")
+    in_prefix[shared, :, 0] = float("-inf")
+    in_own[own, :, 0] = float("-inf")
+    want = run(device, dtype, given)
+    got = run(device, dtype, [given[0], everywhere, *given[2:]])
+    assert got[:, :4].isnan().all() and torch.equal(got[:, 4:], want[:, 4:])
+    got = run(device, dtype, [given[0], in_prefix, *given[2:]])
+    alone = run(device, dtype, [*given[:4], torch.zeros_like(given[4]), *given[5:]])
+    assert torch.equal(got[:2, :4], alone[:2, :4]) and got[2, :4].isnan().all()
+    got = run(device, dtype, [given[0], in_own, *given[2:]])
+    alone = run(device, dtype, [*given[:7], torch.zeros_like(given[7]), given[8]])
+    assert torch.equal(got[:, :4], alone[:, :4])
