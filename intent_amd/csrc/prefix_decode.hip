@@ -3,9 +3,8 @@
 //
 // For query head h of sequence s, over the prefix's tokens and the sequence's own:
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = exp2(scale * log2(e) * (q . k_j) - peak)        0 where there is no token
-// Products are summed in f32. Weights enter the second product as two numbers of the queries' type each: two of f16 hold 21 bits, at 2^11
-// times their share of the largest, which leaves out no more than 2^-36 of that; two of bf16 hold 16. The sum that divides is of the
-// weights as they were rounded, so a rounding moves a weight and no more.
+// Products are summed in f32. Weights are f32 and enter the second product whole, as three numbers of the queries' type each, but for what
+// f16 leaves below 2^-35 of the largest.
 //
 // Design. One launch does two kinds of jobs, whose states (peak, sum of weights, weighted sum of values) a second kernel joins:
 //   * the prefix: the query heads of all sequences that share a key head are the rows of one product, so the prefix is read once for 64
@@ -87,59 +86,61 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-constexpr int kParts = 2;              // numbers of a weight
+constexpr int kParts = 3;              // numbers of a weight
 // Weights are held at this power of two (times 2^kSlack they stay below the largest f16).
 template <typename E>
 constexpr float kRaise = std::is_same_v<E, f16_t> ? 11.0f : 0.0f;
 
-// Two weights as kParts numbers each. No part of a weight that counts is 0, so that an infinite value gives an infinity and not 0 times
-// it: of f16 the first number is cut off below the weight, which leaves a second of 2^-10 of it at least (for weights from 2^-25 of the
-// largest on); of bf16 a second number of 0 becomes 2^-126, unless the first is 0 too: a weight of 0 stays 0.
+// Two weights as kParts numbers each, every one what those before it leave, cut off: three of bf16 hold all 24 bits of a weight, and so do
+// three of f16 down to f16's last, 2^-24, which is 2^-35 of the largest weight. No number of a weight that counts is 0, so that an infinite
+// value gives an infinity and not 0 times it: where the first is not 0, the others are the least of their type at least (f16 2^-24, bf16
+// 2^-126).
 template <typename E>
 __device__ __forceinline__ void rounded(float a, float b, uint32_t (&part)[kParts]) {
-  if constexpr (std::is_same_v<E, f16_t>) {
-    constexpr float kBelow = 1.0f - 0x1p-10f;
-    const f16x2_t high = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_cvt_pkrtz(a * kBelow, b * kBelow));
-    const f16x2_t low = __builtin_convertvector(f32x2_t{a - static_cast<float>(high[0]), b - static_cast<float>(high[1])}, f16x2_t);
-    part[0] = __builtin_bit_cast(uint32_t, high), part[1] = __builtin_bit_cast(uint32_t, low);
-  } else {
-    // The first 8 bits cut off, the rest rounded to 8.
-    const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
-    const float rest_a = a - __uint_as_float(u & 0xFFFF0000u), rest_b = b - __uint_as_float(v & 0xFFFF0000u);
-    const bf16x2_t low = __builtin_convertvector(f32x2_t{rest_a, rest_b}, bf16x2_t);
-    part[0] = __builtin_amdgcn_perm(v, u, 0x07060302);
-    const u16x2_t least = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, part[0]), u16x2_t{0x0080, 0x0080});
-    part[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, low), least));
+  constexpr bool kHalf = std::is_same_v<E, f16_t>;
+  constexpr unsigned short kLeast = kHalf ? 0x0001 : 0x0080;
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    if constexpr (kHalf) {
+      const f16x2_t h = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+      part[i] = __builtin_bit_cast(uint32_t, h);
+      a = fmaf(static_cast<float>(h[0]), -1.0f, a), b = fmaf(static_cast<float>(h[1]), -1.0f, b);
+    } else {
+      const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
+      part[i] = __builtin_amdgcn_perm(v, u, 0x07060302);
+      a -= __uint_as_float(u & 0xFFFF0000u), b -= __uint_as_float(v & 0xFFFF0000u);
+    }
   }
+  const u16x2_t least = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, part[0]), u16x2_t{kLeast, kLeast});
+#pragma unroll
+  for (int i = 1; i < kParts; ++i)
+    part[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, part[i]), least));
 }
 
 // The state of 16 query rows, weights being exp2(score + base): lane (r, g) has row r's base (+inf before any score has counted), the sum
-// of its weights (in each of the four), and in sums[j][i] the weighted values of row 4 g + i of product j, C = D / 16 products: column 16
-// j + 4 g + i of the prefix's, whose values come through the LDS, column C (4 g + i) + j of a sequence's own. The sum is a product with
-// ones, so it is of the weights as the values met them.
+// of the weights that it formed (a quarter of the row's), and in sums[j][i] the weighted values of row 4 g + i of product j, C = D / 16
+// products: column 16 j + 4 g + i of the prefix's, whose values come through the LDS, column C (4 g + i) + j of a sequence's own.
 template <int D>
 struct State {
   static constexpr int C = D / 16;
-  float base;
-  f32x4_t total, sums[C];
+  float base, total;
+  f32x4_t sums[C];
   __device__ __forceinline__ void clear() {
-    base = INFINITY, total = f32x4_t{0, 0, 0, 0};
+    base = INFINITY, total = 0.0f;
 #pragma unroll
     for (int j = 0; j < C; ++j) sums[j] = f32x4_t{0, 0, 0, 0};
   }
 };
 
-// Eight ones.
-template <typename E>
-__device__ __forceinline__ uint4 ones() {
-  constexpr uint32_t two = std::is_same_v<E, f16_t> ? 0x3C003C00u : 0x3F803F80u;
-  return make_uint4(two, two, two, two);
-}
-
 // Largest over the four lanes of a query row.
 __device__ __forceinline__ float largest_of_row(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
   return fmaxf(v, __shfl_xor(v, 32));
+}
+
+__device__ __forceinline__ float sum_of_row(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
 }
 
 __device__ __forceinline__ float largest(float a, float b, float c) {
@@ -181,11 +182,16 @@ __device__ __forceinline__ void powers(State<D> (&state)[NQ], const f32x4_t (&s)
   }
 }
 
+// The weights as the second product takes them; their sum is added to `total`.
 template <typename E>
-__device__ __forceinline__ void weigh(const float (&z)[8], uint4 (&weights)[kParts]) {
+__device__ __forceinline__ void weigh(const float (&z)[8], uint4 (&weights)[kParts], float &total) {
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(z[i]);
+  total += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   uint32_t words[4][kParts];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) rounded<E>(__builtin_amdgcn_exp2f(z[i]), __builtin_amdgcn_exp2f(z[i + 1]), words[i / 2]);
+  for (int i = 0; i < 4; ++i) rounded<E>(w[2 * i], w[2 * i + 1], words[i]);
 #pragma unroll
   for (int n = 0; n < kParts; ++n) weights[n] = make_uint4(words[0][n], words[1][n], words[2][n], words[3][n]);
 }
@@ -248,7 +254,8 @@ __device__ __forceinline__ int place(int row) {
 template <int D>
 __device__ __forceinline__ void keep(const Decode &p, const State<D> &state, int64_t at, int g, bool any) {
   constexpr int C = D / 16;
-  if (g == 0) p.peak[at] = -state.base, p.total[at] = any ? state.total[0] : kNoToken;
+  const float total = sum_of_row(state.total);
+  if (g == 0) p.peak[at] = -state.base, p.total[at] = any ? total : kNoToken;
   if (!any) return;
   float *to = p.sums + at * D + 4 * g;
 #pragma unroll
@@ -378,24 +385,15 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, const uin
       uint4 weights[NQ][kParts];
       float z[NQ][8];
       powers<E, D, NQ>(state, s, scale, last - first - step * kStep, g, z);
-      weigh<E>(z[0], weights[0]);
+      weigh<E>(z[0], weights[0], state[0].total);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {                   // the next tile's weights beside this one's products
-        if (n + 1 < NQ) weigh<E>(z[n + 1], weights[n + 1]);
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) state[n].total = mfma<E>(ones<E>(), weights[n][k], state[n].total);
+        if (n + 1 < NQ) weigh<E>(z[n + 1], weights[n + 1], state[n + 1].total);
 #pragma unroll
         for (int j = 0; j < C; ++j)
 #pragma unroll
           for (int k = 0; k < kParts; ++k) state[n].sums[j] = mfma<E>(column[j], weights[n][k], state[n].sums[j]);
-        if (n + 1 < NQ) {
-#pragma unroll
-          for (int j = 0; j < (C + 1) * kParts; ++j) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x402, 4, 0);
-          }
-        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -541,15 +539,13 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
     const int live = last - first - t * kStep;
     powers<E, D, 1>(of_row, s, scale, live, g, z);
     uint4 weights[kParts];
-    weigh<E>(z[0], weights);
+    weigh<E>(z[0], weights, state.total);
     if (live < kStep) {                                // values of keys behind the last token: zeros
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int c = 0; c < C / 2; ++c) values[i][c] = i / 4 * 16 + g * 4 + i % 4 < live ? values[i][c] : 0;
     }
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) state.total = mfma<E>(ones<E>(), weights[k], state.total);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const uint4 v = column<C>(values, j);
@@ -564,7 +560,8 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
   float peak = -INFINITY;
   for (int i = 0; i < min(kWaves, count); ++i) peak = fmaxf(peak, peaks[i * 16 + r]);
   const float share = wave >= count ? 0.0f : peak == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-state.base - peak);
-  if (g == 0) peaks[(kWaves + wave) * 16 + r] = wave < count ? state.total[0] * share : 0.0f;
+  const float total = sum_of_row(state.total);
+  if (g == 0) peaks[(kWaves + wave) * 16 + r] = wave < count ? total * share : 0.0f;
   // Wave w joins rows 4 w .. 4 w + 3, a lane the D / 16 columns of one from r D / 16 on.
   const int row = wave * 4 + g, of_group = tile * 16 + row;
   float joined[C];
