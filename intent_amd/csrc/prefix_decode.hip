@@ -229,11 +229,11 @@ template <int T>
 struct WaveTile {
   int page, in, most;
   // `entries`: of the table; 0 where the entry is known to be one of its.
-  __device__ __forceinline__ void find(const Decode &p, const int32_t *table, int entries, int begin, int token, int last) {
-    const int base = min(token, last - 1) & ~(T - 1), entry = page_of(p, base);
+  __device__ __forceinline__ void find(const Decode &p, const int32_t *table, int entries, int begin, uint32_t token, int last) {
+    const int base = static_cast<int>(min(token, static_cast<uint32_t>(last - 1))) & ~(T - 1), entry = page_of(p, base);
     page = page_of_wave(table, entries, begin + entry);
     in = base - entry * p.ps, most = last - 1 - base;
-    if (token >= last) in += most, most = 0;           // a tile behind the last token reads that one alone
+    if (token >= static_cast<uint32_t>(last)) in += most, most = 0;           // a tile behind the last token reads that one alone
   }
   // Its first row, of keys (0) or of values (1).
   __device__ __forceinline__ const uint16_t *rows(const Decode &p, const uint16_t *cache, int which) const {
@@ -304,7 +304,7 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, const uin
           continue;
         }
         const int row = __builtin_amdgcn_readfirstlane((i * kWaves + wave) * kWave / kRowUnits);
-        next[i].find(p, p.prefix, 0, 0, first + min(t, count - 1) * kStep + row / T * T, last);
+        next[i].find(p, p.prefix, 0, 0, static_cast<uint32_t>(first + min(t, count - 1) * kStep + row / T * T), last);
       }
     };
     // Where this lane's unit of each load lies from its tile's first row on.
@@ -474,12 +474,14 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
   struct Step {
     WaveTile<T> tile[kHalves];
   };
+  // A token's place behind the last step may pass 2^31, so it is counted without a sign until it is clamped.
+  const auto token_at = [&](int t, int row) { return static_cast<uint32_t>(first) + static_cast<uint32_t>(t) * kStep + row; };
   const auto find = [&](int t) {
     Step found{};
     if constexpr (kTile > 0) {
 #pragma unroll
       for (int i = 0; i < kHalves; ++i)
-        found.tile[i].find(p, p.indices, p.positions, sequence.first, first + t * kStep + i * T, last);
+        found.tile[i].find(p, p.indices, p.positions, sequence.first, token_at(t, i * T), last);
     }
     return found;
   };
@@ -492,7 +494,7 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
       return tile.rows(p, cache, which) + (static_cast<uint32_t>(min(row % T, tile.most)) * p.of_token[which] + at * 2) / 2;
     } else {
       const int64_t(&strides)[3] = which ? p.vs : p.ks;
-      const int token = min(first + t * kStep + row, last - 1), entry = page_of(p, token);
+      const int token = static_cast<int>(min(token_at(t, row), static_cast<uint32_t>(last - 1))), entry = page_of(p, token);
       return cache + physical(p, p.indices, p.positions, sequence.first + entry) * strides[0] + (token - entry * p.ps) * strides[1] + at;
     }
   };
@@ -504,7 +506,7 @@ __device__ __forceinline__ void own_job(const Decode &p, int block, float *sums,
       for (int c = 0; c < kChunks; ++c) to[half][c] = *reinterpret_cast<const uint4 *>(key + c * 32);
     }
   };
-  const int count = (last - first + kStep - 1) / kStep;
+  const int count = static_cast<int>((static_cast<uint32_t>(last - first) + kStep - 1) / kStep);
   uint4 next_keys[2][kChunks];
   Step next = find(wave), after = find(wave + kWaves);
   if (wave < count) load_keys(next, wave, next_keys);

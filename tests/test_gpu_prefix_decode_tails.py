@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.gpu_util import announce
-from tests.test_gpu_prefix_decode import case, run
+from tests.test_gpu_prefix_decode import case, i32, kernel, run
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,19 @@ def test_no_score_is_a_number_above_minus_infinity(device, dtype):
     got = run(device, dtype, [given[0], in_own, *given[2:]])
     alone = run(device, dtype, [*given[:7], torch.zeros_like(given[7]), given[8]])
     assert torch.equal(got[:, :4], alone[:, :4])
+
+
+@pytest.mark.parametrize("ps", [4095, 4096])
+def test_as_many_tokens_as_a_length_counts(device, ps):
+    """2^31 - 1 own tokens, whose pages are one: equal keys and values of powers of two, so the output is those values exactly, whatever
+    the order of the sums."""
+    announce("decode behind a prefix, 2^31 - 1 tokens", ps)
+    length, d = 2 ** 31 - 1, 64
+    positions = -(-length // ps)
+    q = torch.ones((1, 1, d), dtype=torch.bfloat16, device=device)
+    keys = torch.zeros((1, ps, 1, d), dtype=torch.bfloat16, device=device)
+    values = (2.0 ** (torch.arange(d, device=device) % 7 - 3)).bfloat16().expand(1, ps, 1, d).contiguous()
+    tables = [i32(v).to(device) for v in ([], [0], [0, positions])]
+    pages = torch.zeros(positions, dtype=torch.int32, device=device)
+    got = kernel("bf16", 1).run(q, keys, values, *tables, pages, i32([length]).to(device), 0.125)
+    assert torch.equal(got[0, 0], values[0, 0, 0])
