@@ -62,7 +62,7 @@ __global__ __launch_bounds__(W *kWave) void quantize_rows(Quantize p) {
   const RowQuant quant(most[0]);
 #pragma unroll
   for (int j = 0; j < P; ++j) store_piece(p.q + row * p.qs, at, j, quant.piece(a[j]));
-  if (at.thread == 0) p.scales[row] = row_scale(most[0], 1.0f);
+  if (at.thread == 0) p.scales[row] = row_scale(most[0]);
 }
 
 // How a row lies over threads: pieces of a thread, and the waves that its kernel is built for. Two pieces from rows of 1024 on leave fewer

@@ -101,7 +101,9 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_rows(Norm p) {
   if constexpr (kI8) {
     row_reduce(sum, most, p.waves, second);
     const float unit = rsqrtf(sum[0] * p.inverse_d + p.eps);
-    const RowQuant quant(most[0]);
+    // max|y| says what the row is; where the root is 0 or infinite it is not what max|h w| would say. Elements of 0 go without a quotient.
+    const uint32_t top = magnitude(__uint_as_float(most[0]) * unit);
+    const RowQuant quant(top > 0 && top < kInfinity ? most[0] : kInfinity);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       float v[kPiece];
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(W *kWave) void residual_norm_rows(Norm p) {
       for (int i = 0; i < kPiece; ++i) v[i] = h[j][i] * w[j][i];
       store_piece(p.q + token * p.os, at, j, quant.piece(v));
     }
-    if (at.thread == 0) p.scales[token] = row_scale(most[0], unit);
+    if (at.thread == 0) p.scales[token] = row_scale(top);
   } else {
     RowSlots<1> &slots = *reinterpret_cast<RowSlots<1> *>(&second);
     row_reduce(sum, p.waves, slots);

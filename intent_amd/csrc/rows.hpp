@@ -251,9 +251,9 @@ struct RowQuant {
   }
 };
 
-// What an integer counts: `unit` times m / 127.
-__device__ __forceinline__ float row_scale(uint32_t bits, float unit) {
-  return bits < kInfinity ? __uint_as_float(bits) * unit / 127.0f : __uint_as_float(0x7FC00000u);
+// What an integer counts: m / 127.
+__device__ __forceinline__ float row_scale(uint32_t bits) {
+  return bits < kInfinity ? __uint_as_float(bits) / 127.0f : __uint_as_float(0x7FC00000u);
 }
 
 constexpr int kMaxRow = kPiece * kWave * kMaxRowWaves * 2;      // 16384 elements: two pieces of 16 waves' threads
