@@ -17,7 +17,7 @@
 
 #include <type_traits>
 
-#include "common.hpp"
+#include "stages.hpp"
 
 namespace intent_hip {
 namespace {
@@ -27,7 +27,6 @@ constexpr int kFewWaves = 16;
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void lds_void_t;
 
 struct Linear {
   const int8_t *x, *w;
@@ -40,21 +39,6 @@ struct Linear {
   int full;                            // linear_big: tiles of I = 4
   int wide;                            // y takes stores of so many elements (1, 4 or 8)
 };
-
-// s_waitcnt with only the vector-memory counter constrained (vmcnt <= n).
-#define INTENT_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt((((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4) | (0xF << 8)))
-#define INTENT_WAIT_LGKMCNT0() __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4))
-
-// s_barrier with an acquire fence alone: a release fence would wait for every load into the LDS that is on its way.
-__device__ __forceinline__ void stage_barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-  __builtin_amdgcn_sched_barrier(0);
-}
-
-// What is read behind K.
-__device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
 
 __device__ __forceinline__ i32x4_t mfma(uint4 a, uint4 b, i32x4_t c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);

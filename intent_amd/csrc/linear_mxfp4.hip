@@ -26,6 +26,7 @@
 #include <type_traits>
 
 #include "mx.hpp"
+#include "stages.hpp"
 
 namespace intent_hip {
 namespace {
@@ -191,22 +192,6 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few(Linear p) {
   const int n = n0 + g * kSums + wave;
   if (n < p.n) p.y[r * p.ldy + n] = from_f32<E>(total).bits;
 }
-
-typedef __attribute__((address_space(3))) void lds_void_t;
-
-// s_waitcnt with only the vector-memory counter constrained (vmcnt <= n).
-#define INTENT_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt((((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4) | (0xF << 8)))
-
-// s_barrier with an acquire fence alone: a release fence would wait for every load into the LDS that is on its way.
-__device__ __forceinline__ void stage_barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-  __builtin_amdgcn_sched_barrier(0);
-}
-
-// What is read of x behind K.
-__device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
 
 // 16 MT rows of x by 16 NT weight rows for each of W waves; S stages of 128 columns are on their way or in use. Each has an LDS array
 // of its own, and the loop is unrolled by S: the compiler then knows which loads into the LDS a read has to wait for.

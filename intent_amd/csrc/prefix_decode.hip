@@ -24,7 +24,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.hpp"
+#include "stages.hpp"
 
 namespace intent_hip {
 namespace {
@@ -46,7 +46,6 @@ typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) void lds_void_t;
 
 struct Decode {
   const uint16_t *q, *k, *v;
@@ -64,19 +63,6 @@ struct Decode {
   // States: of the prefix [parts][batch][q_heads] (and [D]), then of the jobs [jobs][q_heads] (and [D]).
   float *peak, *total, *sums;
 };
-
-#define INTENT_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt((((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4) | (0xF << 8)))
-
-// s_barrier with an acquire fence alone: a release fence would wait for every load into the LDS that is on its way.
-__device__ __forceinline__ void stage_barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-  __builtin_amdgcn_sched_barrier(0);
-}
-
-// What keys behind the last token have as values: a weight of 0 times that token's own, were it infinite, would not be 0.
-__device__ const uint4 kZeroUnit = {0u, 0u, 0u, 0u};
 
 template <typename E>
 __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
@@ -325,7 +311,9 @@ __device__ __forceinline__ void prefix_job(const Decode &p, int block, const uin
         const uint16_t *k, *v;
         if constexpr (kTile > 0) {
           k = next[i].rows(p, keys_of, 0), v = next[i].rows(p, values_of, 1);
-          if (next[i].most < T - 1) {                  // a tile that not all of counts: the last row again, as values zeros
+          // A tile that not all of counts: the last row again, as values zeros (a weight of 0 times that row's own, were they infinite, would
+          // not be 0).
+          if (next[i].most < T - 1) {
             const uint32_t row = min(row_of[i] % T, next[i].most);
             k += (row * p.of_token[0] + unit_of[i] * 2) / 2;
             v = begin + row_of[i] < last ? v + (row * p.of_token[1] + unit_of[i] * 2) / 2 : zeros;
