@@ -690,14 +690,15 @@ struct Cut {
   int nq, row_tiles, parts, head_tiles, job_pages, jobs;
 };
 
-// NQ = 2 reads the LDS half as often, NQ = 1 leaves room for more waves: us with NQ = 1 and 2 of 32 rows for a key head and 128 dimensions
-// (8 sequences, 8191 + 512 tokens, 8 key heads) 23.5 and 26.8, of 64 (16 sequences) 28.1 and 31.9, of 512 (64 sequences, 16384 + 1000) 118 and
-// 108; of 64 dimensions, 128 rows 24.3 and 28.1, 512 rows 65.4 and 62.6. Parts of the prefix for three workgroups a CU in place of two: 25.7
-// for 23.8 (one sequence, 16384 tokens), 107.0 for 106.5.
+// NQ = 2 reads the LDS half as often, NQ = 1 leaves room for more waves, which the own tokens' jobs need too. us with NQ = 1 and 2, of 128
+// dimensions, bf16, 8 key heads: 128 rows for a key head behind 8192 tokens, up to 512 of their own, 28.1 and 37.3; 512 rows 65 and 70, behind
+// 16384 with up to 1000 110 and 113, with 1 92 and 85; 768 rows behind 8192 88 and 87, behind 16384 alone 136 and 122; of 64 dimensions, 256 rows
+// 27.0 and 30.3, 512 rows 42.7 and 42.7, behind 16384 alone 65 and 60, 1024 rows 73 and 70. Parts of the prefix for three workgroups a CU in
+// place of two: 23.5 for 21.5 (one sequence, 16384 tokens), 118 for 113 (512 rows, 16384 + 1000).
 Cut cut(int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, int64_t prefix_positions, int64_t positions) {
   Cut c{};
   const int64_t rows = batch * group, cus = device_cus();
-  c.nq = rows <= (d == 64 ? 128 : 64) ? 1 : 2;
+  c.nq = rows <= 4 * d ? 1 : 2;
   c.row_tiles = static_cast<int>((rows + kWaves * 16 * c.nq - 1) / (kWaves * 16 * c.nq));
   const int64_t tokens = prefix_positions * ps, tiles = std::max<int64_t>(c.row_tiles * kv_heads, 1);
   const int64_t most = (tokens + 127) / 128;           // a part walks four steps at least
