@@ -11,8 +11,9 @@
 //   * linear_tiles, 64 or 128 x 128 results: x through the LDS, weights to registers, K over several workgroups. 32 x 4096 x 14336 20 us, of
 //     which the fold is 4; 128 x 14336 x 4096 30.5, 256 40.
 //   * linear_big, 256 or 128 x 256 results of four waves: both operands through the LDS. 4096 x 14336 x 4096 247 us, 8192^3 510 (2160
-//     TOP/s), 1024 x 14336 x 4096 73, 512 51; 1021 x 4096 x 14336 97, K in two parts, 11 of them the fold. At 4096 x 4096 x 14336 (2180
-//     TOP/s) the clock falls to 1.9 GHz under this load, which is what bounds it then.
+//     TOP/s), 1024 x 14336 x 4096 73, 512 51; 1021 x 4096 x 14336 97, K in two parts, 11 of them the fold. The matrix pipe is busy in 52%
+//     of the cycles at 4096 x 14336 x 4096, in 64% at 8192^3 (a library's product without scales: 72%), at clocks that fall to 1.6 .. 1.75 GHz under
+//     this load; what the other cycles wait for has not been found.
 #include <stdio.h>
 
 #include <type_traits>

@@ -15,10 +15,10 @@
 // + 3 in lane (r, g), where the second product wants them: columns of the values as rows, 32 keys (4 of each 16 a lane) summed over. The
 // LDS gives those columns turned (ds_read_b64_tr_b16); from memory a lane reads D / 16 columns of its eight keys and pairs them with
 // v_perm. The peak is raised only when a score passes it by 2^4.
-// Measured: 64 sequences behind 16384 tokens, up to 1000 of their own, 64 heads on 8, bf16, 105.5 us; the prefix alone 80 (matrix pipe 33%
-// busy, vector pipe 25%: two waves a SIMD, each of whose steps waits for its own LDS reads, products and weights in turn; three waves
-// spilled), the own tokens alone 52 (2.7 TB/s), the join 12 of each; own jobs between those of the prefix instead of behind them 130. 8
-// sequences behind 8191 tokens, up to 512, 32 heads on 8, f16, 21.8 us, of which the join is 5.
+// Measured: 64 sequences behind 16384 tokens, up to 1000 of their own, 64 heads on 8, bf16, 111 us (matrix pipe 32% busy, vector pipe 33%: two
+// or three waves a SIMD, each of whose steps waits for its own LDS reads, products and weights in turn); the prefix alone 94, the own tokens
+// alone 47 (2.8 TB/s), the join 12 of each; own jobs between those of the prefix instead of behind them 130, before weights were whole. 8
+// sequences behind 8191 tokens, up to 512, 32 heads on 8, f16, 19.6 us, of which the join is 5. Weights of two numbers, 16 bits in bf16: 101 and 18.8.
 #include <stdio.h>
 
 #include <algorithm>
@@ -704,7 +704,8 @@ Cut cut(int64_t batch, int64_t kv_heads, int64_t group, int64_t d, int64_t ps, i
   const int64_t most = (tokens + 127) / 128;           // a part walks four steps at least
   c.parts = static_cast<int>(tokens == 0 ? 0 : std::max<int64_t>(1, std::min<int64_t>(most, 2 * cus / tiles)));
   c.head_tiles = static_cast<int>((group + 15) / 16);
-  // Jobs of 128 tokens, of more where that makes over two a CU: the 8 sequences 21.8 us (256: 23.5, 512: 26.3), the 64 106.5 (256: 108.5).
+  // Jobs of 128 tokens, of more where that makes over two a CU: 8 sequences behind 8191 tokens 19.6 us (256: 20.2), 16 24.6 (25.3); of 64
+  // dimensions 256 would take less where there are many (32 sequences behind 8192 20.5 for 23.2) and more where there are few (one 14.5 for 13.7).
   const int64_t own = positions * ps, aim = 2 * cus / std::max<int64_t>(kv_heads * c.head_tiles, 1);
   const int64_t of_job = std::max<int64_t>(128, (own + std::max<int64_t>(aim, 1) - 1) / std::max<int64_t>(aim, 1));
   c.job_pages = ps > 0 ? static_cast<int>(std::max<int64_t>(1, (of_job + ps - 1) / ps)) : 1;

@@ -280,7 +280,8 @@ __global__ __launch_bounds__(16 * kFoldParts) void residual_norm_fold(const floa
 struct Layout {
   int pieces, most;
 };
-// Forward: 16384 x 2048 takes 50.9 us in one piece a thread, 53.0 in two, and 16384 x 4096 99.7 in two, 97.1 in one (8-bit rows 90.2 and 91.8).
+// Forward: 16384 x 2048 takes 50.9 us in one piece a thread, 53.0 in two, and 16384 x 4096 99.7 in two, 97.1 in one; 8-bit rows 90.2 in two, 91.8
+// in one. One rule for both kinds, so plain rows of 4096 take 3% longer than they could.
 // Backward: one piece leaves registers for the rows of the next token (8192 x 8192 184 us; two pieces of 8 waves 191).
 Layout forward_layout(int64_t d) { return row_waves(d, 1) <= 4 ? Layout{1, 4} : Layout{2, 16}; }
 Layout backward_layout(int64_t d) { return row_waves(d, 1) <= 8 ? Layout{1, 8} : row_waves(d, 1) <= 16 ? Layout{1, 16} : Layout{2, 16}; }
