@@ -618,8 +618,8 @@ int intent_hip_linear_i8(int dtype, const int8_t *x, const int8_t *weight, const
  * prefix_indices [prefix_positions]; sequence s adds the first lengths[s] tokens of the pages page_offsets[s] .. page_offsets[s + 1] of
  * page_indices [positions], lengths[s] not counting the prefix; no more than the tables hold; output is 0 where there is no token.
  * page_offsets [batch + 1] start at 0 or above and do not decrease; entries and pages outside their arrays read the nearest. Products are
- * summed in f32; weights are f32 and enter the second product whole, as three numbers of the rows' type (but for what lies below 2^-35 of
- * the largest in f16); one rounding at the end. Nothing depends on the host's knowledge of lengths and offsets, so they may change under a captured graph. Rows of
+ * summed in f32; weights are f32 and enter the second product whole, as three numbers of the rows' type (but for 2^-36 of the largest in
+ * f16); one rounding at the end. Nothing depends on the host's knowledge of lengths and offsets, so they may change under a captured graph. Rows of
  * q and of the caches 16-byte aligned, their strides multiples of 8. The states of jobs meet in the workspace
  * (intent_hip_paged_gqa_decode_prefix_workspace_bytes bytes, 16-byte aligned).
  * strides[14]: q[3], key_cache[4], value_cache[4], output[3]. */

@@ -4,7 +4,7 @@
 // For query head h of sequence s, over the prefix's tokens and the sequence's own:
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = exp2(scale * log2(e) * (q . k_j) - peak)        0 where there is no token
 // Products are summed in f32. Weights are f32 and enter the second product whole, as three numbers of the queries' type each, but for what
-// f16 leaves below 2^-35 of the largest.
+// 2^-36 of the largest in f16.
 //
 // Design. One launch does two kinds of jobs, whose states (peak, sum of weights, weighted sum of values) a second kernel joins:
 //   * the prefix: the query heads of all sequences that share a key head are the rows of one product, so the prefix is read once for 64
@@ -73,18 +73,17 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
 }
 
 constexpr int kParts = 3;              // numbers of a weight
-// Weights are held at this power of two (times 2^kSlack they stay below the largest f16).
+// The largest weight is held at this power of two, and 2^kSlack times that before the peak is raised: just below the largest f16.
 template <typename E>
-constexpr float kRaise = std::is_same_v<E, f16_t> ? 11.0f : 0.0f;
+constexpr float kRaise = std::is_same_v<E, f16_t> ? 11.9375f : 0.0f;
 
 // Two weights as kParts numbers each, every one what those before it leave, cut off: three of bf16 hold all 24 bits of a weight, and so do
-// three of f16 down to f16's last, 2^-24, which is 2^-35 of the largest weight. No number of a weight that counts is 0, so that an infinite
-// value gives an infinity and not 0 times it: where the first is not 0, the others are the least of their type at least (f16 2^-24, bf16
-// 2^-126).
+// three of f16 down to f16's last, 2^-24, which is about 2^-36 of the largest weight. No number of a weight that counts is 0, so that an
+// infinite value gives an infinity and not 0 times it: the second and third are the least of their type at least (2^-126 in bf16). In f16,
+// whose least is 2^-24, only where the first has all its bits (2^-13, 2^-25 of the largest): smaller weights would move by more than the cut.
 template <typename E>
 __device__ __forceinline__ void rounded(float a, float b, uint32_t (&part)[kParts]) {
   constexpr bool kHalf = std::is_same_v<E, f16_t>;
-  constexpr unsigned short kLeast = kHalf ? 0x0001 : 0x0080;
 #pragma unroll
   for (int i = 0; i < kParts; ++i) {
     if constexpr (kHalf) {
@@ -97,7 +96,9 @@ __device__ __forceinline__ void rounded(float a, float b, uint32_t (&part)[kPart
       a -= __uint_as_float(u & 0xFFFF0000u), b -= __uint_as_float(v & 0xFFFF0000u);
     }
   }
-  const u16x2_t least = __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, part[0]), u16x2_t{kLeast, kLeast});
+  const u16x2_t first = __builtin_bit_cast(u16x2_t, part[0]);
+  const u16x2_t least = kHalf ? __builtin_elementwise_min(first >> u16x2_t{11, 11}, u16x2_t{1, 1})
+                              : __builtin_elementwise_min(first, u16x2_t{0x0080, 0x0080});
 #pragma unroll
   for (int i = 1; i < kParts; ++i)
     part[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, part[i]), least));

@@ -8,8 +8,8 @@ pages hold. Query head h attends to key head h / HEAD_GROUP over both:
 
   output = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q . k_j - max)        0 where there is no token
 
-Sums and weights are f32; weights enter the second product whole, as three numbers of the rows' type (but for what lies below 2^-35 of the
-largest in f16). An infinite value gives an infinity, or NaN where its weight is below 2^-35 (f16) or 2^-126 (bf16) of the largest; a row all
+Sums and weights are f32; weights enter the second product whole, as three numbers of the rows' type (but for 2^-36 of the largest in
+f16). An infinite value gives an infinity, or NaN where its weight is below 2^-25 (f16) or 2^-126 (bf16) of the largest; a row all
 of whose scores are -inf gives NaN. page_offsets start at 0 or above and do not decrease. Table entries outside their table and pages outside the cache read the nearest. Lengths, offsets and tables are read as they are
 at the launch, so a captured graph follows them. D is 64 or 128.
 
