@@ -6,7 +6,7 @@ a weight, and an error of a weight stands out in it.
 
 Bound. A score is one product, exact; the factor scale * log2(e) is off by two roundings and its product with the score by one more: 3 * 2^-24
 of a_j = |score| * log2(e). The sum with the peak rounds once, by half a step of a number below 2 (bf16) or below 16 (f16, whose weights are held
-at 2^11). exp2 is off by 2^-22. So a weight is off by a share e_j, and the output by sum p_j e_j |v_j - out|. Three tokens of three numbers each are
+near 2^12). exp2 is off by 2^-22. So a weight is off by a share e_j, and the output by sum p_j e_j |v_j - out|. Three tokens of three numbers each are
 9 terms, each rounding by 2^-23 of the magnitudes (sums that are cut off); the divisor's sum and the division add 3. Then half a step of the type."""
 import torch
 
